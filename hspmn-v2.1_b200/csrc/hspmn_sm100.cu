@@ -1,7 +1,7 @@
 // C ABI of libhspmn_sm100.so (declared in include/hspmn_sm100.h): argument
 // validation, launch configuration and TMA descriptor encoding for the
-// router gate and selection, row gather/scatter and SQDK attention (forward and
-// backward) kernels. One translation unit so all kernels share the device
+// router gate and selection, row gather/scatter, SQDK attention (forward and
+// backward) and paged K/V cache kernels. One translation unit so all kernels share the device
 // error word.
 
 #include <cuda.h>
@@ -11,11 +11,14 @@
 #include <cmath>
 #include <cstdint>
 #include <cstring>
+#include <initializer_list>
 #include <mutex>
 #include <type_traits>
 
 #include "common.cuh"
 #include "gate.cuh"
+#include "paged.cuh"
+#include "paged_attn.cuh"
 #include "router.cuh"
 #include "rows.cuh"
 #include "sqdk.cuh"
@@ -771,6 +774,215 @@ int hspmn_sqdk_fwd_noalloc(const void* q, const int64_t* qs, const void* k, cons
   // scratch stands in for the caller's workspace
   return sqdk_fwd_impl(q, qs, k, ks, v, vs, idx, idx_sb, idx_sk, o, os, nullptr, 0, 0, B, K, S, H, Hkv, hd, dtype,
                        sm_scale, nullptr, 0, true, stream);
+}
+
+}  // extern "C"
+
+namespace {
+
+// log2 of a page size the cache kernels take (a power of two from 8 to 4096), else -1.
+int page_shift(int64_t page_size) {
+  for (int s = 3; s <= 12; ++s)
+    if (page_size == (1 << s)) return s;
+  return -1;
+}
+
+// Whether every stride is non-negative and, in bytes, a multiple of 16.
+int check_strides(std::initializer_list<int64_t> strides, int64_t es) {
+  for (int64_t s : strides)
+    if (s < 0) return HSPMN_ERR_INVALID;
+  for (int64_t s : strides)
+    if ((s * es) % 16) return HSPMN_ERR_ALIGN;
+  return HSPMN_OK;
+}
+
+template <typename T>
+void launch_paged_write(const PagedWriteParams& prm, bool f32_tables, unsigned grid, cudaStream_t st) {
+  if (f32_tables) rope_paged_write_kernel<T, float><<<grid, kRowThreads, 0, st>>>(prm);
+  else rope_paged_write_kernel<T, T><<<grid, kRowThreads, 0, st>>>(prm);
+}
+
+template <int HD, bool kBF16>
+int launch_paged_attn(const PagedAttnParams& prm, int runs, cudaStream_t st) {
+  auto kern = paged_attn_kernel<HD, kBF16>;
+  constexpr int smem = PagedLayout<HD>::kBytes;
+  if (cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, smem) != cudaSuccess)
+    return HSPMN_ERR_CUDA;
+  kern<<<static_cast<unsigned>(runs), kPagedThreads, smem, st>>>(prm);
+  if (int rc = launch_status()) return rc;
+  if (runs > 1) paged_merge_kernel<HD, kBF16><<<static_cast<unsigned>(runs - 1), 32 * kMergeWarps, 0, st>>>(prm, runs);
+  return launch_status();
+}
+
+int64_t paged_part_o_bytes(int64_t runs, int64_t hdp) { return 2 * runs * kPagedRows * hdp * 4; }
+
+}  // namespace
+
+extern "C" {
+
+int hspmn_paged_slots(int32_t* block_table, int64_t table_rs, const int32_t* seq_lens, const int32_t* new_lens,
+                      const int32_t* free_pages, int64_t num_free, int64_t R, int64_t P, int64_t page_size, int64_t N,
+                      int32_t* cu_new, int32_t* kv_lens, int64_t* positions, int64_t* slots, int32_t* taken,
+                      void* stream) {
+  if (R < 0 || P < 0 || N < 0 || num_free < 0 || !cu_new || !taken) return HSPMN_ERR_INVALID;
+  if (R > 0 && (!seq_lens || !new_lens || !kv_lens)) return HSPMN_ERR_INVALID;
+  if (R > 0 && P > 0 && (!block_table || table_rs < P)) return HSPMN_ERR_INVALID;
+  if ((num_free > 0 && !free_pages) || (N > 0 && (!positions || !slots))) return HSPMN_ERR_INVALID;
+  const int shift = page_shift(page_size);
+  if (shift < 0 || R > kSlotsMaxRequests) return HSPMN_ERR_UNSUPPORTED;
+  if (N > 0x7FFFFFFF || num_free > 0x7FFFFFFF || R * P > 0x7FFFFFFF || P > 0x7FFFFFFF) return HSPMN_ERR_INVALID;
+  if (int rc = check_device()) return rc;
+  int sms = 0;
+  if (int rc = sm_count(&sms)) return rc;
+  SlotsParams prm;
+  prm.table = block_table;
+  prm.table_rs = table_rs;
+  prm.seq_lens = seq_lens;
+  prm.new_lens = new_lens;
+  prm.free_pages = free_pages;
+  prm.R = static_cast<int>(R);
+  prm.P = static_cast<int>(P);
+  prm.F = static_cast<int>(num_free);
+  prm.shift = shift;
+  prm.N = N;
+  prm.cu = cu_new;
+  prm.kv_lens = kv_lens;
+  prm.pos = positions;
+  prm.slots = slots;
+  prm.taken = taken;
+  const size_t smem = static_cast<size_t>(2 * (R + 1) * 4);
+  if (smem > 48 * 1024 &&
+      cudaFuncSetAttribute(paged_slots_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize,
+                           2 * (kSlotsMaxRequests + 1) * 4) != cudaSuccess)
+    return HSPMN_ERR_CUDA;
+  const int64_t need = std::max<int64_t>(1, (N + kSlotsThreads - 1) / kSlotsThreads);
+  const unsigned grid = static_cast<unsigned>(std::min<int64_t>(need, 2LL * sms));
+  paged_slots_kernel<<<grid, kSlotsThreads, smem, static_cast<cudaStream_t>(stream)>>>(prm);
+  return launch_status();
+}
+
+int hspmn_rope_paged_write(const void* k, int64_t k_sn, int64_t k_sh, const void* v, int64_t v_sn, int64_t v_sh,
+                           const void* cos_tab, const void* sin_tab, int64_t tab_ss, int64_t tab_rows, int tab_dtype,
+                           const int64_t* positions, const int64_t* slots, void* k_cache, int64_t kc_sp,
+                           int64_t kc_ss, int64_t kc_sh, void* v_cache, int64_t vc_sp, int64_t vc_ss, int64_t vc_sh,
+                           int64_t N, int64_t Hkv, int64_t hd, int64_t num_pages, int64_t page_size, int dtype,
+                           void* stream) {
+  if (N < 0 || Hkv < 1 || hd < 1 || num_pages < 0 || (cos_tab == nullptr) != (sin_tab == nullptr))
+    return HSPMN_ERR_INVALID;
+  if (!valid_dtype(dtype) || (cos_tab && tab_dtype != dtype && tab_dtype != HSPMN_F32)) return HSPMN_ERR_DTYPE;
+  const int64_t es = dtype == HSPMN_F32 ? 4 : 2;
+  const int shift = page_shift(page_size);
+  if (shift < 0 || (hd * es) % (cos_tab ? 32 : 16) || Hkv * hd > 0x7FFFFFFF) return HSPMN_ERR_UNSUPPORTED;
+  if (cos_tab && (tab_ss < hd || tab_rows < 0)) return HSPMN_ERR_INVALID;
+  if (int rc = check_strides({k_sn, k_sh, v_sn, v_sh, kc_sp, kc_ss, kc_sh, vc_sp, vc_ss, vc_sh}, es)) return rc;
+  const int64_t tes = tab_dtype == HSPMN_F32 ? 4 : 2;
+  if (cos_tab && (tab_ss * tes) % 16) return HSPMN_ERR_ALIGN;
+  if (!aligned(k, 16) || !aligned(v, 16) || !aligned(cos_tab, 16) || !aligned(sin_tab, 16) || !aligned(k_cache, 16) ||
+      !aligned(v_cache, 16))
+    return HSPMN_ERR_ALIGN;
+  if (N == 0) return HSPMN_OK;
+  if (!k || !v || !slots || (cos_tab && !positions) || (num_pages > 0 && (!k_cache || !v_cache)))
+    return HSPMN_ERR_INVALID;
+  if (int rc = check_device()) return rc;
+  int sms = 0;
+  if (int rc = sm_count(&sms)) return rc;
+  PagedWriteParams prm;
+  prm.k = static_cast<const char*>(k);
+  prm.v = static_cast<const char*>(v);
+  prm.k_sn = k_sn * es, prm.k_sh = k_sh * es, prm.v_sn = v_sn * es, prm.v_sh = v_sh * es;
+  prm.cos_tab = static_cast<const char*>(cos_tab);
+  prm.sin_tab = static_cast<const char*>(sin_tab);
+  prm.tab_ss = tab_ss * tes;
+  prm.tab_rows = tab_rows;
+  prm.pos = positions;
+  prm.slots = slots;
+  prm.kc = static_cast<char*>(k_cache);
+  prm.vc = static_cast<char*>(v_cache);
+  prm.kc_sp = kc_sp * es, prm.kc_ss = kc_ss * es, prm.kc_sh = kc_sh * es;
+  prm.vc_sp = vc_sp * es, prm.vc_ss = vc_ss * es, prm.vc_sh = vc_sh * es;
+  prm.N = N;
+  prm.num_pages = num_pages;
+  prm.shift = shift;
+  prm.Hkv = static_cast<int>(Hkv);
+  prm.hd = static_cast<int>(hd);
+  const int64_t need = (N + kRowWarps - 1) / kRowWarps;
+  const unsigned grid = static_cast<unsigned>(std::min<int64_t>(need, 64LL * sms));
+  cudaStream_t st = static_cast<cudaStream_t>(stream);
+  const bool f32_tables = cos_tab && tab_dtype == HSPMN_F32;
+  if (dtype == HSPMN_BF16) launch_paged_write<__nv_bfloat16>(prm, f32_tables, grid, st);
+  else if (dtype == HSPMN_F16) launch_paged_write<__half>(prm, f32_tables, grid, st);
+  else launch_paged_write<float>(prm, true, grid, st);
+  return launch_status();
+}
+
+int64_t hspmn_sqdk_paged_workspace_size(int64_t hd) {
+  int sms = 0;
+  if (sm_count(&sms) != HSPMN_OK) return -1;
+  const int64_t runs = static_cast<int64_t>(sms) * kPagedCtasPerSm;
+  return paged_part_o_bytes(runs, hd > 64 ? 128 : 64) + 2 * runs * kPagedRows * 2 * 4;
+}
+
+int hspmn_sqdk_paged_fwd(const void* q, int64_t q_sn, int64_t q_sh, const void* k_cache, int64_t kc_sp, int64_t kc_ss,
+                         int64_t kc_sh, const void* v_cache, int64_t vc_sp, int64_t vc_ss, int64_t vc_sh,
+                         const int32_t* block_table, int64_t table_rs, const int32_t* kv_lens, const int32_t* cu_q,
+                         const int64_t* positions, void* o, int64_t o_sn, int64_t o_sh, int64_t N, int64_t R,
+                         int64_t P, int64_t num_pages, int64_t page_size, int64_t H, int64_t Hkv, int64_t hd,
+                         int dtype, float sm_scale, int64_t max_q, void* workspace, size_t workspace_bytes,
+                         void* stream) {
+  if (N < 0 || R < 0 || P < 0 || num_pages < 0 || H < 1 || Hkv < 1 || max_q < 0 || !(sm_scale > 0.0f) ||
+      !std::isfinite(sm_scale))
+    return HSPMN_ERR_INVALID;
+  if (dtype != HSPMN_BF16 && dtype != HSPMN_F16) return HSPMN_ERR_DTYPE;
+  const int shift = page_shift(page_size);
+  if (shift < 0 || hd < 8 || hd > 128 || hd % 8 != 0) return HSPMN_ERR_UNSUPPORTED;
+  if (H % Hkv != 0 || H / Hkv > kSqdkBM) return HSPMN_ERR_UNSUPPORTED;
+  if (N > 0x7FFFFFFF / H || R > 0x7FFFFFFE || P > (0x7FFFFFFF >> shift) || num_pages > 0x7FFFFFFF)
+    return HSPMN_ERR_INVALID;
+  const int64_t es = 2;
+  if (int rc = check_strides({q_sn, q_sh, kc_sp, kc_ss, kc_sh, vc_sp, vc_ss, vc_sh, o_sn, o_sh}, es)) return rc;
+  if (!aligned(q, 16) || !aligned(k_cache, 16) || !aligned(v_cache, 16) || !aligned(o, 16) || !aligned(workspace, 16))
+    return HSPMN_ERR_ALIGN;
+  if (N == 0) return HSPMN_OK;
+  if (!q || !o || !cu_q || !positions) return HSPMN_ERR_INVALID;
+  if (R > 0 && (!kv_lens || (P > 0 && (!block_table || table_rs < P)))) return HSPMN_ERR_INVALID;
+  if (num_pages > 0 && (!k_cache || !v_cache)) return HSPMN_ERR_INVALID;
+  if (int rc = check_device()) return rc;
+  int sms = 0;
+  if (int rc = sm_count(&sms)) return rc;
+  if (!workspace || workspace_bytes < static_cast<size_t>(hspmn_sqdk_paged_workspace_size(hd)))
+    return HSPMN_ERR_INVALID;
+  const int runs = sms * kPagedCtasPerSm;
+  PagedAttnParams prm;
+  prm.q = static_cast<const char*>(q);
+  prm.k = static_cast<const char*>(k_cache);
+  prm.v = static_cast<const char*>(v_cache);
+  prm.o = static_cast<char*>(o);
+  prm.q_sn = q_sn * es, prm.q_sh = q_sh * es, prm.o_sn = o_sn * es, prm.o_sh = o_sh * es;
+  prm.k_sp = kc_sp * es, prm.k_ss = kc_ss * es, prm.k_sh = kc_sh * es;
+  prm.v_sp = vc_sp * es, prm.v_ss = vc_ss * es, prm.v_sh = vc_sh * es;
+  prm.table = block_table;
+  prm.table_rs = table_rs;
+  prm.kv_lens = kv_lens;
+  prm.cu_q = cu_q;
+  prm.pos = positions;
+  prm.part_o = static_cast<float*>(workspace);
+  prm.part_ml = reinterpret_cast<float*>(static_cast<char*>(workspace) + paged_part_o_bytes(runs, hd > 64 ? 128 : 64));
+  prm.N = N;
+  prm.R = static_cast<int>(R);
+  prm.P = static_cast<int>(P);
+  prm.num_pages = static_cast<int>(num_pages);
+  prm.shift = shift;
+  prm.H = static_cast<int>(H);
+  prm.Hkv = static_cast<int>(Hkv);
+  prm.G = static_cast<int>(H / Hkv);
+  prm.hd = static_cast<int>(hd);
+  prm.scale_log2 = sm_scale * 1.4426950408889634f;
+  cudaStream_t st = static_cast<cudaStream_t>(stream);
+  if (hd > 64)
+    return dtype == HSPMN_BF16 ? launch_paged_attn<128, true>(prm, runs, st)
+                              : launch_paged_attn<128, false>(prm, runs, st);
+  return dtype == HSPMN_BF16 ? launch_paged_attn<64, true>(prm, runs, st)
+                             : launch_paged_attn<64, false>(prm, runs, st);
 }
 
 int hspmn_device_errors(unsigned* bits, int clear, void* stream) {

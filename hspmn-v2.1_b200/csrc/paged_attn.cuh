@@ -1,0 +1,620 @@
+// Sparse-query dense-key causal attention over a paged K/V cache, for requests
+// whose query rows are few: single tokens and short runs of them.
+//
+//   o[i,h,:] = sum_m softmax_m(scale q[i,h,:].K[m,g,:]) V[m,g,:],  g = h / (H / Hkv),
+//   m over the positions of the query's request with m <= pos[i], m < kv_len
+//   and a page in the table
+//
+// Work unit: 64 keys of one (request, K/V head, 16 query rows) item; the rows
+// of a request and K/V head are numbered query * G + head, so a single token's
+// G heads share the keys that are read. All units of a call form one list
+// (requests, then row tiles, then heads, then keys) which is cut into as many
+// equal contiguous runs as there are CTAs: ragged lengths cost no idle CTA and
+// need no plan from the host, which knows neither lengths nor offsets. An item
+// that a cut divides leaves one partial result a run in the workspace (a run
+// has two at most: its first item and its last), and the merge kernel adds them
+// in run order, so results do not depend on timing.
+//
+// Bound: reading K and V once (4 query heads a key: 4 flops a byte). Each of a
+// CTA's four warps owns 16 keys of every unit and runs on its own: its K and V
+// rows come by cp.async into a private ring (kStages deep), Q K^T and P V are
+// m16n8k16 products with the softmax between them in registers, and the warps
+// meet only at the end of an item. Sums, maxima and O are fp32.
+#pragma once
+
+#include "sqdk.cuh"
+
+namespace hspmn {
+
+constexpr int kPagedRows = 16;     // query rows of an item
+constexpr int kPagedKeys = 64;     // keys of a unit
+constexpr int kPagedWarps = 4;     // 16 keys of the unit each
+constexpr int kPagedThreads = 32 * kPagedWarps;
+constexpr int kPagedStages = 3;
+constexpr int kPagedCtasPerSm = 2;
+
+// Row sum of a part that holds no key its row sees (a true sum is not negative).
+constexpr float kUnseen = -1.0f;
+
+struct PagedAttnParams {
+  const char* q;
+  const char* k;
+  const char* v;
+  char* o;
+  int64_t q_sn, q_sh, o_sn, o_sh;                    // bytes
+  int64_t k_sp, k_ss, k_sh, v_sp, v_ss, v_sh;        // bytes: page, slot in the page, head
+  const int* table;  // [R,P], row stride table_rs
+  int64_t table_rs;
+  const int* kv_lens;
+  const int* cu_q;
+  const int64_t* pos;
+  float* part_o;   // [2 * runs][16][HD] unnormalised O
+  float* part_ml;  // [2 * runs][16][2] maximum (log2 units), row sum
+  int64_t N;
+  int R, P, num_pages, shift, H, Hkv, G, hd;
+  float scale_log2;
+};
+
+// A request's share of the list. Request R stands for the rows behind the last
+// sequence, which see nothing and are written as zeros.
+struct PagedRequest {
+  int q0, rows;    // first query row of q, rows = queries * G
+  int kv;          // visible keys at most
+  int tiles;       // 16-row tiles
+  int nb;          // units of an item (one at least: it writes the rows)
+  int64_t units;   // tiles * Hkv * nb
+};
+
+__device__ __forceinline__ PagedRequest paged_request(const PagedAttnParams& p, int r) {
+  PagedRequest q;
+  const int N = static_cast<int>(p.N);
+  const int a = min(max(__ldg(p.cu_q + r), 0), N);
+  const int b = r < p.R ? min(max(__ldg(p.cu_q + r + 1), 0), N) : N;
+  const int64_t cap = static_cast<int64_t>(p.P) << p.shift;
+  const int64_t kv = r < p.R ? max(__ldg(p.kv_lens + r), 0) : 0;
+  q.q0 = a;
+  q.rows = max(b - a, 0) * p.G;
+  q.kv = static_cast<int>(min(kv, cap));
+  q.tiles = (q.rows + kPagedRows - 1) / kPagedRows;
+  q.nb = max(1, (q.kv + kPagedKeys - 1) / kPagedKeys);
+  q.units = static_cast<int64_t>(q.tiles) * p.Hkv * q.nb;
+  return q;
+}
+
+// Units of the whole list; every lane of the warp gets the sum.
+__device__ __forceinline__ int64_t paged_total(const PagedAttnParams& p, int lane) {
+  int64_t n = 0;
+  for (int r = lane; r <= p.R; r += 32) n += paged_request(p, r).units;
+#pragma unroll
+  for (int d = 16; d > 0; d >>= 1) n += __shfl_xor_sync(0xFFFFFFFFu, n, d);
+  return n;
+}
+
+// The request that unit u (< the total) belongs to and the list's units before
+// it, found by the whole warp.
+__device__ __forceinline__ int paged_locate(const PagedAttnParams& p, int64_t u, int lane, int64_t& before) {
+  int64_t base = 0;
+  for (int r0 = 0; r0 <= p.R; r0 += 32) {
+    const int r = r0 + lane;
+    const int64_t mine = r <= p.R ? paged_request(p, r).units : 0;
+    int64_t sum = mine;
+#pragma unroll
+    for (int d = 1; d < 32; d <<= 1) {
+      const int64_t x = __shfl_up_sync(0xFFFFFFFFu, sum, d);
+      if (lane >= d) sum += x;
+    }
+    const unsigned past = __ballot_sync(0xFFFFFFFFu, base + sum > u);
+    if (past) {
+      const int l = __ffs(past) - 1;
+      before = base + __shfl_sync(0xFFFFFFFFu, sum - mine, l);
+      return r0 + l;
+    }
+    base += __shfl_sync(0xFFFFFFFFu, sum, 31);
+  }
+  before = base;
+  return p.R;  // not reached for u below the total
+}
+
+// First unit of run c of `runs`.
+__device__ __forceinline__ int64_t run_start(int64_t total, int64_t runs, int64_t c) {
+  return total / runs * c + total % runs * c / runs;
+}
+
+// The run that holds unit u (the last one that starts at or before u).
+__device__ __forceinline__ int run_of(int64_t total, int64_t runs, int64_t u) {
+  int64_t lo = 0, hi = runs;
+  while (hi - lo > 1) {
+    const int64_t mid = (lo + hi) >> 1;
+    if (run_start(total, runs, mid) <= u) lo = mid;
+    else hi = mid;
+  }
+  return static_cast<int>(lo);
+}
+
+// A place in the list: request, row tile, head and key unit.
+struct PagedCursor {
+  PagedRequest req;
+  int r, tile, head, j;
+  __device__ __forceinline__ void set(const PagedAttnParams& p, int request, int64_t local) {
+    r = request;
+    req = paged_request(p, r);
+    const int64_t item = local / req.nb;
+    j = static_cast<int>(local - item * req.nb);
+    tile = static_cast<int>(item / p.Hkv);
+    head = static_cast<int>(item - static_cast<int64_t>(tile) * p.Hkv);
+  }
+  // Only called while a next unit exists.
+  __device__ __forceinline__ void next(const PagedAttnParams& p) {
+    if (++j < req.nb) return;
+    j = 0;
+    if (++head < p.Hkv) return;
+    head = 0;
+    if (++tile < req.tiles) return;
+    tile = 0;
+    do req = paged_request(p, ++r);
+    while (req.units == 0 && r < p.R);
+  }
+};
+
+// Byte offset of query row `row` (q0 * G + ...) of K/V head `head`.
+__device__ __forceinline__ int64_t paged_row(int q0, int row, int head, int G, int64_t sn, int64_t sh) {
+  const int qi = row / G;
+  return (static_cast<int64_t>(q0) + qi) * sn + static_cast<int64_t>(head * G + (row - qi * G)) * sh;
+}
+
+__device__ __forceinline__ void cp_async16(uint32_t dst, const void* src, bool full) {
+  asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(dst), "l"(src), "r"(full ? 16 : 0) : "memory");
+}
+__device__ __forceinline__ void cp_async_commit() { asm volatile("cp.async.commit_group;" ::: "memory"); }
+template <int n>
+__device__ __forceinline__ void cp_async_wait() {
+  asm volatile("cp.async.wait_group %0;" ::"n"(n) : "memory");
+}
+
+__device__ __forceinline__ void ldmatrix_x4(uint32_t (&r)[4], uint32_t addr) {
+  asm volatile("ldmatrix.sync.aligned.m8n8.x4.shared.b16 {%0,%1,%2,%3}, [%4];"
+               : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3])
+               : "r"(addr)
+               : "memory");
+}
+__device__ __forceinline__ void ldmatrix_x4_trans(uint32_t (&r)[4], uint32_t addr) {
+  asm volatile("ldmatrix.sync.aligned.m8n8.x4.trans.shared.b16 {%0,%1,%2,%3}, [%4];"
+               : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3])
+               : "r"(addr)
+               : "memory");
+}
+
+// c += a b, 16 x 8 x 16, fp32 accumulation.
+template <bool kBF16>
+__device__ __forceinline__ void mma16816(float (&c)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1) {
+  if constexpr (kBF16)
+    asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
+                 : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3])
+                 : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
+  else
+    asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
+                 : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3])
+                 : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
+}
+
+// Whether a 32-bit word of two 16-bit elements holds an infinity or a NaN.
+template <bool kBF16>
+__device__ __forceinline__ bool not_finite2(uint32_t w) {
+  constexpr uint32_t e = kBF16 ? 0x7F80u : 0x7C00u;
+  return (w & e) == e || ((w >> 16) & e) == e;
+}
+
+template <bool kBF16>
+__device__ __forceinline__ float half_to_float(uint16_t h) {
+  if constexpr (kBF16) return __uint_as_float(static_cast<uint32_t>(h) << 16);
+  else return __half2float(__ushort_as_half(h));
+}
+
+template <int HD>
+struct PagedLayout {
+  static constexpr int kRow = HD * 2;                             // bytes of a key's K or V in shared memory
+  static constexpr int kWarpStage = 2 * 16 * kRow;                // 16 keys of K and of V
+  static constexpr int kStage = kPagedWarps * kWarpStage;
+  static constexpr int kBytes = kPagedStages * kStage;
+  // at the end of an item a warp leaves its 16 x HD fp32 O in the stage it has just consumed
+  static_assert(kWarpStage == kPagedRows * HD * 4, "an O tile fits a warp's stage exactly");
+};
+
+// Word index of O element (row, col) in a warp's stage: 8-column groups are
+// permuted by the row so the accumulator layout's writes spread over the banks.
+template <int HD>
+__device__ __forceinline__ int paged_o_word(int row, int col) {
+  return row * HD + ((((col >> 3) ^ row) & (HD / 8 - 1)) << 3) + (col & 7);
+}
+
+template <int HD, bool kBF16>
+__global__ void __launch_bounds__(kPagedThreads, kPagedCtasPerSm) paged_attn_kernel(const PagedAttnParams p) {
+  using L = PagedLayout<HD>;
+  extern __shared__ __align__(128) uint8_t paged_smem[];
+  __shared__ float s_m[kPagedWarps][kPagedRows], s_l[kPagedWarps][kPagedRows];
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  const int g = lane >> 2, t2 = (lane & 3) * 2;  // accumulator row and first column of this lane
+  const int64_t total = paged_total(p, lane);
+  const int64_t runs = min(static_cast<int64_t>(gridDim.x), total);
+  if (blockIdx.x >= runs) return;
+  const int64_t u0 = run_start(total, runs, blockIdx.x), u1 = run_start(total, runs, blockIdx.x + 1);
+  int64_t before;
+  const int r0 = paged_locate(p, u0, lane, before);
+  PagedCursor cur, ahead;
+  cur.set(p, r0, u0 - before);
+  ahead = cur;
+  const uint32_t wbase = smem_u32(paged_smem) + warp * L::kWarpStage;
+  constexpr int kChunks = HD / 8;           // 16-byte chunks of a row
+  constexpr int kPerIter = 32 / kChunks;    // rows a warp-wide copy covers
+  const int ld_row = lane / kChunks, ld_chunk = lane % kChunks;
+  const bool ld_col = ld_chunk * 8 < p.hd;  // columns past head_dim are zero
+
+  // This warp's 16 keys of the unit `ahead` points at, into ring stage s. Keys
+  // past the visible range or in a page that does not exist arrive as zeros.
+  auto request = [&](int s) {
+    const int key0 = ahead.j * kPagedKeys + warp * 16;
+    const uint32_t kdst = wbase + s * L::kStage, vdst = kdst + 16 * L::kRow;
+    const int* row = p.table + static_cast<int64_t>(ahead.r) * p.table_rs;
+    int page[2];  // pages of the first and of the second 8 keys
+#pragma unroll
+    for (int i = 0; i < 2; ++i) {
+      const int key = key0 + 8 * i;
+      page[i] = key < ahead.req.kv ? __ldg(row + (key >> p.shift)) : -1;
+      if (key < ahead.req.kv && (page[i] < 0 || page[i] >= p.num_pages)) {
+        page[i] = -1;
+        if (lane == 0) raise_device_error(HSPMN_DEVERR_PAGE);
+      }
+    }
+#pragma unroll
+    for (int i = 0; i < 16 / kPerIter; ++i) {
+      const int kr = i * kPerIter + ld_row;
+      const int pg = kr < 8 ? page[0] : page[1];
+      const int key = key0 + kr;
+      const bool there = pg >= 0 && key < ahead.req.kv && ld_col;
+      const int64_t off = key & ((1 << p.shift) - 1);
+      const int64_t pgl = there ? pg : 0;
+      const int64_t o = there ? off : 0;
+      const int64_t col = there ? ld_chunk * 16 : 0;
+      const uint32_t d = kr * L::kRow + ((ld_chunk ^ (kr & 7)) << 4);
+      cp_async16(kdst + d, p.k + pgl * p.k_sp + o * p.k_ss + ahead.head * p.k_sh + col, there);
+      cp_async16(vdst + d, p.v + pgl * p.v_sp + o * p.v_ss + ahead.head * p.v_sh + col, there);
+    }
+  };
+
+  int64_t ua = u0;
+#pragma unroll
+  for (int s = 0; s < kPagedStages - 1; ++s) {
+    if (ua < u1) {
+      if (ua > u0) ahead.next(p);
+      request(s);
+      ++ua;
+    }
+    cp_async_commit();
+  }
+
+  uint32_t qa[HD / 16][4];
+  float acc[HD / 8][4];
+  float m_run[2] = {}, l_run[2] = {};
+  bool seen[2] = {};  // the row has met a key that it sees
+  int lim[2] = {}, lim_min = 0, lim_max = 0;
+  bool fresh = true;  // the next unit opens an item (or this run's part of one)
+  int64_t seg0 = u0;
+  int stage = 0;
+  for (int64_t u = u0; u < u1; ++u) {
+    if (fresh) {
+      fresh = false;
+      seg0 = u;
+      // rows of this tile: q fragments, and the last key that each row sees
+      lim_min = 0x7FFFFFFF;
+      lim_max = -1;
+#pragma unroll
+      for (int i = 0; i < 2; ++i) {
+        const int row = cur.tile * kPagedRows + g + 8 * i;
+        lim[i] = -1;
+        if (row < cur.req.rows) {
+          const int64_t ps = __ldg(p.pos + cur.req.q0 + row / p.G);
+          if (ps >= cur.req.kv && cur.r < p.R) raise_device_error(HSPMN_DEVERR_POSITION);
+          lim[i] = static_cast<int>(min(max(ps, static_cast<int64_t>(-1)), static_cast<int64_t>(cur.req.kv) - 1));
+          if (lim[i] >= 0) lim_min = min(lim_min, lim[i]);
+          lim_max = max(lim_max, lim[i]);
+        }
+        const char* src = p.q + paged_row(cur.req.q0, row < cur.req.rows ? row : 0, cur.head, p.G, p.q_sn, p.q_sh);
+#pragma unroll
+        for (int kk = 0; kk < HD / 16; ++kk) {
+#pragma unroll
+          for (int c = 0; c < 2; ++c) {
+            const int col = kk * 16 + c * 8 + t2;
+            qa[kk][2 * c + i] =
+                row < cur.req.rows && col < p.hd ? __ldg(reinterpret_cast<const uint32_t*>(src + col * 2)) : 0u;
+          }
+        }
+        m_run[i] = -INFINITY;
+        l_run[i] = 0.0f;
+        seen[i] = false;
+      }
+      lim_min = __reduce_min_sync(0xFFFFFFFFu, lim_min);
+      lim_max = __reduce_max_sync(0xFFFFFFFFu, lim_max);
+#pragma unroll
+      for (int n = 0; n < HD / 8; ++n)
+#pragma unroll
+        for (int e = 0; e < 4; ++e) acc[n][e] = 0.0f;
+    }
+    cp_async_wait<kPagedStages - 2>();
+    __syncwarp();
+    const int key0 = cur.j * kPagedKeys + warp * 16;
+    const uint32_t kst = wbase + stage * L::kStage, vst = kst + 16 * L::kRow;
+    if (key0 <= lim_max) {
+      // S = Q K^T, 16 rows x 16 keys
+      float s[2][4] = {};
+#pragma unroll
+      for (int kk = 0; kk < HD / 16; ++kk) {
+        const int kr = ((lane >> 4) << 3) + (lane & 7), chunk = kk * 2 + ((lane >> 3) & 1);
+        uint32_t b[4];
+        ldmatrix_x4(b, kst + kr * L::kRow + ((chunk ^ (kr & 7)) << 4));
+        mma16816<kBF16>(s[0], qa[kk], b[0], b[1]);
+        mma16816<kBF16>(s[1], qa[kk], b[2], b[3]);
+      }
+      // the pages are looked up again: a missing one masks its 8 keys
+      const int* row = p.table + static_cast<int64_t>(cur.r) * p.table_rs;
+      bool gone[2];
+#pragma unroll
+      for (int n = 0; n < 2; ++n) {
+        const int key = key0 + 8 * n;
+        const int pg = key < cur.req.kv ? __ldg(row + (key >> p.shift)) : 0;
+        gone[n] = pg < 0 || pg >= p.num_pages;
+      }
+      const bool masked = key0 + 15 > lim_min || lim_min == 0x7FFFFFFF || gone[0] || gone[1];
+      if (masked) {
+#pragma unroll
+        for (int n = 0; n < 2; ++n)
+#pragma unroll
+          for (int e = 0; e < 4; ++e) {
+            const int key = key0 + 8 * n + t2 + (e & 1);
+            if (key > lim[e >> 1] || gone[n]) s[n][e] = -INFINITY;
+          }
+      }
+      // online softmax of rows g and g + 8
+      float alpha[2];
+      bool grew = false;
+#pragma unroll
+      for (int i = 0; i < 2; ++i) {
+        float mx = fmaxf(fmaxf(s[0][2 * i], s[0][2 * i + 1]), fmaxf(s[1][2 * i], s[1][2 * i + 1]));
+        mx = fmaxf(mx, __shfl_xor_sync(0xFFFFFFFFu, mx, 1));
+        mx = fmaxf(mx, __shfl_xor_sync(0xFFFFFFFFu, mx, 2));
+        const float m_new = fmaxf(m_run[i], mx * p.scale_log2);
+        alpha[i] = m_new > m_run[i] ? fast_exp2(m_run[i] - m_new) : 1.0f;
+        grew |= m_new > m_run[i];
+        const float neg = m_new == -INFINITY ? 0.0f : -m_new;
+        float sum = 0.0f;
+#pragma unroll
+        for (int n = 0; n < 2; ++n)
+#pragma unroll
+          for (int c = 0; c < 2; ++c) {
+            const float e = fast_exp2(fmaf(s[n][2 * i + c], p.scale_log2, neg));
+            s[n][2 * i + c] = e;
+            sum += e;
+          }
+        l_run[i] = l_run[i] * alpha[i] + sum;
+        seen[i] |= (key0 <= lim[i] && !gone[0]) || (key0 + 8 <= lim[i] && !gone[1]);
+        m_run[i] = m_new;
+      }
+      if (__any_sync(0xFFFFFFFFu, grew)) {
+#pragma unroll
+        for (int n = 0; n < HD / 8; ++n) {
+          acc[n][0] *= alpha[0], acc[n][1] *= alpha[0];
+          acc[n][2] *= alpha[1], acc[n][3] *= alpha[1];
+        }
+      }
+      // Where some row sees a key and another does not, an infinity or NaN in
+      // that key's V must not reach the other (0 * inf): such a step adds its
+      // products one by one.
+      bool wild = false;
+      if (masked) {
+        bool mine = false;
+#pragma unroll
+        for (int i = 0; i < 16 / kPerIter; ++i) {
+          const int kr = i * kPerIter + ld_row;
+          uint4 w;
+          asm volatile("ld.shared.v4.u32 {%0,%1,%2,%3}, [%4];"
+                       : "=r"(w.x), "=r"(w.y), "=r"(w.z), "=r"(w.w)
+                       : "r"(vst + kr * L::kRow + ((ld_chunk ^ (kr & 7)) << 4)));
+          mine |= not_finite2<kBF16>(w.x) || not_finite2<kBF16>(w.y) || not_finite2<kBF16>(w.z) ||
+                  not_finite2<kBF16>(w.w);
+        }
+        wild = __any_sync(0xFFFFFFFFu, mine);
+      }
+      if (!wild) {
+        // P in the operands' type: its rounding (half a step) is of the size
+        // of the output's own
+        const uint32_t pa[4] = {pack2<kBF16>(s[0][0], s[0][1]), pack2<kBF16>(s[0][2], s[0][3]),
+                                pack2<kBF16>(s[1][0], s[1][1]), pack2<kBF16>(s[1][2], s[1][3])};
+#pragma unroll
+        for (int n = 0; n < HD / 16; ++n) {
+          const int kr = (((lane >> 3) & 1) << 3) + (lane & 7), chunk = n * 2 + (lane >> 4);
+          uint32_t b[4];
+          ldmatrix_x4_trans(b, vst + kr * L::kRow + ((chunk ^ (kr & 7)) << 4));
+          mma16816<kBF16>(acc[2 * n], pa, b[0], b[1]);
+          mma16816<kBF16>(acc[2 * n + 1], pa, b[2], b[3]);
+        }
+      } else {
+#pragma unroll
+        for (int kr = 0; kr < 16; ++kr) {
+          const int src = (lane & ~3) | ((kr & 7) >> 1);  // the lane of this quad that holds the key's column
+          float w[2];
+          bool sees[2];
+#pragma unroll
+          for (int i = 0; i < 2; ++i) {
+            w[i] = __shfl_sync(0xFFFFFFFFu, s[kr >> 3][2 * i + (kr & 1)], src);
+            sees[i] = key0 + kr <= lim[i] && !gone[kr >> 3];
+          }
+#pragma unroll
+          for (int n = 0; n < HD / 8; ++n) {
+            uint32_t two;
+            asm volatile("ld.shared.u32 %0, [%1];" : "=r"(two) : "r"(vst + kr * L::kRow + ((n ^ (kr & 7)) << 4) + t2 * 2));
+            const float x = half_to_float<kBF16>(static_cast<uint16_t>(two)), y = half_to_float<kBF16>(two >> 16);
+#pragma unroll
+            for (int i = 0; i < 2; ++i)
+              if (sees[i]) acc[n][2 * i] = fmaf(w[i], x, acc[n][2 * i]), acc[n][2 * i + 1] = fmaf(w[i], y, acc[n][2 * i + 1]);
+          }
+        }
+      }
+    }
+    const bool item_end = cur.j == cur.req.nb - 1;
+    if (item_end || u + 1 == u1) {
+      // the warps' results of this item: O in the stage each has just
+      // consumed, maxima and sums beside it
+      __syncwarp();
+      float* mine = reinterpret_cast<float*>(paged_smem + warp * L::kWarpStage + stage * L::kStage);
+#pragma unroll
+      for (int n = 0; n < HD / 8; ++n)
+#pragma unroll
+        for (int i = 0; i < 2; ++i)
+          *reinterpret_cast<float2*>(mine + paged_o_word<HD>(g + 8 * i, n * 8 + t2)) =
+              make_float2(acc[n][2 * i], acc[n][2 * i + 1]);
+#pragma unroll
+      for (int i = 0; i < 2; ++i) {
+        float l = l_run[i];
+        l += __shfl_xor_sync(0xFFFFFFFFu, l, 1);
+        l += __shfl_xor_sync(0xFFFFFFFFu, l, 2);
+        if ((lane & 3) == 0) s_m[warp][g + 8 * i] = m_run[i], s_l[warp][g + 8 * i] = seen[i] ? l : kUnseen;
+      }
+      __syncthreads();
+      const bool whole = item_end && seg0 + cur.req.nb == u + 1;
+      const int64_t slot = 2 * static_cast<int64_t>(blockIdx.x) + (seg0 == u0 ? 0 : 1);
+      constexpr int kQuads = HD / 4;  // 4-column groups of a row
+      for (int i = threadIdx.x; i < kPagedRows * kQuads; i += kPagedThreads) {
+        const int lr = i / kQuads, c = (i % kQuads) * 4;
+        const int row = cur.tile * kPagedRows + lr;
+        if (row >= cur.req.rows || c >= p.hd) continue;
+        float M = s_m[0][lr];
+#pragma unroll
+        for (int w = 1; w < kPagedWarps; ++w) M = fmaxf(M, s_m[w][lr]);
+        float l = 0.0f;
+        bool none = true;
+        float4 o = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+#pragma unroll
+        for (int w = 0; w < kPagedWarps; ++w) {
+          if (s_l[w][lr] == kUnseen) continue;
+          none = false;
+          const float mw = s_m[w][lr], f = mw == M ? 1.0f : fast_exp2(mw - M);
+          const float4 x = *reinterpret_cast<const float4*>(
+              reinterpret_cast<const float*>(paged_smem + w * L::kWarpStage + stage * L::kStage) +
+              paged_o_word<HD>(lr, c));
+          l += f * s_l[w][lr];
+          o.x += f * x.x, o.y += f * x.y, o.z += f * x.z, o.w += f * x.w;
+        }
+        if (whole) {
+          const float inv = 1.0f / l;
+          uint2 w;
+          w.x = none ? 0u : pack2<kBF16>(o.x * inv, o.y * inv);
+          w.y = none ? 0u : pack2<kBF16>(o.z * inv, o.w * inv);
+          *reinterpret_cast<uint2*>(p.o + paged_row(cur.req.q0, row, cur.head, p.G, p.o_sn, p.o_sh) + c * 2) = w;
+        } else {
+          *reinterpret_cast<float4*>(p.part_o + (slot * kPagedRows + lr) * HD + c) = o;
+          if (c == 0) reinterpret_cast<float2*>(p.part_ml)[slot * kPagedRows + lr] = make_float2(M, none ? kUnseen : l);
+        }
+      }
+      __syncthreads();
+      fresh = true;
+    }
+    // refill the stage that this unit has left (its readers are this warp, or
+    // have passed the barrier above)
+    __syncwarp();
+    if (ua < u1) {
+      ahead.next(p);
+      request((stage + kPagedStages - 1) % kPagedStages);
+      ++ua;
+    }
+    cp_async_commit();
+    stage = stage + 1 == kPagedStages ? 0 : stage + 1;
+    if (u + 1 < u1) cur.next(p);
+  }
+  cp_async_wait<0>();
+}
+
+constexpr int kMergeWarps = 16;
+
+// Adds the partial results of the item that the end of run blockIdx.x divides,
+// if this is the first run of that item: O = sum 2^(m_s - M) O_s / sum 2^(m_s - M) l_s
+// over the runs in order. A warp takes one row and a share of the runs.
+template <int HD, bool kBF16>
+__global__ void __launch_bounds__(32 * kMergeWarps) paged_merge_kernel(const PagedAttnParams p, int most_runs) {
+  __shared__ float4 s_o[kMergeWarps][HD / 4];
+  __shared__ float2 s_ml[kMergeWarps];
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  const int64_t total = paged_total(p, lane);
+  const int64_t runs = min(static_cast<int64_t>(most_runs), total);
+  if (blockIdx.x + 1 >= runs) return;
+  const int64_t cut = run_start(total, runs, blockIdx.x + 1);
+  int64_t before;
+  const int r = paged_locate(p, cut, lane, before);
+  PagedCursor cur;
+  cur.set(p, r, cut - before);
+  const int64_t a = cut - cur.j, b = a + cur.req.nb;  // the item's units
+  if (cur.j == 0 || run_of(total, runs, a) != static_cast<int>(blockIdx.x)) return;
+  const int c0 = static_cast<int>(blockIdx.x), c1 = run_of(total, runs, b - 1);
+  const int rows = min(kPagedRows, cur.req.rows - cur.tile * kPagedRows);
+  const int shares = max(1, kMergeWarps / rows);  // warps of a row
+  const float2* ml = reinterpret_cast<const float2*>(p.part_ml);
+  for (int row0 = 0; row0 < rows; row0 += kMergeWarps / shares) {
+    const int lr = row0 + warp / shares, part = warp % shares;
+    const bool live = lr < rows && warp / shares < kMergeWarps / shares;
+    float M = -INFINITY, l = 0.0f;
+    bool none = true;
+    float4 o = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+    if (live) {
+      // run c's part of the item is its first piece unless the item opens inside it
+      auto slot_of = [&](int c) { return (2 * static_cast<int64_t>(c) + (run_start(total, runs, c) < a ? 1 : 0)) * kPagedRows + lr; };
+      const int n = c1 - c0 + 1, per = (n + shares - 1) / shares;
+      const int lo = c0 + part * per, hi = min(c1 + 1, lo + per);
+      for (int c = lo + lane; c < hi; c += 32) M = fmaxf(M, ml[slot_of(c)].x);
+#pragma unroll
+      for (int d = 16; d > 0; d >>= 1) M = fmaxf(M, __shfl_xor_sync(0xFFFFFFFFu, M, d));
+#pragma unroll 4
+      for (int c = lo; c < hi; ++c) {
+        const int64_t s = slot_of(c);
+        const float2 x = ml[s];
+        if (x.y == kUnseen) continue;
+        none = false;
+        const float f = x.x == M ? 1.0f : fast_exp2(x.x - M);
+        l += f * x.y;
+        if (lane * 4 < p.hd && lane < HD / 4) {
+          const float4 v = *reinterpret_cast<const float4*>(p.part_o + s * HD + lane * 4);
+          o.x += f * v.x, o.y += f * v.y, o.z += f * v.z, o.w += f * v.w;
+        }
+      }
+    }
+    if (lane < HD / 4) s_o[warp][lane] = o;
+    if (lane == 0) s_ml[warp] = make_float2(M, none ? kUnseen : l);
+    __syncthreads();
+    if (live && part == 0) {
+      float top = -INFINITY;
+      for (int w = 0; w < shares; ++w) top = fmaxf(top, s_ml[warp + w].x);
+      float sum = 0.0f;
+      bool empty = true;
+      float4 y = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+      for (int w = 0; w < shares; ++w) {
+        const float2 x = s_ml[warp + w];
+        if (x.y == kUnseen) continue;
+        empty = false;
+        const float f = x.x == top ? 1.0f : fast_exp2(x.x - top);
+        sum += f * x.y;
+        if (lane < HD / 4) {
+          const float4 v = s_o[warp + w][lane];
+          y.x += f * v.x, y.y += f * v.y, y.z += f * v.z, y.w += f * v.w;
+        }
+      }
+      const int row = cur.tile * kPagedRows + lr;
+      const float inv = 1.0f / sum;
+      if (lane * 4 < p.hd && lane < HD / 4) {
+        uint2 w;
+        w.x = empty ? 0u : pack2<kBF16>(y.x * inv, y.y * inv);
+        w.y = empty ? 0u : pack2<kBF16>(y.z * inv, y.w * inv);
+        *reinterpret_cast<uint2*>(p.o + paged_row(cur.req.q0, row, cur.head, p.G, p.o_sn, p.o_sh) + lane * 8) = w;
+      }
+    }
+    __syncthreads();
+  }
+}
+
+}  // namespace hspmn

@@ -15,7 +15,7 @@ LIB_NAME = "libhspmn_sm100.so"
 LIB_PATH = os.path.join(os.path.dirname(os.path.abspath(__file__)), LIB_NAME)
 
 HSPMN_F32, HSPMN_F16, HSPMN_BF16 = 0, 1, 2
-DEVERR_POSITION, DEVERR_UNSORTED, DEVERR_TIMEOUT = 1, 2, 4
+DEVERR_POSITION, DEVERR_UNSORTED, DEVERR_TIMEOUT, DEVERR_PAGE = 1, 2, 4, 8
 
 # name -> (restype, argtypes)
 _i64 = ctypes.c_int64
@@ -47,6 +47,15 @@ _SIGNATURES = {
                                _i64, _int, _vp]),
     "hspmn_scatter_add_rows": (_int, [_vp, _i64, _i64, _vp, _i64, _vp, _i64, _i64, _i64, _i64, _i64, _i64,
                                       _int, _vp]),
+    "hspmn_paged_slots": (_int, [_vp, _i64, _vp, _vp, _vp, _i64, _i64, _i64, _i64, _i64, _vp, _vp, _vp, _vp, _vp,
+                                 _vp]),
+    "hspmn_rope_paged_write": (_int, [_vp, _i64, _i64, _vp, _i64, _i64, _vp, _vp, _i64, _i64, _int, _vp, _vp,
+                                      _vp, _i64, _i64, _i64, _vp, _i64, _i64, _i64, _i64, _i64, _i64, _i64, _i64,
+                                      _int, _vp]),
+    "hspmn_sqdk_paged_workspace_size": (_i64, [_i64]),
+    "hspmn_sqdk_paged_fwd": (_int, [_vp, _i64, _i64, _vp, _i64, _i64, _i64, _vp, _i64, _i64, _i64, _vp, _i64, _vp,
+                                    _vp, _vp, _vp, _i64, _i64, _i64, _i64, _i64, _i64, _i64, _i64, _i64, _i64, _int,
+                                    ctypes.c_float, _i64, _vp, ctypes.c_size_t, _vp]),
     "hspmn_device_errors": (_int, [ctypes.POINTER(ctypes.c_uint), _int, _vp]),
 }
 EXPORTED = tuple(_SIGNATURES)

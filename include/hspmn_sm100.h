@@ -5,7 +5,8 @@
  *   (fp32 gate ->) router top-K  ->  gather selected queries  ->  SQDK causal attention
  *                 ->  scatter back into the [B,S,D] stream
  *
- * and, for training, the backward of the SQDK attention.
+ * for training, the backward of the SQDK attention, and for serving the page
+ * bookkeeping, the writes and the attention of a paged K/V cache.
  *
  * Conventions
  *   - All buffers are device memory allocated by the caller; the library never
@@ -54,6 +55,7 @@ enum hspmn_status {
 #define HSPMN_DEVERR_POSITION 1u /* a query/selected position outside [0, S) */
 #define HSPMN_DEVERR_UNSORTED 2u /* indices not ascending where an entry point requires it (scatter, backward) */
 #define HSPMN_DEVERR_TIMEOUT 4u  /* a bounded pipeline wait in attention gave up */
+#define HSPMN_DEVERR_PAGE 8u     /* a page outside the cache, or no free page left */
 
 /* Library version, major*10000 + minor*100 + patch. */
 HSPMN_API int hspmn_version(void);
@@ -302,6 +304,94 @@ HSPMN_API int hspmn_sqdk_bwd(const void* q, const int64_t* q_strides,
                    int64_t B, int64_t K, int64_t S, int64_t H, int64_t Hkv,
                    int64_t hd, int dtype, float sm_scale,
                    void* workspace, size_t workspace_bytes, void* stream);
+
+/*
+ * Paged K/V cache. A cache is [num_pages, page_size, Hkv, hd] (K and V each,
+ * separate or strided parts of one allocation); page_size is a power of two
+ * from 8 to 4096. Token `pos` of request r is in page
+ * block_table[r, pos / page_size] at offset pos % page_size; its slot is
+ * page * page_size + offset. The reference has no counterpart: it computes the
+ * keys of a whole sequence on every call (hspmn_v2_1.py:218-227).
+ *
+ * hspmn_paged_slots: the bookkeeping of one step, from the lengths alone. For
+ * each request r with seq_lens[r] tokens cached and new_lens[r] to come:
+ *   cu_new[0..R]   offsets of the requests' new tokens in the packed batch
+ *   kv_lens[r]     seq_lens[r] + new_lens[r]
+ *   block_table    the entries of the pages that the new tokens open are taken
+ *                  from free_pages in order (request by request); older entries
+ *                  stay. taken[0] is how many pages were needed.
+ *   positions[t], slots[t]  of packed token t < N; -1 for t >= cu_new[R]
+ * block_table: int32 [R,P], row stride table_rs. N: capacity of positions and
+ * slots, at least the number of new tokens (further ones are dropped and
+ * HSPMN_DEVERR_POSITION is set, as for a negative length or one that P pages
+ * do not hold). Where free_pages ends, entries and slots are -1 and
+ * HSPMN_DEVERR_PAGE is set. R <= 8192. All lengths, cu_new, kv_lens, taken,
+ * block_table and free_pages are int32, positions and slots int64.
+ */
+HSPMN_API int hspmn_paged_slots(int32_t* block_table, int64_t table_rs, const int32_t* seq_lens,
+                                const int32_t* new_lens, const int32_t* free_pages, int64_t num_free,
+                                int64_t R, int64_t P, int64_t page_size, int64_t N,
+                                int32_t* cu_new, int32_t* kv_lens, int64_t* positions, int64_t* slots,
+                                int32_t* taken, void* stream);
+
+/*
+ * Cache write of N tokens, with the rotary embedding of K:
+ *   k_cache[slot of t, h, :] = T(k[t,h,:] * cos[pos,:] + rot(k[t,h,:]) * sin[pos,:])
+ *   v_cache[slot of t, h, :] = v[t,h,:]
+ * with rot() as in hspmn_rope_gather_rows, the products and sum in float32 and
+ * one rounding (hspmn_rope_rows rounds each of the reference's three tensor
+ * operations). k, v: [N,Hkv,hd] of `dtype`, strides (elements) of token and
+ * head. cos/sin: tables of tab_rows rows, row stride tab_ss, of tab_dtype
+ * (`dtype` or HSPMN_F32); both NULL stores k as it is, and positions is then
+ * not read. Cache strides (elements): page, offset, head. Tokens with slot < 0
+ * are skipped; a page outside the cache or a position outside the tables sets
+ * HSPMN_DEVERR_PAGE / HSPMN_DEVERR_POSITION and the token is skipped. Slots
+ * must not repeat. hd a multiple of 16 bytes; with tables of 32 bytes
+ * (HSPMN_ERR_UNSUPPORTED). Bases and strides multiples of 16 bytes.
+ */
+HSPMN_API int hspmn_rope_paged_write(const void* k, int64_t k_sn, int64_t k_sh, const void* v, int64_t v_sn,
+                                     int64_t v_sh, const void* cos_tab, const void* sin_tab, int64_t tab_ss,
+                                     int64_t tab_rows, int tab_dtype, const int64_t* positions,
+                                     const int64_t* slots, void* k_cache, int64_t kc_sp, int64_t kc_ss,
+                                     int64_t kc_sh, void* v_cache, int64_t vc_sp, int64_t vc_ss, int64_t vc_sh,
+                                     int64_t N, int64_t Hkv, int64_t hd, int64_t num_pages, int64_t page_size,
+                                     int dtype, void* stream);
+
+/* Bytes of device workspace hspmn_sqdk_paged_fwd needs on the current device
+ * for this head_dim, whatever the lengths (-1: the device could not be queried). */
+HSPMN_API int64_t hspmn_sqdk_paged_workspace_size(int64_t hd);
+
+/*
+ * Sparse-query dense-key causal attention of packed query rows over a paged
+ * cache. Rows cu_q[r] <= i < cu_q[r+1] of q are queries of request r, at
+ * position positions[i]:
+ *   o[i,h,:] = sum_m softmax_m(sm_scale * q[i,h,:].k[m,g,:]) v[m,g,:],  g = h / (H / Hkv),
+ *   m over the cached positions of r with m <= positions[i], m < kv_lens[r]
+ * A decode step (one query a request), a chunk of new tokens and the rows that
+ * a router selected of one are all calls of this function; requests may differ.
+ * Rows that see no key (position or kv_lens below 1 key) and rows i >= cu_q[R]
+ * are written as zeros. A position >= kv_lens[r] sees all kv_lens[r] keys and
+ * sets HSPMN_DEVERR_POSITION; keys whose page is outside the cache are left
+ * out and set HSPMN_DEVERR_PAGE. Whatever the cache holds behind kv_lens[r],
+ * NaN included, does not reach the result, nor does a key's value reach rows
+ * that do not see the key.
+ * q, o: [N,H,hd], strides (elements) of row and head; caches as above, strides
+ * of page, offset and head. dtype HSPMN_BF16 or HSPMN_F16. hd: a multiple of 8
+ * up to 128; H % Hkv == 0, H / Hkv <= 128. block_table, kv_lens, cu_q int32;
+ * positions int64, in any order. Bases and strides multiples of 16 bytes.
+ * max_q: the largest number of query rows of one request if the caller knows
+ * it, else 0; it only chooses kernels, any value is correct.
+ * workspace: hspmn_sqdk_paged_workspace_size() bytes (16-byte aligned);
+ * launches that overlap on the GPU need separate workspaces.
+ */
+HSPMN_API int hspmn_sqdk_paged_fwd(const void* q, int64_t q_sn, int64_t q_sh, const void* k_cache, int64_t kc_sp,
+                                   int64_t kc_ss, int64_t kc_sh, const void* v_cache, int64_t vc_sp, int64_t vc_ss,
+                                   int64_t vc_sh, const int32_t* block_table, int64_t table_rs,
+                                   const int32_t* kv_lens, const int32_t* cu_q, const int64_t* positions, void* o,
+                                   int64_t o_sn, int64_t o_sh, int64_t N, int64_t R, int64_t P, int64_t num_pages,
+                                   int64_t page_size, int64_t H, int64_t Hkv, int64_t hd, int dtype,
+                                   float sm_scale, int64_t max_q, void* workspace, size_t workspace_bytes,
+                                   void* stream);
 
 /*
  * Read (and optionally clear) the current device's HSPMN_DEVERR_* flag word.

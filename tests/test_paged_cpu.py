@@ -1,0 +1,103 @@
+"""Host side of the paged K/V cache operators: argument checks of the C ABI and
+of the Python entry points (no kernel launches), and the tests' plain forms
+against the oracle."""
+
+import ctypes
+
+import numpy as np
+import pytest
+import torch
+
+import oracle
+from hspmn_b200 import _native as N
+from hspmn_b200 import ops
+from tests import paged_ref as ref
+
+P = ctypes.c_void_p(4096)
+INVALID, DTYPE, ALIGN, UNSUPPORTED = -1, -2, -3, -4
+
+
+def test_slots_refusals():
+    def slots(table=P, rs=8, seq=P, new=P, free=P, nfree=4, R=2, Pw=8, page=16, n=4, cu=P, kv=P, pos=P, out=P, taken=P):
+        return N.lib().hspmn_paged_slots(table, rs, seq, new, free, nfree, R, Pw, page, n, cu, kv, pos, out, taken, None)
+
+    for over in (dict(table=None), dict(seq=None), dict(new=None), dict(free=None), dict(cu=None), dict(kv=None),
+                 dict(pos=None), dict(out=None), dict(taken=None), dict(rs=7), dict(R=-1), dict(n=-1), dict(nfree=-1),
+                 dict(Pw=-1), dict(n=1 << 31), dict(R=8192, Pw=1 << 19, rs=1 << 19)):
+        assert slots(**over) == INVALID, over
+    for over in (dict(page=0), dict(page=4), dict(page=24), dict(page=8192), dict(R=8193)):
+        assert slots(**over) == UNSUPPORTED, over
+
+
+def test_write_refusals():
+    def write(k=P, sn=512, sh=128, v=P, cos=P, sin=P, ts=128, rows=9, tdt=2, pos=P, slots=P, kc=P, sp=8192, ss=512, vc=P,
+              n=3, heads=4, hd=128, pages=5, page=16, dt=2):
+        return N.lib().hspmn_rope_paged_write(k, sn, sh, v, sn, sh, cos, sin, ts, rows, tdt, pos, slots, kc, sp, ss, sh,
+                                              vc, sp, ss, sh, n, heads, hd, pages, page, dt, None)
+
+    for over in (dict(k=None), dict(v=None), dict(sin=None), dict(cos=None), dict(pos=None), dict(slots=None),
+                 dict(kc=None), dict(vc=None), dict(n=-1), dict(heads=0), dict(ts=127), dict(rows=-1), dict(sn=-512)):
+        assert write(**over) == INVALID, over
+    for over in (dict(dt=9), dict(tdt=1)):
+        assert write(**over) == DTYPE, over
+    for over in (dict(page=12), dict(hd=24, ts=24), dict(hd=12, cos=None, sin=None)):
+        assert write(**over) == UNSUPPORTED, over
+    odd = ctypes.c_void_p(4104)
+    for over in (dict(k=odd), dict(v=odd), dict(cos=odd), dict(kc=odd), dict(vc=odd), dict(sn=516), dict(ss=516),
+                 dict(ts=132)):
+        assert write(**over) == ALIGN, over
+    assert write(n=0) == 0 and write(n=0, k=None) == 0
+
+
+def test_attention_refusals():
+    def fwd(q=P, sn=2048, sh=128, kc=P, sp=8192, ss=512, vc=P, table=P, rs=8, kv=P, cu=P, pos=P, o=P, n=3, R=2, Pw=8,
+            pages=5, page=16, H=16, Hkv=4, hd=128, dt=2, scale=0.1, max_q=0, ws=P, wsb=1 << 30):
+        return N.lib().hspmn_sqdk_paged_fwd(q, sn, sh, kc, sp, ss, sh, vc, sp, ss, sh, table, rs, kv, cu, pos, o, sn, sh,
+                                            n, R, Pw, pages, page, H, Hkv, hd, dt, scale, max_q, ws, wsb, None)
+
+    for over in (dict(q=None), dict(o=None), dict(kc=None), dict(vc=None), dict(table=None), dict(kv=None), dict(cu=None),
+                 dict(pos=None), dict(n=-1), dict(R=-1), dict(rs=7), dict(scale=0.0), dict(scale=float("nan")),
+                 dict(max_q=-1), dict(sn=-2048), dict(n=1 << 28), dict(Pw=1 << 28, rs=1 << 28)):
+        assert fwd(**over) == INVALID, over
+    for over in (dict(dt=0), dict(dt=7)):
+        assert fwd(**over) == DTYPE, over
+    for over in (dict(hd=12), dict(hd=136), dict(H=14), dict(H=516), dict(page=48)):
+        assert fwd(**over) == UNSUPPORTED, over
+    odd = ctypes.c_void_p(4104)
+    for over in (dict(q=odd), dict(o=odd), dict(kc=odd), dict(vc=odd), dict(ws=odd), dict(sn=2052), dict(ss=516)):
+        assert fwd(**over) == ALIGN, over
+    assert fwd(n=0) == 0 and fwd(n=0, q=None) == 0
+
+
+def test_ops_refuse_cpu_tensors():
+    t, i, x = torch.zeros((1, 2), dtype=torch.int32), torch.zeros(1, dtype=torch.int32), torch.zeros((1, 2, 16))
+    c, j = torch.zeros((2, 8, 2, 16)), torch.zeros(1, dtype=torch.int64)
+    with pytest.raises(RuntimeError, match="CUDA tensors"):
+        ops.paged_slots_(t, i, i, i, 8, 1)
+    with pytest.raises(RuntimeError, match="CUDA tensors"):
+        ops.rope_paged_write_(x, x, None, None, j, j, c, c)
+    with pytest.raises(RuntimeError, match="CUDA tensors"):
+        ops.sqdk_paged_fwd(x, c, c, t, i, i, j, 0.1)
+
+
+def test_plain_attention_is_the_oracles():
+    g = torch.Generator().manual_seed(0)
+    B, S, H, Hkv, hd, page = 2, 45, 6, 2, 16, 8
+    k, v = torch.randn((B, 48, Hkv, hd), generator=g), torch.randn((B, 48, Hkv, hd), generator=g)
+    idx = torch.stack([torch.randperm(S, generator=g)[:9].sort().values for _ in range(B)])
+    q = torch.randn((B, 9, H, hd), generator=g)
+    want = oracle.sqdk_fp32(q.numpy(), k[:, :S].numpy(), v[:, :S].numpy(), idx.numpy())
+    order = torch.randperm(12, generator=g)
+    kc, vc = torch.empty((12, page, Hkv, hd)), torch.empty((12, page, Hkv, hd))
+    kc[order], vc[order] = k.reshape(12, page, Hkv, hd), v.reshape(12, page, Hkv, hd)
+    got, _ = ref.attend_ref(q.reshape(-1, H, hd).half(), kc, vc, order.view(B, 6), [S, S], [0, 9, 18], idx.reshape(-1),
+                            hd ** -0.5)
+    got32, _ = ref.attend_ref(q.reshape(-1, H, hd), kc, vc, order.view(B, 6), [S, S], [0, 9, 18], idx.reshape(-1), hd ** -0.5)
+    np.testing.assert_allclose(got32.numpy().reshape(want.shape), want, atol=2e-5)
+    assert got.dtype == torch.float64
+
+
+def test_plain_slots():
+    table, cu, kv, pos, slots, taken = ref.slots_ref([[7, -1], [3, 4]], [6, 16], [4, 0], [9, 2], 8, 5)
+    assert table == [[7, 9], [3, 4]] and cu == [0, 4, 4] and kv == [10, 16] and taken == 1
+    assert pos == [6, 7, 8, 9, -1] and slots == [62, 63, 72, 73, -1]

@@ -1,0 +1,492 @@
+"""Paged K/V cache operators against their 64-bit forms (tests/paged_ref.py)."""
+
+import pytest
+import torch
+
+from hspmn_b200 import _native as N
+from hspmn_b200 import ops
+from tests import paged_ref as ref
+
+pytestmark = pytest.mark.gpu
+DEV = "cuda"
+
+
+def i32(x):
+    return torch.tensor(x, dtype=torch.int32, device=DEV)
+
+
+# ---------------------------------------------------------------------------
+# paged_slots_
+# ---------------------------------------------------------------------------
+
+
+def run_slots(seq, new, page, n, free=None, width=None, view=False):
+    R = len(seq)
+    g = torch.Generator().manual_seed(R + page)
+    held = [-(-max(c, 0) // page) for c in seq]
+    want = [-(-(max(c, 0) + max(m, 0)) // page) for c, m in zip(seq, new)]
+    width = max(want + [1]) + 1 if width is None else width
+    pages = torch.randperm(sum(want) + 7, generator=g).tolist()
+    rows, at = [], 0
+    for h in held:
+        rows.append((pages[at:at + h] + [-5] * width)[:width])
+        at += h
+    free = pages[at:] if free is None else pages[at:at + free]
+    table = torch.full((R, 2 * width + 3), -9, dtype=torch.int32, device=DEV)
+    if R:
+        table[:, 1:1 + width] = i32(rows)
+    t = table[:, 1:1 + width] if view else table[:, 1:1 + width].contiguous()
+    got = ops.paged_slots_(t, i32(seq), i32(new), i32(free), page, n)
+    want = ref.slots_ref(rows, seq, new, free, page, n)
+    assert t.tolist() == want[0]
+    for name, a, b in zip(("cu", "kv_lens", "positions", "slots"), got, want[1:5]):
+        assert a.tolist() == b, name
+    assert got[4].tolist() == [want[5]]
+    if view:  # the columns beside the view are left as they were
+        assert (table[:, 0] == -9).all() and (table[:, 1 + width:] == -9).all()
+    return got
+
+
+@pytest.mark.parametrize("page", [8, 16, 64, 4096])
+@pytest.mark.parametrize("seq,new,pad", [
+    ([0], [1], 0), ([0], [0], 3), ([5], [0], 0), ([15, 16, 17, 0, 63], [1, 1, 1, 1, 1], 0),
+    ([0, 0, 0], [0, 700, 0], 5), ([4095, 4096, 1, 8191], [1, 1, 9000, 2], 1), ([7] * 300, [3] * 300, 0)])
+def test_slots(page, seq, new, pad):
+    run_slots(seq, new, page, sum(new) + pad, view=pad % 2 == 1)
+    assert ops.device_errors() == 0
+
+
+@pytest.mark.parametrize("R", [255, 256, 257, 1000, 8192])
+def test_slots_many_requests(R):
+    g = torch.Generator().manual_seed(R)
+    seq = torch.randint(0, 200, (R,), generator=g).tolist()
+    new = torch.randint(0, 40, (R,), generator=g).tolist()
+    run_slots(seq, new, 16, sum(new) + 11)
+    assert ops.device_errors() == 0
+
+
+def test_slots_empty_batch():
+    run_slots([], [], 16, 0)
+    run_slots([], [], 16, 4)
+    assert ops.device_errors() == 0
+
+
+def test_slots_flags_what_does_not_fit():
+    run_slots([10, 0, 30], [20, 40, 5], 8, 65, free=4)  # the free list ends
+    assert ops.device_errors() == N.DEVERR_PAGE
+    run_slots([10, 0], [20, 40], 8, 60, width=4)  # the table is too narrow
+    assert ops.device_errors() == N.DEVERR_POSITION
+    run_slots([10, 0], [20, 40], 8, 33)  # more tokens than places
+    assert ops.device_errors() == N.DEVERR_POSITION
+    run_slots([-3, 4], [2, -7], 8, 4)  # negative lengths count as zero
+    assert ops.device_errors() == N.DEVERR_POSITION
+    t = torch.zeros((3, 4), dtype=torch.int32, device=DEV)
+    big = 2 ** 31 - 1
+    got = ops.paged_slots_(t, i32([big, 0, big]), i32([big, big, big]), i32([1, 2]), 8, 40)
+    assert got[1].tolist() == [big] * 3 and got[3].max().item() < 3 * 8
+    assert ops.device_errors() == N.DEVERR_POSITION | N.DEVERR_PAGE
+
+
+# ---------------------------------------------------------------------------
+# rope_paged_write_
+# ---------------------------------------------------------------------------
+
+
+def tables(L, hd, dtype, gen):
+    ang = torch.rand((L, hd), generator=gen, dtype=torch.float64) * 6.28
+    return ang.cos().to(dtype).to(DEV), ang.sin().to(dtype).to(DEV)
+
+
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16, torch.float32])
+@pytest.mark.parametrize("tab", ["same", "f32", None])
+@pytest.mark.parametrize("n,Hkv,hd,page,joint", [(1, 4, 128, 64, False), (61, 4, 64, 16, True), (130, 3, 48, 8, True),
+                                                 (33, 16, 16, 32, False), (700, 1, 256, 128, True)])
+def test_write(dtype, tab, n, Hkv, hd, page, joint):
+    g = torch.Generator().manual_seed(n + hd)
+    pages, L = -(-n // page) + 3, 2 * n + 5
+    kv = torch.randn((pages, 2, page, Hkv, hd), generator=g).to(dtype).to(DEV)
+    kc, vc = (kv[:, 0], kv[:, 1]) if joint else (kv[:, 0].contiguous(), kv[:, 1].contiguous())
+    k0, v0 = kc.clone(), vc.clone()
+    k = torch.randn((n, Hkv, hd), generator=g).to(dtype).to(DEV)
+    v = torch.randn((n, Hkv, hd), generator=g).to(dtype).to(DEV)
+    pos = torch.randint(0, L, (n,), generator=g).to(DEV)
+    slots = torch.randperm(pages * page, generator=g)[:n].to(DEV)
+    slots[n // 2] = -1  # padding
+    cos, sin = (None, None) if tab is None else tables(L, hd, dtype if tab == "same" else torch.float32, g)
+    ops.rope_paged_write_(k, v, cos, sin, pos, slots, kc, vc)
+    live = slots >= 0
+    page_i, off = slots[live] // page, slots[live] % page
+    assert torch.equal(vc[page_i, off], v[live])
+    got = kc[page_i, off].double()
+    if tab is None:
+        assert torch.equal(got, k[live].double())
+    else:
+        want, size = ref.rope_ref(k[live], cos, sin, pos[live])
+        # one rounding to the type, and three float32 operations before it
+        u = torch.finfo(dtype).eps / 2
+        tiny = torch.finfo(dtype).tiny * torch.finfo(dtype).eps
+        assert ((got - want).abs() <= u * want.abs() * (1 + 1e-6) + 3 * 2.0 ** -24 * size + tiny).all()
+    v0[page_i, off] = v[live]
+    k0[page_i, off] = kc[page_i, off]
+    assert torch.equal(kc, k0) and torch.equal(vc, v0)  # nothing else was touched
+    assert ops.device_errors() == 0
+
+
+def test_write_takes_views_and_block_tables():
+    """K and V as halves of one projection, tables as RotaryEmbedding keeps them."""
+    from hspmn_b200 import RotaryEmbedding
+    n, Hkv, hd, page = 37, 4, 64, 16
+    kv = torch.randn(n, 2 * Hkv * hd, dtype=torch.bfloat16, device=DEV)
+    k, v = kv[:, :Hkv * hd].view(n, Hkv, hd), kv[:, Hkv * hd:].view(n, Hkv, hd)
+    rope = RotaryEmbedding(hd, 64).to(DEV)
+    cos, sin = rope.cached_cos, rope.cached_sin  # float32 [1,1,L,hd]
+    kc, vc = (torch.zeros((4, page, Hkv, hd), dtype=torch.bfloat16, device=DEV) for _ in range(2))
+    pos, slots = torch.arange(n, device=DEV), torch.arange(n, device=DEV) + 3
+    ops.rope_paged_write_(k, v, cos, sin, pos, slots, kc, vc)
+    want, _ = ref.rope_ref(k, cos[0, 0], sin[0, 0], pos)
+    got = kc.view(-1, Hkv, hd)[3:3 + n]
+    assert torch.allclose(got.double(), want, rtol=2.0 ** -8, atol=2.0 ** -20)
+    assert torch.equal(vc.view(-1, Hkv, hd)[3:3 + n], v)
+
+
+def test_write_flags_bad_slots_and_positions():
+    Hkv, hd, page = 2, 32, 8
+    kc, vc = (torch.zeros((2, page, Hkv, hd), dtype=torch.float16, device=DEV) for _ in range(2))
+    k = torch.ones((3, Hkv, hd), dtype=torch.float16, device=DEV)
+    cos = torch.ones((4, hd), dtype=torch.float16, device=DEV)
+    ops.rope_paged_write_(k, k, cos, cos, torch.tensor([0, 1, 2], device=DEV), torch.tensor([16, 5, 1 << 40], device=DEV),
+                          kc, vc)
+    assert ops.device_errors() == N.DEVERR_PAGE
+    assert vc.view(16, -1).sum(1).nonzero().flatten().tolist() == [5]
+    ops.rope_paged_write_(k, k, cos, cos, torch.tensor([4, 3, -1], device=DEV), torch.tensor([0, 6, 2], device=DEV), kc, vc)
+    assert ops.device_errors() == N.DEVERR_POSITION
+    assert vc.view(16, -1).sum(1).nonzero().flatten().tolist() == [5, 6]
+    # without tables the positions are not read
+    ops.rope_paged_write_(k, k, None, None, torch.tensor([9, 9, -9], device=DEV), torch.tensor([0, 1, 2], device=DEV), kc, vc)
+    assert ops.device_errors() == 0 and vc.view(16, -1).sum(1).nonzero().flatten().tolist() == [0, 1, 2, 5, 6]
+
+
+# ---------------------------------------------------------------------------
+# sqdk_paged_fwd
+# ---------------------------------------------------------------------------
+
+
+def batch(kv_lens, positions, H, Hkv, hd, dtype, page, seed, joint=False, tail=0, fill=None):
+    """``positions``: for each request its query positions."""
+    g = torch.Generator().manual_seed(seed)
+    kc, vc, table = ref.make_cache(kv_lens, page, Hkv, hd, dtype, g, DEV, joint, fill=fill)
+    cu = [0]
+    for ps in positions:
+        cu.append(cu[-1] + len(ps))
+    flat = [p for ps in positions for p in ps] + [0] * tail
+    q = torch.randn((len(flat), H, hd), generator=g).to(dtype).to(DEV)
+    return q, kc, vc, table, kv_lens, cu, torch.tensor(flat, dtype=torch.int64, device=DEV)
+
+
+def attend(q, kc, vc, table, kv_lens, cu, pos, scale=None, max_q=0):
+    return ops.sqdk_paged_fwd(q, kc, vc, table, i32(kv_lens), i32(cu), pos,
+                              q.shape[-1] ** -0.5 if scale is None else scale, max_q)
+
+
+def check(args, scale=None, max_qs=(0,)):
+    q = args[0]
+    want, tol = ref.attend_ref(*args, q.shape[-1] ** -0.5 if scale is None else scale)
+    for max_q in max_qs:
+        o = attend(*args, scale=scale, max_q=max_q)
+        assert o.dtype == q.dtype and o.shape == q.shape and o.is_contiguous()
+        err = (o.double() - want).abs()
+        assert (err <= tol).all(), (max_q, err.max().item(), (err - tol).max().item())
+
+
+HEADS = [(16, 4, 128), (16, 16, 64), (12, 4, 64), (6, 2, 96), (8, 1, 128), (4, 4, 8), (32, 1, 48), (128, 1, 64),
+         (16, 2, 120)]
+
+
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16])
+@pytest.mark.parametrize("H,Hkv,hd", HEADS)
+def test_decode_heads(dtype, H, Hkv, hd):
+    lens = [1, 7, 8, 63, 64, 65, 200]
+    check(batch(lens, [[n - 1] for n in lens], H, Hkv, hd, dtype, 16, seed=H + hd, joint=hd == 64), max_qs=(0, 1))
+    assert ops.device_errors() == 0
+
+
+@pytest.mark.parametrize("page", [8, 16, 32, 64, 128, 1024])
+@pytest.mark.parametrize("joint", [False, True])
+def test_decode_pages(page, joint):
+    lens = [1500, 3, page, page + 1, 2 * page - 1, 900]
+    check(batch(lens, [[n - 1] for n in lens], 16, 4, 128, torch.bfloat16, page, seed=page, joint=joint), max_qs=(0, 1))
+    assert ops.device_errors() == 0
+
+
+@pytest.mark.parametrize("R,n", [(1, 1), (1, 64), (1, 65), (1, 5000), (2, 20000), (300, 40), (40, 700)])
+def test_decode_batches(R, n):
+    """From fewer units than CTAs to many a CTA: items whole, cut once and cut often."""
+    lens = [max(1, n - 13 * (r % 5)) for r in range(R)]
+    check(batch(lens, [[m - 1] for m in lens], 8, 2, 64, torch.bfloat16, 16, seed=R + n), max_qs=(1,))
+    assert ops.device_errors() == 0
+
+
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16])
+@pytest.mark.parametrize("H,Hkv,hd", [(16, 4, 128), (12, 4, 64), (6, 2, 96), (4, 4, 64), (32, 1, 128), (40, 2, 16)])
+def test_chunks(dtype, H, Hkv, hd):
+    """Whole prompts, chunks behind cached tokens, selected rows, short runs and single tokens in one batch."""
+    lens = [150, 331, 64, 40, 257, 500]
+    positions = [list(range(150)), list(range(200, 331)), list(range(0, 64, 5)), [39], [254, 255, 256],
+                 list(range(3, 500, 7))]
+    check(batch(lens, positions, H, Hkv, hd, dtype, 16, seed=hd, joint=True), max_qs=(0, 150, 1))
+    assert ops.device_errors() == 0
+
+
+@pytest.mark.parametrize("page", [8, 16, 32, 64, 256])
+def test_chunk_pages(page):
+    lens = [300, 77]
+    check(batch(lens, [list(range(100, 300)), list(range(77))], 8, 2, 128, torch.bfloat16, page, seed=page),
+          max_qs=(200,))
+    assert ops.device_errors() == 0
+
+
+def test_positions_in_any_order_and_repeated():
+    lens = [200, 90]
+    g = torch.Generator().manual_seed(5)
+    positions = [torch.randperm(200, generator=g)[:77].tolist() + [13, 13, 13], [89, 0, 44, 44]]
+    check(batch(lens, positions, 8, 2, 64, torch.bfloat16, 32, seed=1), max_qs=(0, 80))
+    assert ops.device_errors() == 0
+
+
+def test_rows_that_see_nothing_are_zero():
+    lens = [0, 100, 70, 0, 64]
+    positions = [[0], [-1, 5, 99, -7], list(range(70)), [], [63]]
+    args = batch(lens, positions, 8, 2, 64, torch.bfloat16, 16, seed=2, tail=21)
+    check(args, max_qs=(0, 70, 1))
+    o = attend(*args)
+    cu = args[5]
+    assert not o[0].any() and not o[cu[1]].any() and not o[cu[1] + 3].any() and not o[cu[-1]:].any()
+    assert ops.device_errors() == N.DEVERR_POSITION  # position 0 of a request with nothing cached
+    none = attend(*batch([], [], 8, 2, 64, torch.bfloat16, 16, seed=2, tail=3))
+    assert none.shape[0] == 3 and not none.any()
+    assert attend(*batch([4], [[]], 8, 2, 64, torch.bfloat16, 16, seed=2)).shape == (0, 8, 64)
+    assert ops.device_errors() == 0
+
+
+@pytest.mark.parametrize("fill", [float("nan"), float("inf")])
+@pytest.mark.parametrize("page", [16, 64])
+def test_what_lies_behind_the_last_token_does_not_count(fill, page):
+    lens = [1, 50, 64, 65, 130, 300]
+    positions = [[0], [49], [63], [64], list(range(100, 130)), list(range(60, 300))]
+    check(batch(lens, positions, 16, 4, 64, torch.bfloat16, page, seed=3, fill=fill), max_qs=(0, 240))
+    assert ops.device_errors() == 0
+
+
+@pytest.mark.parametrize("bad", [float("nan"), float("inf"), float("-inf")])
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16])
+def test_a_value_reaches_only_the_rows_that_see_its_key(bad, dtype):
+    lens = [200, 40]
+    args = batch(lens, [list(range(200)), [36, 37, 38, 39]], 8, 2, 64, dtype, 16, seed=4)
+    q, kc, vc, table, _, cu, pos = args
+    for r, p in ((0, 77), (0, 150), (1, 38)):
+        vc[table[r, p // 16].item(), p % 16, 0, 5] = bad
+        kc[table[r, p // 16].item(), p % 16, 1, 9] = bad
+    want, tol = ref.attend_ref(*args, 0.125)
+    for max_q in (0, 200):
+        o = attend(*args, scale=0.125, max_q=max_q).double()
+        assert torch.equal(o.isnan(), want.isnan())
+        assert torch.equal(o[o.isinf()], want[o.isinf()]) and torch.equal(o.isinf(), want.isinf())
+        fine = want.isfinite()
+        assert ((o - want).abs()[fine] <= tol.nan_to_num(0.0)[fine]).all()
+
+
+def test_large_scores():
+    """Rows whose maximum grows by far from block to block, and ties at the top."""
+    lens = [600, 600]
+    args = batch(lens, [[599], list(range(400, 600))], 8, 2, 64, torch.float16, 32, seed=6)
+    q, kc = args[0], args[1]
+    kc.mul_(8.0)
+    q.mul_(4.0)
+    check(args, max_qs=(0, 200))
+    assert ops.device_errors() == 0
+
+
+def test_positions_behind_the_last_token_are_flagged_and_see_all():
+    args = batch([50], [[49, 50, 1000]], 4, 2, 64, torch.bfloat16, 16, seed=7)
+    check(args, max_qs=(0, 3))
+    assert ops.device_errors() == N.DEVERR_POSITION
+
+
+def test_missing_pages_are_left_out_and_flagged():
+    lens = [160, 64]
+    for many in (False, True):
+        positions = [list(range(100, 160)), [63] * (50 if many else 1)]
+        args = batch(lens, positions, 4, 2, 64, torch.bfloat16, 16, seed=8)
+        q, kc, vc, table, kv, cu, pos = args
+        table[0, 3], table[0, 5] = -1, kc.shape[0]
+        table[1] = 1 << 20
+        o = attend(*args, max_q=60)
+        assert ops.device_errors() == N.DEVERR_PAGE
+        assert not o[60:].any()
+        # the same with the two pages' keys taken out of the row
+        keep = [p for p in range(160) if p // 16 not in (3, 5)]
+        k = torch.cat([kc[table[0, p // 16].item(), p % 16][None] for p in keep])
+        v = torch.cat([vc[table[0, p // 16].item(), p % 16][None] for p in keep])
+        n = len(keep)
+        k2, v2 = (torch.zeros((-(-n // 16) * 16, 2, 64), dtype=k.dtype, device=DEV) for _ in range(2))
+        k2[:n], v2[:n] = k, v
+        want, tol = ref.attend_ref(q[:60], k2.view(-1, 16, 2, 64), v2.view(-1, 16, 2, 64),
+                                   torch.arange(len(k2) // 16, device=DEV)[None], [n], [0, 60], pos[:60] - 32, 0.125)
+        assert ((o[:60].double() - want).abs() <= tol).all()
+
+
+def test_strided_operands():
+    args = batch([90, 200], [[88, 89], list(range(150, 200))], 8, 2, 64, torch.bfloat16, 16, seed=9)
+    q, kc, vc, table, kv, cu, pos = args
+    want = attend(*args)
+    wide = torch.zeros((q.shape[0], 3, 8, 64), dtype=q.dtype, device=DEV)
+    wide[:, 1] = q
+    assert torch.equal(attend(wide[:, 1], *args[1:]), want)
+    off = torch.zeros(q.numel() + 1, dtype=q.dtype, device=DEV)[1:].view(q.shape)  # base not on 16 bytes
+    off.copy_(q)
+    assert torch.equal(attend(off, *args[1:]), want)
+    heads_first = kc.permute(0, 2, 1, 3).contiguous().permute(0, 2, 1, 3)  # [pages, Hkv, page, hd] memory
+    assert torch.equal(attend(q, heads_first, vc, *args[3:]), want)
+    tab = torch.full((2, 40), 10 ** 6, dtype=torch.int32, device=DEV)
+    tab[:, :table.shape[1]] = table
+    assert torch.equal(attend(q, kc, vc, tab[:, :table.shape[1]], *args[4:]), want)
+    assert torch.equal(attend(q, kc, vc, tab, *args[4:]), want)  # a wider table: entries behind kv_lens are not read
+    assert ops.device_errors() == 0
+
+
+def test_results_do_not_depend_on_the_run():
+    lens = [3000, 10, 700]
+    args = batch(lens, [[2999], list(range(10)), list(range(300, 700))], 16, 4, 128, torch.bfloat16, 64, seed=10)
+    first = attend(*args, max_q=400)
+    for _ in range(5):
+        assert torch.equal(attend(*args, max_q=400), first)
+
+
+def test_offsets_past_32_bits():
+    """Pages far into a cache of more than 2^32 bytes."""
+    page, Hkv, hd = 64, 4, 128
+    pages = 75_000  # 4.9 GB each
+    kc = torch.empty((pages, page, Hkv, hd), dtype=torch.bfloat16, device=DEV)
+    vc = torch.empty_like(kc)
+    far = [pages - 1, 2, pages - 7, 70_000]
+    for c in (kc, vc):
+        for pg in far:
+            c[pg] = torch.randn((page, Hkv, hd), device=DEV).to(torch.bfloat16)
+    table = i32([far])
+    k = torch.randn((1, Hkv, hd), device=DEV).to(torch.bfloat16)
+    slot = torch.tensor([(pages - 7) * page + 9], device=DEV)
+    ops.rope_paged_write_(k, k, None, None, slot, slot, kc, vc)
+    assert torch.equal(kc[pages - 7, 9], k[0]) and torch.equal(vc[pages - 7, 9], k[0])
+    for rows in (1, 60):
+        q = torch.randn((rows, 16, hd), device=DEV).to(torch.bfloat16)
+        pos = torch.arange(256 - rows, 256, device=DEV)
+        check((q, kc, vc, table, [256], [0, rows], pos), max_qs=(rows,))
+    assert ops.device_errors() == 0
+
+
+# ---------------------------------------------------------------------------
+# streams, graphs, the operators together
+# ---------------------------------------------------------------------------
+
+
+def test_other_stream():
+    args = batch([500, 300], [[499], list(range(100, 300))], 8, 2, 128, torch.bfloat16, 16, seed=11)
+    want = attend(*args, max_q=200)
+    torch.cuda.synchronize()
+    side = torch.cuda.Stream()
+    with torch.cuda.stream(side):
+        got = attend(*args, max_q=200)
+    side.synchronize()
+    assert torch.equal(got, want)
+
+
+def test_captured_step_replays_with_new_lengths():
+    """A padded decode step captured once and replayed while requests grow and change."""
+    R, P, page, H, Hkv, hd, cap = 4, 12, 16, 8, 2, 64, 6
+    g = torch.Generator().manual_seed(12)
+    kc, vc = (torch.zeros((60, page, Hkv, hd), dtype=torch.bfloat16, device=DEV) for _ in range(2))
+    table = torch.full((R, P), -1, dtype=torch.int32, device=DEV)
+    seq, new = i32([0] * R), i32([0] * R)
+    free = i32(list(range(60)))
+    cos, sin = tables(P * page, hd, torch.float32, g)
+    k, v = (torch.zeros((cap, Hkv, hd), dtype=torch.bfloat16, device=DEV) for _ in range(2))
+    q = torch.zeros((cap, H, hd), dtype=torch.bfloat16, device=DEV)
+
+    def step():
+        cu, kv_lens, pos, slots, taken = ops.paged_slots_(table, seq, new, free, page, cap)
+        ops.rope_paged_write_(k, v, cos, sin, pos, slots, kc, vc)
+        return cu, kv_lens, pos, taken, ops.sqdk_paged_fwd(q, kc, vc, table, kv_lens, cu, pos, 0.125, 3)
+
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        step()
+    torch.cuda.current_stream().wait_stream(side)
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        out = step()
+    held = [0] * R
+    for i, lens in enumerate([[1, 3, 0, 2], [1, 0, 1, 1], [2, 1, 1, 1], [0, 0, 1, 0]] * 6):
+        seq.copy_(i32(held))
+        new.copy_(i32(lens))
+        for t in (k, v, q):
+            t.copy_(torch.randn(t.shape, generator=g))
+        graph.replay()
+        cu, kv_lens, pos, taken, o = out
+        held = [a + b for a, b in zip(held, lens)]
+        assert kv_lens.tolist() == held
+        want, tol = ref.attend_ref(q, kc, vc, table, held, cu.tolist(), pos, 0.125)
+        assert ((o.double() - want).abs() <= tol).all() and not o[cu[-1].item():].any()
+        free.copy_(torch.roll(free, -taken.item()))
+    assert ops.device_errors() == 0
+
+
+def test_prefill_in_chunks_and_decode_equal_the_whole_sequence():
+    """Prompts brought in chunk by chunk and then token by token give what sqdk_fwd gives on the whole sequence."""
+    B, S, H, Hkv, hd, page = 3, 200, 8, 2, 64, 16
+    g = torch.Generator().manual_seed(13)
+    q, k, v = (torch.randn((B, S, h, hd), generator=g).to(torch.bfloat16).to(DEV) for h in (H, Hkv, Hkv))
+    cos, sin = tables(S, hd, torch.float32, g)
+    kc, vc = (torch.full((64, page, Hkv, hd), float("nan"), dtype=torch.bfloat16, device=DEV) for _ in range(2))
+    table = torch.full((B, -(-S // page)), -1, dtype=torch.int32, device=DEV)
+    free = i32(torch.randperm(64, generator=g).tolist())
+    held, rows = [0] * B, [[] for _ in range(B)]
+    plan = [[70, 1, 33], [0, 100, 64], [60, 64, 1]] + [[1, 1, 1]] * 35
+    for new in plan:
+        pick = [slice(h, h + m) for h, m in zip(held, new)]
+        cu, kv_lens, pos, slots, taken = ops.paged_slots_(table, i32(held), i32(new), free, page, sum(new))
+        ops.rope_paged_write_(torch.cat([k[b, s] for b, s in enumerate(pick)]),
+                              torch.cat([v[b, s] for b, s in enumerate(pick)]), cos, sin, pos, slots, kc, vc)
+        o = ops.sqdk_paged_fwd(torch.cat([q[b, s] for b, s in enumerate(pick)]), kc, vc, table, kv_lens, cu, pos, 0.125,
+                               max(new))
+        free = free[taken.item():]
+        at = 0
+        for b, m in enumerate(new):
+            rows[b].append(o[at:at + m])
+            at += m
+        held = [h + m for h, m in zip(held, new)]
+    n = min(held)
+    assert n == 133
+    got = torch.stack([torch.cat(r)[:n] for r in rows])
+    rot = torch.stack([ref.rope_ref(k[b, :n], cos, sin, torch.arange(n, device=DEV))[0] for b in range(B)]).to(torch.bfloat16)
+    idx = torch.arange(n, device=DEV).expand(B, n).contiguous()
+    dense = ops.sqdk_fwd(q[:, :n].contiguous(), rot, v[:, :n].contiguous(), idx, 0.125)
+    want, tol = ref.attend_ref(q[:, :n].reshape(-1, H, hd), rot.view(B, n, Hkv, hd), v[:, :n],
+                               torch.arange(B, device=DEV)[:, None], [n] * B, [0, n, 2 * n, 3 * n], idx.reshape(-1), 0.125)
+    assert ((got.reshape(-1, H, hd).double() - want).abs() <= tol).all()
+    # two kernels, each within its bound
+    assert ((got - dense).double().abs().reshape(-1, H, hd) <= 2 * tol + 2.0 ** -8 * want.abs()).all()
+    assert ops.device_errors() == 0
+
+
+def test_registered_operators_trace():
+    args = batch([20], [[19]], 4, 2, 64, torch.bfloat16, 16, seed=14)
+    q, kc, vc, table, kv, cu, pos = args
+    checks = ("test_schema", "test_faketensor")
+    torch.library.opcheck(torch.ops.hspmn.sqdk_paged_fwd.default, (q, kc, vc, table, i32(kv), i32(cu), pos, 0.125, 1),
+                          test_utils=checks)
+    torch.library.opcheck(torch.ops.hspmn.paged_slots_.default, (table, i32([16]), i32([4]), i32([0, 1]), 16, 4),
+                          test_utils=checks)
+    k = torch.zeros((1, 2, 64), dtype=torch.bfloat16, device=DEV)
+    torch.library.opcheck(torch.ops.hspmn.rope_paged_write_.default, (k, k, None, None, pos, pos, kc, vc),
+                          test_utils=checks)
