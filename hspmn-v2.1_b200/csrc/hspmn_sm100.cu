@@ -19,6 +19,7 @@
 #include "gate.cuh"
 #include "paged.cuh"
 #include "paged_attn.cuh"
+#include "paged_chunk.cuh"
 #include "router.cuh"
 #include "rows.cuh"
 #include "sqdk.cuh"
@@ -787,10 +788,10 @@ int page_shift(int64_t page_size) {
   return -1;
 }
 
-// Whether every stride is non-negative and, in bytes, a multiple of 16.
+// Whether every stride is positive and, in bytes, a multiple of 16.
 int check_strides(std::initializer_list<int64_t> strides, int64_t es) {
   for (int64_t s : strides)
-    if (s < 0) return HSPMN_ERR_INVALID;
+    if (s <= 0) return HSPMN_ERR_INVALID;
   for (int64_t s : strides)
     if ((s * es) % 16) return HSPMN_ERR_ALIGN;
   return HSPMN_OK;
@@ -814,7 +815,29 @@ int launch_paged_attn(const PagedAttnParams& prm, int runs, cudaStream_t st) {
   return launch_status();
 }
 
-int64_t paged_part_o_bytes(int64_t runs, int64_t hdp) { return 2 * runs * kPagedRows * hdp * 4; }
+// Rows (queries * G) of a request up to which its tiles are the 16-row kernel's.
+constexpr int kPagedSplitRows = 16;
+
+// Whether a call has, by its arguments, a request for the chunk kernel.
+bool paged_has_chunks(int64_t N, int64_t G, int64_t max_q) {
+  return (max_q > 0 ? std::min(max_q, N) : N) * G > kPagedSplitRows;
+}
+
+int64_t paged_part_rows(int sms) { return 2LL * sms * kPagedCtasPerSm * kPagedRows; }
+int64_t chunk_part_rows(int sms) { return 2LL * sms * kChunkCtasPerSm * kSqdkBM; }
+
+template <int HD, bool kBF16>
+int launch_paged_chunk(const CUtensorMap& mq, const CUtensorMap& mk, const CUtensorMap& mv, const ChunkParams& prm,
+                       int runs, cudaStream_t st) {
+  using L = ChunkLayout<HD>;
+  auto kern = paged_chunk_kernel<HD, kBF16>;
+  if (cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, L::kAlloc) != cudaSuccess)
+    return HSPMN_ERR_CUDA;
+  kern<<<static_cast<unsigned>(runs), kChunkThreads, L::kAlloc, st>>>(mq, mk, mv, prm);
+  if (int rc = launch_status()) return rc;
+  paged_chunk_merge_kernel<HD, kBF16><<<static_cast<unsigned>(runs - 1), 32 * kChunkMergeWarps, 0, st>>>(prm, runs);
+  return launch_status();
+}
 
 }  // namespace
 
@@ -874,6 +897,10 @@ int hspmn_rope_paged_write(const void* k, int64_t k_sn, int64_t k_sh, const void
   const int shift = page_shift(page_size);
   if (shift < 0 || (hd * es) % (cos_tab ? 32 : 16) || Hkv * hd > 0x7FFFFFFF) return HSPMN_ERR_UNSUPPORTED;
   if (cos_tab && (tab_ss < hd || tab_rows < 0)) return HSPMN_ERR_INVALID;
+  // the stride of a dimension of one element is never used: any is accepted
+  if (N == 1) k_sn = v_sn = Hkv * hd;
+  if (Hkv == 1) k_sh = v_sh = kc_sh = vc_sh = hd;
+  if (num_pages == 1) kc_sp = vc_sp = page_size * Hkv * hd;
   if (int rc = check_strides({k_sn, k_sh, v_sn, v_sh, kc_sp, kc_ss, kc_sh, vc_sp, vc_ss, vc_sh}, es)) return rc;
   const int64_t tes = tab_dtype == HSPMN_F32 ? 4 : 2;
   if (cos_tab && (tab_ss * tes) % 16) return HSPMN_ERR_ALIGN;
@@ -915,11 +942,12 @@ int hspmn_rope_paged_write(const void* k, int64_t k_sn, int64_t k_sh, const void
   return launch_status();
 }
 
-int64_t hspmn_sqdk_paged_workspace_size(int64_t hd) {
+int64_t hspmn_sqdk_paged_workspace_size(int64_t N, int64_t H, int64_t Hkv, int64_t hd, int64_t max_q) {
+  if (N < 1 || H < 1 || Hkv < 1 || hd < 1 || max_q < 0) return 0;
   int sms = 0;
   if (sm_count(&sms) != HSPMN_OK) return -1;
-  const int64_t runs = static_cast<int64_t>(sms) * kPagedCtasPerSm;
-  return paged_part_o_bytes(runs, hd > 64 ? 128 : 64) + 2 * runs * kPagedRows * 2 * 4;
+  const int64_t rows = paged_part_rows(sms) + (paged_has_chunks(N, H / Hkv, max_q) ? chunk_part_rows(sms) : 0);
+  return rows * ((hd > 64 ? 128 : 64) + 2) * 4;
 }
 
 int hspmn_sqdk_paged_fwd(const void* q, int64_t q_sn, int64_t q_sh, const void* k_cache, int64_t kc_sp, int64_t kc_ss,
@@ -939,6 +967,11 @@ int hspmn_sqdk_paged_fwd(const void* q, int64_t q_sn, int64_t q_sh, const void* 
   if (N > 0x7FFFFFFF / H || R > 0x7FFFFFFE || P > (0x7FFFFFFF >> shift) || num_pages > 0x7FFFFFFF)
     return HSPMN_ERR_INVALID;
   const int64_t es = 2;
+  // the stride of a dimension of one element is never used: any is accepted
+  if (N == 1) q_sn = o_sn = H * hd;
+  if (H == 1) q_sh = o_sh = hd;
+  if (Hkv == 1) kc_sh = vc_sh = hd;
+  if (num_pages == 1) kc_sp = vc_sp = page_size * Hkv * hd;
   if (int rc = check_strides({q_sn, q_sh, kc_sp, kc_ss, kc_sh, vc_sp, vc_ss, vc_sh, o_sn, o_sh}, es)) return rc;
   if (!aligned(q, 16) || !aligned(k_cache, 16) || !aligned(v_cache, 16) || !aligned(o, 16) || !aligned(workspace, 16))
     return HSPMN_ERR_ALIGN;
@@ -949,7 +982,7 @@ int hspmn_sqdk_paged_fwd(const void* q, int64_t q_sn, int64_t q_sh, const void* 
   if (int rc = check_device()) return rc;
   int sms = 0;
   if (int rc = sm_count(&sms)) return rc;
-  if (!workspace || workspace_bytes < static_cast<size_t>(hspmn_sqdk_paged_workspace_size(hd)))
+  if (!workspace || workspace_bytes < static_cast<size_t>(hspmn_sqdk_paged_workspace_size(N, H, Hkv, hd, max_q)))
     return HSPMN_ERR_INVALID;
   const int runs = sms * kPagedCtasPerSm;
   PagedAttnParams prm;
@@ -966,7 +999,8 @@ int hspmn_sqdk_paged_fwd(const void* q, int64_t q_sn, int64_t q_sh, const void* 
   prm.cu_q = cu_q;
   prm.pos = positions;
   prm.part_o = static_cast<float*>(workspace);
-  prm.part_ml = reinterpret_cast<float*>(static_cast<char*>(workspace) + paged_part_o_bytes(runs, hd > 64 ? 128 : 64));
+  const int64_t hdp = hd > 64 ? 128 : 64;
+  prm.part_ml = prm.part_o + paged_part_rows(sms) * hdp;
   prm.N = N;
   prm.R = static_cast<int>(R);
   prm.P = static_cast<int>(P);
@@ -977,7 +1011,45 @@ int hspmn_sqdk_paged_fwd(const void* q, int64_t q_sn, int64_t q_sh, const void* 
   prm.G = static_cast<int>(H / Hkv);
   prm.hd = static_cast<int>(hd);
   prm.scale_log2 = sm_scale * 1.4426950408889634f;
+  prm.split_rows = 0x7FFFFFFF;
   cudaStream_t st = static_cast<cudaStream_t>(stream);
+  // The host knows neither lengths nor offsets: a call that may hold chunks runs
+  // both kernels, each on its own requests.
+  if (paged_has_chunks(N, prm.G, max_q) && R > 0 && P > 0 && num_pages > 0) {
+    prm.split_rows = kPagedSplitRows;
+    ChunkParams ch;
+    ch.a = prm;
+    ch.a.part_o = prm.part_ml + paged_part_rows(sms) * 2;
+    ch.a.part_ml = ch.a.part_o + chunk_part_rows(sms) * hdp;
+    ch.QT = kSqdkBM / prm.G;
+    ch.box_rows = static_cast<int>(std::min<int64_t>(page_size, kSqdkBN));
+    const CUtensorMapDataType dt =
+        dtype == HSPMN_BF16 ? CU_TENSOR_MAP_DATA_TYPE_BFLOAT16 : CU_TENSOR_MAP_DATA_TYPE_FLOAT16;
+    CUtensorMap mq, mk, mv;
+    const uint64_t qd[4] = {static_cast<uint64_t>(hd), static_cast<uint64_t>(H), static_cast<uint64_t>(N), 1u};
+    const uint64_t qs[3] = {static_cast<uint64_t>(prm.q_sh), static_cast<uint64_t>(prm.q_sn),
+                            static_cast<uint64_t>(prm.q_sn)};
+    const uint32_t qb[4] = {64u, static_cast<uint32_t>(prm.G), static_cast<uint32_t>(ch.QT), 1u};
+    if (int rc = encode_4d(&mq, q, dt, qd, qs, qb)) return rc;
+    const uint64_t kd[4] = {static_cast<uint64_t>(hd), static_cast<uint64_t>(Hkv), static_cast<uint64_t>(page_size),
+                            static_cast<uint64_t>(num_pages)};
+    const uint64_t ks[3] = {static_cast<uint64_t>(prm.k_sh), static_cast<uint64_t>(prm.k_ss),
+                            static_cast<uint64_t>(prm.k_sp)};
+    const uint64_t vs[3] = {static_cast<uint64_t>(prm.v_sh), static_cast<uint64_t>(prm.v_ss),
+                            static_cast<uint64_t>(prm.v_sp)};
+    const uint32_t kb[4] = {64u, 1u, static_cast<uint32_t>(ch.box_rows), 1u};
+    if (int rc = encode_4d(&mk, k_cache, dt, kd, ks, kb)) return rc;
+    if (int rc = encode_4d(&mv, v_cache, dt, kd, vs, kb)) return rc;
+    const int chunk_runs = sms * kChunkCtasPerSm;
+    int rc;
+    if (hd > 64)
+      rc = dtype == HSPMN_BF16 ? launch_paged_chunk<128, true>(mq, mk, mv, ch, chunk_runs, st)
+                               : launch_paged_chunk<128, false>(mq, mk, mv, ch, chunk_runs, st);
+    else
+      rc = dtype == HSPMN_BF16 ? launch_paged_chunk<64, true>(mq, mk, mv, ch, chunk_runs, st)
+                               : launch_paged_chunk<64, false>(mq, mk, mv, ch, chunk_runs, st);
+    if (rc) return rc;
+  }
   if (hd > 64)
     return dtype == HSPMN_BF16 ? launch_paged_attn<128, true>(prm, runs, st)
                               : launch_paged_attn<128, false>(prm, runs, st);

@@ -52,6 +52,7 @@ struct PagedAttnParams {
   float* part_ml;  // [2 * runs][16][2] maximum (log2 units), row sum
   int64_t N;
   int R, P, num_pages, shift, H, Hkv, G, hd;
+  int split_rows;  // requests with more rows (queries * G) than this are not this kernel's
   float scale_log2;
 };
 
@@ -65,7 +66,8 @@ struct PagedRequest {
   int64_t units;   // tiles * Hkv * nb
 };
 
-__device__ __forceinline__ PagedRequest paged_request(const PagedAttnParams& p, int r) {
+// The request's rows and keys (its tiles not counted).
+__device__ __forceinline__ PagedRequest paged_rows(const PagedAttnParams& p, int r) {
   PagedRequest q;
   const int N = static_cast<int>(p.N);
   const int a = min(max(__ldg(p.cu_q + r), 0), N);
@@ -75,7 +77,12 @@ __device__ __forceinline__ PagedRequest paged_request(const PagedAttnParams& p, 
   q.q0 = a;
   q.rows = max(b - a, 0) * p.G;
   q.kv = static_cast<int>(min(kv, cap));
-  q.tiles = (q.rows + kPagedRows - 1) / kPagedRows;
+  return q;
+}
+
+__device__ __forceinline__ PagedRequest paged_request(const PagedAttnParams& p, int r) {
+  PagedRequest q = paged_rows(p, r);
+  q.tiles = r < p.R && q.rows > p.split_rows ? 0 : (q.rows + kPagedRows - 1) / kPagedRows;
   q.nb = max(1, (q.kv + kPagedKeys - 1) / kPagedKeys);
   q.units = static_cast<int64_t>(q.tiles) * p.Hkv * q.nb;
   return q;
@@ -202,6 +209,15 @@ template <bool kBF16>
 __device__ __forceinline__ bool not_finite2(uint32_t w) {
   constexpr uint32_t e = kBF16 ? 0x7F80u : 0x7C00u;
   return (w & e) == e || ((w >> 16) & e) == e;
+}
+
+// The word with infinities and NaN replaced by zero.
+template <bool kBF16>
+__device__ __forceinline__ uint32_t finite2(uint32_t w) {
+  constexpr uint32_t e = kBF16 ? 0x7F80u : 0x7C00u;
+  if ((w & e) == e) w &= 0xFFFF0000u;
+  if (((w >> 16) & e) == e) w &= 0x0000FFFFu;
+  return w;
 }
 
 template <bool kBF16>

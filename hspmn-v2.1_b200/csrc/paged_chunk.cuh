@@ -1,0 +1,771 @@
+// Sparse-query dense-key causal attention over a paged K/V cache, for requests
+// with many query rows (prompt chunks, whole or router-selected): the products
+// of sqdk_fwd_kernel on tcgen05 / TMEM / TMA with the keys fetched page by page.
+//
+// Tile: one request, one K/V head, QT = 128 / G consecutive query rows of the
+// packed batch with the G heads that read that K/V head (128 rows), against
+// 64-key blocks. S = Q K^T and O += P V as in sqdk.cuh (two S buffers, P over
+// S in tensor memory, optimistic running maximum, O in tensor memory for the
+// whole tile); K and V blocks land through TMA boxes of min(page_size, 64)
+// rows, one box a page, found through the block table by the producer warp.
+//
+// Schedule: requests have any lengths, the host knows none of them, and a tile
+// costs from one block to thousands. The tiles form one list (request, head,
+// tile) with an estimated cost each, linear in the tile's number between the
+// request's first and last position; the list is cut into equal runs, one a
+// CTA (two CTAs an SM). A CTA takes the tiles that lie in its run whole, in
+// order, then the pieces that its run's two ends cut off: their O goes to the
+// workspace and a merge kernel adds the pieces in run order. Whole tiles first,
+// because the tiles of a head then start together at its first key and stream
+// the same K/V blocks out of L2. Estimates only set the balance: which keys a
+// piece covers is computed from the cut and the tile's true key count, the same
+// way by every CTA that holds a piece.
+//
+// Warp roles (192 threads): warp 0 requests Q, K and V (one lane a page box),
+// warp 1 allocates tensor memory and issues the products, warps 2..5 do the
+// softmax and the epilogue (one thread a row). The K, V and S rings run on
+// across tiles, so the next tile's keys load while this one ends.
+#pragma once
+
+#include "paged_attn.cuh"
+
+namespace hspmn {
+
+constexpr int kChunkThreads = 192;
+constexpr int kChunkCtasPerSm = 2;
+constexpr int kChunkUnit = 16;           // cost units of a 64-key block
+constexpr int kChunkTileCost = 3;        // blocks' worth of time to open and close a tile
+constexpr int kChunkMinPiece = 4;        // blocks of work below which another run is not opened
+constexpr int kChunkEpilogueBar = 1;     // named barrier of the four softmax warps
+
+template <int HD>
+struct ChunkLayout {
+  static constexpr int kChunks = HD / 64;
+  static constexpr int kQChunkBytes = kSqdkBM * 128;
+  static constexpr int kKVChunkBytes = kSqdkBN * 128;
+  static constexpr int kKVBytes = kChunks * kKVChunkBytes;
+  static constexpr int kQOff = 0;
+  static constexpr int kKOff = kChunks * kQChunkBytes;
+  static constexpr int kVOff = kKOff + 2 * kKVBytes;
+  static constexpr int kOOff = kVOff + 2 * kKVBytes;  // epilogue staging: 32 rows x 64 bytes a warp
+  static constexpr int kBytes = kOOff + 4 * 32 * 64;
+  static constexpr int kAlloc = kBytes + 1024;
+  static constexpr uint32_t kTmemCols = 256;  // S0 | S1 | O
+  static constexpr int kOCol = 2 * kSqdkBN;
+};
+
+struct ChunkParams {
+  PagedAttnParams a;  // part_o / part_ml: [2 * runs][128] rows here
+  int QT, box_rows;
+};
+
+// A request's tiles. Costs are linear in the tile number: first + t * slope.
+struct ChunkRequest {
+  int q0, len, kv, tiles;
+  int64_t first, slope, head;  // head: the sum over a head's tiles
+};
+
+__device__ __forceinline__ ChunkRequest chunk_request(const ChunkParams& p, int r) {
+  ChunkRequest c;
+  const PagedRequest q = paged_rows(p.a, r);
+  c.q0 = q.q0;
+  c.len = q.rows / p.a.G;
+  c.kv = q.kv;
+  c.tiles = 0;
+  c.first = c.slope = c.head = 0;
+  if (q.rows <= p.a.split_rows) return c;  // the 16-row kernel's
+  c.tiles = (c.len + p.QT - 1) / p.QT;
+  const int64_t top = static_cast<int64_t>(c.kv) - 1;
+  const int64_t lo = min(max(__ldg(p.a.pos + c.q0 + min(p.QT, c.len) - 1), static_cast<int64_t>(0)), max(top, static_cast<int64_t>(0)));
+  const int64_t hi = min(max(__ldg(p.a.pos + c.q0 + c.len - 1), static_cast<int64_t>(0)), max(top, static_cast<int64_t>(0)));
+  constexpr int kShift = 2;  // 64 keys = kChunkUnit units
+  static_assert(kSqdkBN >> kShift == kChunkUnit, "cost units");
+  c.first = (lo >> kShift) + kChunkUnit * (1 + kChunkTileCost);
+  c.slope = c.tiles > 1 ? max((hi - lo) >> kShift, static_cast<int64_t>(0)) / (c.tiles - 1) : 0;
+  c.head = c.first * c.tiles + c.slope * (static_cast<int64_t>(c.tiles) * (c.tiles - 1) / 2);
+  return c;
+}
+
+struct ChunkTile {
+  ChunkRequest req;
+  int r, head, t;
+  int64_t start, cost;  // place in the list
+  __device__ __forceinline__ int64_t before(int n) const {
+    return req.first * n + req.slope * (static_cast<int64_t>(n) * (n - 1) / 2);
+  }
+  // Only called while a next tile exists.
+  __device__ __forceinline__ void next(const ChunkParams& p) {
+    start += cost;
+    if (++t == req.tiles) {
+      t = 0;
+      if (++head == p.a.Hkv) {
+        head = 0;
+        do req = chunk_request(p, ++r);
+        while (req.tiles == 0 && r + 1 < p.a.R);
+      }
+    }
+    cost = req.first + req.slope * t;
+  }
+};
+
+__device__ __forceinline__ int64_t chunk_total(const ChunkParams& p, int lane) {
+  int64_t n = 0;
+  for (int r = lane; r < p.a.R; r += 32) n += chunk_request(p, r).head * p.a.Hkv;
+#pragma unroll
+  for (int d = 16; d > 0; d >>= 1) n += __shfl_xor_sync(0xFFFFFFFFu, n, d);
+  return n;
+}
+
+// Runs that a list of this cost is cut into.
+__device__ __forceinline__ int64_t chunk_runs(int64_t total, int64_t most) {
+  return min(most, max(total / (kChunkUnit * kChunkMinPiece), static_cast<int64_t>(1)));
+}
+
+// The tile that holds list place w (< the total), found by the whole warp.
+__device__ __forceinline__ ChunkTile chunk_locate(const ChunkParams& p, int64_t w, int lane) {
+  ChunkTile c;
+  int64_t base = 0;
+  c.r = p.a.R - 1;
+  for (int r0 = 0; r0 < p.a.R; r0 += 32) {
+    const int r = r0 + lane;
+    const int64_t mine = r < p.a.R ? chunk_request(p, r).head * p.a.Hkv : 0;
+    int64_t sum = mine;
+#pragma unroll
+    for (int d = 1; d < 32; d <<= 1) {
+      const int64_t x = __shfl_up_sync(0xFFFFFFFFu, sum, d);
+      if (lane >= d) sum += x;
+    }
+    const unsigned past = __ballot_sync(0xFFFFFFFFu, base + sum > w);
+    if (past) {
+      const int l = __ffs(past) - 1;
+      base += __shfl_sync(0xFFFFFFFFu, sum - mine, l);
+      c.r = r0 + l;
+      break;
+    }
+    base += __shfl_sync(0xFFFFFFFFu, sum, 31);
+  }
+  c.req = chunk_request(p, c.r);
+  const int64_t rel = w - base;
+  c.head = static_cast<int>(rel / c.req.head);
+  const int64_t in_head = rel - c.head * c.req.head;
+  int lo = 0, hi = c.req.tiles;
+  while (hi - lo > 1) {
+    const int mid = (lo + hi) >> 1;
+    if (c.before(mid) <= in_head) lo = mid;
+    else hi = mid;
+  }
+  c.t = lo;
+  c.start = base + c.head * c.req.head + c.before(lo);
+  c.cost = c.req.first + c.req.slope * lo;
+  return c;
+}
+
+// Where run c begins: an equal share of the list, moved to the nearer end of its
+// tile when that is so close that the piece would not be worth its merge.
+__device__ __forceinline__ int64_t chunk_cut(const ChunkParams& p, int64_t total, int64_t runs, int64_t c, int lane,
+                                             ChunkTile& tile) {
+  if (c >= runs) return total;
+  const int64_t w = run_start(total, runs, c);
+  tile = chunk_locate(p, w, lane);
+  const int64_t near = min(total / runs / 16, static_cast<int64_t>(8 * kChunkUnit));
+  if (w - tile.start <= near) return tile.start;
+  if (tile.start + tile.cost - w <= near) return tile.start + tile.cost;
+  return w;
+}
+
+// Key block at list place w of a tile with nblk blocks.
+__device__ __forceinline__ int chunk_block_at(const ChunkTile& c, int64_t w, int nblk) {
+  const int64_t x = min(max(w - c.start, static_cast<int64_t>(0)), c.cost);
+  return static_cast<int>(x * nblk / c.cost);
+}
+
+// The largest and smallest last key that the tile's rows see, over the rows
+// that see any (the whole warp; max -1 where none does).
+__device__ __forceinline__ void chunk_limits(const ChunkParams& p, const ChunkTile& c, int lane, int& lo, int& hi) {
+  lo = 0x7FFFFFFF;
+  hi = -1;
+  const int n = min(p.QT, c.req.len - c.t * p.QT);
+  for (int i = lane; i < n; i += 32) {
+    const int64_t ps = __ldg(p.a.pos + c.req.q0 + c.t * p.QT + i);
+    const int lim = static_cast<int>(min(max(ps, static_cast<int64_t>(-1)), static_cast<int64_t>(c.req.kv) - 1));
+    if (lim >= 0) lo = min(lo, lim);
+    hi = max(hi, lim);
+  }
+  lo = __reduce_min_sync(0xFFFFFFFFu, lo);
+  hi = __reduce_max_sync(0xFFFFFFFFu, hi);
+}
+
+// One piece of work of a CTA.
+struct ChunkSegment {
+  ChunkTile tile;
+  int lo, hi;    // limits of the tile's rows
+  int j0, nblk;  // its key blocks
+  int slot;      // workspace slot, or -1 for a tile done whole
+};
+
+// Walks a run's segments: the whole tiles in order, then the piece at the run's
+// start, then the one at its end. Every warp of the CTA walks the same ones.
+struct ChunkWalk {
+  ChunkTile first, cur;
+  int64_t w0, w1;
+  int stage;  // 0: whole tiles, 1: piece at the start, 2: piece at the end, 3: done
+  bool started;
+  __device__ __forceinline__ void open(const ChunkParams& p, int64_t total, int64_t runs, int64_t c, int lane) {
+    ChunkTile t;
+    w0 = chunk_cut(p, total, runs, c, lane, t);
+    w1 = chunk_cut(p, total, runs, c + 1, lane, t);
+    stage = 3;
+    started = false;
+    if (w0 >= w1) return;
+    first = cur = chunk_locate(p, w0, lane);
+    stage = 0;
+  }
+  __device__ __forceinline__ void cover(const ChunkParams& p, ChunkSegment& s, int64_t a, int64_t b, int lane) {
+    chunk_limits(p, s.tile, lane, s.lo, s.hi);
+    const int all = s.hi < 0 ? 0 : s.hi / kSqdkBN + 1;
+    s.j0 = chunk_block_at(s.tile, a, all);
+    s.nblk = chunk_block_at(s.tile, b, all) - s.j0;
+  }
+  __device__ __forceinline__ bool next(const ChunkParams& p, ChunkSegment& s, int lane) {
+    while (stage == 0) {
+      if (started) {
+        if (cur.start + cur.cost >= w1) {
+          stage = 1;
+          break;
+        }
+        cur.next(p);
+      }
+      started = true;
+      if (cur.start < w0) continue;
+      if (cur.start + cur.cost > w1) {
+        stage = 1;
+        break;
+      }
+      s.tile = cur;
+      cover(p, s, cur.start, cur.start + cur.cost, lane);
+      s.slot = -1;
+      return true;
+    }
+    // cur is the run's last tile now
+    if (stage == 1) {
+      stage = 2;
+      if (first.start < w0) {
+        s.tile = first;
+        cover(p, s, w0, w1, lane);
+        s.slot = 2 * static_cast<int>(blockIdx.x);
+        if (first.start + first.cost >= w1) stage = 3;  // the run lies inside one tile
+        return true;
+      }
+    }
+    if (stage == 2) {
+      stage = 3;
+      if (cur.start + cur.cost > w1) {
+        s.tile = cur;
+        cover(p, s, w0, w1, lane);
+        s.slot = 2 * static_cast<int>(blockIdx.x) + 1;
+        return true;
+      }
+    }
+    return false;
+  }
+};
+
+template <int HD, bool kBF16>
+__global__ void __launch_bounds__(kChunkThreads, kChunkCtasPerSm)
+    paged_chunk_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant__ CUtensorMap tmK,
+                       const __grid_constant__ CUtensorMap tmV, const __grid_constant__ ChunkParams p) {
+  using L = ChunkLayout<HD>;
+  extern __shared__ uint8_t chunk_smem_raw[];
+  // Blocks are numbered through the whole run: block n uses S buffer, K stage
+  // and V stage n & 1, and phase n >> 1 of their barriers. One thread issues
+  // every product and they complete in order, so bar_sfull (Q K^T of block n
+  // done) also frees K stage n & 1 and, after a tile's last block, the Q tile.
+  __shared__ __align__(8) uint64_t bar_q, bar_kfull[2], bar_vfull[2], bar_vempty[2], bar_sfull[2], bar_pfull[2];
+  __shared__ __align__(8) uint64_t bar_ofinal, bar_drain;
+  __shared__ uint32_t tmem_base_sh;
+  __shared__ volatile uint32_t abort_flag;
+  // an infinity or NaN was taken out of V for rows that do not see it (by the
+  // segment's parity: one is cleared while the other is in use)
+  __shared__ volatile uint32_t wild_flag[2];
+
+  const uint32_t sbase = (smem_u32(chunk_smem_raw) + 1023u) & ~1023u;
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  const int64_t total = chunk_total(p, lane);
+  const int64_t runs = chunk_runs(total, gridDim.x);
+  if (total == 0 || blockIdx.x >= runs) return;
+  ChunkWalk walk;
+  walk.open(p, total, runs, blockIdx.x, lane);
+  if (walk.stage == 3) return;
+
+  if (threadIdx.x == 0) {
+    mbar_init(&bar_q, 1);
+    for (int s = 0; s < 2; ++s) {
+      mbar_init(&bar_kfull[s], 1);
+      mbar_init(&bar_vfull[s], 1);
+      mbar_init(&bar_vempty[s], 1);
+      mbar_init(&bar_sfull[s], 1);
+      mbar_init(&bar_pfull[s], 4);  // one arrival per softmax warp
+    }
+    mbar_init(&bar_ofinal, 1);
+    mbar_init(&bar_drain, 1);
+    abort_flag = 0u;
+    wild_flag[0] = wild_flag[1] = 0u;
+    fence_mbar_init();
+  }
+  if (warp == 1) {
+    tmem_alloc(&tmem_base_sh, L::kTmemCols);
+    tmem_relinquish();
+  }
+  tc_fence_before();
+  __syncthreads();
+  tc_fence_after();
+  const uint32_t tmem = tmem_base_sh;
+  ChunkSegment s;
+
+  if (warp == 0) {
+    // ------------------------------------------------------------ producer
+    const int boxes = kSqdkBN / p.box_rows;
+    uint32_t nk = 0, nv = 0, segs = 0;
+    bool live = true;
+    while (live && walk.next(p, s, lane)) {
+      if (s.nblk == 0) continue;
+      if (nk > 0) live = __all_sync(0xFFFFFFFFu, mbar_wait(&bar_sfull[(nk - 1) & 1], ((nk - 1) >> 1) & 1, &abort_flag));
+      if (!live) break;
+      if (lane == 0) {
+        mbar_arrive_expect_tx(&bar_q, static_cast<uint32_t>(L::kChunks * p.a.G * p.QT * 128));
+        for (int c = 0; c < L::kChunks; ++c)
+          tma_load_4d(sbase + L::kQOff + c * L::kQChunkBytes, &tmQ, &bar_q, c * 64, s.tile.head * p.a.G,
+                      s.tile.req.q0 + s.tile.t * p.QT, 0);
+      }
+      ++segs;
+      const int* row = p.a.table + static_cast<int64_t>(s.tile.r) * p.a.table_rs;
+      const int mask = (1 << p.a.shift) - 1;
+      // this lane's page of block j; a page that does not exist (and a box
+      // behind the cached tokens) is read from behind the last page: zeros
+      auto page_at = [&](int j) -> int {
+        const int key = (s.j0 + j) * kSqdkBN + lane * p.box_rows;
+        if (lane >= boxes || key >= s.tile.req.kv) return p.a.num_pages;
+        const int pg = __ldg(row + (key >> p.a.shift));
+        if (pg >= 0 && pg < p.a.num_pages) return pg;
+        raise_device_error(HSPMN_DEVERR_PAGE);
+        return p.a.num_pages;
+      };
+      auto load = [&](const CUtensorMap* map, uint64_t* bar, uint32_t dst, int j, int page) {
+        if (lane == 0) mbar_arrive_expect_tx(bar, L::kKVBytes);
+        __syncwarp();
+        if (lane < boxes) {
+          const int off = ((s.j0 + j) * kSqdkBN + lane * p.box_rows) & mask;
+          for (int c = 0; c < L::kChunks; ++c)
+            tma_load_4d(dst + c * L::kKVChunkBytes + lane * p.box_rows * 128, map, bar, c * 64, s.tile.head, off, page);
+        }
+      };
+      int page_k = page_at(0), page_v = page_k;
+      auto load_k = [&](int j) -> bool {
+        const uint32_t st = nk & 1, ph = nk >> 1;
+        if (ph > 0 && !__all_sync(0xFFFFFFFFu, mbar_wait(&bar_sfull[st], (ph - 1) & 1, &abort_flag))) return false;
+        load(&tmK, &bar_kfull[st], sbase + L::kKOff + st * L::kKVBytes, j, page_k);
+        ++nk;
+        return true;
+      };
+      live = load_k(0);
+      for (int j = 0; live && j < s.nblk; ++j) {
+        if (j + 1 < s.nblk) {
+          page_k = page_at(j + 1);
+          live = load_k(j + 1);
+          if (!live) break;
+        }
+        const uint32_t st = nv & 1, ph = nv >> 1;
+        if (ph > 0 && !__all_sync(0xFFFFFFFFu, mbar_wait(&bar_vempty[st], (ph - 1) & 1, &abort_flag))) {
+          live = false;
+          break;
+        }
+        load(&tmV, &bar_vfull[st], sbase + L::kVOff + st * L::kKVBytes, j, page_v);
+        page_v = page_k;
+        ++nv;
+      }
+    }
+    // every copy this warp issued has landed before the CTA may exit
+    if (lane == 0) {
+      if (segs > 0) mbar_wait_drain(&bar_q, (segs - 1) & 1);
+      for (uint32_t st = 0; st < 2; ++st) {
+        if (nk > st) mbar_wait_drain(&bar_kfull[st], ((nk - 1 - st) >> 1) & 1);
+        if (nv > st) mbar_wait_drain(&bar_vfull[st], ((nv - 1 - st) >> 1) & 1);
+      }
+    }
+    __syncwarp();
+  } else if (warp == 1) {
+    // ------------------------------------------------------------ MMA issue
+    constexpr int kAB = kBF16 ? 1 : 0;
+    constexpr uint32_t idesc_s = umma_idesc_f16(kSqdkBM, kSqdkBN, kAB, false, false);
+    constexpr uint32_t idesc_o = umma_idesc_f16(kSqdkBM, HD, kAB, false, true);
+    const uint32_t tO = tmem + L::kOCol;
+    const uint64_t qdesc = sw128_desc(sbase + L::kQOff, 16, 1024);
+    const uint64_t kdesc = sw128_desc(sbase + L::kKOff, 16, 1024);
+    const uint64_t vdesc = sw128_desc(sbase + L::kVOff, L::kKVChunkBytes, 1024);
+    uint32_t n = 0, segs = 0;
+    bool ok = true;
+    auto issue_pv = [&](uint32_t m, bool first) -> bool {
+      const uint32_t sb = m & 1, ph = (m >> 1) & 1;
+      if (!__all_sync(0xFFFFFFFFu, mbar_wait2(&bar_pfull[sb], ph, &bar_vfull[sb], ph, &abort_flag))) return false;
+      tc_fence_after();
+      const uint64_t vd = vdesc + static_cast<uint64_t>((sb * L::kKVBytes) >> 4);
+      const uint32_t ta = tmem + sb * kSqdkBN;
+      umma_ts_warp(tO, ta, vd, idesc_o, first ? 0u : 1u);
+#pragma unroll
+      for (int kk = 1; kk < kSqdkBN / 16; ++kk)
+        umma_ts_warp(tO, ta + kk * 8, vd + static_cast<uint64_t>((kk * 16 * 128) >> 4), idesc_o, 1u);
+      umma_commit_warp(&bar_vempty[sb]);
+      return true;
+    };
+    while (ok && walk.next(p, s, lane)) {
+      if (s.nblk == 0) continue;
+      ok = __all_sync(0xFFFFFFFFu, mbar_wait(&bar_q, segs & 1, &abort_flag));
+      ++segs;
+      if (!ok) break;
+      tc_fence_after();
+      for (int j = 0; ok && j < s.nblk; ++j, ++n) {
+        const uint32_t sb = n & 1;
+        if (!__all_sync(0xFFFFFFFFu, mbar_wait(&bar_kfull[sb], (n >> 1) & 1, &abort_flag))) {
+          ok = false;
+          break;
+        }
+        tc_fence_after();
+        const uint64_t kd = kdesc + static_cast<uint64_t>((sb * L::kKVBytes) >> 4);
+#pragma unroll
+        for (int kk = 0; kk < HD / 16; ++kk) {
+          const int c = kk >> 2, w = kk & 3;
+          umma_ss_warp(tmem + sb * kSqdkBN, qdesc + static_cast<uint64_t>((c * L::kQChunkBytes + w * 32) >> 4),
+                       kd + static_cast<uint64_t>((c * L::kKVChunkBytes + w * 32) >> 4), idesc_s, kk > 0 ? 1u : 0u);
+        }
+        umma_commit_warp(&bar_sfull[sb]);
+        if (j >= 1) ok = issue_pv(n - 1, j == 1);
+      }
+      if (ok) ok = issue_pv(n - 1, s.nblk == 1);
+      if (ok) umma_commit_warp(&bar_ofinal);
+    }
+    umma_commit_warp(&bar_drain);
+    if (lane == 0) mbar_wait_drain(&bar_drain, 0);
+    __syncwarp();
+  } else {
+    // ------------------------------------------------------------ softmax
+    const int sw = warp & 3;  // tensor memory lanes 32 * sw ..
+    const uint32_t lane_base = static_cast<uint32_t>(32 * sw) << 16;
+    const uint32_t tS = tmem + lane_base;
+    const uint32_t tO = tmem + lane_base + L::kOCol;
+    const int r = 32 * sw + lane;
+    const int qloc = r / p.a.G;
+    const float c2 = p.a.scale_log2;
+    uint32_t n = 0, segs = 0, walked = 0;
+    bool ok = true;
+    while (ok && walk.next(p, s, lane)) {
+      const ChunkTile& tile = s.tile;
+      const int qi = tile.t * p.QT + qloc;  // query row of the request
+      const bool row_valid = qloc < p.QT && qi < tile.req.len;
+      // rows that see nothing run along like the tile's last row; what they
+      // compute is not stored
+      int lim = s.hi;
+      bool blind = true;
+      if (row_valid) {
+        const int64_t ps = __ldg(p.a.pos + tile.req.q0 + qi);
+        if (ps >= tile.req.kv) raise_device_error(HSPMN_DEVERR_POSITION);
+        blind = ps < 0 || tile.req.kv == 0;
+        if (!blind) lim = static_cast<int>(min(ps, static_cast<int64_t>(tile.req.kv) - 1));
+      }
+      const int* row = p.a.table + static_cast<int64_t>(tile.r) * p.a.table_rs;
+      // pages of this piece that do not exist (flagged by the producer)
+      bool holes = false;
+      if (s.nblk > 0) {
+        const int end = min((s.j0 + s.nblk) * kSqdkBN, tile.req.kv);
+        for (int pg = ((s.j0 * kSqdkBN) >> p.a.shift) + lane; pg <= ((end - 1) >> p.a.shift); pg += 32) {
+          const int x = __ldg(row + pg);
+          holes |= x < 0 || x >= p.a.num_pages;
+        }
+        holes = __any_sync(0xFFFFFFFFu, holes);
+      }
+      bool seen = !blind && lim >= s.j0 * kSqdkBN && s.nblk > 0;
+      if (holes) seen = false;
+      float m_run = -INFINITY, l_run = 0.0f;
+      for (int j = 0; j < s.nblk; ++j, ++n) {
+        const uint32_t sb = n & 1;
+        ok = __all_sync(0xFFFFFFFFu, mbar_wait(&bar_sfull[sb], (n >> 1) & 1, &abort_flag));
+        if (!ok) break;
+        tc_fence_after();
+        float sv[kSqdkBN];
+        {
+          uint32_t r0[32], r1[32];
+          tmem_ld32(tS + sb * kSqdkBN, r0);
+          tmem_ld32(tS + sb * kSqdkBN + 32, r1);
+          tmem_wait_ld();
+#pragma unroll
+          for (int i = 0; i < 32; ++i) {
+            sv[i] = __uint_as_float(r0[i]);
+            sv[32 + i] = __uint_as_float(r1[i]);
+          }
+        }
+        const int key0 = (s.j0 + j) * kSqdkBN;
+        const int left = lim - key0;  // columns <= left are visible to this row
+        // the same for every warp: does any row of the tile not see all of this block?
+        const bool edge = key0 + kSqdkBN - 1 > s.lo;
+        if (edge) {
+#pragma unroll
+          for (int c = 0; c < kSqdkBN; ++c) sv[c] = (c <= left) ? sv[c] : -INFINITY;
+        }
+        if (holes) {
+          for (int c0 = 0; c0 < kSqdkBN; c0 += 8) {
+            const int x = key0 + c0 < tile.req.kv ? __ldg(row + ((key0 + c0) >> p.a.shift)) : -1;
+            const bool gone = x < 0 || x >= p.a.num_pages;
+            seen |= !gone && !blind && c0 <= left;
+#pragma unroll
+            for (int c = 0; c < kSqdkBN; ++c)
+              if ((c & ~7) == c0 && gone) sv[c] = -INFINITY;
+          }
+        }
+        uint32_t pk[kSqdkBN / 2];
+        // p = 2^(s*c2 - m), packed; returns the block's row sum
+        auto exponentiate = [&](float m) -> float {
+          const float neg_m = (m == -INFINITY) ? 0.0f : -m;
+          const uint64_t cc = f2_pack(c2, c2), nm = f2_pack(neg_m, neg_m);
+          uint64_t acc0 = f2_pack(0.0f, 0.0f), acc1 = acc0;
+#pragma unroll
+          for (int c = 0; c < kSqdkBN; c += 2) {
+            float x0, x1;
+            f2_unpack(f2_fma(f2_pack(sv[c], sv[c + 1]), cc, nm), x0, x1);
+            const float p0 = fast_exp2(x0), p1 = fast_exp2(x1);
+            if ((c >> 1) & 1) acc1 = f2_add(acc1, f2_pack(p0, p1));
+            else acc0 = f2_add(acc0, f2_pack(p0, p1));
+            pk[c >> 1] = pack2<kBF16>(p0, p1);
+          }
+          float a0, a1, b0, b1;
+          f2_unpack(acc0, a0, a1);
+          f2_unpack(acc1, b0, b1);
+          return (a0 + a1) + (b0 + b1);
+        };
+        bool done = false;
+        if (__all_sync(0xFFFFFFFFu, m_run != -INFINITY)) {
+          const float lb = exponentiate(m_run);
+          if (__all_sync(0xFFFFFFFFu, lb < kSqdkSumBound<kBF16>)) {
+            l_run += lb;
+            done = true;
+          }
+        }
+        if (!done) {
+          float mq[4] = {sv[0], sv[1], sv[2], sv[3]};
+#pragma unroll
+          for (int c = 4; c < kSqdkBN; c += 4) {
+#pragma unroll
+            for (int u = 0; u < 4; ++u) mq[u] = fmaxf(mq[u], sv[c + u]);
+          }
+          const float mx = fmaxf(fmaxf(mq[0], mq[1]), fmaxf(mq[2], mq[3]));
+          const float m_new = fmaxf(m_run, mx * c2);
+          const bool need_o = j > 0 && (m_run != -INFINITY) && (m_new > m_run);
+          if (__any_sync(0xFFFFFFFFu, need_o)) {
+            // P V of the block before must have landed in O
+            ok = __all_sync(0xFFFFFFFFu, mbar_wait(&bar_vempty[(n - 1) & 1], ((n - 1) >> 1) & 1, &abort_flag));
+            if (!ok) break;
+            tc_fence_after();
+            const float alpha = need_o ? fast_exp2(m_run - m_new) : 1.0f;
+#pragma unroll 1
+            for (int c = 0; c < HD; c += 32) {
+              uint32_t x[32];
+              tmem_ld32(tO + c, x);
+              tmem_wait_ld();
+#pragma unroll
+              for (int i = 0; i < 32; ++i) x[i] = __float_as_uint(__uint_as_float(x[i]) * alpha);
+              tmem_st32(tO + c, x);
+            }
+            tmem_wait_st();
+          }
+          if (m_new != m_run) {
+            l_run = (m_run == -INFINITY) ? 0.0f : l_run * fast_exp2(m_run - m_new);
+            m_run = m_new;
+          }
+          l_run += exponentiate(m_run);
+        }
+        tmem_st32(tS + sb * kSqdkBN, pk);
+        tmem_wait_st();
+        tc_fence_before();
+        if (edge) {
+          // P is zero where a row does not see a key, but 0 * inf is not: V
+          // rows that no row sees (the page's unwritten end) become zeros, and
+          // infinities and NaN leave the rows that only some see (the epilogue
+          // gives them back to those that do). 16 keys a warp.
+          ok = __all_sync(0xFFFFFFFFu, mbar_wait(&bar_vfull[sb], (n >> 1) & 1, &abort_flag));
+          if (!ok) break;
+          const uint32_t vst = sbase + L::kVOff + sb * L::kKVBytes;
+          bool found = false;
+#pragma unroll 1
+          for (int i = lane; i < 16 * 8 * L::kChunks; i += 32) {
+            const int kr = 16 * sw + (i >> 3) % 16, key = key0 + kr;
+            const uint32_t addr = vst + (i >> 7) * L::kKVChunkBytes + kr * 128 + (i & 7) * 16;
+            if (key > s.hi) {
+              st_shared_v4(addr, make_uint4(0u, 0u, 0u, 0u));
+            } else if (key > s.lo) {
+              uint4 w;
+              asm volatile("ld.shared.v4.u32 {%0,%1,%2,%3}, [%4];" : "=r"(w.x), "=r"(w.y), "=r"(w.z), "=r"(w.w) : "r"(addr));
+              if (not_finite2<kBF16>(w.x) || not_finite2<kBF16>(w.y) || not_finite2<kBF16>(w.z) || not_finite2<kBF16>(w.w)) {
+                found = true;
+                w.x = finite2<kBF16>(w.x), w.y = finite2<kBF16>(w.y), w.z = finite2<kBF16>(w.z), w.w = finite2<kBF16>(w.w);
+                st_shared_v4(addr, w);
+              }
+            }
+          }
+          if (found) wild_flag[walked & 1] = 1u;
+          fence_proxy_async_smem();
+        }
+        __syncwarp();
+        if (lane == 0) mbar_arrive(&bar_pfull[sb]);
+      }
+      // ---------------------------------------------------------- epilogue
+      if (ok && s.nblk > 0) ok = __all_sync(0xFFFFFFFFu, mbar_wait(&bar_ofinal, segs & 1, &abort_flag));
+      if (s.nblk > 0) ++segs;
+      // between the barriers every warp has set this segment's flag and none
+      // has left its epilogue: it is read, and the last segment's is cleared
+      if (threadIdx.x == 64) wild_flag[(walked + 1) & 1] = 0u;
+      const bool live = named_bar_and(kChunkEpilogueBar, 128, ok);
+      const bool wild = wild_flag[walked & 1] != 0u;
+      named_bar_sync(kChunkEpilogueBar, 128);
+      ++walked;
+      if (!live) {
+        ok = false;
+        break;
+      }
+      tc_fence_after();
+      const bool none = !seen;
+      const float inv_l = s.slot >= 0 ? 1.0f : 1.0f / l_run;
+#pragma unroll 1
+      for (int c = 0; c < HD; c += 32) {
+        float o[32];
+        if (s.nblk > 0) {
+          uint32_t x[32];
+          tmem_ld32(tO + c, x);
+          tmem_wait_ld();
+#pragma unroll
+          for (int i = 0; i < 32; ++i) o[i] = __uint_as_float(x[i]);
+        } else {
+#pragma unroll
+          for (int i = 0; i < 32; ++i) o[i] = 0.0f;
+        }
+        if (wild && row_valid && !blind) {
+          // infinities and NaN that this row does see, from the cache
+          const int from = max(s.lo + 1, s.j0 * kSqdkBN), to = min(lim, (s.j0 + s.nblk) * kSqdkBN - 1);
+          for (int key = from; key <= to; ++key) {
+            const int pg = __ldg(row + (key >> p.a.shift));
+            if (pg < 0 || pg >= p.a.num_pages) continue;
+            const char* v = p.a.v + pg * p.a.v_sp + (key & ((1 << p.a.shift) - 1)) * p.a.v_ss + tile.head * p.a.v_sh;
+#pragma unroll
+            for (int i = 0; i < 32; ++i) {
+              if (c + i >= p.a.hd) continue;
+              const uint16_t w = __ldg(reinterpret_cast<const unsigned short*>(v) + c + i);
+              if (not_finite2<kBF16>(w)) o[i] += half_to_float<kBF16>(w);
+            }
+          }
+        }
+        if (s.slot >= 0) {
+          // unnormalised O of this piece
+          if (row_valid) {
+            float* dst = p.a.part_o + (static_cast<int64_t>(s.slot) * kSqdkBM + r) * HD + c;
+#pragma unroll
+            for (int v = 0; v < 8; ++v)
+              reinterpret_cast<float4*>(dst)[v] = make_float4(o[4 * v], o[4 * v + 1], o[4 * v + 2], o[4 * v + 3]);
+          }
+          continue;
+        }
+        // 32 columns of the warp's 32 rows through shared memory, so that a
+        // row's 64 bytes leave together
+        const uint32_t stage = sbase + L::kOOff + sw * 32 * 64;
+#pragma unroll
+        for (int v = 0; v < 4; ++v) {
+          uint4 w;
+          w.x = none ? 0u : pack2<kBF16>(o[8 * v + 0] * inv_l, o[8 * v + 1] * inv_l);
+          w.y = none ? 0u : pack2<kBF16>(o[8 * v + 2] * inv_l, o[8 * v + 3] * inv_l);
+          w.z = none ? 0u : pack2<kBF16>(o[8 * v + 4] * inv_l, o[8 * v + 5] * inv_l);
+          w.w = none ? 0u : pack2<kBF16>(o[8 * v + 6] * inv_l, o[8 * v + 7] * inv_l);
+          st_shared_v4(stage + lane * 64 + ((v ^ ((lane >> 1) & 3)) << 4), w);
+        }
+        __syncwarp();
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+          const int lr = i * 8 + (lane >> 2), unit = lane & 3;
+          const int rr = 32 * sw + lr, ql = rr / p.a.G;
+          uint4 w;
+          asm volatile("ld.shared.v4.u32 {%0,%1,%2,%3}, [%4];"
+                       : "=r"(w.x), "=r"(w.y), "=r"(w.z), "=r"(w.w)
+                       : "r"(stage + lr * 64 + ((unit ^ ((lr >> 1) & 3)) << 4)));
+          if (ql < p.QT && tile.t * p.QT + ql < tile.req.len && c + unit * 8 < p.a.hd)
+            *reinterpret_cast<uint4*>(p.a.o + static_cast<int64_t>(tile.req.q0 + tile.t * p.QT + ql) * p.a.o_sn +
+                                      static_cast<int64_t>(tile.head * p.a.G + rr - ql * p.a.G) * p.a.o_sh +
+                                      (c + unit * 8) * 2) = w;
+        }
+        __syncwarp();
+      }
+      if (s.slot >= 0 && row_valid)
+        reinterpret_cast<float2*>(p.a.part_ml)[static_cast<int64_t>(s.slot) * kSqdkBM + r] =
+            make_float2(m_run, none ? kUnseen : l_run);
+      tc_fence_before();  // O has been read: the next tile's first P V (behind this warp's arrival) may write it
+    }
+  }
+
+  tc_fence_before();
+  __syncthreads();
+  if (warp == 1) {
+    tc_fence_after();
+    tmem_dealloc(tmem, L::kTmemCols);
+  }
+}
+
+constexpr int kChunkMergeWarps = 16;
+
+// Adds the pieces of the tile that the end of run blockIdx.x cuts, if that is
+// the tile's first piece. A warp takes a row at a time.
+template <int HD, bool kBF16>
+__global__ void __launch_bounds__(32 * kChunkMergeWarps) paged_chunk_merge_kernel(const __grid_constant__ ChunkParams p,
+                                                                                  int most_runs) {
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  const int64_t total = chunk_total(p, lane);
+  if (total == 0) return;
+  const int64_t runs = chunk_runs(total, most_runs);
+  const int64_t c0 = blockIdx.x;
+  if (c0 + 1 >= runs) return;
+  ChunkTile tile, t;
+  const int64_t cut = chunk_cut(p, total, runs, c0 + 1, lane, tile);
+  // a cut at a tile's end cuts nothing; the first piece is the one whose run
+  // does not begin inside the tile
+  if (cut <= tile.start || cut >= tile.start + tile.cost) return;
+  if (chunk_cut(p, total, runs, c0, lane, t) > tile.start) return;
+  // the last piece's run is the first that ends at or behind the tile's end
+  int64_t c1 = c0 + 1;
+  while (c1 + 1 < runs && run_start(total, runs, c1 + 1) < tile.start + tile.cost) ++c1;
+  if (c1 + 1 <= runs && chunk_cut(p, total, runs, c1, lane, t) >= tile.start + tile.cost) --c1;
+  const float2* ml = reinterpret_cast<const float2*>(p.a.part_ml);
+  const int rows = min(p.QT, tile.req.len - tile.t * p.QT) * p.a.G;
+  for (int r = warp; r < rows; r += kChunkMergeWarps) {
+    float M = -INFINITY, l = 0.0f;
+    bool none = true;
+    float4 o = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+    // run c0's piece is its last, the others' their first
+    for (int64_t c = c0; c <= c1; ++c) M = fmaxf(M, ml[(2 * c + (c == c0 ? 1 : 0)) * kSqdkBM + r].x);
+    for (int64_t c = c0; c <= c1; ++c) {
+      const int64_t sl = (2 * c + (c == c0 ? 1 : 0)) * kSqdkBM + r;
+      const float2 x = ml[sl];
+      if (x.y == kUnseen) continue;
+      none = false;
+      const float f = x.x == M ? 1.0f : fast_exp2(x.x - M);
+      l += f * x.y;
+      if (lane < HD / 4) {
+        const float4 v = *reinterpret_cast<const float4*>(p.a.part_o + sl * HD + lane * 4);
+        o.x += f * v.x, o.y += f * v.y, o.z += f * v.z, o.w += f * v.w;
+      }
+    }
+    const float inv = 1.0f / l;
+    if (lane < HD / 4 && lane * 4 < p.a.hd) {
+      const int ql = r / p.a.G;
+      uint2 w;
+      w.x = none ? 0u : pack2<kBF16>(o.x * inv, o.y * inv);
+      w.y = none ? 0u : pack2<kBF16>(o.z * inv, o.w * inv);
+      *reinterpret_cast<uint2*>(p.a.o + static_cast<int64_t>(tile.req.q0 + tile.t * p.QT + ql) * p.a.o_sn +
+                                static_cast<int64_t>(tile.head * p.a.G + r - ql * p.a.G) * p.a.o_sh + lane * 8) = w;
+    }
+  }
+}
+
+}  // namespace hspmn

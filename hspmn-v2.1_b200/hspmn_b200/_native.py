@@ -52,7 +52,7 @@ _SIGNATURES = {
     "hspmn_rope_paged_write": (_int, [_vp, _i64, _i64, _vp, _i64, _i64, _vp, _vp, _i64, _i64, _int, _vp, _vp,
                                       _vp, _i64, _i64, _i64, _vp, _i64, _i64, _i64, _i64, _i64, _i64, _i64, _i64,
                                       _int, _vp]),
-    "hspmn_sqdk_paged_workspace_size": (_i64, [_i64]),
+    "hspmn_sqdk_paged_workspace_size": (_i64, [_i64, _i64, _i64, _i64, _i64]),
     "hspmn_sqdk_paged_fwd": (_int, [_vp, _i64, _i64, _vp, _i64, _i64, _i64, _vp, _i64, _i64, _i64, _vp, _i64, _vp,
                                     _vp, _vp, _vp, _i64, _i64, _i64, _i64, _i64, _i64, _i64, _i64, _i64, _i64, _int,
                                     ctypes.c_float, _i64, _vp, ctypes.c_size_t, _vp]),

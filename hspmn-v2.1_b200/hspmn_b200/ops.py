@@ -650,7 +650,8 @@ def _check_caches(name: str, k_cache: torch.Tensor, v_cache: torch.Tensor, dtype
 def _rows3(t: torch.Tensor) -> torch.Tensor:
     """[N,H,hd] operand with a contiguous head row and 16-byte strides and base; copied where it is not."""
     es = t.element_size()
-    if t.stride(2) != 1 or (t.stride(0) * es) % 16 or (t.stride(1) * es) % 16 or t.data_ptr() % 16:
+    a, b, c = t.stride()
+    if c != 1 or a <= 0 or b <= 0 or (a * es) % 16 or (b * es) % 16 or t.data_ptr() % 16:
         t = t.clone(memory_format=torch.contiguous_format)
     return t
 
@@ -823,7 +824,7 @@ def _sqdk_paged_fwd_impl(q, k_cache, v_cache, block_table, kv_lens, cu_q, positi
     kc, vc = k_cache.stride(), v_cache.stride()
     with _on_device(dev), _launch("sqdk_paged_fwd", dev):
         lib = N.lib()
-        ws_bytes = lib.hspmn_sqdk_paged_workspace_size(hd)
+        ws_bytes = lib.hspmn_sqdk_paged_workspace_size(n, H, Hkv, hd, max_q)
         if ws_bytes < 0:
             raise N.HSPMNNativeError("hspmn_sqdk_paged_workspace_size: device query failed")
         ws = torch.empty(ws_bytes, dtype=torch.uint8, device=dev)

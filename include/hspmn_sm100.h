@@ -358,8 +358,9 @@ HSPMN_API int hspmn_rope_paged_write(const void* k, int64_t k_sn, int64_t k_sh, 
                                      int dtype, void* stream);
 
 /* Bytes of device workspace hspmn_sqdk_paged_fwd needs on the current device
- * for this head_dim, whatever the lengths (-1: the device could not be queried). */
-HSPMN_API int64_t hspmn_sqdk_paged_workspace_size(int64_t hd);
+ * for these arguments, whatever the requests' lengths (-1: the device could not
+ * be queried). */
+HSPMN_API int64_t hspmn_sqdk_paged_workspace_size(int64_t N, int64_t H, int64_t Hkv, int64_t hd, int64_t max_q);
 
 /*
  * Sparse-query dense-key causal attention of packed query rows over a paged
