@@ -1,8 +1,10 @@
-"""Build libhspmn_sm100.so, the sm_100a CUDA library behind hspmn_b200.
+"""Build libhspmn_sm100.so, the sm_100a CUDA library behind hspmn_b200, and
+libhspmn_torch.so, which registers its paged-cache operators with PyTorch.
 
-The library is compiled in-tree (next to the Python package) with nvcc for
-``sm_100a`` only; the product has no other target. Rebuilds only when a
-source under ``csrc/`` or ``include/`` is newer than the library.
+Both are compiled in-tree (next to the Python package): the CUDA library with
+nvcc for ``sm_100a`` only (the product has no other target), the operators
+with the host compiler against the installed PyTorch. Each is rebuilt only
+when a source it is made from is newer.
 
     python hspmn-v2.1_b200/build_native.py [--force] [-v]
 """
@@ -21,6 +23,8 @@ REPO = os.path.dirname(HERE)
 CSRC = os.path.join(HERE, "csrc")
 INCLUDE = os.path.join(REPO, "include")
 LIB = os.path.join(HERE, "hspmn_b200", "libhspmn_sm100.so")
+TORCH_LIB = os.path.join(HERE, "hspmn_b200", "libhspmn_torch.so")
+TORCH_SOURCE = os.path.join(CSRC, "torch_ops.cpp")
 
 NVCC_FLAGS = [
     "-gencode", "arch=compute_100a,code=sm_100a",
@@ -43,28 +47,47 @@ def sources():
                   + glob.glob(os.path.join(INCLUDE, "*.h")))
 
 
-def up_to_date() -> bool:
-    if not os.path.exists(LIB):
+def up_to_date(lib: str = LIB, made_from=None) -> bool:
+    if not os.path.exists(lib):
         return False
-    t = os.path.getmtime(LIB)
-    return all(os.path.getmtime(s) <= t for s in sources())
+    t = os.path.getmtime(lib)
+    return all(os.path.getmtime(s) <= t for s in (made_from or sources()))
 
 
-def build(force: bool = False, verbose: bool = False) -> str:
-    if not force and up_to_date():
-        return LIB
-    out = LIB
-    cmd = [nvcc(), *NVCC_FLAGS, "-I", INCLUDE, "-I", CSRC,
-           os.path.join(CSRC, "hspmn_sm100.cu"), "-o", out + ".tmp"]
-    if verbose:
-        cmd.insert(1, "-Xptxas=-v")
+def run(cmd, out: str, verbose: bool) -> None:
     r = subprocess.run(cmd, capture_output=True, text=True)
     if r.returncode != 0:
-        raise RuntimeError("nvcc failed:\n" + " ".join(cmd) + "\n" + r.stdout + r.stderr)
+        raise RuntimeError(f"{os.path.basename(cmd[0])} failed:\n" + " ".join(cmd) + "\n" + r.stdout + r.stderr)
     if verbose:
         sys.stderr.write(r.stdout + r.stderr)
     os.replace(out + ".tmp", out)
-    return out
+
+
+def build_torch_ops(force: bool = False, verbose: bool = False) -> str:
+    header = os.path.join(INCLUDE, "hspmn_sm100.h")
+    if not force and up_to_date(TORCH_LIB, [TORCH_SOURCE, header]):
+        return TORCH_LIB
+    import torch
+    from torch.utils.cpp_extension import include_paths, library_paths
+    cuda_include = os.path.join(os.path.dirname(os.path.dirname(os.path.realpath(nvcc()))), "include")
+    cmd = [os.environ.get("CXX", "g++"), "-O2", "-std=c++17", "-fPIC", "-shared", "-fvisibility=hidden",
+           f"-D_GLIBCXX_USE_CXX11_ABI={int(torch._C._GLIBCXX_USE_CXX11_ABI)}",
+           *(f"-isystem{p}" for p in include_paths()), f"-isystem{cuda_include}", "-I", INCLUDE, TORCH_SOURCE,
+           "-o", TORCH_LIB + ".tmp", "-L", os.path.dirname(LIB), "-l:" + os.path.basename(LIB), "-Wl,-rpath,$ORIGIN",
+           *(f"-L{p}" for p in library_paths()), "-lc10", "-lc10_cuda", "-ltorch_cpu", "-ldl"]
+    run(cmd, TORCH_LIB, verbose)
+    return TORCH_LIB
+
+
+def build(force: bool = False, verbose: bool = False) -> str:
+    if force or not up_to_date():
+        cmd = [nvcc(), *NVCC_FLAGS, "-I", INCLUDE, "-I", CSRC,
+               os.path.join(CSRC, "hspmn_sm100.cu"), "-o", LIB + ".tmp"]
+        if verbose:
+            cmd.insert(1, "-Xptxas=-v")
+        run(cmd, LIB, verbose)
+    build_torch_ops(force, verbose)
+    return LIB
 
 
 if __name__ == "__main__":

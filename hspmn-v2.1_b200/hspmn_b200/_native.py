@@ -13,6 +13,7 @@ import threading
 
 LIB_NAME = "libhspmn_sm100.so"
 LIB_PATH = os.path.join(os.path.dirname(os.path.abspath(__file__)), LIB_NAME)
+TORCH_LIB_PATH = os.path.join(os.path.dirname(LIB_PATH), "libhspmn_torch.so")
 
 HSPMN_F32, HSPMN_F16, HSPMN_BF16 = 0, 1, 2
 DEVERR_POSITION, DEVERR_UNSORTED, DEVERR_TIMEOUT, DEVERR_PAGE = 1, 2, 4, 8
@@ -90,6 +91,22 @@ def lib() -> ctypes.CDLL:
                 fn.argtypes = args
             _lib = handle
     return _lib
+
+
+def torch_ops_available() -> bool:
+    return os.path.exists(TORCH_LIB_PATH) and available()
+
+
+def load_torch_ops() -> None:
+    """Register the C++ operators of libhspmn_torch.so with PyTorch; raise if it
+    is not built. (Loading a library again does nothing.)"""
+    if not torch_ops_available():
+        raise RuntimeError(
+            f"{os.path.basename(TORCH_LIB_PATH)} is not built (expected at {TORCH_LIB_PATH}); run "
+            "`python hspmn-v2.1_b200/build_native.py` on a machine with the CUDA toolkit")
+    import torch
+    lib()
+    torch.ops.load_library(TORCH_LIB_PATH)
 
 
 def strerror(status: int) -> str:

@@ -607,53 +607,40 @@ def sqdk_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, indices: t
 # paged K/V cache
 # ---------------------------------------------------------------------------
 
-# The operators of a decode step run for microseconds, so their Python side
-# counts: they are registered through torch.library's define / impl, whose
-# dispatch costs 2 us of host time a call where a custom_op's costs 10.
-_paged_lib = torch.library.Library("hspmn", "FRAGMENT")
-_paged_lib.define("paged_slots_(Tensor(a!) block_table, Tensor seq_lens, Tensor new_lens, Tensor free_pages, "
-                  "int page_size, SymInt num_tokens) -> (Tensor, Tensor, Tensor, Tensor, Tensor)")
-_paged_lib.define("rope_paged_write_(Tensor k, Tensor v, Tensor? cos, Tensor? sin, Tensor positions, Tensor slots, "
-                  "Tensor(a!) k_cache, Tensor(b!) v_cache) -> ()")
-_paged_lib.define("sqdk_paged_fwd(Tensor q, Tensor k_cache, Tensor v_cache, Tensor block_table, Tensor kv_lens, "
-                  "Tensor cu_q, Tensor positions, float sm_scale, int max_q) -> Tensor")
+# These operators are registered from C++ (csrc/torch_ops.cpp): a decode step
+# calls them for microseconds of GPU work each, so host time per call counts.
 
 
-def _int32(name: str, what: str, t: torch.Tensor, dim: int) -> torch.Tensor:
-    if t.dtype != torch.int32 or t.dim() != dim:
-        raise ValueError(f"{name}: {what} must be a {dim}-D int32 tensor, got {t.dtype} {tuple(t.shape)}")
-    return t if t.dim() == 0 or t.stride(-1) == 1 or t.shape[-1] <= 1 else t.contiguous()
+_paged_ops = {}
 
 
-def _index64(name: str, what: str, t: torch.Tensor, n: int) -> torch.Tensor:
-    if t.dtype != torch.int64 or t.dim() != 1 or t.shape[0] != n:
-        raise ValueError(f"{name}: {what} must be int64 [{n}], got {t.dtype} {tuple(t.shape)}")
-    return t.contiguous()
+def _load_paged_ops() -> None:
+    N.load_torch_ops()
+    for name, fake in (("paged_slots_", _paged_slots_fake), ("rope_paged_write_", lambda *args: None),
+                       ("sqdk_paged_fwd", _sqdk_paged_fwd_fake)):
+        torch.library.register_fake("hspmn::" + name, fake)
+        _paged_ops[name] = getattr(torch.ops.hspmn, name).default
 
 
-def _no_grad_needed(name: str, *tensors: torch.Tensor) -> None:
-    if torch.is_grad_enabled() and any(t.requires_grad for t in tensors):
-        raise RuntimeError(f"{name}: has no backward; call it under torch.no_grad() or detach its inputs")
-
-
-def _check_caches(name: str, k_cache: torch.Tensor, v_cache: torch.Tensor, dtype: torch.dtype, heads: int,
-                  hd: int) -> None:
-    if k_cache.dim() != 4 or k_cache.shape != v_cache.shape or k_cache.shape[2] != heads or k_cache.shape[3] != hd:
-        raise ValueError(f"{name}: caches must both be [num_pages, page_size, {heads}, {hd}], got "
-                         f"{tuple(k_cache.shape)} and {tuple(v_cache.shape)}")
-    if k_cache.dtype != dtype or v_cache.dtype != dtype:
-        raise TypeError(f"{name}: the caches ({k_cache.dtype}, {v_cache.dtype}) must have the operands' dtype {dtype}")
-    if hd > 1 and (k_cache.stride(3) != 1 or v_cache.stride(3) != 1):
-        raise ValueError(f"{name}: the caches' last dimension must be contiguous (they are used in place)")
-
-
-def _rows3(t: torch.Tensor) -> torch.Tensor:
-    """[N,H,hd] operand with a contiguous head row and 16-byte strides and base; copied where it is not."""
-    es = t.element_size()
-    a, b, c = t.stride()
-    if c != 1 or a <= 0 or b <= 0 or (a * es) % 16 or (b * es) % 16 or t.data_ptr() % 16:
-        t = t.clone(memory_format=torch.contiguous_format)
-    return t
+def _call_paged(name: str, dev: torch.device, *args):
+    """One operator call; counted and, while a ``KernelTimer`` is active, timed
+    as the other launches are."""
+    if not _paged_ops:
+        _load_paged_ops()  # raises: the library was not there at import
+    op = _paged_ops[name]
+    if torch.compiler.is_compiling():
+        return op(*args)
+    try:
+        if LaunchStats.timer is not None:
+            with _launch(name.rstrip("_"), dev):
+                return op(*args)
+        out = op(*args)
+    except RuntimeError as e:
+        if " (status -" in str(e):  # a library entry point refused the call
+            raise N.HSPMNNativeError(str(e).splitlines()[0]) from None
+        raise
+    LaunchStats.launches += 1
+    return out
 
 
 def paged_slots_(block_table: torch.Tensor, seq_lens: torch.Tensor, new_lens: torch.Tensor, free_pages: torch.Tensor,
@@ -676,35 +663,8 @@ def paged_slots_(block_table: torch.Tensor, seq_lens: torch.Tensor, new_lens: to
     entries and slots are -1 and ``DEVERR_PAGE`` is set in ``device_errors()``;
     negative lengths, tokens beyond N and lengths beyond P pages set
     ``DEVERR_POSITION``. At most 8192 requests a call."""
-    return torch.ops.hspmn.paged_slots_.default(block_table, seq_lens, new_lens, free_pages, page_size, num_tokens)
-
-
-def _paged_slots_impl(block_table, seq_lens, new_lens, free_pages, page_size, num_tokens):
-    dev = _require_cuda(block_table, seq_lens, new_lens, free_pages)
-    seq_lens = _int32("paged_slots_", "seq_lens", seq_lens, 1)
-    new_lens = _int32("paged_slots_", "new_lens", new_lens, 1)
-    free_pages = _int32("paged_slots_", "free_pages", free_pages, 1)
-    if block_table.dtype != torch.int32 or block_table.dim() != 2:
-        raise ValueError("paged_slots_: block_table must be int32 [R,P]")
-    R, P = block_table.shape
-    if seq_lens.shape[0] != R or new_lens.shape[0] != R:
-        raise ValueError(f"paged_slots_: {R} table rows, {seq_lens.shape[0]} seq_lens, {new_lens.shape[0]} new_lens")
-    if (P > 1 and block_table.stride(1) != 1) or (R > 1 and block_table.stride(0) < P):
-        raise ValueError("paged_slots_: block_table is written in place: its rows must be dense and must not overlap")
-    if num_tokens < 0:
-        raise ValueError(f"paged_slots_: num_tokens={num_tokens}")
-    cu = torch.empty(R + 1, dtype=torch.int32, device=dev)
-    kv_lens = torch.empty(R, dtype=torch.int32, device=dev)
-    positions = torch.empty(num_tokens, dtype=torch.int64, device=dev)
-    slots = torch.empty(num_tokens, dtype=torch.int64, device=dev)
-    taken = torch.empty(1, dtype=torch.int32, device=dev)
-    with _on_device(dev), _launch("paged_slots", dev):
-        rc = N.lib().hspmn_paged_slots(
-            block_table.data_ptr(), max(P, block_table.stride(0)), seq_lens.data_ptr(), new_lens.data_ptr(),
-            free_pages.data_ptr(), free_pages.shape[0], R, P, page_size, num_tokens, cu.data_ptr(),
-            kv_lens.data_ptr(), positions.data_ptr(), slots.data_ptr(), taken.data_ptr(), _stream(dev))
-        N.check(rc, "hspmn_paged_slots")
-    return cu, kv_lens, positions, slots, taken
+    return _call_paged("paged_slots_", block_table.device, block_table, seq_lens, new_lens, free_pages,
+                       page_size, num_tokens)
 
 
 def _paged_slots_fake(block_table, seq_lens, new_lens, free_pages, page_size, num_tokens):
@@ -729,46 +689,7 @@ def rope_paged_write_(k: torch.Tensor, v: torch.Tensor, cos: Optional[torch.Tens
     and their sum are float32 with one rounding, where ``rope_rows`` rounds each
     of the reference's tensor operations. A slot outside the cache or a position
     outside the tables sets ``DEVERR_PAGE`` / ``DEVERR_POSITION`` and is skipped."""
-    torch.ops.hspmn.rope_paged_write_.default(k, v, cos, sin, positions, slots, k_cache, v_cache)
-
-
-def _rope_paged_write_impl(k, v, cos, sin, positions, slots, k_cache, v_cache):
-    name = "rope_paged_write_"
-    if (cos is None) != (sin is None):
-        raise ValueError(f"{name}: cos and sin must both be given or both be None")
-    dev = _require_cuda(k, v, positions, slots, k_cache, v_cache, *(() if cos is None else (cos, sin)))
-    _no_grad_needed(name, k, v, k_cache, v_cache)
-    if k.dim() != 3 or k.shape != v.shape:
-        raise ValueError(f"{name}: k and v must both be [N,Hkv,hd], got {tuple(k.shape)} and {tuple(v.shape)}")
-    n, heads, hd = k.shape
-    if v.dtype != k.dtype:
-        raise TypeError(f"{name}: k ({k.dtype}) and v ({v.dtype}) must share one dtype")
-    code = dtype_code(k.dtype)
-    _check_caches(name, k_cache, v_cache, k.dtype, heads, hd)
-    positions, slots = _index64(name, "positions", positions, n), _index64(name, "slots", slots, n)
-    cos_ptr = sin_ptr = tab_ss = tab_rows = 0
-    tab_code = code
-    if cos is not None:
-        if cos.dtype != sin.dtype or cos.dtype not in (k.dtype, torch.float32):
-            raise TypeError(f"{name}: cos/sin must both have k's dtype or float32")
-        if cos.shape[-1] != hd or cos.shape != sin.shape:
-            raise ValueError(f"{name}: cos/sin must both be [L,{hd}], got {tuple(cos.shape)} and {tuple(sin.shape)}")
-        cos, sin = cos.reshape(-1, hd), sin.reshape(-1, hd)
-        if cos.stride(1) != 1 or sin.stride(1) != 1 or cos.stride(0) != sin.stride(0) or cos.stride(0) < hd:
-            cos, sin = cos.contiguous(), sin.contiguous()
-        cos_ptr, sin_ptr, tab_ss, tab_rows = cos.data_ptr(), sin.data_ptr(), cos.stride(0), cos.shape[0]
-        tab_code = dtype_code(cos.dtype)
-    if n == 0:
-        return
-    k, v = _rows3(k), _rows3(v)
-    kc, vc = k_cache.stride(), v_cache.stride()
-    with _on_device(dev), _launch("rope_paged_write", dev):
-        rc = N.lib().hspmn_rope_paged_write(
-            k.data_ptr(), k.stride(0), k.stride(1), v.data_ptr(), v.stride(0), v.stride(1), cos_ptr, sin_ptr, tab_ss,
-            tab_rows, tab_code, positions.data_ptr(), slots.data_ptr(), k_cache.data_ptr(), kc[0], kc[1], kc[2],
-            v_cache.data_ptr(), vc[0], vc[1], vc[2], n, heads, hd, k_cache.shape[0], k_cache.shape[1], code,
-            _stream(dev))
-        N.check(rc, "hspmn_rope_paged_write")
+    _call_paged("rope_paged_write_", k.device, k, v, cos, sin, positions, slots, k_cache, v_cache)
 
 
 def sqdk_paged_fwd(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tensor, block_table: torch.Tensor,
@@ -789,64 +710,16 @@ def sqdk_paged_fwd(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tensor
     behind ``cu_q[R]`` are zeros. A position beyond kv_lens sets
     ``DEVERR_POSITION``, a page outside the cache ``DEVERR_PAGE`` (its keys are
     left out) in ``device_errors()``. No backward."""
-    return torch.ops.hspmn.sqdk_paged_fwd.default(q, k_cache, v_cache, block_table, kv_lens, cu_q, positions, sm_scale,
-                                                  max_q)
-
-
-def _sqdk_paged_fwd_impl(q, k_cache, v_cache, block_table, kv_lens, cu_q, positions, sm_scale, max_q=0):
-    name = "sqdk_paged_fwd"
-    dev = _require_cuda(q, k_cache, v_cache, block_table, kv_lens, cu_q, positions)
-    _no_grad_needed(name, q, k_cache, v_cache)
-    if q.dim() != 3:
-        raise ValueError(f"{name}: q must be [N,H,hd], got {tuple(q.shape)}")
-    n, H, hd = q.shape
-    if q.dtype not in (torch.bfloat16, torch.float16):
-        raise TypeError(f"{name}: q dtype {q.dtype} unsupported (bf16 or f16)")
-    if k_cache.dim() != 4:
-        raise ValueError(f"{name}: caches must be [num_pages, page_size, Hkv, hd], got {tuple(k_cache.shape)}")
-    Hkv = k_cache.shape[2]
-    _check_caches(name, k_cache, v_cache, q.dtype, Hkv, hd)
-    if Hkv == 0 or H % Hkv != 0:
-        raise ValueError(f"{name}: num_heads {H} is not a multiple of num_kv_heads {Hkv}")
-    block_table = _int32(name, "block_table", block_table, 2)
-    kv_lens, cu_q = _int32(name, "kv_lens", kv_lens, 1), _int32(name, "cu_q", cu_q, 1)
-    R, P = block_table.shape
-    if kv_lens.shape[0] != R or cu_q.shape[0] != R + 1:
-        raise ValueError(f"{name}: {R} table rows need kv_lens [{R}] and cu_q [{R + 1}], got {kv_lens.shape[0]} and "
-                         f"{cu_q.shape[0]}")
-    if R > 1 and block_table.stride(0) < P:
-        block_table = block_table.contiguous()
-    positions = _index64(name, "positions", positions, n)
-    q = _rows3(q)
-    o = torch.empty((n, H, hd), dtype=q.dtype, device=dev)
-    if n == 0:
-        return o
-    kc, vc = k_cache.stride(), v_cache.stride()
-    with _on_device(dev), _launch("sqdk_paged_fwd", dev):
-        lib = N.lib()
-        ws_bytes = lib.hspmn_sqdk_paged_workspace_size(n, H, Hkv, hd, max_q)
-        if ws_bytes < 0:
-            raise N.HSPMNNativeError("hspmn_sqdk_paged_workspace_size: device query failed")
-        ws = torch.empty(ws_bytes, dtype=torch.uint8, device=dev)
-        rc = lib.hspmn_sqdk_paged_fwd(
-            q.data_ptr(), q.stride(0), q.stride(1), k_cache.data_ptr(), kc[0], kc[1], kc[2], v_cache.data_ptr(), vc[0],
-            vc[1], vc[2], block_table.data_ptr(), max(P, block_table.stride(0)), kv_lens.data_ptr(), cu_q.data_ptr(),
-            positions.data_ptr(), o.data_ptr(), H * hd, hd, n, R, P, k_cache.shape[0], k_cache.shape[1], H, Hkv, hd,
-            N.HSPMN_BF16 if q.dtype == torch.bfloat16 else N.HSPMN_F16, sm_scale, max_q, ws.data_ptr(), ws_bytes,
-            _stream(dev))
-        N.check(rc, "hspmn_sqdk_paged_fwd")
-    return o
+    return _call_paged("sqdk_paged_fwd", q.device, q, k_cache, v_cache, block_table, kv_lens, cu_q,
+                       positions, sm_scale, max_q)
 
 
 def _sqdk_paged_fwd_fake(q, k_cache, v_cache, block_table, kv_lens, cu_q, positions, sm_scale, max_q=0):
     return torch.empty_like(q, memory_format=torch.contiguous_format)
 
 
-for _name, _impl, _fake in (("paged_slots_", _paged_slots_impl, _paged_slots_fake),
-                            ("rope_paged_write_", _rope_paged_write_impl, lambda *args: None),
-                            ("sqdk_paged_fwd", _sqdk_paged_fwd_impl, _sqdk_paged_fwd_fake)):
-    _paged_lib.impl(_name, _impl, "CompositeExplicitAutograd")
-    torch.library.register_fake("hspmn::" + _name, _fake, lib=_paged_lib)
+if N.torch_ops_available():
+    _load_paged_ops()
 
 
 def device_errors(device: Optional[torch.device] = None, clear: bool = True) -> int:
