@@ -355,6 +355,16 @@ __host__ __device__ constexpr uint32_t umma_idesc_f16(int M, int N, int ab, bool
 }
 
 // ---------------------------------------------------------------------------
+// dependent launches
+// ---------------------------------------------------------------------------
+
+// The next kernel of the stream, if launched as a programmatic dependent, may
+// begin; it waits for this grid's results with grid_dependency_wait().
+__device__ __forceinline__ void grid_dependents_launch() { asm volatile("griddepcontrol.launch_dependents;" ::: "memory"); }
+// Waits until the grid before this one has finished and its writes are visible.
+__device__ __forceinline__ void grid_dependency_wait() { asm volatile("griddepcontrol.wait;" ::: "memory"); }
+
+// ---------------------------------------------------------------------------
 // small math
 // ---------------------------------------------------------------------------
 

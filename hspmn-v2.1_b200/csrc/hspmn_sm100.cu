@@ -803,6 +803,23 @@ void launch_paged_write(const PagedWriteParams& prm, bool f32_tables, unsigned g
   else rope_paged_write_kernel<T, T><<<grid, kRowThreads, 0, st>>>(prm);
 }
 
+// Launches kern as a programmatic dependent of the kernel before it in the
+// stream: its launch overlaps that kernel's end (it must wait for the results
+// itself, with grid_dependency_wait).
+template <typename Params>
+int launch_dependent(void (*kern)(Params), unsigned grid, unsigned threads, const Params& prm, cudaStream_t st) {
+  cudaLaunchConfig_t cfg = {};
+  cfg.gridDim = dim3(grid);
+  cfg.blockDim = dim3(threads);
+  cfg.stream = st;
+  cudaLaunchAttribute attr[1];
+  attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  attr[0].val.programmaticStreamSerializationAllowed = 1;
+  cfg.attrs = attr;
+  cfg.numAttrs = 1;
+  return cudaLaunchKernelEx(&cfg, kern, prm) == cudaSuccess ? HSPMN_OK : HSPMN_ERR_CUDA;
+}
+
 template <int HD, bool kBF16>
 int launch_paged_attn(const PagedAttnParams& prm, int runs, cudaStream_t st) {
   auto kern = paged_attn_kernel<HD, kBF16>;
@@ -811,8 +828,7 @@ int launch_paged_attn(const PagedAttnParams& prm, int runs, cudaStream_t st) {
     return HSPMN_ERR_CUDA;
   kern<<<static_cast<unsigned>(runs), kPagedThreads, smem, st>>>(prm);
   if (int rc = launch_status()) return rc;
-  if (runs > 1) paged_merge_kernel<HD, kBF16><<<static_cast<unsigned>(runs - 1), 32 * kMergeWarps, 0, st>>>(prm, runs);
-  return launch_status();
+  return launch_dependent(paged_merge_kernel<HD, kBF16>, static_cast<unsigned>(runs), 32 * kMergeWarps, prm, st);
 }
 
 // Rows (queries * G) of a request up to which its tiles are the 16-row kernel's.
@@ -823,8 +839,15 @@ bool paged_has_chunks(int64_t N, int64_t G, int64_t max_q) {
   return (max_q > 0 ? std::min(max_q, N) : N) * G > kPagedSplitRows;
 }
 
-int64_t paged_part_rows(int sms) { return 2LL * sms * kPagedCtasPerSm * kPagedRows; }
-int64_t chunk_part_rows(int sms) { return 2LL * sms * kChunkCtasPerSm * kSqdkBM; }
+// Workspace of one of the two kernels: two pieces a run (O, maximum and sum of
+// each row), and a note a run for the merge.
+int64_t paged_ws_bytes(int64_t runs, int rows, int64_t hdp) { return runs * (2 * rows * (hdp + 2) * 4 + 16); }
+
+void paged_ws_carve(PagedAttnParams* prm, void* ws, int64_t runs, int rows, int64_t hdp) {
+  prm->part_o = static_cast<float*>(ws);
+  prm->part_ml = prm->part_o + 2 * runs * rows * hdp;
+  prm->merges = reinterpret_cast<int4*>(prm->part_ml + 2 * runs * rows * 2);
+}
 
 template <int HD, bool kBF16>
 int launch_paged_chunk(const CUtensorMap& mq, const CUtensorMap& mk, const CUtensorMap& mv, const ChunkParams& prm,
@@ -835,8 +858,8 @@ int launch_paged_chunk(const CUtensorMap& mq, const CUtensorMap& mk, const CUten
     return HSPMN_ERR_CUDA;
   kern<<<static_cast<unsigned>(runs), kChunkThreads, L::kAlloc, st>>>(mq, mk, mv, prm);
   if (int rc = launch_status()) return rc;
-  paged_chunk_merge_kernel<HD, kBF16><<<static_cast<unsigned>(runs - 1), 32 * kChunkMergeWarps, 0, st>>>(prm, runs);
-  return launch_status();
+  return launch_dependent(paged_chunk_merge_kernel<HD, kBF16>, static_cast<unsigned>(runs), 32 * kChunkMergeWarps, prm,
+                          st);
 }
 
 }  // namespace
@@ -946,8 +969,11 @@ int64_t hspmn_sqdk_paged_workspace_size(int64_t N, int64_t H, int64_t Hkv, int64
   if (N < 1 || H < 1 || Hkv < 1 || hd < 1 || max_q < 0) return 0;
   int sms = 0;
   if (sm_count(&sms) != HSPMN_OK) return -1;
-  const int64_t rows = paged_part_rows(sms) + (paged_has_chunks(N, H / Hkv, max_q) ? chunk_part_rows(sms) : 0);
-  return rows * ((hd > 64 ? 128 : 64) + 2) * 4;
+  const int64_t hdp = hd > 64 ? 128 : 64;
+  int64_t bytes = paged_ws_bytes(static_cast<int64_t>(sms) * kPagedCtasPerSm, kPagedRows, hdp);
+  if (paged_has_chunks(N, H / Hkv, max_q))
+    bytes += paged_ws_bytes(static_cast<int64_t>(sms) * kChunkCtasPerSm, kSqdkBM, hdp);
+  return bytes;
 }
 
 int hspmn_sqdk_paged_fwd(const void* q, int64_t q_sn, int64_t q_sh, const void* k_cache, int64_t kc_sp, int64_t kc_ss,
@@ -998,9 +1024,8 @@ int hspmn_sqdk_paged_fwd(const void* q, int64_t q_sn, int64_t q_sh, const void* 
   prm.kv_lens = kv_lens;
   prm.cu_q = cu_q;
   prm.pos = positions;
-  prm.part_o = static_cast<float*>(workspace);
   const int64_t hdp = hd > 64 ? 128 : 64;
-  prm.part_ml = prm.part_o + paged_part_rows(sms) * hdp;
+  paged_ws_carve(&prm, workspace, runs, kPagedRows, hdp);
   prm.N = N;
   prm.R = static_cast<int>(R);
   prm.P = static_cast<int>(P);
@@ -1019,8 +1044,8 @@ int hspmn_sqdk_paged_fwd(const void* q, int64_t q_sn, int64_t q_sh, const void* 
     prm.split_rows = kPagedSplitRows;
     ChunkParams ch;
     ch.a = prm;
-    ch.a.part_o = prm.part_ml + paged_part_rows(sms) * 2;
-    ch.a.part_ml = ch.a.part_o + chunk_part_rows(sms) * hdp;
+    const int chunk_runs = sms * kChunkCtasPerSm;
+    paged_ws_carve(&ch.a, static_cast<char*>(workspace) + paged_ws_bytes(runs, kPagedRows, hdp), chunk_runs, kSqdkBM, hdp);
     ch.QT = kSqdkBM / prm.G;
     ch.box_rows = static_cast<int>(std::min<int64_t>(page_size, kSqdkBN));
     const CUtensorMapDataType dt =
@@ -1040,7 +1065,6 @@ int hspmn_sqdk_paged_fwd(const void* q, int64_t q_sn, int64_t q_sh, const void* 
     const uint32_t kb[4] = {64u, 1u, static_cast<uint32_t>(ch.box_rows), 1u};
     if (int rc = encode_4d(&mk, k_cache, dt, kd, ks, kb)) return rc;
     if (int rc = encode_4d(&mv, v_cache, dt, kd, vs, kb)) return rc;
-    const int chunk_runs = sms * kChunkCtasPerSm;
     int rc;
     if (hd > 64)
       rc = dtype == HSPMN_BF16 ? launch_paged_chunk<128, true>(mq, mk, mv, ch, chunk_runs, st)

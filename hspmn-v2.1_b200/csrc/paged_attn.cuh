@@ -50,6 +50,7 @@ struct PagedAttnParams {
   const int64_t* pos;
   float* part_o;   // [2 * runs][16][HD] unnormalised O
   float* part_ml;  // [2 * runs][16][2] maximum (log2 units), row sum
+  int4* merges;    // [runs] what is to be merged from this run on; .w < 0: nothing
   int64_t N;
   int R, P, num_pages, shift, H, Hkv, G, hd;
   int split_rows;  // requests with more rows (queries * G) than this are not this kernel's
@@ -250,9 +251,13 @@ __global__ void __launch_bounds__(kPagedThreads, kPagedCtasPerSm) paged_attn_ker
   __shared__ float s_m[kPagedWarps][kPagedRows], s_l[kPagedWarps][kPagedRows];
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   const int g = lane >> 2, t2 = (lane & 3) * 2;  // accumulator row and first column of this lane
+  grid_dependents_launch();
   const int64_t total = paged_total(p, lane);
   const int64_t runs = min(static_cast<int64_t>(gridDim.x), total);
-  if (blockIdx.x >= runs) return;
+  if (blockIdx.x >= runs) {
+    if (threadIdx.x == 0) p.merges[blockIdx.x] = make_int4(0, 0, 0, -1);
+    return;
+  }
   const int64_t u0 = run_start(total, runs, blockIdx.x), u1 = run_start(total, runs, blockIdx.x + 1);
   int64_t before;
   const int r0 = paged_locate(p, u0, lane, before);
@@ -494,9 +499,19 @@ __global__ void __launch_bounds__(kPagedThreads, kPagedCtasPerSm) paged_attn_ker
         l += __shfl_xor_sync(0xFFFFFFFFu, l, 2);
         if ((lane & 3) == 0) s_m[warp][g + 8 * i] = m_run[i], s_l[warp][g + 8 * i] = seen[i] ? l : kUnseen;
       }
+      if (u + 1 == u1 && threadIdx.x == 0) {
+        // an item that opens in this run and goes on behind it is merged from here
+        const int64_t open = u - cur.j;
+        const bool first = !item_end && open >= u0;
+        p.merges[blockIdx.x] =
+            make_int4(cur.req.q0, cur.tile * kPagedRows,
+                      cur.head * kPagedRows + min(kPagedRows, cur.req.rows - cur.tile * kPagedRows) - 1,
+                      first ? run_of(total, runs, open + cur.req.nb - 1) : -1);
+      }
       __syncthreads();
       const bool whole = item_end && seg0 + cur.req.nb == u + 1;
-      const int64_t slot = 2 * static_cast<int64_t>(blockIdx.x) + (seg0 == u0 ? 0 : 1);
+      // a run holds the last piece of one item at most, and the first of one
+      const int64_t slot = 2 * static_cast<int64_t>(blockIdx.x) + (u - cur.j >= u0 ? 1 : 0);
       constexpr int kQuads = HD / 4;  // 4-column groups of a row
       for (int i = threadIdx.x; i < kPagedRows * kQuads; i += kPagedThreads) {
         const int lr = i / kQuads, c = (i % kQuads) * 4;
@@ -550,86 +565,70 @@ __global__ void __launch_bounds__(kPagedThreads, kPagedCtasPerSm) paged_attn_ker
 
 constexpr int kMergeWarps = 16;
 
-// Adds the partial results of the item that the end of run blockIdx.x divides,
-// if this is the first run of that item: O = sum 2^(m_s - M) O_s / sum 2^(m_s - M) l_s
-// over the runs in order. A warp takes one row and a share of the runs.
+// Adds the partial results of the item that opens in run blockIdx.x and goes on
+// behind it, as that run noted: O = sum 2^(m_c - M) O_c / sum 2^(m_c - M) l_c over
+// the runs in order. A warp takes one row and a share of the runs.
 template <int HD, bool kBF16>
-__global__ void __launch_bounds__(32 * kMergeWarps) paged_merge_kernel(const PagedAttnParams p, int most_runs) {
+__global__ void __launch_bounds__(32 * kMergeWarps) paged_merge_kernel(const __grid_constant__ PagedAttnParams p) {
   __shared__ float4 s_o[kMergeWarps][HD / 4];
   __shared__ float2 s_ml[kMergeWarps];
+  grid_dependency_wait();
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-  const int64_t total = paged_total(p, lane);
-  const int64_t runs = min(static_cast<int64_t>(most_runs), total);
-  if (blockIdx.x + 1 >= runs) return;
-  const int64_t cut = run_start(total, runs, blockIdx.x + 1);
-  int64_t before;
-  const int r = paged_locate(p, cut, lane, before);
-  PagedCursor cur;
-  cur.set(p, r, cut - before);
-  const int64_t a = cut - cur.j, b = a + cur.req.nb;  // the item's units
-  if (cur.j == 0 || run_of(total, runs, a) != static_cast<int>(blockIdx.x)) return;
-  const int c0 = static_cast<int>(blockIdx.x), c1 = run_of(total, runs, b - 1);
-  const int rows = min(kPagedRows, cur.req.rows - cur.tile * kPagedRows);
+  const int4 note = p.merges[blockIdx.x];
+  const int c0 = static_cast<int>(blockIdx.x), c1 = note.w;
+  if (c1 < 0) return;
+  const int rows = note.z % kPagedRows + 1, head = note.z / kPagedRows;
   const int shares = max(1, kMergeWarps / rows);  // warps of a row
+  const int lr = warp / shares, part = warp % shares;
+  const bool live = lr < rows;
   const float2* ml = reinterpret_cast<const float2*>(p.part_ml);
-  for (int row0 = 0; row0 < rows; row0 += kMergeWarps / shares) {
-    const int lr = row0 + warp / shares, part = warp % shares;
-    const bool live = lr < rows && warp / shares < kMergeWarps / shares;
-    float M = -INFINITY, l = 0.0f;
-    bool none = true;
-    float4 o = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
-    if (live) {
-      // run c's part of the item is its first piece unless the item opens inside it
-      auto slot_of = [&](int c) { return (2 * static_cast<int64_t>(c) + (run_start(total, runs, c) < a ? 1 : 0)) * kPagedRows + lr; };
-      const int n = c1 - c0 + 1, per = (n + shares - 1) / shares;
-      const int lo = c0 + part * per, hi = min(c1 + 1, lo + per);
-      for (int c = lo + lane; c < hi; c += 32) M = fmaxf(M, ml[slot_of(c)].x);
-#pragma unroll
-      for (int d = 16; d > 0; d >>= 1) M = fmaxf(M, __shfl_xor_sync(0xFFFFFFFFu, M, d));
+  float M = -INFINITY, l = 0.0f;
+  bool none = true;
+  float4 o = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+  if (live) {
+    const int per = (c1 - c0 + shares) / shares, lo = c0 + part * per, hi = min(c1 + 1, lo + per);
 #pragma unroll 4
-      for (int c = lo; c < hi; ++c) {
-        const int64_t s = slot_of(c);
-        const float2 x = ml[s];
-        if (x.y == kUnseen) continue;
-        none = false;
-        const float f = x.x == M ? 1.0f : fast_exp2(x.x - M);
-        l += f * x.y;
-        if (lane * 4 < p.hd && lane < HD / 4) {
-          const float4 v = *reinterpret_cast<const float4*>(p.part_o + s * HD + lane * 4);
-          o.x += f * v.x, o.y += f * v.y, o.z += f * v.z, o.w += f * v.w;
-        }
-      }
+    for (int c = lo; c < hi; ++c) {
+      // run c0's piece is its last, the others' their first
+      const int64_t s = (2 * static_cast<int64_t>(c) + (c == c0 ? 1 : 0)) * kPagedRows + lr;
+      const float2 x = ml[s];
+      const float4 v = lane < HD / 4 ? *reinterpret_cast<const float4*>(p.part_o + s * HD + lane * 4)
+                                     : make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+      if (x.y == kUnseen) continue;
+      none = false;
+      const float top = fmaxf(M, x.x);
+      const float f = x.x == top ? 1.0f : fast_exp2(x.x - top), g = M == top ? 1.0f : fast_exp2(M - top);
+      M = top;
+      l = g * l + f * x.y;
+      o.x = g * o.x + f * v.x, o.y = g * o.y + f * v.y, o.z = g * o.z + f * v.z, o.w = g * o.w + f * v.w;
     }
-    if (lane < HD / 4) s_o[warp][lane] = o;
-    if (lane == 0) s_ml[warp] = make_float2(M, none ? kUnseen : l);
-    __syncthreads();
-    if (live && part == 0) {
-      float top = -INFINITY;
-      for (int w = 0; w < shares; ++w) top = fmaxf(top, s_ml[warp + w].x);
-      float sum = 0.0f;
-      bool empty = true;
-      float4 y = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
-      for (int w = 0; w < shares; ++w) {
-        const float2 x = s_ml[warp + w];
-        if (x.y == kUnseen) continue;
-        empty = false;
-        const float f = x.x == top ? 1.0f : fast_exp2(x.x - top);
-        sum += f * x.y;
-        if (lane < HD / 4) {
-          const float4 v = s_o[warp + w][lane];
-          y.x += f * v.x, y.y += f * v.y, y.z += f * v.z, y.w += f * v.w;
-        }
-      }
-      const int row = cur.tile * kPagedRows + lr;
-      const float inv = 1.0f / sum;
-      if (lane * 4 < p.hd && lane < HD / 4) {
-        uint2 w;
-        w.x = empty ? 0u : pack2<kBF16>(y.x * inv, y.y * inv);
-        w.y = empty ? 0u : pack2<kBF16>(y.z * inv, y.w * inv);
-        *reinterpret_cast<uint2*>(p.o + paged_row(cur.req.q0, row, cur.head, p.G, p.o_sn, p.o_sh) + lane * 8) = w;
-      }
+  }
+  if (lane < HD / 4) s_o[warp][lane] = o;
+  if (lane == 0) s_ml[warp] = make_float2(M, none ? kUnseen : l);
+  __syncthreads();
+  if (!live || part != 0) return;
+  float top = -INFINITY, sum = 0.0f;
+  bool empty = true;
+  for (int w = warp; w < warp + shares; ++w)
+    if (s_ml[w].y != kUnseen) top = fmaxf(top, s_ml[w].x);
+  float4 y = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+  for (int w = warp; w < warp + shares; ++w) {
+    const float2 x = s_ml[w];
+    if (x.y == kUnseen) continue;
+    empty = false;
+    const float f = x.x == top ? 1.0f : fast_exp2(x.x - top);
+    sum += f * x.y;
+    if (lane < HD / 4) {
+      const float4 v = s_o[w][lane];
+      y.x += f * v.x, y.y += f * v.y, y.z += f * v.z, y.w += f * v.w;
     }
-    __syncthreads();
+  }
+  const float inv = 1.0f / sum;
+  if (lane * 4 < p.hd && lane < HD / 4) {
+    uint2 w;
+    w.x = empty ? 0u : pack2<kBF16>(y.x * inv, y.y * inv);
+    w.y = empty ? 0u : pack2<kBF16>(y.z * inv, y.w * inv);
+    *reinterpret_cast<uint2*>(p.o + paged_row(note.x, note.y + lr, head, p.G, p.o_sn, p.o_sh) + lane * 8) = w;
   }
 }
 

@@ -59,6 +59,17 @@ struct ChunkParams {
   int QT, box_rows;
 };
 
+// One piece of work as the producer posts it to the other warps.
+struct ChunkJob {
+  int row0, queries;  // first query row of q, queries of the tile
+  int r, head, kv;
+  int lo, hi;      // smallest and largest last key that the tile's rows see, over rows that see any
+  int j0, nblk;    // key blocks; nblk -1: no more work
+  int slot;        // workspace slot, or -1 for a tile done whole
+  int holes;       // some page of these blocks does not exist
+  int lim[kSqdkBM];  // last key each query sees, -1 for none
+};
+
 // A request's tiles. Costs are linear in the tile number: first + t * slope.
 struct ChunkRequest {
   int q0, len, kv, tiles;
@@ -160,73 +171,42 @@ __device__ __forceinline__ ChunkTile chunk_locate(const ChunkParams& p, int64_t 
   return c;
 }
 
-// Where run c begins: an equal share of the list, moved to the nearer end of its
-// tile when that is so close that the piece would not be worth its merge.
-__device__ __forceinline__ int64_t chunk_cut(const ChunkParams& p, int64_t total, int64_t runs, int64_t c, int lane,
-                                             ChunkTile& tile) {
+// How near to an end of its tile a cut is moved to that end: the piece would not
+// be worth its merge.
+__device__ __forceinline__ int64_t chunk_near(int64_t total, int64_t runs) {
+  return min(total / runs / 16, static_cast<int64_t>(8 * kChunkUnit));
+}
+
+// Where run c begins: an equal share of the list, or the near end of its tile.
+__device__ __forceinline__ int64_t chunk_cut(const ChunkParams& p, int64_t total, int64_t runs, int64_t c, int lane) {
   if (c >= runs) return total;
   const int64_t w = run_start(total, runs, c);
-  tile = chunk_locate(p, w, lane);
-  const int64_t near = min(total / runs / 16, static_cast<int64_t>(8 * kChunkUnit));
+  const ChunkTile tile = chunk_locate(p, w, lane);
+  const int64_t near = chunk_near(total, runs);
   if (w - tile.start <= near) return tile.start;
   if (tile.start + tile.cost - w <= near) return tile.start + tile.cost;
   return w;
 }
 
-// Key block at list place w of a tile with nblk blocks.
-__device__ __forceinline__ int chunk_block_at(const ChunkTile& c, int64_t w, int nblk) {
-  const int64_t x = min(max(w - c.start, static_cast<int64_t>(0)), c.cost);
-  return static_cast<int>(x * nblk / c.cost);
-}
-
-// The largest and smallest last key that the tile's rows see, over the rows
-// that see any (the whole warp; max -1 where none does).
-__device__ __forceinline__ void chunk_limits(const ChunkParams& p, const ChunkTile& c, int lane, int& lo, int& hi) {
-  lo = 0x7FFFFFFF;
-  hi = -1;
-  const int n = min(p.QT, c.req.len - c.t * p.QT);
-  for (int i = lane; i < n; i += 32) {
-    const int64_t ps = __ldg(p.a.pos + c.req.q0 + c.t * p.QT + i);
-    const int lim = static_cast<int>(min(max(ps, static_cast<int64_t>(-1)), static_cast<int64_t>(c.req.kv) - 1));
-    if (lim >= 0) lo = min(lo, lim);
-    hi = max(hi, lim);
-  }
-  lo = __reduce_min_sync(0xFFFFFFFFu, lo);
-  hi = __reduce_max_sync(0xFFFFFFFFu, hi);
-}
-
-// One piece of work of a CTA.
-struct ChunkSegment {
-  ChunkTile tile;
-  int lo, hi;    // limits of the tile's rows
-  int j0, nblk;  // its key blocks
-  int slot;      // workspace slot, or -1 for a tile done whole
-};
-
-// Walks a run's segments: the whole tiles in order, then the piece at the run's
-// start, then the one at its end. Every warp of the CTA walks the same ones.
+// Walks a run's pieces: the whole tiles in order, then the piece at the run's
+// start, then the one at its end.
 struct ChunkWalk {
   ChunkTile first, cur;
   int64_t w0, w1;
   int stage;  // 0: whole tiles, 1: piece at the start, 2: piece at the end, 3: done
   bool started;
   __device__ __forceinline__ void open(const ChunkParams& p, int64_t total, int64_t runs, int64_t c, int lane) {
-    ChunkTile t;
-    w0 = chunk_cut(p, total, runs, c, lane, t);
-    w1 = chunk_cut(p, total, runs, c + 1, lane, t);
     stage = 3;
     started = false;
+    if (c >= runs || total == 0) return;
+    w0 = chunk_cut(p, total, runs, c, lane);
+    w1 = chunk_cut(p, total, runs, c + 1, lane);
     if (w0 >= w1) return;
     first = cur = chunk_locate(p, w0, lane);
     stage = 0;
   }
-  __device__ __forceinline__ void cover(const ChunkParams& p, ChunkSegment& s, int64_t a, int64_t b, int lane) {
-    chunk_limits(p, s.tile, lane, s.lo, s.hi);
-    const int all = s.hi < 0 ? 0 : s.hi / kSqdkBN + 1;
-    s.j0 = chunk_block_at(s.tile, a, all);
-    s.nblk = chunk_block_at(s.tile, b, all) - s.j0;
-  }
-  __device__ __forceinline__ bool next(const ChunkParams& p, ChunkSegment& s, int lane) {
+  // The next piece's tile; slot and merge say what it is.
+  __device__ __forceinline__ bool next(const ChunkParams& p, ChunkTile& tile, int& slot) {
     while (stage == 0) {
       if (started) {
         if (cur.start + cur.cost >= w1) {
@@ -241,18 +221,16 @@ struct ChunkWalk {
         stage = 1;
         break;
       }
-      s.tile = cur;
-      cover(p, s, cur.start, cur.start + cur.cost, lane);
-      s.slot = -1;
+      tile = cur;
+      slot = -1;
       return true;
     }
     // cur is the run's last tile now
     if (stage == 1) {
       stage = 2;
       if (first.start < w0) {
-        s.tile = first;
-        cover(p, s, w0, w1, lane);
-        s.slot = 2 * static_cast<int>(blockIdx.x);
+        tile = first;
+        slot = 2 * static_cast<int>(blockIdx.x);
         if (first.start + first.cost >= w1) stage = 3;  // the run lies inside one tile
         return true;
       }
@@ -260,15 +238,66 @@ struct ChunkWalk {
     if (stage == 2) {
       stage = 3;
       if (cur.start + cur.cost > w1) {
-        s.tile = cur;
-        cover(p, s, w0, w1, lane);
-        s.slot = 2 * static_cast<int>(blockIdx.x) + 1;
+        tile = cur;
+        slot = 2 * static_cast<int>(blockIdx.x) + 1;
         return true;
       }
     }
     return false;
   }
 };
+
+// Key block at list place w of a tile with nblk blocks.
+__device__ __forceinline__ int chunk_block_at(const ChunkTile& c, int64_t w, int nblk) {
+  const int64_t x = min(max(w - c.start, static_cast<int64_t>(0)), c.cost);
+  return static_cast<int>(x * nblk / c.cost);
+}
+
+// Fills in a job for list places [a, b) of a tile (the whole warp).
+__device__ __forceinline__ void chunk_job(const ChunkParams& p, const ChunkTile& c, int64_t a, int64_t b, int slot,
+                                          volatile ChunkJob& job, int lane) {
+  int lo = 0x7FFFFFFF, hi = -1;
+  const int n = min(p.QT, c.req.len - c.t * p.QT);
+  bool beyond = false;
+  for (int i = lane; i < n; i += 32) {
+    const int64_t ps = __ldg(p.a.pos + c.req.q0 + c.t * p.QT + i);
+    const int lim = static_cast<int>(min(max(ps, static_cast<int64_t>(-1)), static_cast<int64_t>(c.req.kv) - 1));
+    beyond |= ps >= c.req.kv;
+    job.lim[i] = lim;
+    if (lim >= 0) lo = min(lo, lim);
+    hi = max(hi, lim);
+  }
+  if (beyond) raise_device_error(HSPMN_DEVERR_POSITION);
+  lo = __reduce_min_sync(0xFFFFFFFFu, lo);
+  hi = __reduce_max_sync(0xFFFFFFFFu, hi);
+  const int all = hi < 0 ? 0 : hi / kSqdkBN + 1;
+  const int j0 = chunk_block_at(c, a, all), nblk = chunk_block_at(c, b, all) - j0;
+  bool holes = false;
+  if (nblk > 0) {
+    const int* row = p.a.table + static_cast<int64_t>(c.r) * p.a.table_rs;
+    const int last = (min((j0 + nblk) * kSqdkBN, c.req.kv) - 1) >> p.a.shift;
+    for (int pg = ((j0 * kSqdkBN) >> p.a.shift) + lane; pg <= last; pg += 32) {
+      const int x = __ldg(row + pg);
+      holes |= x < 0 || x >= p.a.num_pages;
+    }
+    holes = __any_sync(0xFFFFFFFFu, holes);
+    if (holes && lane == 0) raise_device_error(HSPMN_DEVERR_PAGE);
+  }
+  if (lane == 0) {
+    job.row0 = c.req.q0 + c.t * p.QT;
+    job.queries = n;
+    job.r = c.r;
+    job.head = c.head;
+    job.kv = c.req.kv;
+    job.lo = lo;
+    job.hi = hi;
+    job.j0 = j0;
+    job.nblk = nblk;
+    job.slot = slot;
+    job.holes = holes;
+  }
+  __syncwarp();
+}
 
 template <int HD, bool kBF16>
 __global__ void __launch_bounds__(kChunkThreads, kChunkCtasPerSm)
@@ -281,21 +310,17 @@ __global__ void __launch_bounds__(kChunkThreads, kChunkCtasPerSm)
   // every product and they complete in order, so bar_sfull (Q K^T of block n
   // done) also frees K stage n & 1 and, after a tile's last block, the Q tile.
   __shared__ __align__(8) uint64_t bar_q, bar_kfull[2], bar_vfull[2], bar_vempty[2], bar_sfull[2], bar_pfull[2];
-  __shared__ __align__(8) uint64_t bar_ofinal, bar_drain;
+  __shared__ __align__(8) uint64_t bar_ofinal, bar_drain, bar_job[2], bar_jobdone[2];
+  __shared__ volatile ChunkJob jobs[2];  // by the job's number: the next is posted while one is worked on
   __shared__ uint32_t tmem_base_sh;
   __shared__ volatile uint32_t abort_flag;
   // an infinity or NaN was taken out of V for rows that do not see it (by the
-  // segment's parity: one is cleared while the other is in use)
+  // job's parity: one is cleared while the other is in use)
   __shared__ volatile uint32_t wild_flag[2];
 
   const uint32_t sbase = (smem_u32(chunk_smem_raw) + 1023u) & ~1023u;
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-  const int64_t total = chunk_total(p, lane);
-  const int64_t runs = chunk_runs(total, gridDim.x);
-  if (total == 0 || blockIdx.x >= runs) return;
-  ChunkWalk walk;
-  walk.open(p, total, runs, blockIdx.x, lane);
-  if (walk.stage == 3) return;
+  grid_dependents_launch();
 
   if (threadIdx.x == 0) {
     mbar_init(&bar_q, 1);
@@ -305,6 +330,8 @@ __global__ void __launch_bounds__(kChunkThreads, kChunkCtasPerSm)
       mbar_init(&bar_vempty[s], 1);
       mbar_init(&bar_sfull[s], 1);
       mbar_init(&bar_pfull[s], 4);  // one arrival per softmax warp
+      mbar_init(&bar_job[s], 1);
+      mbar_init(&bar_jobdone[s], 5);  // the MMA warp and the softmax warps
     }
     mbar_init(&bar_ofinal, 1);
     mbar_init(&bar_drain, 1);
@@ -320,43 +347,71 @@ __global__ void __launch_bounds__(kChunkThreads, kChunkCtasPerSm)
   __syncthreads();
   tc_fence_after();
   const uint32_t tmem = tmem_base_sh;
-  ChunkSegment s;
 
   if (warp == 0) {
     // ------------------------------------------------------------ producer
     const int boxes = kSqdkBN / p.box_rows;
-    uint32_t nk = 0, nv = 0, segs = 0;
+    const int64_t total = chunk_total(p, lane);
+    const int64_t runs = chunk_runs(total, gridDim.x);
+    ChunkWalk walk;
+    walk.open(p, total, runs, blockIdx.x, lane);
+    uint32_t nk = 0, nv = 0, segs = 0, posted = 0;
     bool live = true;
-    while (live && walk.next(p, s, lane)) {
-      if (s.nblk == 0) continue;
+    int merge_to = -1;
+    ChunkTile tile;
+    int slot;
+    while (live) {
+      const bool more = walk.next(p, tile, slot);
+      volatile ChunkJob& job = jobs[posted & 1];
+      if (posted > 1 && !__all_sync(0xFFFFFFFFu, mbar_wait(&bar_jobdone[posted & 1], ((posted >> 1) - 1) & 1, &abort_flag)))
+        break;
+      if (more) {
+        chunk_job(p, tile, slot < 0 ? tile.start : walk.w0, slot < 0 ? tile.start + tile.cost : walk.w1, slot, job, lane);
+      } else if (lane == 0) {
+        job.nblk = -1;
+      }
+      if (lane == 0) mbar_arrive(&bar_job[posted & 1]);
+      ++posted;
+      __syncwarp();
+      if (!more) break;
+      if (slot >= 0 && (slot & 1)) {
+        // the first piece of its tile: its merge goes up to the last run that
+        // begins inside the tile
+        const int64_t end = tile.start + tile.cost;
+        merge_to = run_of(total, runs, end - 1);
+        if (end - run_start(total, runs, merge_to) <= chunk_near(total, runs)) --merge_to;
+        if (lane == 0)
+          p.a.merges[blockIdx.x] = make_int4(tile.req.q0 + tile.t * p.QT, min(p.QT, tile.req.len - tile.t * p.QT),
+                                             tile.head, merge_to);
+      }
+      const int nblk = job.nblk, j0 = job.j0;
+      if (nblk == 0) continue;
       if (nk > 0) live = __all_sync(0xFFFFFFFFu, mbar_wait(&bar_sfull[(nk - 1) & 1], ((nk - 1) >> 1) & 1, &abort_flag));
       if (!live) break;
       if (lane == 0) {
         mbar_arrive_expect_tx(&bar_q, static_cast<uint32_t>(L::kChunks * p.a.G * p.QT * 128));
         for (int c = 0; c < L::kChunks; ++c)
-          tma_load_4d(sbase + L::kQOff + c * L::kQChunkBytes, &tmQ, &bar_q, c * 64, s.tile.head * p.a.G,
-                      s.tile.req.q0 + s.tile.t * p.QT, 0);
+          tma_load_4d(sbase + L::kQOff + c * L::kQChunkBytes, &tmQ, &bar_q, c * 64, tile.head * p.a.G,
+                      tile.req.q0 + tile.t * p.QT, 0);
       }
       ++segs;
-      const int* row = p.a.table + static_cast<int64_t>(s.tile.r) * p.a.table_rs;
+      const int* row = p.a.table + static_cast<int64_t>(tile.r) * p.a.table_rs;
       const int mask = (1 << p.a.shift) - 1;
       // this lane's page of block j; a page that does not exist (and a box
       // behind the cached tokens) is read from behind the last page: zeros
       auto page_at = [&](int j) -> int {
-        const int key = (s.j0 + j) * kSqdkBN + lane * p.box_rows;
-        if (lane >= boxes || key >= s.tile.req.kv) return p.a.num_pages;
+        const int key = (j0 + j) * kSqdkBN + lane * p.box_rows;
+        if (lane >= boxes || key >= tile.req.kv) return p.a.num_pages;
         const int pg = __ldg(row + (key >> p.a.shift));
-        if (pg >= 0 && pg < p.a.num_pages) return pg;
-        raise_device_error(HSPMN_DEVERR_PAGE);
-        return p.a.num_pages;
+        return pg >= 0 && pg < p.a.num_pages ? pg : p.a.num_pages;
       };
       auto load = [&](const CUtensorMap* map, uint64_t* bar, uint32_t dst, int j, int page) {
         if (lane == 0) mbar_arrive_expect_tx(bar, L::kKVBytes);
         __syncwarp();
         if (lane < boxes) {
-          const int off = ((s.j0 + j) * kSqdkBN + lane * p.box_rows) & mask;
+          const int off = ((j0 + j) * kSqdkBN + lane * p.box_rows) & mask;
           for (int c = 0; c < L::kChunks; ++c)
-            tma_load_4d(dst + c * L::kKVChunkBytes + lane * p.box_rows * 128, map, bar, c * 64, s.tile.head, off, page);
+            tma_load_4d(dst + c * L::kKVChunkBytes + lane * p.box_rows * 128, map, bar, c * 64, tile.head, off, page);
         }
       };
       int page_k = page_at(0), page_v = page_k;
@@ -368,8 +423,8 @@ __global__ void __launch_bounds__(kChunkThreads, kChunkCtasPerSm)
         return true;
       };
       live = load_k(0);
-      for (int j = 0; live && j < s.nblk; ++j) {
-        if (j + 1 < s.nblk) {
+      for (int j = 0; live && j < nblk; ++j) {
+        if (j + 1 < nblk) {
           page_k = page_at(j + 1);
           live = load_k(j + 1);
           if (!live) break;
@@ -384,6 +439,7 @@ __global__ void __launch_bounds__(kChunkThreads, kChunkCtasPerSm)
         ++nv;
       }
     }
+    if (lane == 0 && merge_to < 0) p.a.merges[blockIdx.x] = make_int4(0, 0, 0, -1);
     // every copy this warp issued has landed before the CTA may exit
     if (lane == 0) {
       if (segs > 0) mbar_wait_drain(&bar_q, (segs - 1) & 1);
@@ -417,13 +473,19 @@ __global__ void __launch_bounds__(kChunkThreads, kChunkCtasPerSm)
       umma_commit_warp(&bar_vempty[sb]);
       return true;
     };
-    while (ok && walk.next(p, s, lane)) {
-      if (s.nblk == 0) continue;
+    for (uint32_t i = 0; ok; ++i) {
+      ok = __all_sync(0xFFFFFFFFu, mbar_wait(&bar_job[i & 1], (i >> 1) & 1, &abort_flag));
+      if (!ok) break;
+      const int nblk = jobs[i & 1].nblk;
+      __syncwarp();
+      if (lane == 0) mbar_arrive(&bar_jobdone[i & 1]);
+      if (nblk < 0) break;
+      if (nblk == 0) continue;
       ok = __all_sync(0xFFFFFFFFu, mbar_wait(&bar_q, segs & 1, &abort_flag));
       ++segs;
       if (!ok) break;
       tc_fence_after();
-      for (int j = 0; ok && j < s.nblk; ++j, ++n) {
+      for (int j = 0; ok && j < nblk; ++j, ++n) {
         const uint32_t sb = n & 1;
         if (!__all_sync(0xFFFFFFFFu, mbar_wait(&bar_kfull[sb], (n >> 1) & 1, &abort_flag))) {
           ok = false;
@@ -440,7 +502,7 @@ __global__ void __launch_bounds__(kChunkThreads, kChunkCtasPerSm)
         umma_commit_warp(&bar_sfull[sb]);
         if (j >= 1) ok = issue_pv(n - 1, j == 1);
       }
-      if (ok) ok = issue_pv(n - 1, s.nblk == 1);
+      if (ok) ok = issue_pv(n - 1, nblk == 1);
       if (ok) umma_commit_warp(&bar_ofinal);
     }
     umma_commit_warp(&bar_drain);
@@ -457,35 +519,23 @@ __global__ void __launch_bounds__(kChunkThreads, kChunkCtasPerSm)
     const float c2 = p.a.scale_log2;
     uint32_t n = 0, segs = 0, walked = 0;
     bool ok = true;
-    while (ok && walk.next(p, s, lane)) {
-      const ChunkTile& tile = s.tile;
-      const int qi = tile.t * p.QT + qloc;  // query row of the request
-      const bool row_valid = qloc < p.QT && qi < tile.req.len;
+    while (ok) {
+      ok = __all_sync(0xFFFFFFFFu, mbar_wait(&bar_job[walked & 1], (walked >> 1) & 1, &abort_flag));
+      if (!ok) break;
+      volatile ChunkJob& job = jobs[walked & 1];
+      const int nblk = job.nblk, j0 = job.j0;
+      if (nblk < 0) break;
+      const bool row_valid = qloc < p.QT && qloc < job.queries;
       // rows that see nothing run along like the tile's last row; what they
       // compute is not stored
-      int lim = s.hi;
-      bool blind = true;
-      if (row_valid) {
-        const int64_t ps = __ldg(p.a.pos + tile.req.q0 + qi);
-        if (ps >= tile.req.kv) raise_device_error(HSPMN_DEVERR_POSITION);
-        blind = ps < 0 || tile.req.kv == 0;
-        if (!blind) lim = static_cast<int>(min(ps, static_cast<int64_t>(tile.req.kv) - 1));
-      }
-      const int* row = p.a.table + static_cast<int64_t>(tile.r) * p.a.table_rs;
-      // pages of this piece that do not exist (flagged by the producer)
-      bool holes = false;
-      if (s.nblk > 0) {
-        const int end = min((s.j0 + s.nblk) * kSqdkBN, tile.req.kv);
-        for (int pg = ((s.j0 * kSqdkBN) >> p.a.shift) + lane; pg <= ((end - 1) >> p.a.shift); pg += 32) {
-          const int x = __ldg(row + pg);
-          holes |= x < 0 || x >= p.a.num_pages;
-        }
-        holes = __any_sync(0xFFFFFFFFu, holes);
-      }
-      bool seen = !blind && lim >= s.j0 * kSqdkBN && s.nblk > 0;
-      if (holes) seen = false;
+      const int tile_hi = job.hi, tile_lo = job.lo;
+      const bool holes = job.holes != 0;
+      int lim = row_valid ? job.lim[qloc] : -1;
+      const bool blind = lim < 0;
+      if (blind) lim = tile_hi;
+      bool seen = !blind && lim >= j0 * kSqdkBN && nblk > 0 && !holes;
       float m_run = -INFINITY, l_run = 0.0f;
-      for (int j = 0; j < s.nblk; ++j, ++n) {
+      for (int j = 0; j < nblk; ++j, ++n) {
         const uint32_t sb = n & 1;
         ok = __all_sync(0xFFFFFFFFu, mbar_wait(&bar_sfull[sb], (n >> 1) & 1, &abort_flag));
         if (!ok) break;
@@ -502,17 +552,18 @@ __global__ void __launch_bounds__(kChunkThreads, kChunkCtasPerSm)
             sv[32 + i] = __uint_as_float(r1[i]);
           }
         }
-        const int key0 = (s.j0 + j) * kSqdkBN;
+        const int key0 = (j0 + j) * kSqdkBN;
         const int left = lim - key0;  // columns <= left are visible to this row
         // the same for every warp: does any row of the tile not see all of this block?
-        const bool edge = key0 + kSqdkBN - 1 > s.lo;
+        const bool edge = key0 + kSqdkBN - 1 > tile_lo;
         if (edge) {
 #pragma unroll
           for (int c = 0; c < kSqdkBN; ++c) sv[c] = (c <= left) ? sv[c] : -INFINITY;
         }
         if (holes) {
+          const int* row = p.a.table + static_cast<int64_t>(job.r) * p.a.table_rs;
           for (int c0 = 0; c0 < kSqdkBN; c0 += 8) {
-            const int x = key0 + c0 < tile.req.kv ? __ldg(row + ((key0 + c0) >> p.a.shift)) : -1;
+            const int x = key0 + c0 < job.kv ? __ldg(row + ((key0 + c0) >> p.a.shift)) : -1;
             const bool gone = x < 0 || x >= p.a.num_pages;
             seen |= !gone && !blind && c0 <= left;
 #pragma unroll
@@ -593,13 +644,14 @@ __global__ void __launch_bounds__(kChunkThreads, kChunkCtasPerSm)
           if (!ok) break;
           const uint32_t vst = sbase + L::kVOff + sb * L::kKVBytes;
           bool found = false;
-#pragma unroll 1
-          for (int i = lane; i < 16 * 8 * L::kChunks; i += 32) {
+          if (key0 + 16 * sw + 15 > tile_lo)
+#pragma unroll 4
+            for (int i = lane; i < 16 * 8 * L::kChunks; i += 32) {
             const int kr = 16 * sw + (i >> 3) % 16, key = key0 + kr;
             const uint32_t addr = vst + (i >> 7) * L::kKVChunkBytes + kr * 128 + (i & 7) * 16;
-            if (key > s.hi) {
+            if (key > tile_hi) {
               st_shared_v4(addr, make_uint4(0u, 0u, 0u, 0u));
-            } else if (key > s.lo) {
+            } else if (key > tile_lo) {
               uint4 w;
               asm volatile("ld.shared.v4.u32 {%0,%1,%2,%3}, [%4];" : "=r"(w.x), "=r"(w.y), "=r"(w.z), "=r"(w.w) : "r"(addr));
               if (not_finite2<kBF16>(w.x) || not_finite2<kBF16>(w.y) || not_finite2<kBF16>(w.z) || not_finite2<kBF16>(w.w)) {
@@ -616,10 +668,10 @@ __global__ void __launch_bounds__(kChunkThreads, kChunkCtasPerSm)
         if (lane == 0) mbar_arrive(&bar_pfull[sb]);
       }
       // ---------------------------------------------------------- epilogue
-      if (ok && s.nblk > 0) ok = __all_sync(0xFFFFFFFFu, mbar_wait(&bar_ofinal, segs & 1, &abort_flag));
-      if (s.nblk > 0) ++segs;
-      // between the barriers every warp has set this segment's flag and none
-      // has left its epilogue: it is read, and the last segment's is cleared
+      if (ok && nblk > 0) ok = __all_sync(0xFFFFFFFFu, mbar_wait(&bar_ofinal, segs & 1, &abort_flag));
+      if (nblk > 0) ++segs;
+      // between the barriers every warp has set this job's flag and none has
+      // left its epilogue: it is read, and the last job's is cleared
       if (threadIdx.x == 64) wild_flag[(walked + 1) & 1] = 0u;
       const bool live = named_bar_and(kChunkEpilogueBar, 128, ok);
       const bool wild = wild_flag[walked & 1] != 0u;
@@ -631,11 +683,12 @@ __global__ void __launch_bounds__(kChunkThreads, kChunkCtasPerSm)
       }
       tc_fence_after();
       const bool none = !seen;
-      const float inv_l = s.slot >= 0 ? 1.0f : 1.0f / l_run;
+      const int slot = job.slot, row0 = job.row0, head = job.head;
+      const float inv_l = slot >= 0 ? 1.0f : 1.0f / l_run;
 #pragma unroll 1
       for (int c = 0; c < HD; c += 32) {
         float o[32];
-        if (s.nblk > 0) {
+        if (nblk > 0) {
           uint32_t x[32];
           tmem_ld32(tO + c, x);
           tmem_wait_ld();
@@ -647,11 +700,12 @@ __global__ void __launch_bounds__(kChunkThreads, kChunkCtasPerSm)
         }
         if (wild && row_valid && !blind) {
           // infinities and NaN that this row does see, from the cache
-          const int from = max(s.lo + 1, s.j0 * kSqdkBN), to = min(lim, (s.j0 + s.nblk) * kSqdkBN - 1);
+          const int* row = p.a.table + static_cast<int64_t>(job.r) * p.a.table_rs;
+          const int from = max(tile_lo + 1, j0 * kSqdkBN), to = min(lim, (j0 + nblk) * kSqdkBN - 1);
           for (int key = from; key <= to; ++key) {
             const int pg = __ldg(row + (key >> p.a.shift));
             if (pg < 0 || pg >= p.a.num_pages) continue;
-            const char* v = p.a.v + pg * p.a.v_sp + (key & ((1 << p.a.shift) - 1)) * p.a.v_ss + tile.head * p.a.v_sh;
+            const char* v = p.a.v + pg * p.a.v_sp + (key & ((1 << p.a.shift) - 1)) * p.a.v_ss + head * p.a.v_sh;
 #pragma unroll
             for (int i = 0; i < 32; ++i) {
               if (c + i >= p.a.hd) continue;
@@ -660,10 +714,10 @@ __global__ void __launch_bounds__(kChunkThreads, kChunkCtasPerSm)
             }
           }
         }
-        if (s.slot >= 0) {
+        if (slot >= 0) {
           // unnormalised O of this piece
           if (row_valid) {
-            float* dst = p.a.part_o + (static_cast<int64_t>(s.slot) * kSqdkBM + r) * HD + c;
+            float* dst = p.a.part_o + (static_cast<int64_t>(slot) * kSqdkBM + r) * HD + c;
 #pragma unroll
             for (int v = 0; v < 8; ++v)
               reinterpret_cast<float4*>(dst)[v] = make_float4(o[4 * v], o[4 * v + 1], o[4 * v + 2], o[4 * v + 3]);
@@ -691,17 +745,19 @@ __global__ void __launch_bounds__(kChunkThreads, kChunkCtasPerSm)
           asm volatile("ld.shared.v4.u32 {%0,%1,%2,%3}, [%4];"
                        : "=r"(w.x), "=r"(w.y), "=r"(w.z), "=r"(w.w)
                        : "r"(stage + lr * 64 + ((unit ^ ((lr >> 1) & 3)) << 4)));
-          if (ql < p.QT && tile.t * p.QT + ql < tile.req.len && c + unit * 8 < p.a.hd)
-            *reinterpret_cast<uint4*>(p.a.o + static_cast<int64_t>(tile.req.q0 + tile.t * p.QT + ql) * p.a.o_sn +
-                                      static_cast<int64_t>(tile.head * p.a.G + rr - ql * p.a.G) * p.a.o_sh +
+          if (ql < job.queries && c + unit * 8 < p.a.hd)
+            *reinterpret_cast<uint4*>(p.a.o + static_cast<int64_t>(row0 + ql) * p.a.o_sn +
+                                      static_cast<int64_t>(head * p.a.G + rr - ql * p.a.G) * p.a.o_sh +
                                       (c + unit * 8) * 2) = w;
         }
         __syncwarp();
       }
-      if (s.slot >= 0 && row_valid)
-        reinterpret_cast<float2*>(p.a.part_ml)[static_cast<int64_t>(s.slot) * kSqdkBM + r] =
+      if (slot >= 0 && row_valid)
+        reinterpret_cast<float2*>(p.a.part_ml)[static_cast<int64_t>(slot) * kSqdkBM + r] =
             make_float2(m_run, none ? kUnseen : l_run);
       tc_fence_before();  // O has been read: the next tile's first P V (behind this warp's arrival) may write it
+      __syncwarp();
+      if (lane == 0) mbar_arrive(&bar_jobdone[(walked - 1) & 1]);
     }
   }
 
@@ -715,55 +771,53 @@ __global__ void __launch_bounds__(kChunkThreads, kChunkCtasPerSm)
 
 constexpr int kChunkMergeWarps = 16;
 
-// Adds the pieces of the tile that the end of run blockIdx.x cuts, if that is
-// the tile's first piece. A warp takes a row at a time.
+// Adds the pieces of the tile whose first piece ends run blockIdx.x, as that run
+// noted: O = sum 2^(m_c - M) O_c / sum 2^(m_c - M) l_c over the runs in order.
+// Two rows a warp at a time keep four 512-byte loads in flight per lane group.
 template <int HD, bool kBF16>
-__global__ void __launch_bounds__(32 * kChunkMergeWarps) paged_chunk_merge_kernel(const __grid_constant__ ChunkParams p,
-                                                                                  int most_runs) {
+__global__ void __launch_bounds__(32 * kChunkMergeWarps) paged_chunk_merge_kernel(const __grid_constant__ ChunkParams p) {
+  grid_dependency_wait();
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-  const int64_t total = chunk_total(p, lane);
-  if (total == 0) return;
-  const int64_t runs = chunk_runs(total, most_runs);
-  const int64_t c0 = blockIdx.x;
-  if (c0 + 1 >= runs) return;
-  ChunkTile tile, t;
-  const int64_t cut = chunk_cut(p, total, runs, c0 + 1, lane, tile);
-  // a cut at a tile's end cuts nothing; the first piece is the one whose run
-  // does not begin inside the tile
-  if (cut <= tile.start || cut >= tile.start + tile.cost) return;
-  if (chunk_cut(p, total, runs, c0, lane, t) > tile.start) return;
-  // the last piece's run is the first that ends at or behind the tile's end
-  int64_t c1 = c0 + 1;
-  while (c1 + 1 < runs && run_start(total, runs, c1 + 1) < tile.start + tile.cost) ++c1;
-  if (c1 + 1 <= runs && chunk_cut(p, total, runs, c1, lane, t) >= tile.start + tile.cost) --c1;
+  const int4 note = p.a.merges[blockIdx.x];
+  const int c0 = static_cast<int>(blockIdx.x), c1 = note.w;
+  if (c1 < 0) return;
   const float2* ml = reinterpret_cast<const float2*>(p.a.part_ml);
-  const int rows = min(p.QT, tile.req.len - tile.t * p.QT) * p.a.G;
-  for (int r = warp; r < rows; r += kChunkMergeWarps) {
-    float M = -INFINITY, l = 0.0f;
-    bool none = true;
-    float4 o = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
-    // run c0's piece is its last, the others' their first
-    for (int64_t c = c0; c <= c1; ++c) M = fmaxf(M, ml[(2 * c + (c == c0 ? 1 : 0)) * kSqdkBM + r].x);
-    for (int64_t c = c0; c <= c1; ++c) {
-      const int64_t sl = (2 * c + (c == c0 ? 1 : 0)) * kSqdkBM + r;
-      const float2 x = ml[sl];
-      if (x.y == kUnseen) continue;
-      none = false;
-      const float f = x.x == M ? 1.0f : fast_exp2(x.x - M);
-      l += f * x.y;
-      if (lane < HD / 4) {
-        const float4 v = *reinterpret_cast<const float4*>(p.a.part_o + sl * HD + lane * 4);
-        o.x += f * v.x, o.y += f * v.y, o.z += f * v.z, o.w += f * v.w;
+  const int rows = note.y * p.a.G;
+  // run c0's piece is its last, the others' their first
+  auto slot_row = [&](int c, int r) { return (2 * static_cast<int64_t>(c) + (c == c0 ? 1 : 0)) * kSqdkBM + r; };
+  for (int r0 = 2 * warp; r0 < rows; r0 += 2 * kChunkMergeWarps) {
+    float M[2] = {-INFINITY, -INFINITY}, l[2] = {};
+    bool none[2] = {true, true};
+    float4 o[2] = {make_float4(0.0f, 0.0f, 0.0f, 0.0f), make_float4(0.0f, 0.0f, 0.0f, 0.0f)};
+#pragma unroll 2
+    for (int c = c0; c <= c1; ++c) {
+#pragma unroll
+      for (int i = 0; i < 2; ++i) {
+        const int64_t sl = slot_row(c, min(r0 + i, rows - 1));
+        const float2 x = ml[sl];
+        const float4 v = lane < HD / 4 ? *reinterpret_cast<const float4*>(p.a.part_o + sl * HD + lane * 4)
+                                       : make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+        if (x.y == kUnseen) continue;
+        none[i] = false;
+        const float top = fmaxf(M[i], x.x);
+        const float f = x.x == top ? 1.0f : fast_exp2(x.x - top), g = M[i] == top ? 1.0f : fast_exp2(M[i] - top);
+        M[i] = top;
+        l[i] = g * l[i] + f * x.y;
+        o[i].x = g * o[i].x + f * v.x, o[i].y = g * o[i].y + f * v.y;
+        o[i].z = g * o[i].z + f * v.z, o[i].w = g * o[i].w + f * v.w;
       }
     }
-    const float inv = 1.0f / l;
-    if (lane < HD / 4 && lane * 4 < p.a.hd) {
+#pragma unroll
+    for (int i = 0; i < 2; ++i) {
+      const int r = r0 + i;
+      if (r >= rows || lane >= HD / 4 || lane * 4 >= p.a.hd) continue;
+      const float inv = 1.0f / l[i];
       const int ql = r / p.a.G;
       uint2 w;
-      w.x = none ? 0u : pack2<kBF16>(o.x * inv, o.y * inv);
-      w.y = none ? 0u : pack2<kBF16>(o.z * inv, o.w * inv);
-      *reinterpret_cast<uint2*>(p.a.o + static_cast<int64_t>(tile.req.q0 + tile.t * p.QT + ql) * p.a.o_sn +
-                                static_cast<int64_t>(tile.head * p.a.G + r - ql * p.a.G) * p.a.o_sh + lane * 8) = w;
+      w.x = none[i] ? 0u : pack2<kBF16>(o[i].x * inv, o[i].y * inv);
+      w.y = none[i] ? 0u : pack2<kBF16>(o[i].z * inv, o[i].w * inv);
+      *reinterpret_cast<uint2*>(p.a.o + static_cast<int64_t>(note.x + ql) * p.a.o_sn +
+                                static_cast<int64_t>(note.z * p.a.G + r - ql * p.a.G) * p.a.o_sh + lane * 8) = w;
     }
   }
 }
