@@ -182,43 +182,59 @@ __device__ __forceinline__ void load_table(const char* p, float (&out)[n]) {
 // One warp a token: lanes take the K row in pairs of 16-byte groups (a group of
 // a head's low half and its partner in the high half, so x and the tables are
 // read once per pair) and the V row in 16-byte groups. The rotation is formed
-// in fp32 and rounded once, when it is stored.
+// in fp32 and rounded once, when it is stored. A lane's first K pair and first
+// two V groups (the whole rows up to 512 16-bit elements) are requested before
+// the slot and position are known, so that only the table rows wait for those.
 template <typename T, typename Tab>
 __global__ void __launch_bounds__(kRowThreads) rope_paged_write_kernel(const PagedWriteParams p) {
   constexpr int n = 16 / sizeof(T);
   const int lane = threadIdx.x & 31;
   const int half = p.hd / 2;
+  const bool rope = p.cos_tab != nullptr;
+  const int vgroups = p.hd / n, units = p.Hkv * vgroups;  // 16-byte groups of a head, of a row
+  const int pairs = half / n, kunits = rope ? p.Hkv * pairs : units;
+  auto source = [](const char* row, int64_t sh, int h, int c) { return reinterpret_cast<const uint4*>(row + h * sh + c * 16); };
   for (int64_t t = static_cast<int64_t>(blockIdx.x) * kRowWarps + (threadIdx.x >> 5); t < p.N;
        t += static_cast<int64_t>(gridDim.x) * kRowWarps) {
+    const char* krow = p.k + t * p.k_sn;
+    const char* vrow = p.v + t * p.v_sn;
     const int64_t slot = __ldg(p.slots + t);
+    const int64_t pos = rope ? __ldg(p.pos + t) : 0;
+    const int kg = rope ? pairs : vgroups;
+    const int kh = lane / kg, kc = lane - kh * kg;
+    uint4 k_lo = make_uint4(0, 0, 0, 0), k_hi = k_lo, v_0 = k_lo, v_1 = k_lo;
+    if (lane < kunits) {
+      k_lo = __ldcs(source(krow, p.k_sh, kh, kc));
+      if (rope) k_hi = __ldcs(source(krow, p.k_sh, kh, kc + pairs));
+    }
+    if (lane < units) v_0 = __ldcs(source(vrow, p.v_sh, lane / vgroups, lane % vgroups));
+    if (lane + 32 < units) v_1 = __ldcs(source(vrow, p.v_sh, (lane + 32) / vgroups, (lane + 32) % vgroups));
     if (slot < 0) continue;  // padding
     const int64_t page = slot >> p.shift, off = slot & ((1 << p.shift) - 1);
-    const int64_t pos = p.cos_tab ? __ldg(p.pos + t) : 0;
-    if (page >= p.num_pages || pos < 0 || (p.cos_tab && pos >= p.tab_rows)) {
+    if (page >= p.num_pages || pos < 0 || (rope && pos >= p.tab_rows)) {
       if (lane == 0) raise_device_error(page >= p.num_pages ? HSPMN_DEVERR_PAGE : HSPMN_DEVERR_POSITION);
       continue;
     }
-    const char* krow = p.k + t * p.k_sn;
-    const char* vrow = p.v + t * p.v_sn;
     char* kdst = p.kc + page * p.kc_sp + off * p.kc_ss;
     char* vdst = p.vc + page * p.vc_sp + off * p.vc_ss;
-    const int vgroups = p.hd / n;
-    if (p.cos_tab) {
-      const int pairs = half / n;
-      const char* cs = p.cos_tab + pos * p.tab_ss;
-      const char* sn = p.sin_tab + pos * p.tab_ss;
-      for (int i = lane; i < p.Hkv * pairs; i += 32) {
-        const int h = i / pairs, c = (i - h * pairs) * n;
-        const uint4 lo4 = __ldcs(reinterpret_cast<const uint4*>(krow + h * p.k_sh + c * sizeof(T)));
-        const uint4 hi4 = __ldcs(reinterpret_cast<const uint4*>(krow + h * p.k_sh + (c + half) * sizeof(T)));
+    const char* cs = p.cos_tab + pos * p.tab_ss;
+    const char* sn = p.sin_tab + pos * p.tab_ss;
+    for (int i = lane; i < kunits; i += 32) {
+      const int h = i / kg, c = i - h * kg;
+      if (i != lane) {
+        k_lo = __ldcs(source(krow, p.k_sh, h, c));
+        if (rope) k_hi = __ldcs(source(krow, p.k_sh, h, c + pairs));
+      }
+      uint4 out_lo = k_lo;
+      if (rope) {
         float c_lo[n], c_hi[n], s_lo[n], s_hi[n];
-        load_table<Tab, n>(cs + c * sizeof(Tab), c_lo);
-        load_table<Tab, n>(cs + (c + half) * sizeof(Tab), c_hi);
-        load_table<Tab, n>(sn + c * sizeof(Tab), s_lo);
-        load_table<Tab, n>(sn + (c + half) * sizeof(Tab), s_hi);
-        const T* lo = reinterpret_cast<const T*>(&lo4);
-        const T* hi = reinterpret_cast<const T*>(&hi4);
-        uint4 out_lo, out_hi;
+        load_table<Tab, n>(cs + c * n * sizeof(Tab), c_lo);
+        load_table<Tab, n>(cs + (c * n + half) * sizeof(Tab), c_hi);
+        load_table<Tab, n>(sn + c * n * sizeof(Tab), s_lo);
+        load_table<Tab, n>(sn + (c * n + half) * sizeof(Tab), s_hi);
+        const T* lo = reinterpret_cast<const T*>(&k_lo);
+        const T* hi = reinterpret_cast<const T*>(&k_hi);
+        uint4 out_hi;
         T* a = reinterpret_cast<T*>(&out_lo);
         T* b = reinterpret_cast<T*>(&out_hi);
 #pragma unroll
@@ -227,19 +243,14 @@ __global__ void __launch_bounds__(kRowThreads) rope_paged_write_kernel(const Pag
           a[j] = float_to_elt<T>(x * c_lo[j] - y * s_lo[j]);
           b[j] = float_to_elt<T>(y * c_hi[j] + x * s_hi[j]);
         }
-        *reinterpret_cast<uint4*>(kdst + h * p.kc_sh + c * sizeof(T)) = out_lo;
-        *reinterpret_cast<uint4*>(kdst + h * p.kc_sh + (c + half) * sizeof(T)) = out_hi;
+        __stcs(reinterpret_cast<uint4*>(kdst + h * p.kc_sh + (c + pairs) * 16), out_hi);
       }
-    } else {
-      for (int i = lane; i < p.Hkv * vgroups; i += 32) {
-        const int h = i / vgroups, c = (i - h * vgroups) * 16;
-        *reinterpret_cast<uint4*>(kdst + h * p.kc_sh + c) =
-            __ldcs(reinterpret_cast<const uint4*>(krow + h * p.k_sh + c));
-      }
+      __stcs(reinterpret_cast<uint4*>(kdst + h * p.kc_sh + c * 16), out_lo);
     }
-    for (int i = lane; i < p.Hkv * vgroups; i += 32) {
-      const int h = i / vgroups, c = (i - h * vgroups) * 16;
-      *reinterpret_cast<uint4*>(vdst + h * p.vc_sh + c) = __ldcs(reinterpret_cast<const uint4*>(vrow + h * p.v_sh + c));
+    for (int i = lane; i < units; i += 32) {
+      const int h = i / vgroups, c = i - h * vgroups;
+      const uint4 w = i == lane ? v_0 : i == lane + 32 ? v_1 : __ldcs(source(vrow, p.v_sh, h, c));
+      __stcs(reinterpret_cast<uint4*>(vdst + h * p.vc_sh + c * 16), w);
     }
   }
 }

@@ -5,7 +5,7 @@
 //   m over the positions of the query's request with m <= pos[i], m < kv_len
 //   and a page in the table
 //
-// Work unit: 64 keys of one (request, K/V head, 16 query rows) item; the rows
+// Work unit: 64 keys (128 for head_dim <= 64) of one (request, K/V head, 16 query rows) item; the rows
 // of a request and K/V head are numbered query * G + head, so a single token's
 // G heads share the keys that are read. All units of a call form one list
 // (requests, then row tiles, then heads, then keys) which is cut into as many
@@ -16,8 +16,8 @@
 // in run order, so results do not depend on timing.
 //
 // Bound: reading K and V once (4 query heads a key: 4 flops a byte). Each of a
-// CTA's four warps owns 16 keys of every unit and runs on its own: its K and V
-// rows come by cp.async into a private ring (kStages deep), Q K^T and P V are
+// CTA's four warps owns 16 (32) keys of every unit and runs on its own: its K and
+// V rows come by cp.async into a private ring (kStages deep), Q K^T and P V are
 // m16n8k16 products with the softmax between them in registers, and the warps
 // meet only at the end of an item. Sums, maxima and O are fp32.
 #pragma once
@@ -27,8 +27,7 @@
 namespace hspmn {
 
 constexpr int kPagedRows = 16;     // query rows of an item
-constexpr int kPagedKeys = 64;     // keys of a unit
-constexpr int kPagedWarps = 4;     // 16 keys of the unit each
+constexpr int kPagedWarps = 4;     // a quarter of a unit's keys each
 constexpr int kPagedThreads = 32 * kPagedWarps;
 constexpr int kPagedStages = 3;
 constexpr int kPagedCtasPerSm = 2;
@@ -81,18 +80,20 @@ __device__ __forceinline__ PagedRequest paged_rows(const PagedAttnParams& p, int
   return q;
 }
 
+template <int kKeys>
 __device__ __forceinline__ PagedRequest paged_request(const PagedAttnParams& p, int r) {
   PagedRequest q = paged_rows(p, r);
   q.tiles = r < p.R && q.rows > p.split_rows ? 0 : (q.rows + kPagedRows - 1) / kPagedRows;
-  q.nb = max(1, (q.kv + kPagedKeys - 1) / kPagedKeys);
+  q.nb = max(1, (q.kv + kKeys - 1) / kKeys);
   q.units = static_cast<int64_t>(q.tiles) * p.Hkv * q.nb;
   return q;
 }
 
 // Units of the whole list; every lane of the warp gets the sum.
+template <int kKeys>
 __device__ __forceinline__ int64_t paged_total(const PagedAttnParams& p, int lane) {
   int64_t n = 0;
-  for (int r = lane; r <= p.R; r += 32) n += paged_request(p, r).units;
+  for (int r = lane; r <= p.R; r += 32) n += paged_request<kKeys>(p, r).units;
 #pragma unroll
   for (int d = 16; d > 0; d >>= 1) n += __shfl_xor_sync(0xFFFFFFFFu, n, d);
   return n;
@@ -100,11 +101,12 @@ __device__ __forceinline__ int64_t paged_total(const PagedAttnParams& p, int lan
 
 // The request that unit u (< the total) belongs to and the list's units before
 // it, found by the whole warp.
+template <int kKeys>
 __device__ __forceinline__ int paged_locate(const PagedAttnParams& p, int64_t u, int lane, int64_t& before) {
   int64_t base = 0;
   for (int r0 = 0; r0 <= p.R; r0 += 32) {
     const int r = r0 + lane;
-    const int64_t mine = r <= p.R ? paged_request(p, r).units : 0;
+    const int64_t mine = r <= p.R ? paged_request<kKeys>(p, r).units : 0;
     int64_t sum = mine;
 #pragma unroll
     for (int d = 1; d < 32; d <<= 1) {
@@ -123,32 +125,45 @@ __device__ __forceinline__ int paged_locate(const PagedAttnParams& p, int64_t u,
   return p.R;  // not reached for u below the total
 }
 
-// First unit of run c of `runs`.
-__device__ __forceinline__ int64_t run_start(int64_t total, int64_t runs, int64_t c) {
-  return total / runs * c + total % runs * c / runs;
+// a / b; 64-bit divisions are slow, and most operands here fit 32 bits.
+__device__ __forceinline__ int64_t div_wide(int64_t a, int64_t b) {
+  if (((a | b) >> 32) == 0) return static_cast<uint32_t>(a) / static_cast<uint32_t>(b);
+  return a / b;
 }
 
-// The run that holds unit u (the last one that starts at or before u).
-__device__ __forceinline__ int run_of(int64_t total, int64_t runs, int64_t u) {
-  int64_t lo = 0, hi = runs;
-  while (hi - lo > 1) {
-    const int64_t mid = (lo + hi) >> 1;
-    if (run_start(total, runs, mid) <= u) lo = mid;
-    else hi = mid;
+// A list of `total` units cut into n runs whose lengths differ by one at most.
+struct Runs {
+  int64_t share, rem;
+  int n;
+  __device__ __forceinline__ Runs(int64_t total, int64_t runs) {
+    n = static_cast<int>(runs);
+    share = div_wide(total, runs);
+    rem = total - share * runs;
   }
-  return static_cast<int>(lo);
-}
+  __device__ __forceinline__ int64_t start(int64_t c) const { return share * c + min(c, rem); }
+  // The run that holds unit u.
+  __device__ __forceinline__ int of(int64_t u) const {
+    int lo = 0, hi = n;
+    while (hi - lo > 1) {
+      const int mid = (lo + hi) >> 1;
+      if (start(mid) <= u) lo = mid;
+      else hi = mid;
+    }
+    return lo;
+  }
+};
 
 // A place in the list: request, row tile, head and key unit.
+template <int kKeys>
 struct PagedCursor {
   PagedRequest req;
   int r, tile, head, j;
   __device__ __forceinline__ void set(const PagedAttnParams& p, int request, int64_t local) {
     r = request;
-    req = paged_request(p, r);
-    const int64_t item = local / req.nb;
+    req = paged_request<kKeys>(p, r);
+    const int64_t item = div_wide(local, req.nb);
     j = static_cast<int>(local - item * req.nb);
-    tile = static_cast<int>(item / p.Hkv);
+    tile = static_cast<int>(div_wide(item, p.Hkv));
     head = static_cast<int>(item - static_cast<int64_t>(tile) * p.Hkv);
   }
   // Only called while a next unit exists.
@@ -159,7 +174,7 @@ struct PagedCursor {
     head = 0;
     if (++tile < req.tiles) return;
     tile = 0;
-    do req = paged_request(p, ++r);
+    do req = paged_request<kKeys>(p, ++r);
     while (req.units == 0 && r < p.R);
   }
 };
@@ -230,11 +245,13 @@ __device__ __forceinline__ float half_to_float(uint16_t h) {
 template <int HD>
 struct PagedLayout {
   static constexpr int kRow = HD * 2;                             // bytes of a key's K or V in shared memory
-  static constexpr int kWarpStage = 2 * 16 * kRow;                // 16 keys of K and of V
+  static constexpr int kWarpKeys = HD == 64 ? 32 : 16;            // a warp's keys of a unit: 8 KB of K and V
+  static constexpr int kKeys = kPagedWarps * kWarpKeys;
+  static constexpr int kWarpStage = 2 * kWarpKeys * kRow;
   static constexpr int kStage = kPagedWarps * kWarpStage;
   static constexpr int kBytes = kPagedStages * kStage;
   // at the end of an item a warp leaves its 16 x HD fp32 O in the stage it has just consumed
-  static_assert(kWarpStage == kPagedRows * HD * 4, "an O tile fits a warp's stage exactly");
+  static_assert(kWarpStage >= kPagedRows * HD * 4, "an O tile fits a warp's stage");
 };
 
 // Word index of O element (row, col) in a warp's stage: 8-column groups are
@@ -252,16 +269,17 @@ __global__ void __launch_bounds__(kPagedThreads, kPagedCtasPerSm) paged_attn_ker
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   const int g = lane >> 2, t2 = (lane & 3) * 2;  // accumulator row and first column of this lane
   grid_dependents_launch();
-  const int64_t total = paged_total(p, lane);
+  const int64_t total = paged_total<L::kKeys>(p, lane);
   const int64_t runs = min(static_cast<int64_t>(gridDim.x), total);
   if (blockIdx.x >= runs) {
     if (threadIdx.x == 0) p.merges[blockIdx.x] = make_int4(0, 0, 0, -1);
     return;
   }
-  const int64_t u0 = run_start(total, runs, blockIdx.x), u1 = run_start(total, runs, blockIdx.x + 1);
+  const Runs run(total, runs);
+  const int64_t u0 = run.start(blockIdx.x), u1 = run.start(blockIdx.x + 1);
   int64_t before;
-  const int r0 = paged_locate(p, u0, lane, before);
-  PagedCursor cur, ahead;
+  const int r0 = paged_locate<L::kKeys>(p, u0, lane, before);
+  PagedCursor<L::kKeys> cur, ahead;
   cur.set(p, r0, u0 - before);
   ahead = cur;
   const uint32_t wbase = smem_u32(paged_smem) + warp * L::kWarpStage;
@@ -270,36 +288,45 @@ __global__ void __launch_bounds__(kPagedThreads, kPagedCtasPerSm) paged_attn_ker
   const int ld_row = lane / kChunks, ld_chunk = lane % kChunks;
   const bool ld_col = ld_chunk * 8 < p.hd;  // columns past head_dim are zero
 
-  // This warp's 16 keys of the unit `ahead` points at, into ring stage s. Keys
-  // past the visible range or in a page that does not exist arrive as zeros.
+  constexpr int kGroups = L::kWarpKeys / 8;  // of 8 keys: each lies in one page
+  const int mask = (1 << p.shift) - 1;
+  uint32_t gone_ring = 0;  // kGroups bits a stage: the group's page does not exist
+
+  // This warp's keys of the unit `ahead` points at, into ring stage s. Keys past
+  // the visible range or in a page that does not exist arrive as zeros (no bytes
+  // are read; the address then is any valid one).
   auto request = [&](int s) {
-    const int key0 = ahead.j * kPagedKeys + warp * 16;
-    const uint32_t kdst = wbase + s * L::kStage, vdst = kdst + 16 * L::kRow;
+    const int key0 = ahead.j * L::kKeys + warp * L::kWarpKeys;
+    const uint32_t kdst = wbase + s * L::kStage, vdst = kdst + L::kWarpKeys * L::kRow;
     const int* row = p.table + static_cast<int64_t>(ahead.r) * p.table_rs;
-    int page[2];  // pages of the first and of the second 8 keys
+    int page[kGroups];
 #pragma unroll
-    for (int i = 0; i < 2; ++i) {
-      const int key = key0 + 8 * i;
-      page[i] = key < ahead.req.kv ? __ldg(row + (key >> p.shift)) : -1;
-      if (key < ahead.req.kv && (page[i] < 0 || page[i] >= p.num_pages)) {
-        page[i] = -1;
+    for (int i = 0; i < kGroups; ++i) page[i] = key0 + 8 * i < ahead.req.kv ? __ldg(row + ((key0 + 8 * i) >> p.shift)) : -1;
+    uint32_t gone = 0;
+#pragma unroll
+    for (int i = 0; i < kGroups; ++i) {
+      const bool there = page[i] >= 0 && page[i] < p.num_pages;
+      if (!there && key0 + 8 * i < ahead.req.kv) {
+        gone |= 1u << i;
         if (lane == 0) raise_device_error(HSPMN_DEVERR_PAGE);
       }
-    }
+      const int64_t pg = there ? page[i] : 0;
+      const int64_t off = there ? ((key0 + 8 * i) & mask) + ld_row : 0;
+      const int col = there && ld_col ? ld_chunk * 16 : 0;
+      const char* ks = p.k + pg * p.k_sp + off * p.k_ss + ahead.head * p.k_sh + col;
+      const char* vs = p.v + pg * p.v_sp + off * p.v_ss + ahead.head * p.v_sh + col;
+      const int64_t kstep = there ? kPerIter * p.k_ss : 0, vstep = there ? kPerIter * p.v_ss : 0;
+      const int left = there && ld_col ? ahead.req.kv - key0 - 8 * i - ld_row : 0;  // rows from here on that count
 #pragma unroll
-    for (int i = 0; i < 16 / kPerIter; ++i) {
-      const int kr = i * kPerIter + ld_row;
-      const int pg = kr < 8 ? page[0] : page[1];
-      const int key = key0 + kr;
-      const bool there = pg >= 0 && key < ahead.req.kv && ld_col;
-      const int64_t off = key & ((1 << p.shift) - 1);
-      const int64_t pgl = there ? pg : 0;
-      const int64_t o = there ? off : 0;
-      const int64_t col = there ? ld_chunk * 16 : 0;
-      const uint32_t d = kr * L::kRow + ((ld_chunk ^ (kr & 7)) << 4);
-      cp_async16(kdst + d, p.k + pgl * p.k_sp + o * p.k_ss + ahead.head * p.k_sh + col, there);
-      cp_async16(vdst + d, p.v + pgl * p.v_sp + o * p.v_ss + ahead.head * p.v_sh + col, there);
+      for (int x = 0; x < 8 / kPerIter; ++x) {
+        const int kr = 8 * i + x * kPerIter + ld_row;
+        const uint32_t d = kr * L::kRow + ((ld_chunk ^ (kr & 7)) << 4);
+        cp_async16(kdst + d, ks, x * kPerIter < left);
+        cp_async16(vdst + d, vs, x * kPerIter < left);
+        ks += kstep, vs += vstep;
+      }
     }
+    gone_ring = (gone_ring & ~(((1u << kGroups) - 1) << (kGroups * s))) | gone << (kGroups * s);
   };
 
   int64_t ua = u0;
@@ -362,36 +389,32 @@ __global__ void __launch_bounds__(kPagedThreads, kPagedCtasPerSm) paged_attn_ker
     }
     cp_async_wait<kPagedStages - 2>();
     __syncwarp();
-    const int key0 = cur.j * kPagedKeys + warp * 16;
-    const uint32_t kst = wbase + stage * L::kStage, vst = kst + 16 * L::kRow;
+    const int key0 = cur.j * L::kKeys + warp * L::kWarpKeys;
+    const uint32_t kst = wbase + stage * L::kStage, vst = kst + L::kWarpKeys * L::kRow;
     if (key0 <= lim_max) {
-      // S = Q K^T, 16 rows x 16 keys
-      float s[2][4] = {};
+      // S = Q K^T, 16 rows by the warp's keys, in 8-key tiles
+      float s[kGroups][4] = {};
 #pragma unroll
       for (int kk = 0; kk < HD / 16; ++kk) {
-        const int kr = ((lane >> 4) << 3) + (lane & 7), chunk = kk * 2 + ((lane >> 3) & 1);
-        uint32_t b[4];
-        ldmatrix_x4(b, kst + kr * L::kRow + ((chunk ^ (kr & 7)) << 4));
-        mma16816<kBF16>(s[0], qa[kk], b[0], b[1]);
-        mma16816<kBF16>(s[1], qa[kk], b[2], b[3]);
-      }
-      // the pages are looked up again: a missing one masks its 8 keys
-      const int* row = p.table + static_cast<int64_t>(cur.r) * p.table_rs;
-      bool gone[2];
+        const int chunk = kk * 2 + ((lane >> 3) & 1);
 #pragma unroll
-      for (int n = 0; n < 2; ++n) {
-        const int key = key0 + 8 * n;
-        const int pg = key < cur.req.kv ? __ldg(row + (key >> p.shift)) : 0;
-        gone[n] = pg < 0 || pg >= p.num_pages;
+        for (int n = 0; n < kGroups; n += 2) {
+          const int kr = n * 8 + ((lane >> 4) << 3) + (lane & 7);
+          uint32_t b[4];
+          ldmatrix_x4(b, kst + kr * L::kRow + ((chunk ^ (kr & 7)) << 4));
+          mma16816<kBF16>(s[n], qa[kk], b[0], b[1]);
+          mma16816<kBF16>(s[n + 1], qa[kk], b[2], b[3]);
+        }
       }
-      const bool masked = key0 + 15 > lim_min || lim_min == 0x7FFFFFFF || gone[0] || gone[1];
+      const uint32_t gone = (gone_ring >> (kGroups * stage)) & ((1u << kGroups) - 1);
+      const bool masked = key0 + L::kWarpKeys - 1 > lim_min || gone != 0;
       if (masked) {
 #pragma unroll
-        for (int n = 0; n < 2; ++n)
+        for (int n = 0; n < kGroups; ++n)
 #pragma unroll
           for (int e = 0; e < 4; ++e) {
             const int key = key0 + 8 * n + t2 + (e & 1);
-            if (key > lim[e >> 1] || gone[n]) s[n][e] = -INFINITY;
+            if (key > lim[e >> 1] || (gone >> n & 1)) s[n][e] = -INFINITY;
           }
       }
       // online softmax of rows g and g + 8
@@ -399,7 +422,9 @@ __global__ void __launch_bounds__(kPagedThreads, kPagedCtasPerSm) paged_attn_ker
       bool grew = false;
 #pragma unroll
       for (int i = 0; i < 2; ++i) {
-        float mx = fmaxf(fmaxf(s[0][2 * i], s[0][2 * i + 1]), fmaxf(s[1][2 * i], s[1][2 * i + 1]));
+        float mx = fmaxf(s[0][2 * i], s[0][2 * i + 1]);
+#pragma unroll
+        for (int n = 1; n < kGroups; ++n) mx = fmaxf(mx, fmaxf(s[n][2 * i], s[n][2 * i + 1]));
         mx = fmaxf(mx, __shfl_xor_sync(0xFFFFFFFFu, mx, 1));
         mx = fmaxf(mx, __shfl_xor_sync(0xFFFFFFFFu, mx, 2));
         const float m_new = fmaxf(m_run[i], mx * p.scale_log2);
@@ -408,15 +433,16 @@ __global__ void __launch_bounds__(kPagedThreads, kPagedCtasPerSm) paged_attn_ker
         const float neg = m_new == -INFINITY ? 0.0f : -m_new;
         float sum = 0.0f;
 #pragma unroll
-        for (int n = 0; n < 2; ++n)
+        for (int n = 0; n < kGroups; ++n) {
 #pragma unroll
           for (int c = 0; c < 2; ++c) {
             const float e = fast_exp2(fmaf(s[n][2 * i + c], p.scale_log2, neg));
             s[n][2 * i + c] = e;
             sum += e;
           }
+          seen[i] |= key0 + 8 * n <= lim[i] && !(gone >> n & 1);
+        }
         l_run[i] = l_run[i] * alpha[i] + sum;
-        seen[i] |= (key0 <= lim[i] && !gone[0]) || (key0 + 8 <= lim[i] && !gone[1]);
         m_run[i] = m_new;
       }
       if (__any_sync(0xFFFFFFFFu, grew)) {
@@ -433,7 +459,7 @@ __global__ void __launch_bounds__(kPagedThreads, kPagedCtasPerSm) paged_attn_ker
       if (masked) {
         bool mine = false;
 #pragma unroll
-        for (int i = 0; i < 16 / kPerIter; ++i) {
+        for (int i = 0; i < L::kWarpKeys / kPerIter; ++i) {
           const int kr = i * kPerIter + ld_row;
           uint4 w;
           asm volatile("ld.shared.v4.u32 {%0,%1,%2,%3}, [%4];"
@@ -445,28 +471,31 @@ __global__ void __launch_bounds__(kPagedThreads, kPagedCtasPerSm) paged_attn_ker
         wild = __any_sync(0xFFFFFFFFu, mine);
       }
       if (!wild) {
-        // P in the operands' type: its rounding (half a step) is of the size
-        // of the output's own
-        const uint32_t pa[4] = {pack2<kBF16>(s[0][0], s[0][1]), pack2<kBF16>(s[0][2], s[0][3]),
-                                pack2<kBF16>(s[1][0], s[1][1]), pack2<kBF16>(s[1][2], s[1][3])};
 #pragma unroll
-        for (int n = 0; n < HD / 16; ++n) {
-          const int kr = (((lane >> 3) & 1) << 3) + (lane & 7), chunk = n * 2 + (lane >> 4);
-          uint32_t b[4];
-          ldmatrix_x4_trans(b, vst + kr * L::kRow + ((chunk ^ (kr & 7)) << 4));
-          mma16816<kBF16>(acc[2 * n], pa, b[0], b[1]);
-          mma16816<kBF16>(acc[2 * n + 1], pa, b[2], b[3]);
+        for (int k = 0; k < kGroups; k += 2) {
+          // P in the operands' type: its rounding (half a step) is of the size
+          // of the output's own
+          const uint32_t pa[4] = {pack2<kBF16>(s[k][0], s[k][1]), pack2<kBF16>(s[k][2], s[k][3]),
+                                  pack2<kBF16>(s[k + 1][0], s[k + 1][1]), pack2<kBF16>(s[k + 1][2], s[k + 1][3])};
+#pragma unroll
+          for (int n = 0; n < HD / 16; ++n) {
+            const int kr = k * 8 + (((lane >> 3) & 1) << 3) + (lane & 7), chunk = n * 2 + (lane >> 4);
+            uint32_t b[4];
+            ldmatrix_x4_trans(b, vst + kr * L::kRow + ((chunk ^ (kr & 7)) << 4));
+            mma16816<kBF16>(acc[2 * n], pa, b[0], b[1]);
+            mma16816<kBF16>(acc[2 * n + 1], pa, b[2], b[3]);
+          }
         }
       } else {
 #pragma unroll
-        for (int kr = 0; kr < 16; ++kr) {
+        for (int kr = 0; kr < L::kWarpKeys; ++kr) {
           const int src = (lane & ~3) | ((kr & 7) >> 1);  // the lane of this quad that holds the key's column
           float w[2];
           bool sees[2];
 #pragma unroll
           for (int i = 0; i < 2; ++i) {
             w[i] = __shfl_sync(0xFFFFFFFFu, s[kr >> 3][2 * i + (kr & 1)], src);
-            sees[i] = key0 + kr <= lim[i] && !gone[kr >> 3];
+            sees[i] = key0 + kr <= lim[i] && !(gone >> (kr >> 3) & 1);
           }
 #pragma unroll
           for (int n = 0; n < HD / 8; ++n) {
@@ -506,7 +535,7 @@ __global__ void __launch_bounds__(kPagedThreads, kPagedCtasPerSm) paged_attn_ker
         p.merges[blockIdx.x] =
             make_int4(cur.req.q0, cur.tile * kPagedRows,
                       cur.head * kPagedRows + min(kPagedRows, cur.req.rows - cur.tile * kPagedRows) - 1,
-                      first ? run_of(total, runs, open + cur.req.nb - 1) : -1);
+                      first ? run.of(open + cur.req.nb - 1) : -1);
       }
       __syncthreads();
       const bool whole = item_end && seg0 + cur.req.nb == u + 1;
@@ -563,7 +592,7 @@ __global__ void __launch_bounds__(kPagedThreads, kPagedCtasPerSm) paged_attn_ker
   cp_async_wait<0>();
 }
 
-constexpr int kMergeWarps = 16;
+constexpr int kMergeWarps = 32;
 
 // Adds the partial results of the item that opens in run blockIdx.x and goes on
 // behind it, as that run noted: O = sum 2^(m_c - M) O_c / sum 2^(m_c - M) l_c over

@@ -92,7 +92,7 @@ __device__ __forceinline__ ChunkRequest chunk_request(const ChunkParams& p, int 
   constexpr int kShift = 2;  // 64 keys = kChunkUnit units
   static_assert(kSqdkBN >> kShift == kChunkUnit, "cost units");
   c.first = (lo >> kShift) + kChunkUnit * (1 + kChunkTileCost);
-  c.slope = c.tiles > 1 ? max((hi - lo) >> kShift, static_cast<int64_t>(0)) / (c.tiles - 1) : 0;
+  c.slope = c.tiles > 1 ? div_wide(max((hi - lo) >> kShift, static_cast<int64_t>(0)), c.tiles - 1) : 0;
   c.head = c.first * c.tiles + c.slope * (static_cast<int64_t>(c.tiles) * (c.tiles - 1) / 2);
   return c;
 }
@@ -119,74 +119,83 @@ struct ChunkTile {
   }
 };
 
-__device__ __forceinline__ int64_t chunk_total(const ChunkParams& p, int lane) {
-  int64_t n = 0;
-  for (int r = lane; r < p.a.R; r += 32) n += chunk_request(p, r).head * p.a.Hkv;
-#pragma unroll
-  for (int d = 16; d > 0; d >>= 1) n += __shfl_xor_sync(0xFFFFFFFFu, n, d);
-  return n;
-}
-
-// Runs that a list of this cost is cut into.
-__device__ __forceinline__ int64_t chunk_runs(int64_t total, int64_t most) {
-  return min(most, max(total / (kChunkUnit * kChunkMinPiece), static_cast<int64_t>(1)));
-}
-
-// The tile that holds list place w (< the total), found by the whole warp.
-__device__ __forceinline__ ChunkTile chunk_locate(const ChunkParams& p, int64_t w, int lane) {
-  ChunkTile c;
-  int64_t base = 0;
-  c.r = p.a.R - 1;
-  for (int r0 = 0; r0 < p.a.R; r0 += 32) {
-    const int r = r0 + lane;
-    const int64_t mine = r < p.a.R ? chunk_request(p, r).head * p.a.Hkv : 0;
-    int64_t sum = mine;
+// The list of tiles, as one warp sees it: the first 32 requests' shares stay in
+// its lanes, later ones are read again.
+struct ChunkList {
+  const ChunkParams& p;
+  int lane;
+  int64_t mine, upto;  // cost of request `lane`, and with all before it
+  __device__ __forceinline__ ChunkList(const ChunkParams& p_, int lane_) : p(p_), lane(lane_) {
+    mine = cost(lane);
+    upto = scan(mine);
+  }
+  __device__ __forceinline__ int64_t cost(int r) const { return r < p.a.R ? chunk_request(p, r).head * p.a.Hkv : 0; }
+  __device__ __forceinline__ int64_t scan(int64_t x) const {
 #pragma unroll
     for (int d = 1; d < 32; d <<= 1) {
-      const int64_t x = __shfl_up_sync(0xFFFFFFFFu, sum, d);
-      if (lane >= d) sum += x;
+      const int64_t y = __shfl_up_sync(0xFFFFFFFFu, x, d);
+      if (lane >= d) x += y;
     }
-    const unsigned past = __ballot_sync(0xFFFFFFFFu, base + sum > w);
-    if (past) {
-      const int l = __ffs(past) - 1;
-      base += __shfl_sync(0xFFFFFFFFu, sum - mine, l);
-      c.r = r0 + l;
-      break;
+    return x;
+  }
+  __device__ __forceinline__ int64_t total() const {
+    int64_t n = mine;
+    for (int r = lane + 32; r < p.a.R; r += 32) n += cost(r);
+#pragma unroll
+    for (int d = 16; d > 0; d >>= 1) n += __shfl_xor_sync(0xFFFFFFFFu, n, d);
+    return n;
+  }
+  // The tile that holds list place w (below the total).
+  __device__ __forceinline__ ChunkTile locate(int64_t w) const {
+    ChunkTile c;
+    int64_t base = 0, own = mine, sum = upto;
+    c.r = p.a.R - 1;
+    for (int r0 = 0; r0 < p.a.R; r0 += 32) {
+      if (r0 > 0) own = cost(r0 + lane), sum = scan(own);
+      const unsigned past = __ballot_sync(0xFFFFFFFFu, base + sum > w);
+      if (past) {
+        const int l = __ffs(past) - 1;
+        base += __shfl_sync(0xFFFFFFFFu, sum - own, l);
+        c.r = r0 + l;
+        break;
+      }
+      base += __shfl_sync(0xFFFFFFFFu, sum, 31);
     }
-    base += __shfl_sync(0xFFFFFFFFu, sum, 31);
+    c.req = chunk_request(p, c.r);
+    const int64_t rel = w - base;
+    c.head = static_cast<int>(div_wide(rel, c.req.head));
+    const int64_t in_head = rel - c.head * c.req.head;
+    int lo = 0, hi = c.req.tiles;
+    while (hi - lo > 1) {
+      const int mid = (lo + hi) >> 1;
+      if (c.before(mid) <= in_head) lo = mid;
+      else hi = mid;
+    }
+    c.t = lo;
+    c.start = base + c.head * c.req.head + c.before(lo);
+    c.cost = c.req.first + c.req.slope * lo;
+    return c;
   }
-  c.req = chunk_request(p, c.r);
-  const int64_t rel = w - base;
-  c.head = static_cast<int>(rel / c.req.head);
-  const int64_t in_head = rel - c.head * c.req.head;
-  int lo = 0, hi = c.req.tiles;
-  while (hi - lo > 1) {
-    const int mid = (lo + hi) >> 1;
-    if (c.before(mid) <= in_head) lo = mid;
-    else hi = mid;
+};
+
+// The list cut into runs. A cut so near to an end of its tile that the piece
+// would not be worth its merge is moved to that end.
+struct ChunkCuts {
+  Runs run;
+  int64_t total, near;
+  __device__ __forceinline__ ChunkCuts(int64_t total_, int64_t most)
+      : run(total_, min(most, max(total_ / (kChunkUnit * kChunkMinPiece), static_cast<int64_t>(1)))),
+        total(total_),
+        near(min(run.share >> 4, static_cast<int64_t>(8 * kChunkUnit))) {}
+  __device__ __forceinline__ int64_t at(const ChunkList& list, int64_t c) const {
+    if (c >= run.n) return total;
+    const int64_t w = run.start(c);
+    const ChunkTile tile = list.locate(w);
+    if (w - tile.start <= near) return tile.start;
+    if (tile.start + tile.cost - w <= near) return tile.start + tile.cost;
+    return w;
   }
-  c.t = lo;
-  c.start = base + c.head * c.req.head + c.before(lo);
-  c.cost = c.req.first + c.req.slope * lo;
-  return c;
-}
-
-// How near to an end of its tile a cut is moved to that end: the piece would not
-// be worth its merge.
-__device__ __forceinline__ int64_t chunk_near(int64_t total, int64_t runs) {
-  return min(total / runs / 16, static_cast<int64_t>(8 * kChunkUnit));
-}
-
-// Where run c begins: an equal share of the list, or the near end of its tile.
-__device__ __forceinline__ int64_t chunk_cut(const ChunkParams& p, int64_t total, int64_t runs, int64_t c, int lane) {
-  if (c >= runs) return total;
-  const int64_t w = run_start(total, runs, c);
-  const ChunkTile tile = chunk_locate(p, w, lane);
-  const int64_t near = chunk_near(total, runs);
-  if (w - tile.start <= near) return tile.start;
-  if (tile.start + tile.cost - w <= near) return tile.start + tile.cost;
-  return w;
-}
+};
 
 // Walks a run's pieces: the whole tiles in order, then the piece at the run's
 // start, then the one at its end.
@@ -195,14 +204,14 @@ struct ChunkWalk {
   int64_t w0, w1;
   int stage;  // 0: whole tiles, 1: piece at the start, 2: piece at the end, 3: done
   bool started;
-  __device__ __forceinline__ void open(const ChunkParams& p, int64_t total, int64_t runs, int64_t c, int lane) {
+  __device__ __forceinline__ void open(const ChunkList& list, const ChunkCuts& cuts, int64_t c) {
     stage = 3;
     started = false;
-    if (c >= runs || total == 0) return;
-    w0 = chunk_cut(p, total, runs, c, lane);
-    w1 = chunk_cut(p, total, runs, c + 1, lane);
+    if (c >= cuts.run.n || cuts.total == 0) return;
+    w0 = cuts.at(list, c);
+    w1 = cuts.at(list, c + 1);
     if (w0 >= w1) return;
-    first = cur = chunk_locate(p, w0, lane);
+    first = cur = list.locate(w0);
     stage = 0;
   }
   // The next piece's tile; slot and merge say what it is.
@@ -250,7 +259,7 @@ struct ChunkWalk {
 // Key block at list place w of a tile with nblk blocks.
 __device__ __forceinline__ int chunk_block_at(const ChunkTile& c, int64_t w, int nblk) {
   const int64_t x = min(max(w - c.start, static_cast<int64_t>(0)), c.cost);
-  return static_cast<int>(x * nblk / c.cost);
+  return static_cast<int>(div_wide(x * nblk, c.cost));
 }
 
 // Fills in a job for list places [a, b) of a tile (the whole warp).
@@ -312,6 +321,7 @@ __global__ void __launch_bounds__(kChunkThreads, kChunkCtasPerSm)
   __shared__ __align__(8) uint64_t bar_q, bar_kfull[2], bar_vfull[2], bar_vempty[2], bar_sfull[2], bar_pfull[2];
   __shared__ __align__(8) uint64_t bar_ofinal, bar_drain, bar_job[2], bar_jobdone[2];
   __shared__ volatile ChunkJob jobs[2];  // by the job's number: the next is posted while one is worked on
+  __shared__ int64_t row_off[kSqdkBM];  // of a tile's row in o, from the tile's first query and head; -1: no row
   __shared__ uint32_t tmem_base_sh;
   __shared__ volatile uint32_t abort_flag;
   // an infinity or NaN was taken out of V for rows that do not see it (by the
@@ -343,6 +353,10 @@ __global__ void __launch_bounds__(kChunkThreads, kChunkCtasPerSm)
     tmem_alloc(&tmem_base_sh, L::kTmemCols);
     tmem_relinquish();
   }
+  if (threadIdx.x >= 64) {
+    const int rr = threadIdx.x - 64, ql = rr / p.a.G;
+    row_off[rr] = ql < p.QT ? ql * p.a.o_sn + (rr - ql * p.a.G) * p.a.o_sh : -1;
+  }
   tc_fence_before();
   __syncthreads();
   tc_fence_after();
@@ -351,10 +365,10 @@ __global__ void __launch_bounds__(kChunkThreads, kChunkCtasPerSm)
   if (warp == 0) {
     // ------------------------------------------------------------ producer
     const int boxes = kSqdkBN / p.box_rows;
-    const int64_t total = chunk_total(p, lane);
-    const int64_t runs = chunk_runs(total, gridDim.x);
+    const ChunkList list(p, lane);
+    const ChunkCuts cuts(list.total(), gridDim.x);
     ChunkWalk walk;
-    walk.open(p, total, runs, blockIdx.x, lane);
+    walk.open(list, cuts, blockIdx.x);
     uint32_t nk = 0, nv = 0, segs = 0, posted = 0;
     bool live = true;
     int merge_to = -1;
@@ -378,8 +392,8 @@ __global__ void __launch_bounds__(kChunkThreads, kChunkCtasPerSm)
         // the first piece of its tile: its merge goes up to the last run that
         // begins inside the tile
         const int64_t end = tile.start + tile.cost;
-        merge_to = run_of(total, runs, end - 1);
-        if (end - run_start(total, runs, merge_to) <= chunk_near(total, runs)) --merge_to;
+        merge_to = cuts.run.of(end - 1);
+        if (end - cuts.run.start(merge_to) <= cuts.near) --merge_to;
         if (lane == 0)
           p.a.merges[blockIdx.x] = make_int4(tile.req.q0 + tile.t * p.QT, min(p.QT, tile.req.len - tile.t * p.QT),
                                              tile.head, merge_to);
@@ -683,7 +697,8 @@ __global__ void __launch_bounds__(kChunkThreads, kChunkCtasPerSm)
       }
       tc_fence_after();
       const bool none = !seen;
-      const int slot = job.slot, row0 = job.row0, head = job.head;
+      const int slot = job.slot, head = job.head;
+      const int64_t row0 = job.row0;
       const float inv_l = slot >= 0 ? 1.0f : 1.0f / l_run;
 #pragma unroll 1
       for (int c = 0; c < HD; c += 32) {
@@ -715,13 +730,11 @@ __global__ void __launch_bounds__(kChunkThreads, kChunkCtasPerSm)
           }
         }
         if (slot >= 0) {
-          // unnormalised O of this piece
-          if (row_valid) {
-            float* dst = p.a.part_o + (static_cast<int64_t>(slot) * kSqdkBM + r) * HD + c;
+          // unnormalised O of this piece, rows side by side in groups of four
+          // columns: a warp's stores are whole lines
+          float4* dst = reinterpret_cast<float4*>(p.a.part_o) + (static_cast<int64_t>(slot) * (HD / 4) + c / 4) * kSqdkBM + r;
 #pragma unroll
-            for (int v = 0; v < 8; ++v)
-              reinterpret_cast<float4*>(dst)[v] = make_float4(o[4 * v], o[4 * v + 1], o[4 * v + 2], o[4 * v + 3]);
-          }
+          for (int v = 0; v < 8; ++v) dst[v * kSqdkBM] = make_float4(o[4 * v], o[4 * v + 1], o[4 * v + 2], o[4 * v + 3]);
           continue;
         }
         // 32 columns of the warp's 32 rows through shared memory, so that a
@@ -737,18 +750,16 @@ __global__ void __launch_bounds__(kChunkThreads, kChunkCtasPerSm)
           st_shared_v4(stage + lane * 64 + ((v ^ ((lane >> 1) & 3)) << 4), w);
         }
         __syncwarp();
+        char* base = p.a.o + row0 * p.a.o_sn + static_cast<int64_t>(head) * p.a.G * p.a.o_sh + (c + (lane & 3) * 8) * 2;
+        const int rows = job.queries * p.a.G;
 #pragma unroll
         for (int i = 0; i < 4; ++i) {
-          const int lr = i * 8 + (lane >> 2), unit = lane & 3;
-          const int rr = 32 * sw + lr, ql = rr / p.a.G;
+          const int lr = i * 8 + (lane >> 2), rr = 32 * sw + lr;
           uint4 w;
           asm volatile("ld.shared.v4.u32 {%0,%1,%2,%3}, [%4];"
                        : "=r"(w.x), "=r"(w.y), "=r"(w.z), "=r"(w.w)
-                       : "r"(stage + lr * 64 + ((unit ^ ((lr >> 1) & 3)) << 4)));
-          if (ql < job.queries && c + unit * 8 < p.a.hd)
-            *reinterpret_cast<uint4*>(p.a.o + static_cast<int64_t>(row0 + ql) * p.a.o_sn +
-                                      static_cast<int64_t>(head * p.a.G + rr - ql * p.a.G) * p.a.o_sh +
-                                      (c + unit * 8) * 2) = w;
+                       : "r"(stage + lr * 64 + (((lane & 3) ^ ((lr >> 1) & 3)) << 4)));
+          if (rr < rows && c + (lane & 3) * 8 < p.a.hd) *reinterpret_cast<uint4*>(base + row_off[rr]) = w;
         }
         __syncwarp();
       }
@@ -773,7 +784,7 @@ constexpr int kChunkMergeWarps = 16;
 
 // Adds the pieces of the tile whose first piece ends run blockIdx.x, as that run
 // noted: O = sum 2^(m_c - M) O_c / sum 2^(m_c - M) l_c over the runs in order.
-// Two rows a warp at a time keep four 512-byte loads in flight per lane group.
+// A warp takes 8 rows by 16 columns at a time (128-byte reads of the pieces).
 template <int HD, bool kBF16>
 __global__ void __launch_bounds__(32 * kChunkMergeWarps) paged_chunk_merge_kernel(const __grid_constant__ ChunkParams p) {
   grid_dependency_wait();
@@ -782,43 +793,36 @@ __global__ void __launch_bounds__(32 * kChunkMergeWarps) paged_chunk_merge_kerne
   const int c0 = static_cast<int>(blockIdx.x), c1 = note.w;
   if (c1 < 0) return;
   const float2* ml = reinterpret_cast<const float2*>(p.a.part_ml);
+  const float4* part = reinterpret_cast<const float4*>(p.a.part_o);
   const int rows = note.y * p.a.G;
-  // run c0's piece is its last, the others' their first
-  auto slot_row = [&](int c, int r) { return (2 * static_cast<int64_t>(c) + (c == c0 ? 1 : 0)) * kSqdkBM + r; };
-  for (int r0 = 2 * warp; r0 < rows; r0 += 2 * kChunkMergeWarps) {
-    float M[2] = {-INFINITY, -INFINITY}, l[2] = {};
-    bool none[2] = {true, true};
-    float4 o[2] = {make_float4(0.0f, 0.0f, 0.0f, 0.0f), make_float4(0.0f, 0.0f, 0.0f, 0.0f)};
+#pragma unroll 2
+  for (int i = warp; i < (kSqdkBM / 8) * (HD / 16); i += kChunkMergeWarps) {
+    const int r = i / (HD / 16) * 8 + (lane >> 2), q4 = i % (HD / 16) * 4 + (lane & 3);  // row, group of 4 columns
+    if (r >= rows || q4 * 4 >= p.a.hd) continue;
+    float M = -INFINITY, l = 0.0f;
+    bool none = true;
+    float4 o = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
 #pragma unroll 2
     for (int c = c0; c <= c1; ++c) {
-#pragma unroll
-      for (int i = 0; i < 2; ++i) {
-        const int64_t sl = slot_row(c, min(r0 + i, rows - 1));
-        const float2 x = ml[sl];
-        const float4 v = lane < HD / 4 ? *reinterpret_cast<const float4*>(p.a.part_o + sl * HD + lane * 4)
-                                       : make_float4(0.0f, 0.0f, 0.0f, 0.0f);
-        if (x.y == kUnseen) continue;
-        none[i] = false;
-        const float top = fmaxf(M[i], x.x);
-        const float f = x.x == top ? 1.0f : fast_exp2(x.x - top), g = M[i] == top ? 1.0f : fast_exp2(M[i] - top);
-        M[i] = top;
-        l[i] = g * l[i] + f * x.y;
-        o[i].x = g * o[i].x + f * v.x, o[i].y = g * o[i].y + f * v.y;
-        o[i].z = g * o[i].z + f * v.z, o[i].w = g * o[i].w + f * v.w;
-      }
+      // run c0's piece is its last, the others' their first
+      const int64_t slot = 2 * static_cast<int64_t>(c) + (c == c0 ? 1 : 0);
+      const float2 x = ml[slot * kSqdkBM + r];
+      const float4 v = part[(slot * (HD / 4) + q4) * kSqdkBM + r];
+      if (x.y == kUnseen) continue;
+      none = false;
+      const float top = fmaxf(M, x.x);
+      const float f = x.x == top ? 1.0f : fast_exp2(x.x - top), g = M == top ? 1.0f : fast_exp2(M - top);
+      M = top;
+      l = g * l + f * x.y;
+      o.x = g * o.x + f * v.x, o.y = g * o.y + f * v.y, o.z = g * o.z + f * v.z, o.w = g * o.w + f * v.w;
     }
-#pragma unroll
-    for (int i = 0; i < 2; ++i) {
-      const int r = r0 + i;
-      if (r >= rows || lane >= HD / 4 || lane * 4 >= p.a.hd) continue;
-      const float inv = 1.0f / l[i];
-      const int ql = r / p.a.G;
-      uint2 w;
-      w.x = none[i] ? 0u : pack2<kBF16>(o[i].x * inv, o[i].y * inv);
-      w.y = none[i] ? 0u : pack2<kBF16>(o[i].z * inv, o[i].w * inv);
-      *reinterpret_cast<uint2*>(p.a.o + static_cast<int64_t>(note.x + ql) * p.a.o_sn +
-                                static_cast<int64_t>(note.z * p.a.G + r - ql * p.a.G) * p.a.o_sh + lane * 8) = w;
-    }
+    const float inv = 1.0f / l;
+    const int ql = r / p.a.G;
+    uint2 w;
+    w.x = none ? 0u : pack2<kBF16>(o.x * inv, o.y * inv);
+    w.y = none ? 0u : pack2<kBF16>(o.z * inv, o.w * inv);
+    *reinterpret_cast<uint2*>(p.a.o + static_cast<int64_t>(note.x + ql) * p.a.o_sn +
+                              static_cast<int64_t>(note.z * p.a.G + r - ql * p.a.G) * p.a.o_sh + q4 * 8) = w;
   }
 }
 
