@@ -30,6 +30,7 @@ constexpr int kPagedRows = 16;     // query rows of an item
 constexpr int kPagedWarps = 4;     // a quarter of a unit's keys each
 constexpr int kPagedThreads = 32 * kPagedWarps;
 constexpr int kPagedStages = 3;
+constexpr int kPagedItemCost = 1;  // what opening and closing an item takes, in units
 constexpr int kPagedCtasPerSm = 2;
 
 // Row sum of a part that holds no key its row sees (a true sum is not negative).
@@ -63,57 +64,73 @@ struct PagedRequest {
   int kv;          // visible keys at most
   int tiles;       // 16-row tiles
   int nb;          // units of an item (one at least: it writes the rows)
-  int64_t units;   // tiles * Hkv * nb
 };
 
+// A request as it lies in memory.
+struct PagedRaw {
+  int a, b, kv;
+};
+
+__device__ __forceinline__ PagedRaw paged_raw(const PagedAttnParams& p, int r) {
+  PagedRaw x;
+  x.a = r <= p.R ? __ldg(p.cu_q + r) : 0;
+  x.b = r < p.R ? __ldg(p.cu_q + r + 1) : static_cast<int>(p.N);
+  x.kv = r < p.R ? __ldg(p.kv_lens + r) : 0;
+  return x;
+}
+
 // The request's rows and keys (its tiles not counted).
-__device__ __forceinline__ PagedRequest paged_rows(const PagedAttnParams& p, int r) {
+__device__ __forceinline__ PagedRequest paged_rows(const PagedAttnParams& p, const PagedRaw& x) {
   PagedRequest q;
   const int N = static_cast<int>(p.N);
-  const int a = min(max(__ldg(p.cu_q + r), 0), N);
-  const int b = r < p.R ? min(max(__ldg(p.cu_q + r + 1), 0), N) : N;
+  const int a = min(max(x.a, 0), N), b = min(max(x.b, 0), N);
   const int64_t cap = static_cast<int64_t>(p.P) << p.shift;
-  const int64_t kv = r < p.R ? max(__ldg(p.kv_lens + r), 0) : 0;
   q.q0 = a;
   q.rows = max(b - a, 0) * p.G;
-  q.kv = static_cast<int>(min(kv, cap));
+  q.kv = static_cast<int>(min(static_cast<int64_t>(max(x.kv, 0)), cap));
   return q;
 }
 
 template <int kKeys>
-__device__ __forceinline__ PagedRequest paged_request(const PagedAttnParams& p, int r) {
-  PagedRequest q = paged_rows(p, r);
+__device__ __forceinline__ PagedRequest paged_request(const PagedAttnParams& p, const PagedRaw& x, int r) {
+  PagedRequest q = paged_rows(p, x);
   q.tiles = r < p.R && q.rows > p.split_rows ? 0 : (q.rows + kPagedRows - 1) / kPagedRows;
   q.nb = max(1, (q.kv + kKeys - 1) / kKeys);
-  q.units = static_cast<int64_t>(q.tiles) * p.Hkv * q.nb;
   return q;
 }
 
-// Units of the whole list; every lane of the warp gets the sum.
+// A request's cost in the list.
+template <int kKeys>
+__device__ __forceinline__ int64_t paged_cost(const PagedAttnParams& p, int r) {
+  if (r > p.R) return 0;
+  const PagedRequest q = paged_request<kKeys>(p, paged_raw(p, r), r);
+  return static_cast<int64_t>(q.tiles) * p.Hkv * (q.nb + kPagedItemCost);
+}
+
+// Cost of the whole list; every lane of the warp gets the sum.
 template <int kKeys>
 __device__ __forceinline__ int64_t paged_total(const PagedAttnParams& p, int lane) {
   int64_t n = 0;
-  for (int r = lane; r <= p.R; r += 32) n += paged_request<kKeys>(p, r).units;
+  for (int r = lane; r <= p.R; r += 32) n += paged_cost<kKeys>(p, r);
 #pragma unroll
   for (int d = 16; d > 0; d >>= 1) n += __shfl_xor_sync(0xFFFFFFFFu, n, d);
   return n;
 }
 
-// The request that unit u (< the total) belongs to and the list's units before
-// it, found by the whole warp.
+// The request that holds list place w (below the total) and the cost before it,
+// found by the whole warp.
 template <int kKeys>
-__device__ __forceinline__ int paged_locate(const PagedAttnParams& p, int64_t u, int lane, int64_t& before) {
+__device__ __forceinline__ int paged_locate(const PagedAttnParams& p, int64_t w, int lane, int64_t& before) {
   int64_t base = 0;
   for (int r0 = 0; r0 <= p.R; r0 += 32) {
-    const int r = r0 + lane;
-    const int64_t mine = r <= p.R ? paged_request<kKeys>(p, r).units : 0;
+    const int64_t mine = paged_cost<kKeys>(p, r0 + lane);
     int64_t sum = mine;
 #pragma unroll
     for (int d = 1; d < 32; d <<= 1) {
       const int64_t x = __shfl_up_sync(0xFFFFFFFFu, sum, d);
       if (lane >= d) sum += x;
     }
-    const unsigned past = __ballot_sync(0xFFFFFFFFu, base + sum > u);
+    const unsigned past = __ballot_sync(0xFFFFFFFFu, base + sum > w);
     if (past) {
       const int l = __ffs(past) - 1;
       before = base + __shfl_sync(0xFFFFFFFFu, sum - mine, l);
@@ -122,7 +139,7 @@ __device__ __forceinline__ int paged_locate(const PagedAttnParams& p, int64_t u,
     base += __shfl_sync(0xFFFFFFFFu, sum, 31);
   }
   before = base;
-  return p.R;  // not reached for u below the total
+  return p.R;  // not reached for w below the total
 }
 
 // a / b; 64-bit divisions are slow, and most operands here fit 32 bits.
@@ -153,29 +170,54 @@ struct Runs {
   }
 };
 
-// A place in the list: request, row tile, head and key unit.
+// A unit of a run: request, row tile, head and key unit. The next request is
+// read ahead, so that coming to it costs no wait.
 template <int kKeys>
 struct PagedCursor {
   PagedRequest req;
-  int r, tile, head, j;
-  __device__ __forceinline__ void set(const PagedAttnParams& p, int request, int64_t local) {
+  PagedRaw ahead;
+  int r, tile, head;
+  int j, jend;  // unit, and the end of this run's units of the item
+  int64_t a, end;  // the item's place in the list, the run's end
+  __device__ __forceinline__ void cut() {
+    const int64_t left = end - a - kPagedItemCost;
+    jend = static_cast<int>(min(max(left, static_cast<int64_t>(0)), static_cast<int64_t>(req.nb)));
+  }
+  // To the run [w0, w1), whose start lies in request `request` with `before` before it.
+  __device__ __forceinline__ void open(const PagedAttnParams& p, int request, int64_t before, int64_t w0, int64_t w1) {
     r = request;
-    req = paged_request<kKeys>(p, r);
-    const int64_t item = div_wide(local, req.nb);
-    j = static_cast<int>(local - item * req.nb);
+    req = paged_request<kKeys>(p, paged_raw(p, r), r);
+    ahead = paged_raw(p, r + 1);
+    const int64_t local = w0 - before, cost = req.nb + kPagedItemCost;
+    const int64_t item = div_wide(local, cost);
+    j = static_cast<int>(max(local - item * cost - kPagedItemCost, static_cast<int64_t>(0)));
     tile = static_cast<int>(div_wide(item, p.Hkv));
     head = static_cast<int>(item - static_cast<int64_t>(tile) * p.Hkv);
+    a = before + item * cost;
+    end = w1;
+    cut();
   }
-  // Only called while a next unit exists.
+  __device__ __forceinline__ bool valid() const { return j < jend; }
+  // To the run's next unit, if there is one (valid() tells).
   __device__ __forceinline__ void next(const PagedAttnParams& p) {
-    if (++j < req.nb) return;
+    if (++j < jend) return;
+    a += req.nb + kPagedItemCost;
+    if (a + kPagedItemCost >= end) {  // the run ends in front of the next item's first unit
+      jend = 0;
+      return;
+    }
     j = 0;
-    if (++head < p.Hkv) return;
-    head = 0;
-    if (++tile < req.tiles) return;
-    tile = 0;
-    do req = paged_request<kKeys>(p, ++r);
-    while (req.units == 0 && r < p.R);
+    if (++head == p.Hkv) {
+      head = 0;
+      if (++tile == req.tiles) {
+        tile = 0;
+        do {
+          req = paged_request<kKeys>(p, ahead, ++r);
+          ahead = paged_raw(p, r + 1);
+        } while (req.tiles == 0 && r < p.R);
+      }
+    }
+    cut();
   }
 };
 
@@ -187,6 +229,9 @@ __device__ __forceinline__ int64_t paged_row(int q0, int row, int head, int G, i
 
 __device__ __forceinline__ void cp_async16(uint32_t dst, const void* src, bool full) {
   asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(dst), "l"(src), "r"(full ? 16 : 0) : "memory");
+}
+__device__ __forceinline__ void cp_async8(uint32_t dst, const void* src) {
+  asm volatile("cp.async.ca.shared.global [%0], [%1], 8;" ::"r"(dst), "l"(src) : "memory");
 }
 __device__ __forceinline__ void cp_async_commit() { asm volatile("cp.async.commit_group;" ::: "memory"); }
 template <int n>
@@ -249,7 +294,9 @@ struct PagedLayout {
   static constexpr int kKeys = kPagedWarps * kWarpKeys;
   static constexpr int kWarpStage = 2 * kWarpKeys * kRow;
   static constexpr int kStage = kPagedWarps * kWarpStage;
-  static constexpr int kBytes = kPagedStages * kStage;
+  static constexpr int kQSlot = kPagedRows * HD * 2;              // a tile's query rows
+  static constexpr int kQOff = kPagedStages * kStage;
+  static constexpr int kBytes = kQOff + kPagedStages * kQSlot;
   // at the end of an item a warp leaves its 16 x HD fp32 O in the stage it has just consumed
   static_assert(kWarpStage >= kPagedRows * HD * 4, "an O tile fits a warp's stage");
 };
@@ -266,21 +313,26 @@ __global__ void __launch_bounds__(kPagedThreads, kPagedCtasPerSm) paged_attn_ker
   using L = PagedLayout<HD>;
   extern __shared__ __align__(128) uint8_t paged_smem[];
   __shared__ float s_m[kPagedWarps][kPagedRows], s_l[kPagedWarps][kPagedRows];
+  __shared__ __align__(8) int64_t s_pos[kPagedStages][kPagedRows];
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   const int g = lane >> 2, t2 = (lane & 3) * 2;  // accumulator row and first column of this lane
   grid_dependents_launch();
   const int64_t total = paged_total<L::kKeys>(p, lane);
   const int64_t runs = min(static_cast<int64_t>(gridDim.x), total);
-  if (blockIdx.x >= runs) {
+  PagedCursor<L::kKeys> cur, ahead;
+  const Runs run(total, max(runs, static_cast<int64_t>(1)));
+  if (blockIdx.x < runs) {
+    const int64_t w0 = run.start(blockIdx.x), w1 = run.start(blockIdx.x + 1);
+    int64_t before;
+    const int r0 = paged_locate<L::kKeys>(p, w0, lane, before);
+    cur.open(p, r0, before, w0, w1);
+  } else {
+    cur.j = cur.jend = 0;
+  }
+  if (!cur.valid()) {
     if (threadIdx.x == 0) p.merges[blockIdx.x] = make_int4(0, 0, 0, -1);
     return;
   }
-  const Runs run(total, runs);
-  const int64_t u0 = run.start(blockIdx.x), u1 = run.start(blockIdx.x + 1);
-  int64_t before;
-  const int r0 = paged_locate<L::kKeys>(p, u0, lane, before);
-  PagedCursor<L::kKeys> cur, ahead;
-  cur.set(p, r0, u0 - before);
   ahead = cur;
   const uint32_t wbase = smem_u32(paged_smem) + warp * L::kWarpStage;
   constexpr int kChunks = HD / 8;           // 16-byte chunks of a row
@@ -295,6 +347,24 @@ __global__ void __launch_bounds__(kPagedThreads, kPagedCtasPerSm) paged_attn_ker
   // This warp's keys of the unit `ahead` points at, into ring stage s. Keys past
   // the visible range or in a page that does not exist arrive as zeros (no bytes
   // are read; the address then is any valid one).
+  // With an item's first unit come its query rows (a quarter a warp) and their
+  // positions, into slot q_ahead.
+  const uint32_t qbase = smem_u32(paged_smem) + L::kQOff;
+  int q_ahead = 0, q_cur = 0;
+  auto request_rows = [&]() {
+#pragma unroll
+    for (int i = 0; i < 4 / kPerIter; ++i) {
+      const int lr = warp * 4 + i * kPerIter + ld_row, row = ahead.tile * kPagedRows + lr;
+      const bool there = row < ahead.req.rows && ld_col;
+      const char* src = p.q + paged_row(ahead.req.q0, there ? row : 0, ahead.head, p.G, p.q_sn, p.q_sh) +
+                        (there ? ld_chunk * 16 : 0);
+      cp_async16(qbase + q_ahead * L::kQSlot + lr * L::kRow + ((ld_chunk ^ (lr & 7)) << 4), src, there);
+    }
+    const int row = ahead.tile * kPagedRows + lane;
+    if (warp == 0 && lane < kPagedRows && row < ahead.req.rows)
+      cp_async8(smem_u32(&s_pos[q_ahead][lane]), p.pos + ahead.req.q0 + row / p.G);
+    q_ahead = q_ahead + 1 == kPagedStages ? 0 : q_ahead + 1;
+  };
   auto request = [&](int s) {
     const int key0 = ahead.j * L::kKeys + warp * L::kWarpKeys;
     const uint32_t kdst = wbase + s * L::kStage, vdst = kdst + L::kWarpKeys * L::kRow;
@@ -329,13 +399,12 @@ __global__ void __launch_bounds__(kPagedThreads, kPagedCtasPerSm) paged_attn_ker
     gone_ring = (gone_ring & ~(((1u << kGroups) - 1) << (kGroups * s))) | gone << (kGroups * s);
   };
 
-  int64_t ua = u0;
 #pragma unroll
   for (int s = 0; s < kPagedStages - 1; ++s) {
-    if (ua < u1) {
-      if (ua > u0) ahead.next(p);
+    if (ahead.valid()) {
+      if (s == 0 || ahead.j == 0) request_rows();
       request(s);
-      ++ua;
+      ahead.next(p);
     }
     cp_async_commit();
   }
@@ -346,35 +415,33 @@ __global__ void __launch_bounds__(kPagedThreads, kPagedCtasPerSm) paged_attn_ker
   bool seen[2] = {};  // the row has met a key that it sees
   int lim[2] = {}, lim_min = 0, lim_max = 0;
   bool fresh = true;  // the next unit opens an item (or this run's part of one)
-  int64_t seg0 = u0;
+  int seg_j = 0;      // the part's first unit
   int stage = 0;
-  for (int64_t u = u0; u < u1; ++u) {
+  while (cur.valid()) {
+    cp_async_wait<kPagedStages - 2>();
     if (fresh) {
+      // every warp's share of the query rows has arrived, and every warp has
+      // left the item before (its O in a stage, its maxima and sums)
+      __syncthreads();
       fresh = false;
-      seg0 = u;
-      // rows of this tile: q fragments, and the last key that each row sees
+      seg_j = cur.j;
+#pragma unroll
+      for (int kk = 0; kk < HD / 16; ++kk) {
+        const int lr = (lane & 7) + (((lane >> 3) & 1) << 3), chunk = kk * 2 + (lane >> 4);
+        ldmatrix_x4(qa[kk], qbase + q_cur * L::kQSlot + lr * L::kRow + ((chunk ^ (lr & 7)) << 4));
+      }
+      // the last key that each row sees
       lim_min = 0x7FFFFFFF;
       lim_max = -1;
 #pragma unroll
       for (int i = 0; i < 2; ++i) {
-        const int row = cur.tile * kPagedRows + g + 8 * i;
         lim[i] = -1;
-        if (row < cur.req.rows) {
-          const int64_t ps = __ldg(p.pos + cur.req.q0 + row / p.G);
+        if (cur.tile * kPagedRows + g + 8 * i < cur.req.rows) {
+          const int64_t ps = s_pos[q_cur][g + 8 * i];
           if (ps >= cur.req.kv && cur.r < p.R) raise_device_error(HSPMN_DEVERR_POSITION);
           lim[i] = static_cast<int>(min(max(ps, static_cast<int64_t>(-1)), static_cast<int64_t>(cur.req.kv) - 1));
           if (lim[i] >= 0) lim_min = min(lim_min, lim[i]);
           lim_max = max(lim_max, lim[i]);
-        }
-        const char* src = p.q + paged_row(cur.req.q0, row < cur.req.rows ? row : 0, cur.head, p.G, p.q_sn, p.q_sh);
-#pragma unroll
-        for (int kk = 0; kk < HD / 16; ++kk) {
-#pragma unroll
-          for (int c = 0; c < 2; ++c) {
-            const int col = kk * 16 + c * 8 + t2;
-            qa[kk][2 * c + i] =
-                row < cur.req.rows && col < p.hd ? __ldg(reinterpret_cast<const uint32_t*>(src + col * 2)) : 0u;
-          }
         }
         m_run[i] = -INFINITY;
         l_run[i] = 0.0f;
@@ -382,13 +449,14 @@ __global__ void __launch_bounds__(kPagedThreads, kPagedCtasPerSm) paged_attn_ker
       }
       lim_min = __reduce_min_sync(0xFFFFFFFFu, lim_min);
       lim_max = __reduce_max_sync(0xFFFFFFFFu, lim_max);
+      q_cur = q_cur + 1 == kPagedStages ? 0 : q_cur + 1;
 #pragma unroll
       for (int n = 0; n < HD / 8; ++n)
 #pragma unroll
         for (int e = 0; e < 4; ++e) acc[n][e] = 0.0f;
+    } else {
+      __syncwarp();
     }
-    cp_async_wait<kPagedStages - 2>();
-    __syncwarp();
     const int key0 = cur.j * L::kKeys + warp * L::kWarpKeys;
     const uint32_t kst = wbase + stage * L::kStage, vst = kst + L::kWarpKeys * L::kRow;
     if (key0 <= lim_max) {
@@ -509,8 +577,7 @@ __global__ void __launch_bounds__(kPagedThreads, kPagedCtasPerSm) paged_attn_ker
         }
       }
     }
-    const bool item_end = cur.j == cur.req.nb - 1;
-    if (item_end || u + 1 == u1) {
+    if (cur.j + 1 == cur.jend) {
       // the warps' results of this item: O in the stage each has just
       // consumed, maxima and sums beside it
       __syncwarp();
@@ -528,19 +595,15 @@ __global__ void __launch_bounds__(kPagedThreads, kPagedCtasPerSm) paged_attn_ker
         l += __shfl_xor_sync(0xFFFFFFFFu, l, 2);
         if ((lane & 3) == 0) s_m[warp][g + 8 * i] = m_run[i], s_l[warp][g + 8 * i] = seen[i] ? l : kUnseen;
       }
-      if (u + 1 == u1 && threadIdx.x == 0) {
-        // an item that opens in this run and goes on behind it is merged from here
-        const int64_t open = u - cur.j;
-        const bool first = !item_end && open >= u0;
-        p.merges[blockIdx.x] =
-            make_int4(cur.req.q0, cur.tile * kPagedRows,
-                      cur.head * kPagedRows + min(kPagedRows, cur.req.rows - cur.tile * kPagedRows) - 1,
-                      first ? run.of(open + cur.req.nb - 1) : -1);
-      }
+      const bool item_end = cur.jend == cur.req.nb, whole = item_end && seg_j == 0;
+      // an item that opens in this run and goes on behind it is merged from here
+      if (threadIdx.x == 0 && (!item_end || cur.a + cur.req.nb + 2 * kPagedItemCost >= cur.end))
+        p.merges[blockIdx.x] = make_int4(cur.req.q0, cur.tile * kPagedRows,
+                                         cur.head * kPagedRows + min(kPagedRows, cur.req.rows - cur.tile * kPagedRows) - 1,
+                                         !item_end && seg_j == 0 ? run.of(cur.a + kPagedItemCost + cur.req.nb - 1) : -1);
       __syncthreads();
-      const bool whole = item_end && seg0 + cur.req.nb == u + 1;
       // a run holds the last piece of one item at most, and the first of one
-      const int64_t slot = 2 * static_cast<int64_t>(blockIdx.x) + (u - cur.j >= u0 ? 1 : 0);
+      const int64_t slot = 2 * static_cast<int64_t>(blockIdx.x) + (seg_j == 0 ? 1 : 0);
       constexpr int kQuads = HD / 4;  // 4-column groups of a row
       for (int i = threadIdx.x; i < kPagedRows * kQuads; i += kPagedThreads) {
         const int lr = i / kQuads, c = (i % kQuads) * 4;
@@ -574,20 +637,18 @@ __global__ void __launch_bounds__(kPagedThreads, kPagedCtasPerSm) paged_attn_ker
           if (c == 0) reinterpret_cast<float2*>(p.part_ml)[slot * kPagedRows + lr] = make_float2(M, none ? kUnseen : l);
         }
       }
-      __syncthreads();
       fresh = true;
     }
-    // refill the stage that this unit has left (its readers are this warp, or
-    // have passed the barrier above)
+    // refill the stage that the unit before this one has left
     __syncwarp();
-    if (ua < u1) {
-      ahead.next(p);
+    if (ahead.valid()) {
+      if (ahead.j == 0) request_rows();
       request((stage + kPagedStages - 1) % kPagedStages);
-      ++ua;
+      ahead.next(p);
     }
     cp_async_commit();
     stage = stage + 1 == kPagedStages ? 0 : stage + 1;
-    if (u + 1 < u1) cur.next(p);
+    cur.next(p);
   }
   cp_async_wait<0>();
 }

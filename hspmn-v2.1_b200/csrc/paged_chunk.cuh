@@ -78,7 +78,7 @@ struct ChunkRequest {
 
 __device__ __forceinline__ ChunkRequest chunk_request(const ChunkParams& p, int r) {
   ChunkRequest c;
-  const PagedRequest q = paged_rows(p.a, r);
+  const PagedRequest q = paged_rows(p.a, paged_raw(p.a, r));
   c.q0 = q.q0;
   c.len = q.rows / p.a.G;
   c.kv = q.kv;
