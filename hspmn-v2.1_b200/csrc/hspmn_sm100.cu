@@ -999,6 +999,9 @@ int hspmn_sqdk_paged_fwd(const void* q, int64_t q_sn, int64_t q_sh, const void* 
   if (Hkv == 1) kc_sh = vc_sh = hd;
   if (num_pages == 1) kc_sp = vc_sp = page_size * Hkv * hd;
   if (int rc = check_strides({q_sn, q_sh, kc_sp, kc_ss, kc_sh, vc_sp, vc_ss, vc_sh, o_sn, o_sh}, es)) return rc;
+  // the kernels step through pages and slots with 32-bit strides
+  if (kc_sp >= (1LL << 30) || kc_ss >= (1LL << 30) || vc_sp >= (1LL << 30) || vc_ss >= (1LL << 30))
+    return HSPMN_ERR_UNSUPPORTED;
   if (!aligned(q, 16) || !aligned(k_cache, 16) || !aligned(v_cache, 16) || !aligned(o, 16) || !aligned(workspace, 16))
     return HSPMN_ERR_ALIGN;
   if (N == 0) return HSPMN_OK;
@@ -1017,8 +1020,9 @@ int hspmn_sqdk_paged_fwd(const void* q, int64_t q_sn, int64_t q_sh, const void* 
   prm.v = static_cast<const char*>(v_cache);
   prm.o = static_cast<char*>(o);
   prm.q_sn = q_sn * es, prm.q_sh = q_sh * es, prm.o_sn = o_sn * es, prm.o_sh = o_sh * es;
-  prm.k_sp = kc_sp * es, prm.k_ss = kc_ss * es, prm.k_sh = kc_sh * es;
-  prm.v_sp = vc_sp * es, prm.v_ss = vc_ss * es, prm.v_sh = vc_sh * es;
+  prm.k_sp = static_cast<unsigned>(kc_sp * es), prm.k_ss = static_cast<unsigned>(kc_ss * es);
+  prm.v_sp = static_cast<unsigned>(vc_sp * es), prm.v_ss = static_cast<unsigned>(vc_ss * es);
+  prm.k_sh = kc_sh * es, prm.v_sh = vc_sh * es;
   prm.table = block_table;
   prm.table_rs = table_rs;
   prm.kv_lens = kv_lens;

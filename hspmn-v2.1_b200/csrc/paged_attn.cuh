@@ -30,7 +30,7 @@ constexpr int kPagedRows = 16;     // query rows of an item
 constexpr int kPagedWarps = 4;     // a quarter of a unit's keys each
 constexpr int kPagedThreads = 32 * kPagedWarps;
 constexpr int kPagedStages = 3;
-constexpr int kPagedItemCost = 1;  // what opening and closing an item takes, in units
+constexpr int kPagedItemCost = 2;  // what opening and closing an item takes, in units (68.0 us against 86.3 at 0, 68.7 at 1, 69.6 at 3: 37 x 16 items of 1 to 64 units)
 constexpr int kPagedCtasPerSm = 2;
 
 // Row sum of a part that holds no key its row sees (a true sum is not negative).
@@ -41,8 +41,9 @@ struct PagedAttnParams {
   const char* k;
   const char* v;
   char* o;
-  int64_t q_sn, q_sh, o_sn, o_sh;                    // bytes
-  int64_t k_sp, k_ss, k_sh, v_sp, v_ss, v_sh;        // bytes: page, slot in the page, head
+  int64_t q_sn, q_sh, o_sn, o_sh;   // bytes
+  unsigned k_sp, k_ss, v_sp, v_ss;  // bytes: page, slot in the page
+  int64_t k_sh, v_sh;               // bytes: head
   const int* table;  // [R,P], row stride table_rs
   int64_t table_rs;
   const int* kv_lens;
@@ -230,6 +231,9 @@ __device__ __forceinline__ int64_t paged_row(int q0, int row, int head, int G, i
 __device__ __forceinline__ void cp_async16(uint32_t dst, const void* src, bool full) {
   asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(dst), "l"(src), "r"(full ? 16 : 0) : "memory");
 }
+__device__ __forceinline__ void cp_async16(uint32_t dst, const void* src) {
+  asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(dst), "l"(src) : "memory");
+}
 __device__ __forceinline__ void cp_async8(uint32_t dst, const void* src) {
   asm volatile("cp.async.ca.shared.global [%0], [%1], 8;" ::"r"(dst), "l"(src) : "memory");
 }
@@ -344,9 +348,6 @@ __global__ void __launch_bounds__(kPagedThreads, kPagedCtasPerSm) paged_attn_ker
   const int mask = (1 << p.shift) - 1;
   uint32_t gone_ring = 0;  // kGroups bits a stage: the group's page does not exist
 
-  // This warp's keys of the unit `ahead` points at, into ring stage s. Keys past
-  // the visible range or in a page that does not exist arrive as zeros (no bytes
-  // are read; the address then is any valid one).
   // With an item's first unit come its query rows (a quarter a warp) and their
   // positions, into slot q_ahead.
   const uint32_t qbase = smem_u32(paged_smem) + L::kQOff;
@@ -365,37 +366,46 @@ __global__ void __launch_bounds__(kPagedThreads, kPagedCtasPerSm) paged_attn_ker
       cp_async8(smem_u32(&s_pos[q_ahead][lane]), p.pos + ahead.req.q0 + row / p.G);
     q_ahead = q_ahead + 1 == kPagedStages ? 0 : q_ahead + 1;
   };
+  // This warp's keys of the unit `ahead` points at, into ring stage s. Keys past
+  // the visible range or in a page that does not exist arrive as zeros: no byte
+  // is read for them.
+  const int ld_byte = ld_col ? ld_chunk * 16 : 0;
+  const uint32_t ld_dst = ld_row * L::kRow;
   auto request = [&](int s) {
-    const int key0 = ahead.j * L::kKeys + warp * L::kWarpKeys;
-    const uint32_t kdst = wbase + s * L::kStage, vdst = kdst + L::kWarpKeys * L::kRow;
+    const int key0 = ahead.j * L::kKeys + warp * L::kWarpKeys, left = ahead.req.kv - key0;
+    const uint32_t kdst = wbase + s * L::kStage + ld_dst, vdst = kdst + L::kWarpKeys * L::kRow;
     const int* row = p.table + static_cast<int64_t>(ahead.r) * p.table_rs;
+    const char* kh = p.k + static_cast<int64_t>(ahead.head) * p.k_sh + ld_byte;
+    const char* vh = p.v + static_cast<int64_t>(ahead.head) * p.v_sh + ld_byte;
     int page[kGroups];
 #pragma unroll
-    for (int i = 0; i < kGroups; ++i) page[i] = key0 + 8 * i < ahead.req.kv ? __ldg(row + ((key0 + 8 * i) >> p.shift)) : -1;
+    for (int i = 0; i < kGroups; ++i) page[i] = 8 * i < left ? __ldg(row + ((key0 + 8 * i) >> p.shift)) : 0;
     uint32_t gone = 0;
 #pragma unroll
+    for (int i = 0; i < kGroups; ++i) gone |= (static_cast<unsigned>(page[i]) >= static_cast<unsigned>(p.num_pages) ? 1u : 0u) << i;
+    const bool full = left >= L::kWarpKeys && gone == 0 && p.hd == HD;
+#pragma unroll
     for (int i = 0; i < kGroups; ++i) {
-      const bool there = page[i] >= 0 && page[i] < p.num_pages;
-      if (!there && key0 + 8 * i < ahead.req.kv) {
-        gone |= 1u << i;
-        if (lane == 0) raise_device_error(HSPMN_DEVERR_PAGE);
-      }
-      const int64_t pg = there ? page[i] : 0;
-      const int64_t off = there ? ((key0 + 8 * i) & mask) + ld_row : 0;
-      const int col = there && ld_col ? ld_chunk * 16 : 0;
-      const char* ks = p.k + pg * p.k_sp + off * p.k_ss + ahead.head * p.k_sh + col;
-      const char* vs = p.v + pg * p.v_sp + off * p.v_ss + ahead.head * p.v_sh + col;
-      const int64_t kstep = there ? kPerIter * p.k_ss : 0, vstep = there ? kPerIter * p.v_ss : 0;
-      const int left = there && ld_col ? ahead.req.kv - key0 - 8 * i - ld_row : 0;  // rows from here on that count
+      const unsigned pg = gone >> i & 1 ? 0u : static_cast<unsigned>(page[i]);
+      const unsigned off = ((key0 + 8 * i) & mask) + ld_row;
+      const char* ks = kh + static_cast<uint64_t>(pg) * p.k_sp + static_cast<uint64_t>(off) * p.k_ss;
+      const char* vs = vh + static_cast<uint64_t>(pg) * p.v_sp + static_cast<uint64_t>(off) * p.v_ss;
+      const int rows = gone >> i & 1 || !ld_col ? 0 : left - 8 * i - ld_row;  // rows from here on that count
 #pragma unroll
       for (int x = 0; x < 8 / kPerIter; ++x) {
-        const int kr = 8 * i + x * kPerIter + ld_row;
-        const uint32_t d = kr * L::kRow + ((ld_chunk ^ (kr & 7)) << 4);
-        cp_async16(kdst + d, ks, x * kPerIter < left);
-        cp_async16(vdst + d, vs, x * kPerIter < left);
-        ks += kstep, vs += vstep;
+        const int kr = 8 * i + x * kPerIter;
+        const uint32_t d = kr * L::kRow + ((ld_chunk ^ ((kr & 7) + ld_row)) << 4);
+        if (full) {
+          cp_async16(kdst + d, ks);
+          cp_async16(vdst + d, vs);
+        } else {
+          cp_async16(kdst + d, ks, x * kPerIter < rows);
+          cp_async16(vdst + d, vs, x * kPerIter < rows);
+        }
+        ks += kPerIter * p.k_ss, vs += kPerIter * p.v_ss;
       }
     }
+    if (gone && lane == 0) raise_device_error(HSPMN_DEVERR_PAGE);
     gone_ring = (gone_ring & ~(((1u << kGroups) - 1) << (kGroups * s))) | gone << (kGroups * s);
   };
 
@@ -556,23 +566,26 @@ __global__ void __launch_bounds__(kPagedThreads, kPagedCtasPerSm) paged_attn_ker
         }
       } else {
 #pragma unroll
-        for (int kr = 0; kr < L::kWarpKeys; ++kr) {
-          const int src = (lane & ~3) | ((kr & 7) >> 1);  // the lane of this quad that holds the key's column
-          float w[2];
-          bool sees[2];
+        for (int k8 = 0; k8 < kGroups; ++k8) {
+#pragma unroll 1
+          for (int kr = 0; kr < 8; ++kr) {
+            const int src = (lane & ~3) | (kr >> 1);  // the lane of this quad that holds the key's column
+            float w[2];
+            bool sees[2];
 #pragma unroll
-          for (int i = 0; i < 2; ++i) {
-            w[i] = __shfl_sync(0xFFFFFFFFu, s[kr >> 3][2 * i + (kr & 1)], src);
-            sees[i] = key0 + kr <= lim[i] && !(gone >> (kr >> 3) & 1);
-          }
+            for (int i = 0; i < 2; ++i) {
+              w[i] = __shfl_sync(0xFFFFFFFFu, kr & 1 ? s[k8][2 * i + 1] : s[k8][2 * i], src);
+              sees[i] = key0 + 8 * k8 + kr <= lim[i] && !(gone >> k8 & 1);
+            }
 #pragma unroll
-          for (int n = 0; n < HD / 8; ++n) {
-            uint32_t two;
-            asm volatile("ld.shared.u32 %0, [%1];" : "=r"(two) : "r"(vst + kr * L::kRow + ((n ^ (kr & 7)) << 4) + t2 * 2));
-            const float x = half_to_float<kBF16>(static_cast<uint16_t>(two)), y = half_to_float<kBF16>(two >> 16);
+            for (int n = 0; n < HD / 8; ++n) {
+              uint32_t two;
+              asm volatile("ld.shared.u32 %0, [%1];" : "=r"(two) : "r"(vst + (8 * k8 + kr) * L::kRow + ((n ^ kr) << 4) + t2 * 2));
+              const float x = half_to_float<kBF16>(static_cast<uint16_t>(two)), y = half_to_float<kBF16>(two >> 16);
 #pragma unroll
-            for (int i = 0; i < 2; ++i)
-              if (sees[i]) acc[n][2 * i] = fmaf(w[i], x, acc[n][2 * i]), acc[n][2 * i + 1] = fmaf(w[i], y, acc[n][2 * i + 1]);
+              for (int i = 0; i < 2; ++i)
+                if (sees[i]) acc[n][2 * i] = fmaf(w[i], x, acc[n][2 * i]), acc[n][2 * i + 1] = fmaf(w[i], y, acc[n][2 * i + 1]);
+            }
           }
         }
       }

@@ -720,7 +720,8 @@ __global__ void __launch_bounds__(kChunkThreads, kChunkCtasPerSm)
           for (int key = from; key <= to; ++key) {
             const int pg = __ldg(row + (key >> p.a.shift));
             if (pg < 0 || pg >= p.a.num_pages) continue;
-            const char* v = p.a.v + pg * p.a.v_sp + (key & ((1 << p.a.shift) - 1)) * p.a.v_ss + head * p.a.v_sh;
+            const char* v = p.a.v + static_cast<int64_t>(pg) * p.a.v_sp +
+                            static_cast<int64_t>(key & ((1 << p.a.shift) - 1)) * p.a.v_ss + head * p.a.v_sh;
 #pragma unroll
             for (int i = 0; i < 32; ++i) {
               if (c + i >= p.a.hd) continue;

@@ -378,7 +378,8 @@ HSPMN_API int64_t hspmn_sqdk_paged_workspace_size(int64_t N, int64_t H, int64_t 
  * that do not see the key.
  * q, o: [N,H,hd], strides (elements) of row and head; caches as above, strides
  * of page, offset and head. dtype HSPMN_BF16 or HSPMN_F16. hd: a multiple of 8
- * up to 128; H % Hkv == 0, H / Hkv <= 128. block_table, kv_lens, cu_q int32;
+ * up to 128; H % Hkv == 0, H / Hkv <= 128; strides of page and offset below
+ * 2^30 elements. block_table, kv_lens, cu_q int32;
  * positions int64, in any order. Bases and strides multiples of 16 bytes.
  * max_q: the largest number of query rows of one request if the caller knows
  * it, else 0; it only chooses kernels, any value is correct.

@@ -61,7 +61,7 @@ def test_attention_refusals():
         assert fwd(**over) == INVALID, over
     for over in (dict(dt=0), dict(dt=7)):
         assert fwd(**over) == DTYPE, over
-    for over in (dict(hd=12), dict(hd=136), dict(H=14), dict(H=516), dict(page=48)):
+    for over in (dict(hd=12), dict(hd=136), dict(H=14), dict(H=516), dict(page=48), dict(sp=1 << 30)):
         assert fwd(**over) == UNSUPPORTED, over
     odd = ctypes.c_void_p(4104)
     for over in (dict(q=odd), dict(o=odd), dict(kc=odd), dict(vc=odd), dict(ws=odd), dict(sn=2052), dict(ss=516)):
