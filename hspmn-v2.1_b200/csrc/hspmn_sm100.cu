@@ -804,31 +804,22 @@ void launch_paged_write(const PagedWriteParams& prm, bool f32_tables, unsigned g
 }
 
 // Launches kern as a programmatic dependent of the kernel before it in the
-// stream: its launch overlaps that kernel's end (it must wait for the results
-// itself, with grid_dependency_wait).
-template <typename Params>
-int launch_dependent(void (*kern)(Params), unsigned grid, unsigned threads, const Params& prm, cudaStream_t st) {
+// stream: it may begin while that kernel ends (and waits for the results, where
+// it needs them, with grid_dependency_wait).
+template <typename... Params>
+int launch_dependent(void (*kern)(Params...), unsigned grid, unsigned threads, size_t smem, cudaStream_t st,
+                     const Params&... prm) {
   cudaLaunchConfig_t cfg = {};
   cfg.gridDim = dim3(grid);
   cfg.blockDim = dim3(threads);
+  cfg.dynamicSmemBytes = smem;
   cfg.stream = st;
   cudaLaunchAttribute attr[1];
   attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
   attr[0].val.programmaticStreamSerializationAllowed = 1;
   cfg.attrs = attr;
   cfg.numAttrs = 1;
-  return cudaLaunchKernelEx(&cfg, kern, prm) == cudaSuccess ? HSPMN_OK : HSPMN_ERR_CUDA;
-}
-
-template <int HD, bool kBF16>
-int launch_paged_attn(const PagedAttnParams& prm, int runs, cudaStream_t st) {
-  auto kern = paged_attn_kernel<HD, kBF16>;
-  constexpr int smem = PagedLayout<HD>::kBytes;
-  if (cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, smem) != cudaSuccess)
-    return HSPMN_ERR_CUDA;
-  kern<<<static_cast<unsigned>(runs), kPagedThreads, smem, st>>>(prm);
-  if (int rc = launch_status()) return rc;
-  return launch_dependent(paged_merge_kernel<HD, kBF16>, static_cast<unsigned>(runs), 32 * kMergeWarps, prm, st);
+  return cudaLaunchKernelEx(&cfg, kern, prm...) == cudaSuccess ? HSPMN_OK : HSPMN_ERR_CUDA;
 }
 
 // Rows (queries * G) of a request up to which its tiles are the 16-row kernel's.
@@ -850,16 +841,32 @@ void paged_ws_carve(PagedAttnParams* prm, void* ws, int64_t runs, int rows, int6
 }
 
 template <int HD, bool kBF16>
-int launch_paged_chunk(const CUtensorMap& mq, const CUtensorMap& mk, const CUtensorMap& mv, const ChunkParams& prm,
-                       int runs, cudaStream_t st) {
-  using L = ChunkLayout<HD>;
-  auto kern = paged_chunk_kernel<HD, kBF16>;
-  if (cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, L::kAlloc) != cudaSuccess)
+int launch_paged(const PagedAttnParams& prm, int runs, cudaStream_t st) {
+  auto kern = paged_attn_kernel<HD, kBF16>;
+  constexpr int smem = PagedLayout<HD>::kBytes;
+  if (cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, smem) != cudaSuccess)
     return HSPMN_ERR_CUDA;
-  kern<<<static_cast<unsigned>(runs), kChunkThreads, L::kAlloc, st>>>(mq, mk, mv, prm);
+  kern<<<static_cast<unsigned>(runs), kPagedThreads, smem, st>>>(prm);
   if (int rc = launch_status()) return rc;
-  return launch_dependent(paged_chunk_merge_kernel<HD, kBF16>, static_cast<unsigned>(runs), 32 * kChunkMergeWarps, prm,
-                          st);
+  return launch_dependent(paged_merge_kernel<HD, kBF16>, static_cast<unsigned>(runs), 32 * kMergeWarps, 0, st, prm);
+}
+
+// The chunk kernel, the 16-row kernel (which needs nothing of the former and
+// fills the SMs as it ends) and the merge of both.
+template <int HD, bool kBF16>
+int launch_paged_chunks(const CUtensorMap& mq, const CUtensorMap& mk, const CUtensorMap& mv, const ChunkParams& ch,
+                        int chunk_runs, const PagedAttnParams& prm, int runs, cudaStream_t st) {
+  auto chunks = paged_chunk_kernel<HD, kBF16>;
+  auto rows = paged_attn_kernel<HD, kBF16>;
+  constexpr int chunk_smem = ChunkLayout<HD>::kAlloc, smem = PagedLayout<HD>::kBytes;
+  if (cudaFuncSetAttribute(chunks, cudaFuncAttributeMaxDynamicSharedMemorySize, chunk_smem) != cudaSuccess ||
+      cudaFuncSetAttribute(rows, cudaFuncAttributeMaxDynamicSharedMemorySize, smem) != cudaSuccess)
+    return HSPMN_ERR_CUDA;
+  chunks<<<static_cast<unsigned>(chunk_runs), kChunkThreads, chunk_smem, st>>>(mq, mk, mv, ch);
+  if (int rc = launch_status()) return rc;
+  if (int rc = launch_dependent(rows, static_cast<unsigned>(runs), kPagedThreads, smem, st, prm)) return rc;
+  return launch_dependent(paged_both_merge_kernel<HD, kBF16>, static_cast<unsigned>(runs + chunk_runs), 32 * kMergeWarps, 0,
+                          st, prm, ch, runs);
 }
 
 }  // namespace
@@ -1069,20 +1076,15 @@ int hspmn_sqdk_paged_fwd(const void* q, int64_t q_sn, int64_t q_sh, const void* 
     const uint32_t kb[4] = {64u, 1u, static_cast<uint32_t>(ch.box_rows), 1u};
     if (int rc = encode_4d(&mk, k_cache, dt, kd, ks, kb)) return rc;
     if (int rc = encode_4d(&mv, v_cache, dt, kd, vs, kb)) return rc;
-    int rc;
     if (hd > 64)
-      rc = dtype == HSPMN_BF16 ? launch_paged_chunk<128, true>(mq, mk, mv, ch, chunk_runs, st)
-                               : launch_paged_chunk<128, false>(mq, mk, mv, ch, chunk_runs, st);
-    else
-      rc = dtype == HSPMN_BF16 ? launch_paged_chunk<64, true>(mq, mk, mv, ch, chunk_runs, st)
-                               : launch_paged_chunk<64, false>(mq, mk, mv, ch, chunk_runs, st);
-    if (rc) return rc;
+      return dtype == HSPMN_BF16 ? launch_paged_chunks<128, true>(mq, mk, mv, ch, chunk_runs, prm, runs, st)
+                                : launch_paged_chunks<128, false>(mq, mk, mv, ch, chunk_runs, prm, runs, st);
+    return dtype == HSPMN_BF16 ? launch_paged_chunks<64, true>(mq, mk, mv, ch, chunk_runs, prm, runs, st)
+                              : launch_paged_chunks<64, false>(mq, mk, mv, ch, chunk_runs, prm, runs, st);
   }
   if (hd > 64)
-    return dtype == HSPMN_BF16 ? launch_paged_attn<128, true>(prm, runs, st)
-                              : launch_paged_attn<128, false>(prm, runs, st);
-  return dtype == HSPMN_BF16 ? launch_paged_attn<64, true>(prm, runs, st)
-                             : launch_paged_attn<64, false>(prm, runs, st);
+    return dtype == HSPMN_BF16 ? launch_paged<128, true>(prm, runs, st) : launch_paged<128, false>(prm, runs, st);
+  return dtype == HSPMN_BF16 ? launch_paged<64, true>(prm, runs, st) : launch_paged<64, false>(prm, runs, st);
 }
 
 int hspmn_device_errors(unsigned* bits, int clear, void* stream) {

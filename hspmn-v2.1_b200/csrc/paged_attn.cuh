@@ -335,6 +335,7 @@ __global__ void __launch_bounds__(kPagedThreads, kPagedCtasPerSm) paged_attn_ker
   }
   if (!cur.valid()) {
     if (threadIdx.x == 0) p.merges[blockIdx.x] = make_int4(0, 0, 0, -1);
+    grid_dependency_wait();
     return;
   }
   ahead = cur;
@@ -664,21 +665,23 @@ __global__ void __launch_bounds__(kPagedThreads, kPagedCtasPerSm) paged_attn_ker
     cur.next(p);
   }
   cp_async_wait<0>();
+  // the kernel before (the chunks' one, or the caller's) is not needed here, but
+  // what comes next counts on it when this grid has ended
+  grid_dependency_wait();
 }
 
 constexpr int kMergeWarps = 32;
 
-// Adds the partial results of the item that opens in run blockIdx.x and goes on
+// Adds the partial results of the item that opens in run c0 and goes on
 // behind it, as that run noted: O = sum 2^(m_c - M) O_c / sum 2^(m_c - M) l_c over
 // the runs in order. A warp takes one row and a share of the runs.
 template <int HD, bool kBF16>
-__global__ void __launch_bounds__(32 * kMergeWarps) paged_merge_kernel(const __grid_constant__ PagedAttnParams p) {
+__device__ __forceinline__ void paged_merge(const PagedAttnParams& p, int c0) {
   __shared__ float4 s_o[kMergeWarps][HD / 4];
   __shared__ float2 s_ml[kMergeWarps];
-  grid_dependency_wait();
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-  const int4 note = p.merges[blockIdx.x];
-  const int c0 = static_cast<int>(blockIdx.x), c1 = note.w;
+  const int4 note = p.merges[c0];
+  const int c1 = note.w;
   if (c1 < 0) return;
   const int rows = note.z % kPagedRows + 1, head = note.z / kPagedRows;
   const int shares = max(1, kMergeWarps / rows);  // warps of a row
@@ -733,6 +736,12 @@ __global__ void __launch_bounds__(32 * kMergeWarps) paged_merge_kernel(const __g
     w.y = empty ? 0u : pack2<kBF16>(y.z * inv, y.w * inv);
     *reinterpret_cast<uint2*>(p.o + paged_row(note.x, note.y + lr, head, p.G, p.o_sn, p.o_sh) + lane * 8) = w;
   }
+}
+
+template <int HD, bool kBF16>
+__global__ void __launch_bounds__(32 * kMergeWarps) paged_merge_kernel(const __grid_constant__ PagedAttnParams p) {
+  grid_dependency_wait();
+  paged_merge<HD, kBF16>(p, static_cast<int>(blockIdx.x));
 }
 
 }  // namespace hspmn

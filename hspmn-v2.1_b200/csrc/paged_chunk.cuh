@@ -34,7 +34,7 @@ namespace hspmn {
 constexpr int kChunkThreads = 192;
 constexpr int kChunkCtasPerSm = 2;
 constexpr int kChunkUnit = 16;           // cost units of a 64-key block
-constexpr int kChunkTileCost = 3;        // blocks' worth of time to open and close a tile
+constexpr int kChunkTileCost = 5;        // blocks' worth of time to open and close a tile
 constexpr int kChunkMinPiece = 4;        // blocks of work below which another run is not opened
 constexpr int kChunkEpilogueBar = 1;     // named barrier of the four softmax warps
 
@@ -165,15 +165,16 @@ struct ChunkList {
     const int64_t rel = w - base;
     c.head = static_cast<int>(div_wide(rel, c.req.head));
     const int64_t in_head = rel - c.head * c.req.head;
-    int lo = 0, hi = c.req.tiles;
-    while (hi - lo > 1) {
-      const int mid = (lo + hi) >> 1;
-      if (c.before(mid) <= in_head) lo = mid;
-      else hi = mid;
-    }
-    c.t = lo;
-    c.start = base + c.head * c.req.head + c.before(lo);
-    c.cost = c.req.first + c.req.slope * lo;
+    // the last tile t with first t + slope t (t - 1) / 2 <= in_head: the root
+    // in float, set right in integers
+    const float b = static_cast<float>(c.req.first) - 0.5f * static_cast<float>(c.req.slope);
+    const float x = static_cast<float>(in_head), root = sqrtf(b * b + 2.0f * static_cast<float>(c.req.slope) * x);
+    int t = min(max(static_cast<int>(2.0f * x / (b + root)), 0), c.req.tiles - 1);
+    while (t > 0 && c.before(t) > in_head) --t;
+    while (t + 1 < c.req.tiles && c.before(t + 1) <= in_head) ++t;
+    c.t = t;
+    c.start = base + c.head * c.req.head + c.before(t);
+    c.cost = c.req.first + c.req.slope * t;
     return c;
   }
 };
@@ -699,7 +700,9 @@ __global__ void __launch_bounds__(kChunkThreads, kChunkCtasPerSm)
       const bool none = !seen;
       const int slot = job.slot, head = job.head;
       const int64_t row0 = job.row0;
-      const float inv_l = slot >= 0 ? 1.0f : 1.0f / l_run;
+      const float inv_l = 1.0f / l_run;
+      char* base = p.a.o + row0 * p.a.o_sn + static_cast<int64_t>(head) * p.a.G * p.a.o_sh + (lane & 3) * 16;
+      const int rows = job.queries * p.a.G;
 #pragma unroll 1
       for (int c = 0; c < HD; c += 32) {
         float o[32];
@@ -741,18 +744,19 @@ __global__ void __launch_bounds__(kChunkThreads, kChunkCtasPerSm)
         // 32 columns of the warp's 32 rows through shared memory, so that a
         // row's 64 bytes leave together
         const uint32_t stage = sbase + L::kOOff + sw * 32 * 64;
+        const uint32_t keep = none ? 0u : 0xFFFFFFFFu;
 #pragma unroll
         for (int v = 0; v < 4; ++v) {
-          uint4 w;
-          w.x = none ? 0u : pack2<kBF16>(o[8 * v + 0] * inv_l, o[8 * v + 1] * inv_l);
-          w.y = none ? 0u : pack2<kBF16>(o[8 * v + 2] * inv_l, o[8 * v + 3] * inv_l);
-          w.z = none ? 0u : pack2<kBF16>(o[8 * v + 4] * inv_l, o[8 * v + 5] * inv_l);
-          w.w = none ? 0u : pack2<kBF16>(o[8 * v + 6] * inv_l, o[8 * v + 7] * inv_l);
-          st_shared_v4(stage + lane * 64 + ((v ^ ((lane >> 1) & 3)) << 4), w);
+          uint32_t w[4];
+#pragma unroll
+          for (int i = 0; i < 4; ++i) {
+            float a, b;
+            f2_unpack(f2_mul(f2_pack(o[8 * v + 2 * i], o[8 * v + 2 * i + 1]), f2_pack(inv_l, inv_l)), a, b);
+            w[i] = pack2<kBF16>(a, b) & keep;
+          }
+          st_shared_v4(stage + lane * 64 + ((v ^ ((lane >> 1) & 3)) << 4), make_uint4(w[0], w[1], w[2], w[3]));
         }
         __syncwarp();
-        char* base = p.a.o + row0 * p.a.o_sn + static_cast<int64_t>(head) * p.a.G * p.a.o_sh + (c + (lane & 3) * 8) * 2;
-        const int rows = job.queries * p.a.G;
 #pragma unroll
         for (int i = 0; i < 4; ++i) {
           const int lr = i * 8 + (lane >> 2), rr = 32 * sw + lr;
@@ -760,7 +764,7 @@ __global__ void __launch_bounds__(kChunkThreads, kChunkCtasPerSm)
           asm volatile("ld.shared.v4.u32 {%0,%1,%2,%3}, [%4];"
                        : "=r"(w.x), "=r"(w.y), "=r"(w.z), "=r"(w.w)
                        : "r"(stage + lr * 64 + (((lane & 3) ^ ((lr >> 1) & 3)) << 4)));
-          if (rr < rows && c + (lane & 3) * 8 < p.a.hd) *reinterpret_cast<uint4*>(base + row_off[rr]) = w;
+          if (rr < rows && c + (lane & 3) * 8 < p.a.hd) *reinterpret_cast<uint4*>(base + row_off[rr] + c * 2) = w;
         }
         __syncwarp();
       }
@@ -781,23 +785,20 @@ __global__ void __launch_bounds__(kChunkThreads, kChunkCtasPerSm)
   }
 }
 
-constexpr int kChunkMergeWarps = 16;
-
-// Adds the pieces of the tile whose first piece ends run blockIdx.x, as that run
-// noted: O = sum 2^(m_c - M) O_c / sum 2^(m_c - M) l_c over the runs in order.
+// Adds the pieces of the tile whose first piece ends run c0, as that run noted:
+// O = sum 2^(m_c - M) O_c / sum 2^(m_c - M) l_c over the runs in order.
 // A warp takes 8 rows by 16 columns at a time (128-byte reads of the pieces).
 template <int HD, bool kBF16>
-__global__ void __launch_bounds__(32 * kChunkMergeWarps) paged_chunk_merge_kernel(const __grid_constant__ ChunkParams p) {
-  grid_dependency_wait();
+__device__ __forceinline__ void chunk_merge(const ChunkParams& p, int c0) {
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-  const int4 note = p.a.merges[blockIdx.x];
-  const int c0 = static_cast<int>(blockIdx.x), c1 = note.w;
+  const int4 note = p.a.merges[c0];
+  const int c1 = note.w;
   if (c1 < 0) return;
   const float2* ml = reinterpret_cast<const float2*>(p.a.part_ml);
   const float4* part = reinterpret_cast<const float4*>(p.a.part_o);
   const int rows = note.y * p.a.G;
 #pragma unroll 2
-  for (int i = warp; i < (kSqdkBM / 8) * (HD / 16); i += kChunkMergeWarps) {
+  for (int i = warp; i < (kSqdkBM / 8) * (HD / 16); i += kMergeWarps) {
     const int r = i / (HD / 16) * 8 + (lane >> 2), q4 = i % (HD / 16) * 4 + (lane & 3);  // row, group of 4 columns
     if (r >= rows || q4 * 4 >= p.a.hd) continue;
     float M = -INFINITY, l = 0.0f;
@@ -825,6 +826,17 @@ __global__ void __launch_bounds__(32 * kChunkMergeWarps) paged_chunk_merge_kerne
     *reinterpret_cast<uint2*>(p.a.o + static_cast<int64_t>(note.x + ql) * p.a.o_sn +
                               static_cast<int64_t>(note.z * p.a.G + r - ql * p.a.G) * p.a.o_sh + q4 * 8) = w;
   }
+}
+
+// Both kernels' merges in one launch: blocks [0, paged_runs) those of the 16-row
+// kernel, the others the chunks'.
+template <int HD, bool kBF16>
+__global__ void __launch_bounds__(32 * kMergeWarps)
+    paged_both_merge_kernel(const __grid_constant__ PagedAttnParams p, const __grid_constant__ ChunkParams c, int paged_runs) {
+  grid_dependency_wait();
+  const int run = static_cast<int>(blockIdx.x);
+  if (run < paged_runs) paged_merge<HD, kBF16>(p, run);
+  else chunk_merge<HD, kBF16>(c, run - paged_runs);
 }
 
 }  // namespace hspmn
