@@ -797,10 +797,25 @@ int check_strides(std::initializer_list<int64_t> strides, int64_t es) {
   return HSPMN_OK;
 }
 
-template <typename T>
-void launch_paged_write(const PagedWriteParams& prm, bool f32_tables, unsigned grid, cudaStream_t st) {
-  if (f32_tables) rope_paged_write_kernel<T, float><<<grid, kRowThreads, 0, st>>>(prm);
-  else rope_paged_write_kernel<T, T><<<grid, kRowThreads, 0, st>>>(prm);
+template <typename T, typename Tab, int kLanes>
+int launch_paged_write_lanes(const PagedWriteParams& prm, int sms, cudaStream_t st) {
+  auto kern = rope_paged_write_kernel<T, Tab, kLanes>;
+  int per_sm = 0;
+  if (cudaOccupancyMaxActiveBlocksPerMultiprocessor(&per_sm, kern, kRowThreads, 0) != cudaSuccess || per_sm < 1)
+    return HSPMN_ERR_CUDA;
+  const int64_t need = (prm.N + kRowThreads / kLanes - 1) / (kRowThreads / kLanes);
+  const unsigned grid = static_cast<unsigned>(std::min<int64_t>(need, static_cast<int64_t>(sms) * per_sm));
+  kern<<<grid, kRowThreads, 0, st>>>(prm);
+  return launch_status();
+}
+
+template <typename T, typename Tab>
+int launch_paged_write(const PagedWriteParams& prm, int sms, cudaStream_t st) {
+  const int per_vec = 16 / static_cast<int>(sizeof(T));
+  const int64_t units = static_cast<int64_t>(prm.Hkv) * prm.hd / (prm.cos_tab ? 2 * per_vec : per_vec);
+  if (units <= 8) return launch_paged_write_lanes<T, Tab, 8>(prm, sms, st);
+  if (units <= 16) return launch_paged_write_lanes<T, Tab, 16>(prm, sms, st);
+  return launch_paged_write_lanes<T, Tab, 32>(prm, sms, st);
 }
 
 // Launches kern as a programmatic dependent of the kernel before it in the
@@ -865,7 +880,8 @@ int launch_paged_chunks(const CUtensorMap& mq, const CUtensorMap& mk, const CUte
   chunks<<<static_cast<unsigned>(chunk_runs), kChunkThreads, chunk_smem, st>>>(mq, mk, mv, ch);
   if (int rc = launch_status()) return rc;
   if (int rc = launch_dependent(rows, static_cast<unsigned>(runs), kPagedThreads, smem, st, prm)) return rc;
-  return launch_dependent(paged_both_merge_kernel<HD, kBF16>, static_cast<unsigned>(runs + chunk_runs), 32 * kMergeWarps, 0,
+  return launch_dependent(paged_both_merge_kernel<HD, kBF16>, static_cast<unsigned>(runs + chunk_runs * kChunkMergeBlocks),
+                          32 * kMergeWarps, 0,
                           st, prm, ch, runs);
 }
 
@@ -962,14 +978,13 @@ int hspmn_rope_paged_write(const void* k, int64_t k_sn, int64_t k_sh, const void
   prm.shift = shift;
   prm.Hkv = static_cast<int>(Hkv);
   prm.hd = static_cast<int>(hd);
-  const int64_t need = (N + kRowWarps - 1) / kRowWarps;
-  const unsigned grid = static_cast<unsigned>(std::min<int64_t>(need, 64LL * sms));
   cudaStream_t st = static_cast<cudaStream_t>(stream);
   const bool f32_tables = cos_tab && tab_dtype == HSPMN_F32;
-  if (dtype == HSPMN_BF16) launch_paged_write<__nv_bfloat16>(prm, f32_tables, grid, st);
-  else if (dtype == HSPMN_F16) launch_paged_write<__half>(prm, f32_tables, grid, st);
-  else launch_paged_write<float>(prm, true, grid, st);
-  return launch_status();
+  if (dtype == HSPMN_F32) return launch_paged_write<float, float>(prm, sms, st);
+  if (dtype == HSPMN_BF16)
+    return f32_tables ? launch_paged_write<__nv_bfloat16, float>(prm, sms, st)
+                      : launch_paged_write<__nv_bfloat16, __nv_bfloat16>(prm, sms, st);
+  return f32_tables ? launch_paged_write<__half, float>(prm, sms, st) : launch_paged_write<__half, __half>(prm, sms, st);
 }
 
 int64_t hspmn_sqdk_paged_workspace_size(int64_t N, int64_t H, int64_t Hkv, int64_t hd, int64_t max_q) {

@@ -179,48 +179,58 @@ __device__ __forceinline__ void load_table(const char* p, float (&out)[n]) {
   }
 }
 
-// One warp a token: lanes take the K row in pairs of 16-byte groups (a group of
-// a head's low half and its partner in the high half, so x and the tables are
-// read once per pair) and the V row in 16-byte groups. The rotation is formed
-// in fp32 and rounded once, when it is stored. A lane's first K pair and first
-// two V groups (the whole rows up to 512 16-bit elements) are requested before
-// the slot and position are known, so that only the table rows wait for those.
-template <typename T, typename Tab>
+// kLanes lanes a token (the smallest power of two from 8 to 32 that gives each one
+// K unit, where 32 are enough): lanes take the K row in pairs of 16-byte groups
+// (a group of a head's low half and its partner in the high half, so x and the
+// tables are read once per pair) and the V row in 16-byte groups. The rotation is
+// formed in fp32 and rounded once, when it is stored. The slot and position of a
+// lane's next token are read one token ahead, and its first K pair and first two
+// V groups (the whole rows up to 512 16-bit elements) together with the table
+// rows, so that a token waits for memory once.
+template <typename T, typename Tab, int kLanes>
 __global__ void __launch_bounds__(kRowThreads) rope_paged_write_kernel(const PagedWriteParams p) {
   constexpr int n = 16 / sizeof(T);
-  const int lane = threadIdx.x & 31;
+  constexpr int kTokens = kRowThreads / kLanes;  // of a CTA at a time
+  const int lane = threadIdx.x % kLanes;
   const int half = p.hd / 2;
   const bool rope = p.cos_tab != nullptr;
   const int vgroups = p.hd / n, units = p.Hkv * vgroups;  // 16-byte groups of a head, of a row
   const int pairs = half / n, kunits = rope ? p.Hkv * pairs : units;
+  const int kg = rope ? pairs : vgroups;
+  const int kh = lane / kg, kc = lane - kh * kg;
+  const int vh0 = lane / vgroups, vc0 = lane - vh0 * vgroups;
+  const int vh1 = (lane + kLanes) / vgroups, vc1 = lane + kLanes - vh1 * vgroups;
   auto source = [](const char* row, int64_t sh, int h, int c) { return reinterpret_cast<const uint4*>(row + h * sh + c * 16); };
-  for (int64_t t = static_cast<int64_t>(blockIdx.x) * kRowWarps + (threadIdx.x >> 5); t < p.N;
-       t += static_cast<int64_t>(gridDim.x) * kRowWarps) {
+  const int64_t step = static_cast<int64_t>(gridDim.x) * kTokens;
+  int64_t t = static_cast<int64_t>(blockIdx.x) * kTokens + threadIdx.x / kLanes;
+  int64_t slot = t < p.N ? __ldg(p.slots + t) : -1, pos = rope && t < p.N ? __ldg(p.pos + t) : 0;
+  for (; t < p.N; t += step) {
+    const int64_t slot_now = slot, pos_now = pos;
+    if (t + step < p.N) {
+      slot = __ldg(p.slots + t + step);
+      if (rope) pos = __ldg(p.pos + t + step);
+    }
+    if (slot_now < 0) continue;  // padding
+    const int64_t page = slot_now >> p.shift, off = slot_now & ((1 << p.shift) - 1);
+    if (page >= p.num_pages || pos_now < 0 || (rope && pos_now >= p.tab_rows)) {
+      if (lane == 0) raise_device_error(page >= p.num_pages ? HSPMN_DEVERR_PAGE : HSPMN_DEVERR_POSITION);
+      continue;
+    }
     const char* krow = p.k + t * p.k_sn;
     const char* vrow = p.v + t * p.v_sn;
-    const int64_t slot = __ldg(p.slots + t);
-    const int64_t pos = rope ? __ldg(p.pos + t) : 0;
-    const int kg = rope ? pairs : vgroups;
-    const int kh = lane / kg, kc = lane - kh * kg;
     uint4 k_lo = make_uint4(0, 0, 0, 0), k_hi = k_lo, v_0 = k_lo, v_1 = k_lo;
     if (lane < kunits) {
       k_lo = __ldcs(source(krow, p.k_sh, kh, kc));
       if (rope) k_hi = __ldcs(source(krow, p.k_sh, kh, kc + pairs));
     }
-    if (lane < units) v_0 = __ldcs(source(vrow, p.v_sh, lane / vgroups, lane % vgroups));
-    if (lane + 32 < units) v_1 = __ldcs(source(vrow, p.v_sh, (lane + 32) / vgroups, (lane + 32) % vgroups));
-    if (slot < 0) continue;  // padding
-    const int64_t page = slot >> p.shift, off = slot & ((1 << p.shift) - 1);
-    if (page >= p.num_pages || pos < 0 || (rope && pos >= p.tab_rows)) {
-      if (lane == 0) raise_device_error(page >= p.num_pages ? HSPMN_DEVERR_PAGE : HSPMN_DEVERR_POSITION);
-      continue;
-    }
+    if (lane < units) v_0 = __ldcs(source(vrow, p.v_sh, vh0, vc0));
+    if (lane + kLanes < units) v_1 = __ldcs(source(vrow, p.v_sh, vh1, vc1));
     char* kdst = p.kc + page * p.kc_sp + off * p.kc_ss;
     char* vdst = p.vc + page * p.vc_sp + off * p.vc_ss;
-    const char* cs = p.cos_tab + pos * p.tab_ss;
-    const char* sn = p.sin_tab + pos * p.tab_ss;
-    for (int i = lane; i < kunits; i += 32) {
-      const int h = i / kg, c = i - h * kg;
+    const char* cs = p.cos_tab + pos_now * p.tab_ss;
+    const char* sn = p.sin_tab + pos_now * p.tab_ss;
+    for (int i = lane; i < kunits; i += kLanes) {
+      const int h = i == lane ? kh : i / kg, c = i == lane ? kc : i - h * kg;
       if (i != lane) {
         k_lo = __ldcs(source(krow, p.k_sh, h, c));
         if (rope) k_hi = __ldcs(source(krow, p.k_sh, h, c + pairs));
@@ -247,10 +257,11 @@ __global__ void __launch_bounds__(kRowThreads) rope_paged_write_kernel(const Pag
       }
       __stcs(reinterpret_cast<uint4*>(kdst + h * p.kc_sh + c * 16), out_lo);
     }
-    for (int i = lane; i < units; i += 32) {
+    if (lane < units) __stcs(reinterpret_cast<uint4*>(vdst + vh0 * p.vc_sh + vc0 * 16), v_0);
+    if (lane + kLanes < units) __stcs(reinterpret_cast<uint4*>(vdst + vh1 * p.vc_sh + vc1 * 16), v_1);
+    for (int i = lane + 2 * kLanes; i < units; i += kLanes) {
       const int h = i / vgroups, c = i - h * vgroups;
-      const uint4 w = i == lane ? v_0 : i == lane + 32 ? v_1 : __ldcs(source(vrow, p.v_sh, h, c));
-      __stcs(reinterpret_cast<uint4*>(vdst + h * p.vc_sh + c * 16), w);
+      __stcs(reinterpret_cast<uint4*>(vdst + h * p.vc_sh + c * 16), __ldcs(source(vrow, p.v_sh, h, c)));
     }
   }
 }

@@ -51,7 +51,7 @@ struct PagedAttnParams {
   const int64_t* pos;
   float* part_o;   // [2 * runs][16][HD] unnormalised O
   float* part_ml;  // [2 * runs][16][2] maximum (log2 units), row sum
-  int4* merges;    // [runs] what is to be merged from this run on; .w < 0: nothing
+  int4* merges;    // [runs] the item that goes on behind this run, for the merge; .w < 0: none
   int64_t N;
   int R, P, num_pages, shift, H, Hkv, G, hd;
   int split_rows;  // requests with more rows (queries * G) than this are not this kernel's
@@ -108,40 +108,51 @@ __device__ __forceinline__ int64_t paged_cost(const PagedAttnParams& p, int r) {
   return static_cast<int64_t>(q.tiles) * p.Hkv * (q.nb + kPagedItemCost);
 }
 
-// Cost of the whole list; every lane of the warp gets the sum.
+// The list of items, as one warp sees it: the first 32 requests' costs stay in
+// its lanes, later ones are read again.
 template <int kKeys>
-__device__ __forceinline__ int64_t paged_total(const PagedAttnParams& p, int lane) {
-  int64_t n = 0;
-  for (int r = lane; r <= p.R; r += 32) n += paged_cost<kKeys>(p, r);
-#pragma unroll
-  for (int d = 16; d > 0; d >>= 1) n += __shfl_xor_sync(0xFFFFFFFFu, n, d);
-  return n;
-}
-
-// The request that holds list place w (below the total) and the cost before it,
-// found by the whole warp.
-template <int kKeys>
-__device__ __forceinline__ int paged_locate(const PagedAttnParams& p, int64_t w, int lane, int64_t& before) {
-  int64_t base = 0;
-  for (int r0 = 0; r0 <= p.R; r0 += 32) {
-    const int64_t mine = paged_cost<kKeys>(p, r0 + lane);
-    int64_t sum = mine;
+struct PagedList {
+  const PagedAttnParams& p;
+  int lane;
+  int64_t own, upto;  // cost of request `lane`, and with all before it
+  __device__ __forceinline__ PagedList(const PagedAttnParams& p_, int lane_) : p(p_), lane(lane_) {
+    own = paged_cost<kKeys>(p, lane);
+    upto = scan(own);
+  }
+  __device__ __forceinline__ int64_t scan(int64_t x) const {
 #pragma unroll
     for (int d = 1; d < 32; d <<= 1) {
-      const int64_t x = __shfl_up_sync(0xFFFFFFFFu, sum, d);
-      if (lane >= d) sum += x;
+      const int64_t y = __shfl_up_sync(0xFFFFFFFFu, x, d);
+      if (lane >= d) x += y;
     }
-    const unsigned past = __ballot_sync(0xFFFFFFFFu, base + sum > w);
-    if (past) {
-      const int l = __ffs(past) - 1;
-      before = base + __shfl_sync(0xFFFFFFFFu, sum - mine, l);
-      return r0 + l;
-    }
-    base += __shfl_sync(0xFFFFFFFFu, sum, 31);
+    return x;
   }
-  before = base;
-  return p.R;  // not reached for w below the total
-}
+  __device__ __forceinline__ int64_t total() const {
+    int64_t n = __shfl_sync(0xFFFFFFFFu, upto, 31);
+    if (p.R < 32) return n;
+    int64_t more = 0;
+    for (int r = lane + 32; r <= p.R; r += 32) more += paged_cost<kKeys>(p, r);
+#pragma unroll
+    for (int d = 16; d > 0; d >>= 1) more += __shfl_xor_sync(0xFFFFFFFFu, more, d);
+    return n + more;
+  }
+  // The request that holds list place w (below the total) and the cost before it.
+  __device__ __forceinline__ int locate(int64_t w, int64_t& before) const {
+    int64_t base = 0, mine = own, sum = upto;
+    for (int r0 = 0; r0 <= p.R; r0 += 32) {
+      if (r0 > 0) mine = paged_cost<kKeys>(p, r0 + lane), sum = scan(mine);
+      const unsigned past = __ballot_sync(0xFFFFFFFFu, base + sum > w);
+      if (past) {
+        const int l = __ffs(past) - 1;
+        before = base + __shfl_sync(0xFFFFFFFFu, sum - mine, l);
+        return r0 + l;
+      }
+      base += __shfl_sync(0xFFFFFFFFu, sum, 31);
+    }
+    before = base;
+    return p.R;  // not reached for w below the total
+  }
+};
 
 // a / b; 64-bit divisions are slow, and most operands here fit 32 bits.
 __device__ __forceinline__ int64_t div_wide(int64_t a, int64_t b) {
@@ -321,14 +332,15 @@ __global__ void __launch_bounds__(kPagedThreads, kPagedCtasPerSm) paged_attn_ker
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   const int g = lane >> 2, t2 = (lane & 3) * 2;  // accumulator row and first column of this lane
   grid_dependents_launch();
-  const int64_t total = paged_total<L::kKeys>(p, lane);
+  const PagedList<L::kKeys> list(p, lane);
+  const int64_t total = list.total();
   const int64_t runs = min(static_cast<int64_t>(gridDim.x), total);
   PagedCursor<L::kKeys> cur, ahead;
   const Runs run(total, max(runs, static_cast<int64_t>(1)));
   if (blockIdx.x < runs) {
     const int64_t w0 = run.start(blockIdx.x), w1 = run.start(blockIdx.x + 1);
     int64_t before;
-    const int r0 = paged_locate<L::kKeys>(p, w0, lane, before);
+    const int r0 = list.locate(w0, before);
     cur.open(p, r0, before, w0, w1);
   } else {
     cur.j = cur.jend = 0;
@@ -610,11 +622,16 @@ __global__ void __launch_bounds__(kPagedThreads, kPagedCtasPerSm) paged_attn_ker
         if ((lane & 3) == 0) s_m[warp][g + 8 * i] = m_run[i], s_l[warp][g + 8 * i] = seen[i] ? l : kUnseen;
       }
       const bool item_end = cur.jend == cur.req.nb, whole = item_end && seg_j == 0;
-      // an item that opens in this run and goes on behind it is merged from here
-      if (threadIdx.x == 0 && (!item_end || cur.a + cur.req.nb + 2 * kPagedItemCost >= cur.end))
-        p.merges[blockIdx.x] = make_int4(cur.req.q0, cur.tile * kPagedRows,
-                                         cur.head * kPagedRows + min(kPagedRows, cur.req.rows - cur.tile * kPagedRows) - 1,
-                                         !item_end && seg_j == 0 ? run.of(cur.a + kPagedItemCost + cur.req.nb - 1) : -1);
+      // the last item of this run: if it goes on behind it, its runs from the one
+      // in which it opens to this one share its merge
+      if (threadIdx.x == 0 && (!item_end || cur.a + cur.req.nb + 2 * kPagedItemCost >= cur.end)) {
+        const int64_t first = cur.a + kPagedItemCost;
+        p.merges[blockIdx.x] =
+            make_int4(cur.req.q0, cur.tile * kPagedRows,
+                      cur.head * kPagedRows + min(kPagedRows, cur.req.rows - cur.tile * kPagedRows) - 1,
+                      item_end ? -1 : (seg_j == 0 ? static_cast<int>(blockIdx.x) : run.of(first)) << 16 |
+                                          run.of(first + cur.req.nb - 1));
+      }
       __syncthreads();
       // a run holds the last piece of one item at most, and the first of one
       const int64_t slot = 2 * static_cast<int64_t>(blockIdx.x) + (seg_j == 0 ? 1 : 0);
@@ -670,23 +687,27 @@ __global__ void __launch_bounds__(kPagedThreads, kPagedCtasPerSm) paged_attn_ker
   grid_dependency_wait();
 }
 
-constexpr int kMergeWarps = 32;
+constexpr int kMergeWarps = 16;
 
-// Adds the partial results of the item that opens in run c0 and goes on
-// behind it, as that run noted: O = sum 2^(m_c - M) O_c / sum 2^(m_c - M) l_c over
-// the runs in order. A warp takes one row and a share of the runs.
+// Adds the partial results of the item that goes on behind run `block`, as that
+// run noted: O = sum 2^(m_c - M) O_c / sum 2^(m_c - M) l_c over the item's runs in
+// order. All runs it goes on behind share its rows; a warp takes a row and a
+// share of the runs.
 template <int HD, bool kBF16>
-__device__ __forceinline__ void paged_merge(const PagedAttnParams& p, int c0) {
+__device__ __forceinline__ void paged_merge(const PagedAttnParams& p, int block) {
   __shared__ float4 s_o[kMergeWarps][HD / 4];
   __shared__ float2 s_ml[kMergeWarps];
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-  const int4 note = p.merges[c0];
-  const int c1 = note.w;
-  if (c1 < 0) return;
+  const int4 note = p.merges[block];
+  if (note.w < 0) return;
+  const int c0 = note.w >> 16, c1 = note.w & 0xFFFF;
   const int rows = note.z % kPagedRows + 1, head = note.z / kPagedRows;
-  const int shares = max(1, kMergeWarps / rows);  // warps of a row
-  const int lr = warp / shares, part = warp % shares;
-  const bool live = lr < rows;
+  const int blocks = min(rows, c1 - c0), slice = block - c0;
+  if (slice >= blocks) return;
+  const int mine = (rows - slice + blocks - 1) / blocks;  // rows slice, slice + blocks, ..
+  const int shares = kMergeWarps / mine;                  // warps of a row
+  const int part = warp % shares, lr = slice + warp / shares * blocks;
+  const bool live = warp / shares < mine;
   const float2* ml = reinterpret_cast<const float2*>(p.part_ml);
   float M = -INFINITY, l = 0.0f;
   bool none = true;

@@ -533,10 +533,14 @@ __global__ void __launch_bounds__(kChunkThreads, kChunkCtasPerSm)
     const int qloc = r / p.a.G;
     const float c2 = p.a.scale_log2;
     uint32_t n = 0, segs = 0, walked = 0;
-    bool ok = true;
-    while (ok) {
-      ok = __all_sync(0xFFFFFFFFu, mbar_wait(&bar_job[walked & 1], (walked >> 1) & 1, &abort_flag));
-      if (!ok) break;
+    while (true) {
+      // The four warps agree on each job, so that all of them meet at the barrier
+      // of its epilogue even if some wait gives up; behind this one, every warp
+      // has left the job before.
+      const bool posted = __all_sync(0xFFFFFFFFu, mbar_wait(&bar_job[walked & 1], (walked >> 1) & 1, &abort_flag));
+      if (!named_bar_and(kChunkEpilogueBar, 128, posted)) break;
+      if (threadIdx.x == 64) wild_flag[(walked + 1) & 1] = 0u;
+      bool ok = true;
       volatile ChunkJob& job = jobs[walked & 1];
       const int nblk = job.nblk, j0 = job.j0;
       if (nblk < 0) break;
@@ -659,20 +663,24 @@ __global__ void __launch_bounds__(kChunkThreads, kChunkCtasPerSm)
           if (!ok) break;
           const uint32_t vst = sbase + L::kVOff + sb * L::kKVBytes;
           bool found = false;
-          if (key0 + 16 * sw + 15 > tile_lo)
+          if (key0 + 16 * sw + 15 > tile_lo) {
 #pragma unroll 4
             for (int i = lane; i < 16 * 8 * L::kChunks; i += 32) {
-            const int kr = 16 * sw + (i >> 3) % 16, key = key0 + kr;
-            const uint32_t addr = vst + (i >> 7) * L::kKVChunkBytes + kr * 128 + (i & 7) * 16;
-            if (key > tile_hi) {
-              st_shared_v4(addr, make_uint4(0u, 0u, 0u, 0u));
-            } else if (key > tile_lo) {
-              uint4 w;
-              asm volatile("ld.shared.v4.u32 {%0,%1,%2,%3}, [%4];" : "=r"(w.x), "=r"(w.y), "=r"(w.z), "=r"(w.w) : "r"(addr));
-              if (not_finite2<kBF16>(w.x) || not_finite2<kBF16>(w.y) || not_finite2<kBF16>(w.z) || not_finite2<kBF16>(w.w)) {
-                found = true;
-                w.x = finite2<kBF16>(w.x), w.y = finite2<kBF16>(w.y), w.z = finite2<kBF16>(w.z), w.w = finite2<kBF16>(w.w);
-                st_shared_v4(addr, w);
+              const int kr = 16 * sw + (i >> 3) % 16, key = key0 + kr;
+              const uint32_t addr = vst + (i >> 7) * L::kKVChunkBytes + kr * 128 + (i & 7) * 16;
+              if (key > tile_hi) {
+                st_shared_v4(addr, make_uint4(0u, 0u, 0u, 0u));
+              } else if (key > tile_lo) {
+                uint4 w;
+                asm volatile("ld.shared.v4.u32 {%0,%1,%2,%3}, [%4];"
+                             : "=r"(w.x), "=r"(w.y), "=r"(w.z), "=r"(w.w)
+                             : "r"(addr));
+                if (not_finite2<kBF16>(w.x) || not_finite2<kBF16>(w.y) || not_finite2<kBF16>(w.z) ||
+                    not_finite2<kBF16>(w.w)) {
+                  found = true;
+                  w.x = finite2<kBF16>(w.x), w.y = finite2<kBF16>(w.y), w.z = finite2<kBF16>(w.z), w.w = finite2<kBF16>(w.w);
+                  st_shared_v4(addr, w);
+                }
               }
             }
           }
@@ -685,17 +693,10 @@ __global__ void __launch_bounds__(kChunkThreads, kChunkCtasPerSm)
       // ---------------------------------------------------------- epilogue
       if (ok && nblk > 0) ok = __all_sync(0xFFFFFFFFu, mbar_wait(&bar_ofinal, segs & 1, &abort_flag));
       if (nblk > 0) ++segs;
-      // between the barriers every warp has set this job's flag and none has
-      // left its epilogue: it is read, and the last job's is cleared
-      if (threadIdx.x == 64) wild_flag[(walked + 1) & 1] = 0u;
-      const bool live = named_bar_and(kChunkEpilogueBar, 128, ok);
+      const bool live = named_bar_and(kChunkEpilogueBar, 128, ok);  // every warp has set this job's flag
       const bool wild = wild_flag[walked & 1] != 0u;
-      named_bar_sync(kChunkEpilogueBar, 128);
       ++walked;
-      if (!live) {
-        ok = false;
-        break;
-      }
+      if (!live) break;
       tc_fence_after();
       const bool none = !seen;
       const int slot = job.slot, head = job.head;
@@ -787,9 +788,12 @@ __global__ void __launch_bounds__(kChunkThreads, kChunkCtasPerSm)
 
 // Adds the pieces of the tile whose first piece ends run c0, as that run noted:
 // O = sum 2^(m_c - M) O_c / sum 2^(m_c - M) l_c over the runs in order.
-// A warp takes 8 rows by 16 columns at a time (128-byte reads of the pieces).
+// A warp takes 8 rows by 16 columns at a time (128-byte reads of the pieces);
+// kChunkMergeBlocks blocks share a tile.
+constexpr int kChunkMergeBlocks = 4;
+
 template <int HD, bool kBF16>
-__device__ __forceinline__ void chunk_merge(const ChunkParams& p, int c0) {
+__device__ __forceinline__ void chunk_merge(const ChunkParams& p, int c0, int share) {
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   const int4 note = p.a.merges[c0];
   const int c1 = note.w;
@@ -798,7 +802,7 @@ __device__ __forceinline__ void chunk_merge(const ChunkParams& p, int c0) {
   const float4* part = reinterpret_cast<const float4*>(p.a.part_o);
   const int rows = note.y * p.a.G;
 #pragma unroll 2
-  for (int i = warp; i < (kSqdkBM / 8) * (HD / 16); i += kMergeWarps) {
+  for (int i = warp + share * kMergeWarps; i < (kSqdkBM / 8) * (HD / 16); i += kMergeWarps * kChunkMergeBlocks) {
     const int r = i / (HD / 16) * 8 + (lane >> 2), q4 = i % (HD / 16) * 4 + (lane & 3);  // row, group of 4 columns
     if (r >= rows || q4 * 4 >= p.a.hd) continue;
     float M = -INFINITY, l = 0.0f;
@@ -829,14 +833,14 @@ __device__ __forceinline__ void chunk_merge(const ChunkParams& p, int c0) {
 }
 
 // Both kernels' merges in one launch: blocks [0, paged_runs) those of the 16-row
-// kernel, the others the chunks'.
+// kernel, then kChunkMergeBlocks a run of the chunks'.
 template <int HD, bool kBF16>
 __global__ void __launch_bounds__(32 * kMergeWarps)
     paged_both_merge_kernel(const __grid_constant__ PagedAttnParams p, const __grid_constant__ ChunkParams c, int paged_runs) {
   grid_dependency_wait();
-  const int run = static_cast<int>(blockIdx.x);
-  if (run < paged_runs) paged_merge<HD, kBF16>(p, run);
-  else chunk_merge<HD, kBF16>(c, run - paged_runs);
+  const int block = static_cast<int>(blockIdx.x) - paged_runs;
+  if (block < 0) paged_merge<HD, kBF16>(p, static_cast<int>(blockIdx.x));
+  else chunk_merge<HD, kBF16>(c, block / kChunkMergeBlocks, block % kChunkMergeBlocks);
 }
 
 }  // namespace hspmn
