@@ -837,12 +837,9 @@ int launch_dependent(void (*kern)(Params...), unsigned grid, unsigned threads, s
   return cudaLaunchKernelEx(&cfg, kern, prm...) == cudaSuccess ? HSPMN_OK : HSPMN_ERR_CUDA;
 }
 
-// Rows (queries * G) of a request up to which its tiles are the 16-row kernel's.
-constexpr int kPagedSplitRows = 16;
-
-// Whether a call has, by its arguments, a request for the chunk kernel.
+// Whether a call has, by its arguments, requests that the chunk kernel may take.
 bool paged_has_chunks(int64_t N, int64_t G, int64_t max_q) {
-  return (max_q > 0 ? std::min(max_q, N) : N) * G > kPagedSplitRows;
+  return (max_q > 0 ? std::min(max_q, N) : N) * G > kPagedRows;
 }
 
 // Workspace of one of the two kernels: two pieces a run (O, maximum and sum of
@@ -1062,12 +1059,12 @@ int hspmn_sqdk_paged_fwd(const void* q, int64_t q_sn, int64_t q_sh, const void* 
   prm.G = static_cast<int>(H / Hkv);
   prm.hd = static_cast<int>(hd);
   prm.scale_log2 = sm_scale * 1.4426950408889634f;
-  prm.split_rows = 0x7FFFFFFF;
+  prm.has_chunks = 0;
   cudaStream_t st = static_cast<cudaStream_t>(stream);
   // The host knows neither lengths nor offsets: a call that may hold chunks runs
   // both kernels, each on its own requests.
   if (paged_has_chunks(N, prm.G, max_q) && R > 0 && P > 0 && num_pages > 0) {
-    prm.split_rows = kPagedSplitRows;
+    prm.has_chunks = 1;
     ChunkParams ch;
     ch.a = prm;
     const int chunk_runs = sms * kChunkCtasPerSm;

@@ -32,6 +32,8 @@ constexpr int kPagedThreads = 32 * kPagedWarps;
 constexpr int kPagedStages = 3;
 constexpr int kPagedItemCost = 2;  // what opening and closing an item takes, in units (68.0 us against 86.3 at 0, 68.7 at 1, 69.6 at 3: 37 x 16 items of 1 to 64 units)
 constexpr int kPagedCtasPerSm = 2;
+constexpr int kPagedMidRows = 128;      // see paged_split
+constexpr int kPagedMidScore = 14200;
 
 // Row sum of a part that holds no key its row sees (a true sum is not negative).
 constexpr float kUnseen = -1.0f;
@@ -54,7 +56,7 @@ struct PagedAttnParams {
   int4* merges;    // [runs] the item that goes on behind this run, for the merge; .w < 0: none
   int64_t N;
   int R, P, num_pages, shift, H, Hkv, G, hd;
-  int split_rows;  // requests with more rows (queries * G) than this are not this kernel's
+  int has_chunks;  // the chunk kernel takes part in the call
   float scale_log2;
 };
 
@@ -92,19 +94,46 @@ __device__ __forceinline__ PagedRequest paged_rows(const PagedAttnParams& p, con
   return q;
 }
 
+// Rows (queries * G) of a request up to which the 16-row kernel takes it; the
+// chunk kernel takes the others. Up to one tile is always the former's. Requests
+// of two to eight tiles are read by it once a tile, at about 1.5 us a unit and
+// CTA, and by the chunk kernel once, at about 1.75 us a unit and CTA but 12 us
+// later (its setup and the merge of 128-row pieces), so they stay here while
+// that is less in all: 16 us against 27 for one request of 32 rows and 8192 keys,
+// 171 against 118 for 64 requests of 32 rows and 4096 keys. A batch with larger
+// requests has the chunk kernel's setup anyway. Both kernels work this out from
+// the same lengths.
 template <int kKeys>
-__device__ __forceinline__ PagedRequest paged_request(const PagedAttnParams& p, const PagedRaw& x, int r) {
+__device__ __forceinline__ int paged_split(const PagedAttnParams& p, int lane) {
+  if (!p.has_chunks) return 0x7FFFFFFF;
+  constexpr int kMost = 1 << 24;
+  int score = 0;  // quarters of a microsecond and CTA
+  bool large = false;
+  for (int r = lane; r < p.R; r += 32) {
+    const PagedRequest q = paged_rows(p, paged_raw(p, r));
+    large |= q.rows > kPagedMidRows;
+    if (q.rows <= kPagedRows || q.rows > kPagedMidRows) continue;
+    const int64_t units = static_cast<int64_t>(p.Hkv) * ((q.kv + kKeys - 1) / kKeys);
+    const int tiles = (q.rows + kPagedRows - 1) / kPagedRows;
+    score = static_cast<int>(min(score + units * (6 * tiles - 7), static_cast<int64_t>(kMost)));
+  }
+  if (__any_sync(0xFFFFFFFFu, large)) return kPagedRows;
+  return __reduce_add_sync(0xFFFFFFFFu, score) < kPagedMidScore ? kPagedMidRows : kPagedRows;
+}
+
+template <int kKeys>
+__device__ __forceinline__ PagedRequest paged_request(const PagedAttnParams& p, int split, const PagedRaw& x, int r) {
   PagedRequest q = paged_rows(p, x);
-  q.tiles = r < p.R && q.rows > p.split_rows ? 0 : (q.rows + kPagedRows - 1) / kPagedRows;
+  q.tiles = r < p.R && q.rows > split ? 0 : (q.rows + kPagedRows - 1) / kPagedRows;
   q.nb = max(1, (q.kv + kKeys - 1) / kKeys);
   return q;
 }
 
 // A request's cost in the list.
 template <int kKeys>
-__device__ __forceinline__ int64_t paged_cost(const PagedAttnParams& p, int r) {
+__device__ __forceinline__ int64_t paged_cost(const PagedAttnParams& p, int split, int r) {
   if (r > p.R) return 0;
-  const PagedRequest q = paged_request<kKeys>(p, paged_raw(p, r), r);
+  const PagedRequest q = paged_request<kKeys>(p, split, paged_raw(p, r), r);
   return static_cast<int64_t>(q.tiles) * p.Hkv * (q.nb + kPagedItemCost);
 }
 
@@ -113,10 +142,11 @@ __device__ __forceinline__ int64_t paged_cost(const PagedAttnParams& p, int r) {
 template <int kKeys>
 struct PagedList {
   const PagedAttnParams& p;
-  int lane;
+  int split, lane;
   int64_t own, upto;  // cost of request `lane`, and with all before it
-  __device__ __forceinline__ PagedList(const PagedAttnParams& p_, int lane_) : p(p_), lane(lane_) {
-    own = paged_cost<kKeys>(p, lane);
+  __device__ __forceinline__ PagedList(const PagedAttnParams& p_, int split_, int lane_)
+      : p(p_), split(split_), lane(lane_) {
+    own = paged_cost<kKeys>(p, split, lane);
     upto = scan(own);
   }
   __device__ __forceinline__ int64_t scan(int64_t x) const {
@@ -131,7 +161,7 @@ struct PagedList {
     int64_t n = __shfl_sync(0xFFFFFFFFu, upto, 31);
     if (p.R < 32) return n;
     int64_t more = 0;
-    for (int r = lane + 32; r <= p.R; r += 32) more += paged_cost<kKeys>(p, r);
+    for (int r = lane + 32; r <= p.R; r += 32) more += paged_cost<kKeys>(p, split, r);
 #pragma unroll
     for (int d = 16; d > 0; d >>= 1) more += __shfl_xor_sync(0xFFFFFFFFu, more, d);
     return n + more;
@@ -140,7 +170,7 @@ struct PagedList {
   __device__ __forceinline__ int locate(int64_t w, int64_t& before) const {
     int64_t base = 0, mine = own, sum = upto;
     for (int r0 = 0; r0 <= p.R; r0 += 32) {
-      if (r0 > 0) mine = paged_cost<kKeys>(p, r0 + lane), sum = scan(mine);
+      if (r0 > 0) mine = paged_cost<kKeys>(p, split, r0 + lane), sum = scan(mine);
       const unsigned past = __ballot_sync(0xFFFFFFFFu, base + sum > w);
       if (past) {
         const int l = __ffs(past) - 1;
@@ -188,7 +218,7 @@ template <int kKeys>
 struct PagedCursor {
   PagedRequest req;
   PagedRaw ahead;
-  int r, tile, head;
+  int split, r, tile, head;
   int j, jend;  // unit, and the end of this run's units of the item
   int64_t a, end;  // the item's place in the list, the run's end
   __device__ __forceinline__ void cut() {
@@ -196,9 +226,10 @@ struct PagedCursor {
     jend = static_cast<int>(min(max(left, static_cast<int64_t>(0)), static_cast<int64_t>(req.nb)));
   }
   // To the run [w0, w1), whose start lies in request `request` with `before` before it.
-  __device__ __forceinline__ void open(const PagedAttnParams& p, int request, int64_t before, int64_t w0, int64_t w1) {
+  __device__ __forceinline__ void open(const PagedAttnParams& p, int split_, int request, int64_t before, int64_t w0, int64_t w1) {
+    split = split_;
     r = request;
-    req = paged_request<kKeys>(p, paged_raw(p, r), r);
+    req = paged_request<kKeys>(p, split, paged_raw(p, r), r);
     ahead = paged_raw(p, r + 1);
     const int64_t local = w0 - before, cost = req.nb + kPagedItemCost;
     const int64_t item = div_wide(local, cost);
@@ -224,7 +255,7 @@ struct PagedCursor {
       if (++tile == req.tiles) {
         tile = 0;
         do {
-          req = paged_request<kKeys>(p, ahead, ++r);
+          req = paged_request<kKeys>(p, split, ahead, ++r);
           ahead = paged_raw(p, r + 1);
         } while (req.tiles == 0 && r < p.R);
       }
@@ -332,7 +363,8 @@ __global__ void __launch_bounds__(kPagedThreads, kPagedCtasPerSm) paged_attn_ker
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   const int g = lane >> 2, t2 = (lane & 3) * 2;  // accumulator row and first column of this lane
   grid_dependents_launch();
-  const PagedList<L::kKeys> list(p, lane);
+  const int split = paged_split<L::kKeys>(p, lane);
+  const PagedList<L::kKeys> list(p, split, lane);
   const int64_t total = list.total();
   const int64_t runs = min(static_cast<int64_t>(gridDim.x), total);
   PagedCursor<L::kKeys> cur, ahead;
@@ -341,7 +373,7 @@ __global__ void __launch_bounds__(kPagedThreads, kPagedCtasPerSm) paged_attn_ker
     const int64_t w0 = run.start(blockIdx.x), w1 = run.start(blockIdx.x + 1);
     int64_t before;
     const int r0 = list.locate(w0, before);
-    cur.open(p, r0, before, w0, w1);
+    cur.open(p, split, r0, before, w0, w1);
   } else {
     cur.j = cur.jend = 0;
   }

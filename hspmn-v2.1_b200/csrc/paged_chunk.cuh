@@ -35,7 +35,7 @@ constexpr int kChunkThreads = 192;
 constexpr int kChunkCtasPerSm = 2;
 constexpr int kChunkUnit = 16;           // cost units of a 64-key block
 constexpr int kChunkTileCost = 5;        // blocks' worth of time to open and close a tile
-constexpr int kChunkMinPiece = 4;        // blocks of work below which another run is not opened
+constexpr int kChunkMinPiece = 8;        // blocks of work below which another run is not opened
 constexpr int kChunkEpilogueBar = 1;     // named barrier of the four softmax warps
 
 template <int HD>
@@ -76,7 +76,7 @@ struct ChunkRequest {
   int64_t first, slope, head;  // head: the sum over a head's tiles
 };
 
-__device__ __forceinline__ ChunkRequest chunk_request(const ChunkParams& p, int r) {
+__device__ __forceinline__ ChunkRequest chunk_request(const ChunkParams& p, int split, int r) {
   ChunkRequest c;
   const PagedRequest q = paged_rows(p.a, paged_raw(p.a, r));
   c.q0 = q.q0;
@@ -84,7 +84,7 @@ __device__ __forceinline__ ChunkRequest chunk_request(const ChunkParams& p, int 
   c.kv = q.kv;
   c.tiles = 0;
   c.first = c.slope = c.head = 0;
-  if (q.rows <= p.a.split_rows) return c;  // the 16-row kernel's
+  if (q.rows <= split) return c;  // the 16-row kernel's
   c.tiles = (c.len + p.QT - 1) / p.QT;
   const int64_t top = static_cast<int64_t>(c.kv) - 1;
   const int64_t lo = min(max(__ldg(p.a.pos + c.q0 + min(p.QT, c.len) - 1), static_cast<int64_t>(0)), max(top, static_cast<int64_t>(0)));
@@ -99,7 +99,7 @@ __device__ __forceinline__ ChunkRequest chunk_request(const ChunkParams& p, int 
 
 struct ChunkTile {
   ChunkRequest req;
-  int r, head, t;
+  int split, r, head, t;
   int64_t start, cost;  // place in the list
   __device__ __forceinline__ int64_t before(int n) const {
     return req.first * n + req.slope * (static_cast<int64_t>(n) * (n - 1) / 2);
@@ -111,7 +111,7 @@ struct ChunkTile {
       t = 0;
       if (++head == p.a.Hkv) {
         head = 0;
-        do req = chunk_request(p, ++r);
+        do req = chunk_request(p, split, ++r);
         while (req.tiles == 0 && r + 1 < p.a.R);
       }
     }
@@ -123,13 +123,14 @@ struct ChunkTile {
 // its lanes, later ones are read again.
 struct ChunkList {
   const ChunkParams& p;
-  int lane;
+  int split, lane;
   int64_t mine, upto;  // cost of request `lane`, and with all before it
-  __device__ __forceinline__ ChunkList(const ChunkParams& p_, int lane_) : p(p_), lane(lane_) {
+  __device__ __forceinline__ ChunkList(const ChunkParams& p_, int split_, int lane_)
+      : p(p_), split(split_), lane(lane_) {
     mine = cost(lane);
     upto = scan(mine);
   }
-  __device__ __forceinline__ int64_t cost(int r) const { return r < p.a.R ? chunk_request(p, r).head * p.a.Hkv : 0; }
+  __device__ __forceinline__ int64_t cost(int r) const { return r < p.a.R ? chunk_request(p, split, r).head * p.a.Hkv : 0; }
   __device__ __forceinline__ int64_t scan(int64_t x) const {
 #pragma unroll
     for (int d = 1; d < 32; d <<= 1) {
@@ -161,7 +162,8 @@ struct ChunkList {
       }
       base += __shfl_sync(0xFFFFFFFFu, sum, 31);
     }
-    c.req = chunk_request(p, c.r);
+    c.split = split;
+    c.req = chunk_request(p, split, c.r);
     const int64_t rel = w - base;
     c.head = static_cast<int>(div_wide(rel, c.req.head));
     const int64_t in_head = rel - c.head * c.req.head;
@@ -195,6 +197,12 @@ struct ChunkCuts {
     if (w - tile.start <= near) return tile.start;
     if (tile.start + tile.cost - w <= near) return tile.start + tile.cost;
     return w;
+  }
+  // The first run that begins behind list place w (the start of a tile that a cut divides).
+  __device__ __forceinline__ int first_inside(int64_t w) const {
+    int c = run.of(w) + 1;
+    while (run.start(c) - w <= near) ++c;
+    return c;
   }
 };
 
@@ -332,6 +340,14 @@ __global__ void __launch_bounds__(kChunkThreads, kChunkCtasPerSm)
   const uint32_t sbase = (smem_u32(chunk_smem_raw) + 1023u) & ~1023u;
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   grid_dependents_launch();
+  // no request for this kernel: nothing to set up
+  const int split = paged_split<PagedLayout<HD>::kKeys>(p.a, lane);
+  bool any = false;
+  for (int r = lane; r < p.a.R; r += 32) any |= paged_rows(p.a, paged_raw(p.a, r)).rows > split;
+  if (!__any_sync(0xFFFFFFFFu, any)) {
+    if (threadIdx.x == 0) p.a.merges[blockIdx.x] = make_int4(0, 0, 0, -1);
+    return;
+  }
 
   if (threadIdx.x == 0) {
     mbar_init(&bar_q, 1);
@@ -366,13 +382,13 @@ __global__ void __launch_bounds__(kChunkThreads, kChunkCtasPerSm)
   if (warp == 0) {
     // ------------------------------------------------------------ producer
     const int boxes = kSqdkBN / p.box_rows;
-    const ChunkList list(p, lane);
+    const ChunkList list(p, split, lane);
     const ChunkCuts cuts(list.total(), gridDim.x);
     ChunkWalk walk;
     walk.open(list, cuts, blockIdx.x);
     uint32_t nk = 0, nv = 0, segs = 0, posted = 0;
     bool live = true;
-    int merge_to = -1;
+    bool goes_on = false;
     ChunkTile tile;
     int slot;
     while (live) {
@@ -389,15 +405,17 @@ __global__ void __launch_bounds__(kChunkThreads, kChunkCtasPerSm)
       ++posted;
       __syncwarp();
       if (!more) break;
-      if (slot >= 0 && (slot & 1)) {
-        // the first piece of its tile: its merge goes up to the last run that
-        // begins inside the tile
+      if (slot >= 0 && tile.start + tile.cost > walk.w1) {
+        // the tile goes on behind this run: its runs from the one in which it
+        // begins to the last that begins inside it share its merge
         const int64_t end = tile.start + tile.cost;
-        merge_to = cuts.run.of(end - 1);
-        if (end - cuts.run.start(merge_to) <= cuts.near) --merge_to;
+        const int first = slot & 1 ? static_cast<int>(blockIdx.x) : cuts.first_inside(tile.start) - 1;
+        int last = cuts.run.of(end - 1);
+        if (end - cuts.run.start(last) <= cuts.near) --last;
+        goes_on = true;
         if (lane == 0)
           p.a.merges[blockIdx.x] = make_int4(tile.req.q0 + tile.t * p.QT, min(p.QT, tile.req.len - tile.t * p.QT),
-                                             tile.head, merge_to);
+                                             tile.head, first << 16 | last);
       }
       const int nblk = job.nblk, j0 = job.j0;
       if (nblk == 0) continue;
@@ -454,7 +472,7 @@ __global__ void __launch_bounds__(kChunkThreads, kChunkCtasPerSm)
         ++nv;
       }
     }
-    if (lane == 0 && merge_to < 0) p.a.merges[blockIdx.x] = make_int4(0, 0, 0, -1);
+    if (lane == 0 && !goes_on) p.a.merges[blockIdx.x] = make_int4(0, 0, 0, -1);
     // every copy this warp issued has landed before the CTA may exit
     if (lane == 0) {
       if (segs > 0) mbar_wait_drain(&bar_q, (segs - 1) & 1);
@@ -738,8 +756,9 @@ __global__ void __launch_bounds__(kChunkThreads, kChunkCtasPerSm)
           // unnormalised O of this piece, rows side by side in groups of four
           // columns: a warp's stores are whole lines
           float4* dst = reinterpret_cast<float4*>(p.a.part_o) + (static_cast<int64_t>(slot) * (HD / 4) + c / 4) * kSqdkBM + r;
+          if (row_valid)
 #pragma unroll
-          for (int v = 0; v < 8; ++v) dst[v * kSqdkBM] = make_float4(o[4 * v], o[4 * v + 1], o[4 * v + 2], o[4 * v + 3]);
+            for (int v = 0; v < 8; ++v) dst[v * kSqdkBM] = make_float4(o[4 * v], o[4 * v + 1], o[4 * v + 2], o[4 * v + 3]);
           continue;
         }
         // 32 columns of the warp's 32 rows through shared memory, so that a
@@ -786,42 +805,75 @@ __global__ void __launch_bounds__(kChunkThreads, kChunkCtasPerSm)
   }
 }
 
-// Adds the pieces of the tile whose first piece ends run c0, as that run noted:
-// O = sum 2^(m_c - M) O_c / sum 2^(m_c - M) l_c over the runs in order.
-// A warp takes 8 rows by 16 columns at a time (128-byte reads of the pieces);
-// kChunkMergeBlocks blocks share a tile.
+// Adds the pieces of the tile that goes on behind run `run`, as that run noted:
+// O = sum 2^(m_c - M) O_c / sum 2^(m_c - M) l_c over the runs in order. Every run
+// that the tile goes on behind gives kChunkMergeBlocks blocks to it. A warp takes
+// 8 rows by 16 columns at a time (128-byte reads of the pieces); where there are
+// more warps than that needs, several share the pieces.
 constexpr int kChunkMergeBlocks = 4;
 
 template <int HD, bool kBF16>
-__device__ __forceinline__ void chunk_merge(const ChunkParams& p, int c0, int share) {
+__device__ __forceinline__ void chunk_merge(const ChunkParams& p, int run, int share) {
+  __shared__ float s_m[kMergeWarps][32], s_l[kMergeWarps][32];
+  __shared__ float4 s_o[kMergeWarps][32];
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-  const int4 note = p.a.merges[c0];
-  const int c1 = note.w;
-  if (c1 < 0) return;
+  const int4 note = p.a.merges[run];
+  if (note.w < 0) return;
+  const int c0 = note.w >> 16, c1 = note.w & 0xFFFF, pieces = c1 - c0 + 1;
   const float2* ml = reinterpret_cast<const float2*>(p.a.part_ml);
   const float4* part = reinterpret_cast<const float4*>(p.a.part_o);
   const int rows = note.y * p.a.G;
-#pragma unroll 2
-  for (int i = warp + share * kMergeWarps; i < (kSqdkBM / 8) * (HD / 16); i += kMergeWarps * kChunkMergeBlocks) {
+  const int units = (rows + 7) / 8 * (HD / 16), blocks = (c1 - c0) * kChunkMergeBlocks;
+  // warps a unit: a power of two up to 16, two pieces a warp at least
+  int k = 1;
+  while (k < kMergeWarps && 2 * k * units <= blocks * kMergeWarps && 4 * k <= pieces) k *= 2;
+  const int per = (pieces + k - 1) / k, from = c0 + warp % k * per, to = min(c1 + 1, from + per);
+  const int step = blocks * (kMergeWarps / k);
+  // every warp of the block takes as many turns
+  for (int i0 = ((run - c0) * kChunkMergeBlocks + share) * (kMergeWarps / k); i0 < units; i0 += step) {
+    const int i = i0 + warp / k;
     const int r = i / (HD / 16) * 8 + (lane >> 2), q4 = i % (HD / 16) * 4 + (lane & 3);  // row, group of 4 columns
-    if (r >= rows || q4 * 4 >= p.a.hd) continue;
+    const bool live = i < units && r < rows && q4 * 4 < p.a.hd;
     float M = -INFINITY, l = 0.0f;
     bool none = true;
     float4 o = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
-#pragma unroll 2
-    for (int c = c0; c <= c1; ++c) {
-      // run c0's piece is its last, the others' their first
-      const int64_t slot = 2 * static_cast<int64_t>(c) + (c == c0 ? 1 : 0);
-      const float2 x = ml[slot * kSqdkBM + r];
-      const float4 v = part[(slot * (HD / 4) + q4) * kSqdkBM + r];
-      if (x.y == kUnseen) continue;
+    auto add = [&](float m, float s, const float4& v) {
+      if (s == kUnseen) return;
       none = false;
-      const float top = fmaxf(M, x.x);
-      const float f = x.x == top ? 1.0f : fast_exp2(x.x - top), g = M == top ? 1.0f : fast_exp2(M - top);
+      const float top = fmaxf(M, m);
+      const float f = m == top ? 1.0f : fast_exp2(m - top), g = M == top ? 1.0f : fast_exp2(M - top);
       M = top;
-      l = g * l + f * x.y;
+      l = g * l + f * s;
       o.x = g * o.x + f * v.x, o.y = g * o.y + f * v.y, o.z = g * o.z + f * v.z, o.w = g * o.w + f * v.w;
+    };
+    if (live) {
+      // four pieces' loads in flight
+      for (int c = from; c < to; c += 4) {
+        float2 x[4];
+        float4 v[4];
+#pragma unroll
+        for (int u = 0; u < 4; ++u) {
+          if (c + u >= to) continue;
+          // run c0's piece is its last, the others' their first
+          const int64_t slot = 2 * static_cast<int64_t>(c + u) + (c + u == c0 ? 1 : 0);
+          x[u] = ml[slot * kSqdkBM + r];
+          v[u] = part[(slot * (HD / 4) + q4) * kSqdkBM + r];
+        }
+#pragma unroll
+        for (int u = 0; u < 4; ++u)
+          if (c + u < to) add(x[u].x, x[u].y, v[u]);
+      }
     }
+    if (k > 1) {
+      __syncthreads();
+      s_m[warp][lane] = M;
+      s_l[warp][lane] = none ? kUnseen : l;
+      s_o[warp][lane] = o;
+      __syncthreads();
+      if (warp % k == 0)
+        for (int w = warp + 1; w < warp + k; ++w) add(s_m[w][lane], s_l[w][lane], s_o[w][lane]);
+    }
+    if (!live || warp % k != 0) continue;
     const float inv = 1.0f / l;
     const int ql = r / p.a.G;
     uint2 w;
