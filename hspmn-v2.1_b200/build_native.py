@@ -67,14 +67,16 @@ def build_torch_ops(force: bool = False, verbose: bool = False) -> str:
     header = os.path.join(INCLUDE, "hspmn_sm100.h")
     if not force and up_to_date(TORCH_LIB, [TORCH_SOURCE, header]):
         return TORCH_LIB
+    import sysconfig
     import torch
     from torch.utils.cpp_extension import include_paths, library_paths
     cuda_include = os.path.join(os.path.dirname(os.path.dirname(os.path.realpath(nvcc()))), "include")
     cmd = [os.environ.get("CXX", "g++"), "-O2", "-std=c++17", "-fPIC", "-shared", "-fvisibility=hidden",
            f"-D_GLIBCXX_USE_CXX11_ABI={int(torch._C._GLIBCXX_USE_CXX11_ABI)}",
-           *(f"-isystem{p}" for p in include_paths()), f"-isystem{cuda_include}", "-I", INCLUDE, TORCH_SOURCE,
+           *(f"-isystem{p}" for p in (*include_paths(), cuda_include, sysconfig.get_paths()["include"])), "-I", INCLUDE, TORCH_SOURCE,
            "-o", TORCH_LIB + ".tmp", "-L", os.path.dirname(LIB), "-l:" + os.path.basename(LIB), "-Wl,-rpath,$ORIGIN",
-           *(f"-L{p}" for p in library_paths()), "-lc10", "-lc10_cuda", "-ltorch_cpu", "-ldl"]
+           *(f"-L{p}" for p in library_paths()), "-lc10", "-lc10_cuda", "-ltorch_cpu", "-ltorch_cuda",
+           "-ltorch_python", "-ldl"]
     run(cmd, TORCH_LIB, verbose)
     return TORCH_LIB
 

@@ -797,12 +797,42 @@ int check_strides(std::initializer_list<int64_t> strides, int64_t es) {
   return HSPMN_OK;
 }
 
+// Lets kernel kKern use `bytes` of dynamic shared memory on the current device
+// (asked of the runtime once a device: the call takes as long as a launch).
+template <auto kKern>
+int allow_smem(int bytes) {
+  static int allowed[kMaxDevices];
+  int dev = 0;
+  if (cudaGetDevice(&dev) != cudaSuccess || dev < 0 || dev >= kMaxDevices) return HSPMN_ERR_CUDA;
+  if (__atomic_load_n(&allowed[dev], __ATOMIC_ACQUIRE)) return HSPMN_OK;
+  if (cudaFuncSetAttribute(kKern, cudaFuncAttributeMaxDynamicSharedMemorySize, bytes) != cudaSuccess)
+    return HSPMN_ERR_CUDA;
+  __atomic_store_n(&allowed[dev], 1, __ATOMIC_RELEASE);
+  return HSPMN_OK;
+}
+
+// CTAs of kThreads threads of kernel kKern that an SM of the current device
+// holds (asked once a device).
+template <auto kKern, int kThreads>
+int ctas_per_sm(int* out) {
+  static int held[kMaxDevices];
+  int dev = 0;
+  if (cudaGetDevice(&dev) != cudaSuccess || dev < 0 || dev >= kMaxDevices) return HSPMN_ERR_CUDA;
+  int n = __atomic_load_n(&held[dev], __ATOMIC_ACQUIRE);
+  if (n == 0) {
+    if (cudaOccupancyMaxActiveBlocksPerMultiprocessor(&n, kKern, kThreads, 0) != cudaSuccess || n < 1)
+      return HSPMN_ERR_CUDA;
+    __atomic_store_n(&held[dev], n, __ATOMIC_RELEASE);
+  }
+  *out = n;
+  return HSPMN_OK;
+}
+
 template <typename T, typename Tab, int kLanes>
 int launch_paged_write_lanes(const PagedWriteParams& prm, int sms, cudaStream_t st) {
-  auto kern = rope_paged_write_kernel<T, Tab, kLanes>;
+  constexpr auto kern = rope_paged_write_kernel<T, Tab, kLanes>;
   int per_sm = 0;
-  if (cudaOccupancyMaxActiveBlocksPerMultiprocessor(&per_sm, kern, kRowThreads, 0) != cudaSuccess || per_sm < 1)
-    return HSPMN_ERR_CUDA;
+  if (int rc = ctas_per_sm<kern, kRowThreads>(&per_sm)) return rc;
   const int64_t need = (prm.N + kRowThreads / kLanes - 1) / (kRowThreads / kLanes);
   const unsigned grid = static_cast<unsigned>(std::min<int64_t>(need, static_cast<int64_t>(sms) * per_sm));
   kern<<<grid, kRowThreads, 0, st>>>(prm);
@@ -854,10 +884,9 @@ void paged_ws_carve(PagedAttnParams* prm, void* ws, int64_t runs, int rows, int6
 
 template <int HD, bool kBF16>
 int launch_paged(const PagedAttnParams& prm, int runs, cudaStream_t st) {
-  auto kern = paged_attn_kernel<HD, kBF16>;
+  constexpr auto kern = paged_attn_kernel<HD, kBF16>;
   constexpr int smem = PagedLayout<HD>::kBytes;
-  if (cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, smem) != cudaSuccess)
-    return HSPMN_ERR_CUDA;
+  if (int rc = allow_smem<kern>(smem)) return rc;
   kern<<<static_cast<unsigned>(runs), kPagedThreads, smem, st>>>(prm);
   if (int rc = launch_status()) return rc;
   return launch_dependent(paged_merge_kernel<HD, kBF16>, static_cast<unsigned>(runs), 32 * kMergeWarps, 0, st, prm);
@@ -868,12 +897,11 @@ int launch_paged(const PagedAttnParams& prm, int runs, cudaStream_t st) {
 template <int HD, bool kBF16>
 int launch_paged_chunks(const CUtensorMap& mq, const CUtensorMap& mk, const CUtensorMap& mv, const ChunkParams& ch,
                         int chunk_runs, const PagedAttnParams& prm, int runs, cudaStream_t st) {
-  auto chunks = paged_chunk_kernel<HD, kBF16>;
-  auto rows = paged_attn_kernel<HD, kBF16>;
+  constexpr auto chunks = paged_chunk_kernel<HD, kBF16>;
+  constexpr auto rows = paged_attn_kernel<HD, kBF16>;
   constexpr int chunk_smem = ChunkLayout<HD>::kAlloc, smem = PagedLayout<HD>::kBytes;
-  if (cudaFuncSetAttribute(chunks, cudaFuncAttributeMaxDynamicSharedMemorySize, chunk_smem) != cudaSuccess ||
-      cudaFuncSetAttribute(rows, cudaFuncAttributeMaxDynamicSharedMemorySize, smem) != cudaSuccess)
-    return HSPMN_ERR_CUDA;
+  if (int rc = allow_smem<chunks>(chunk_smem)) return rc;
+  if (int rc = allow_smem<rows>(smem)) return rc;
   chunks<<<static_cast<unsigned>(chunk_runs), kChunkThreads, chunk_smem, st>>>(mq, mk, mv, ch);
   if (int rc = launch_status()) return rc;
   if (int rc = launch_dependent(rows, static_cast<unsigned>(runs), kPagedThreads, smem, st, prm)) return rc;
@@ -917,10 +945,9 @@ int hspmn_paged_slots(int32_t* block_table, int64_t table_rs, const int32_t* seq
   prm.slots = slots;
   prm.taken = taken;
   const size_t smem = static_cast<size_t>(2 * (R + 1) * 4);
-  if (smem > 48 * 1024 &&
-      cudaFuncSetAttribute(paged_slots_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize,
-                           2 * (kSlotsMaxRequests + 1) * 4) != cudaSuccess)
-    return HSPMN_ERR_CUDA;
+  if (smem > 48 * 1024) {
+    if (int rc = allow_smem<paged_slots_kernel>(2 * (kSlotsMaxRequests + 1) * 4)) return rc;
+  }
   const int64_t need = std::max<int64_t>(1, (N + kSlotsThreads - 1) / kSlotsThreads);
   const unsigned grid = static_cast<unsigned>(std::min<int64_t>(need, 2LL * sms));
   paged_slots_kernel<<<grid, kSlotsThreads, smem, static_cast<cudaStream_t>(stream)>>>(prm);

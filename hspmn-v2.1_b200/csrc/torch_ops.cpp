@@ -1,12 +1,16 @@
-// torch operators of the paged K/V cache (torch.ops.hspmn.*): argument checks,
-// outputs and workspace from PyTorch's allocator, and the call into the C ABI
-// on the caller's current stream. They are registered from C++ because a decode
-// step calls them for microseconds of GPU work each: through Python checks and
-// ctypes a call took 28 to 37 us of host time, from here 7 to 9.
+// torch operators of the paged K/V cache: argument checks, outputs and workspace
+// from PyTorch's allocator, and the call into the C ABI on the caller's current
+// stream. They are in C++ because a decode step calls them for microseconds of
+// GPU work each (through Python checks and ctypes a call took 28 to 37 us of host
+// time). Registered as torch.ops.hspmn.*, for tracing, and as functions of the
+// Python module libhspmn_torch, which eager calls use: the dispatcher's boxing of
+// the arguments costs 2 us more.
 #include <ATen/ATen.h>
+#include <ATen/cuda/EmptyTensor.h>
 #include <c10/cuda/CUDAGuard.h>
 #include <c10/cuda/CUDAStream.h>
 #include <nvtx3/nvToolsExt.h>
+#include <torch/csrc/utils/pybind.h>
 #include <torch/library.h>
 
 #include <initializer_list>
@@ -52,6 +56,11 @@ int dtype_code(const char* name, at::ScalarType t) {
   }
 }
 
+// at::empty without the dispatcher's part of its cost.
+Tensor empty_on(c10::Device dev, at::IntArrayRef sizes, at::ScalarType dtype) {
+  return at::detail::empty_cuda(sizes, dtype, dev, std::nullopt);
+}
+
 // A 1-D int32 / int64 argument of n elements, contiguous.
 Tensor vector_arg(const char* name, const char* what, const Tensor& t, at::ScalarType dtype, int64_t n) {
   TORCH_CHECK_VALUE(t.scalar_type() == dtype && t.dim() == 1 && (n < 0 || t.size(0) == n), name, ": ", what, " must be ",
@@ -92,9 +101,8 @@ std::tuple<Tensor, Tensor, Tensor, Tensor, Tensor> paged_slots_(const Tensor& bl
                     ": block_table is written in place: its rows must be dense and must not overlap");
   TORCH_CHECK_VALUE(num_tokens >= 0, name, ": num_tokens=", num_tokens);
   const c10::cuda::CUDAGuard guard(dev);
-  const auto i32 = block_table.options(), i64 = i32.dtype(at::kLong);
-  Tensor cu = at::empty({R + 1}, i32), kv_lens = at::empty({R}, i32), taken = at::empty({1}, i32);
-  Tensor positions = at::empty({num_tokens}, i64), slots = at::empty({num_tokens}, i64);
+  Tensor cu = empty_on(dev, {R + 1}, at::kInt), kv_lens = empty_on(dev, {R}, at::kInt), taken = empty_on(dev, {1}, at::kInt);
+  Tensor positions = empty_on(dev, {num_tokens}, at::kLong), slots = empty_on(dev, {num_tokens}, at::kLong);
   const Range range("hspmn::paged_slots");
   check_status(
       hspmn_paged_slots(block_table.data_ptr<int32_t>(), R > 1 ? block_table.stride(0) : P,
@@ -179,11 +187,11 @@ Tensor sqdk_paged_fwd(const Tensor& q_, const Tensor& k_cache, const Tensor& v_c
   const Tensor positions = vector_arg(name, "positions", positions_, at::kLong, n);
   const c10::cuda::CUDAGuard guard(dev);
   const Tensor q = rows_arg(q_);
-  Tensor o = at::empty({n, H, hd}, q.options());
+  Tensor o = empty_on(dev, {n, H, hd}, q.scalar_type());
   if (n == 0) return o;
   const int64_t bytes = hspmn_sqdk_paged_workspace_size(n, H, Hkv, hd, max_q);
   TORCH_CHECK(bytes >= 0, "hspmn_sqdk_paged_workspace_size: device query failed");
-  Tensor ws = at::empty({bytes}, q.options().dtype(at::kByte));
+  Tensor ws = empty_on(dev, {bytes}, at::kByte);
   const Range range("hspmn::sqdk_paged_fwd");
   check_status(
       hspmn_sqdk_paged_fwd(q.const_data_ptr(), q.stride(0), q.stride(1), k_cache.const_data_ptr(), k_cache.stride(0),
@@ -217,4 +225,10 @@ TORCH_LIBRARY_IMPL(hspmn, CompositeExplicitAutograd, m) {
   m.impl("paged_slots_", paged_slots_);
   m.impl("rope_paged_write_", rope_paged_write_);
   m.impl("sqdk_paged_fwd", sqdk_paged_fwd);
+}
+
+PYBIND11_MODULE(libhspmn_torch, m) {
+  m.def("paged_slots_", paged_slots_);
+  m.def("rope_paged_write_", rope_paged_write_);
+  m.def("sqdk_paged_fwd", sqdk_paged_fwd);
 }

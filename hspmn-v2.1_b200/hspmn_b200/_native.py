@@ -97,16 +97,21 @@ def torch_ops_available() -> bool:
     return os.path.exists(TORCH_LIB_PATH) and available()
 
 
-def load_torch_ops() -> None:
-    """Register the C++ operators of libhspmn_torch.so with PyTorch; raise if it
-    is not built. (Loading a library again does nothing.)"""
+def load_torch_ops():
+    """Load libhspmn_torch.so: its operators are then registered with PyTorch.
+    Returns it as a Python module; raises if it is not built."""
     if not torch_ops_available():
         raise RuntimeError(
             f"{os.path.basename(TORCH_LIB_PATH)} is not built (expected at {TORCH_LIB_PATH}); run "
             "`python hspmn-v2.1_b200/build_native.py` on a machine with the CUDA toolkit")
-    import torch
+    import importlib.machinery
+    import importlib.util
+    import torch  # noqa: F401 (the module links against its libraries)
     lib()
-    torch.ops.load_library(TORCH_LIB_PATH)
+    loader = importlib.machinery.ExtensionFileLoader("libhspmn_torch", TORCH_LIB_PATH)
+    module = importlib.util.module_from_spec(importlib.util.spec_from_loader("libhspmn_torch", loader))
+    loader.exec_module(module)
+    return module
 
 
 def strerror(status: int) -> str:

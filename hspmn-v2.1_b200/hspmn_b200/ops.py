@@ -607,34 +607,39 @@ def sqdk_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, indices: t
 # paged K/V cache
 # ---------------------------------------------------------------------------
 
-# These operators are registered from C++ (csrc/torch_ops.cpp): a decode step
-# calls them for microseconds of GPU work each, so host time per call counts.
+# These operators are in C++ (csrc/torch_ops.cpp): a decode step calls them for
+# microseconds of GPU work each, so host time per call counts. Eager calls go to
+# the compiled functions directly, traced ones (and tensor subclasses) through
+# the operators registered as torch.ops.hspmn.*.
 
-
-_paged_ops = {}
+_paged_direct = None  # the compiled functions
+_paged_ops = {}       # the registered operators
 
 
 def _load_paged_ops() -> None:
-    N.load_torch_ops()
+    global _paged_direct
+    direct = N.load_torch_ops()
     for name, fake in (("paged_slots_", _paged_slots_fake), ("rope_paged_write_", lambda *args: None),
                        ("sqdk_paged_fwd", _sqdk_paged_fwd_fake)):
         torch.library.register_fake("hspmn::" + name, fake)
         _paged_ops[name] = getattr(torch.ops.hspmn, name).default
+    _paged_direct = direct
 
 
-def _call_paged(name: str, dev: torch.device, *args):
-    """One operator call; counted and, while a ``KernelTimer`` is active, timed
-    as the other launches are."""
-    if not _paged_ops:
-        _load_paged_ops()  # raises: the library was not there at import
-    op = _paged_ops[name]
+def _call_paged(name: str, first: torch.Tensor, *args):
+    """One operator call (``first``: its first tensor); counted and, while a
+    ``KernelTimer`` is active, timed as the other launches are."""
     if torch.compiler.is_compiling():
-        return op(*args)
+        return _paged_ops[name](first, *args)
+    if _paged_direct is None:
+        _load_paged_ops()  # raises: the library was not there at import
+    plain = type(first) is torch.Tensor and torch._C._len_torch_dispatch_stack() == 0
+    op = getattr(_paged_direct, name) if plain else _paged_ops[name]
     try:
         if LaunchStats.timer is not None:
-            with _launch(name.rstrip("_"), dev):
-                return op(*args)
-        out = op(*args)
+            with _launch(name.rstrip("_"), first.device):
+                return op(first, *args)
+        out = op(first, *args)
     except RuntimeError as e:
         if " (status -" in str(e):  # a library entry point refused the call
             raise N.HSPMNNativeError(str(e).splitlines()[0]) from None
@@ -663,7 +668,7 @@ def paged_slots_(block_table: torch.Tensor, seq_lens: torch.Tensor, new_lens: to
     entries and slots are -1 and ``DEVERR_PAGE`` is set in ``device_errors()``;
     negative lengths, tokens beyond N and lengths beyond P pages set
     ``DEVERR_POSITION``. At most 8192 requests a call."""
-    return _call_paged("paged_slots_", block_table.device, block_table, seq_lens, new_lens, free_pages,
+    return _call_paged("paged_slots_", block_table, seq_lens, new_lens, free_pages,
                        page_size, num_tokens)
 
 
@@ -689,7 +694,7 @@ def rope_paged_write_(k: torch.Tensor, v: torch.Tensor, cos: Optional[torch.Tens
     and their sum are float32 with one rounding, where ``rope_rows`` rounds each
     of the reference's tensor operations. A slot outside the cache or a position
     outside the tables sets ``DEVERR_PAGE`` / ``DEVERR_POSITION`` and is skipped."""
-    _call_paged("rope_paged_write_", k.device, k, v, cos, sin, positions, slots, k_cache, v_cache)
+    _call_paged("rope_paged_write_", k, v, cos, sin, positions, slots, k_cache, v_cache)
 
 
 def sqdk_paged_fwd(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tensor, block_table: torch.Tensor,
@@ -710,7 +715,7 @@ def sqdk_paged_fwd(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tensor
     behind ``cu_q[R]`` are zeros. A position beyond kv_lens sets
     ``DEVERR_POSITION``, a page outside the cache ``DEVERR_PAGE`` (its keys are
     left out) in ``device_errors()``. No backward."""
-    return _call_paged("sqdk_paged_fwd", q.device, q, k_cache, v_cache, block_table, kv_lens, cu_q,
+    return _call_paged("sqdk_paged_fwd", q, k_cache, v_cache, block_table, kv_lens, cu_q,
                        positions, sm_scale, max_q)
 
 
