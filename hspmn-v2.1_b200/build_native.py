@@ -42,6 +42,15 @@ def nvcc() -> str:
     raise RuntimeError("nvcc not found; the HSPMN library needs the CUDA toolkit to build")
 
 
+def cxx() -> str:
+    """The system's host compiler. (A compiler that links its own libstdc++ in
+    statically will not do: PyTorch's streams and the operators' must be one.)"""
+    for cand in ("/usr/bin/g++", shutil.which("g++"), os.environ.get("CXX")):
+        if cand and os.path.exists(cand):
+            return cand
+    raise RuntimeError("g++ not found; the paged-cache operators need a host compiler to build")
+
+
 def sources():
     return sorted(glob.glob(os.path.join(CSRC, "*.cu")) + glob.glob(os.path.join(CSRC, "*.cuh"))
                   + glob.glob(os.path.join(INCLUDE, "*.h")))
@@ -71,13 +80,17 @@ def build_torch_ops(force: bool = False, verbose: bool = False) -> str:
     import torch
     from torch.utils.cpp_extension import include_paths, library_paths
     cuda_include = os.path.join(os.path.dirname(os.path.dirname(os.path.realpath(nvcc()))), "include")
-    cmd = [os.environ.get("CXX", "g++"), "-O2", "-std=c++17", "-fPIC", "-shared", "-fvisibility=hidden",
+    cmd = [cxx(), "-O2", "-std=c++17", "-fPIC", "-shared", "-fvisibility=hidden",
            f"-D_GLIBCXX_USE_CXX11_ABI={int(torch._C._GLIBCXX_USE_CXX11_ABI)}",
            *(f"-isystem{p}" for p in (*include_paths(), cuda_include, sysconfig.get_paths()["include"])), "-I", INCLUDE, TORCH_SOURCE,
            "-o", TORCH_LIB + ".tmp", "-L", os.path.dirname(LIB), "-l:" + os.path.basename(LIB), "-Wl,-rpath,$ORIGIN",
            *(f"-L{p}" for p in library_paths()), "-lc10", "-lc10_cuda", "-ltorch_cpu", "-ltorch_cuda",
            "-ltorch_python", "-ldl"]
     run(cmd, TORCH_LIB, verbose)
+    with open(TORCH_LIB, "rb") as f:
+        if b"libstdc++.so" not in f.read():
+            os.remove(TORCH_LIB)
+            raise RuntimeError(f"{cmd[0]} links libstdc++ statically; build with a compiler that uses the shared one")
     return TORCH_LIB
 
 

@@ -596,8 +596,9 @@ __global__ void __launch_bounds__(kPagedThreads, kPagedCtasPerSm) paged_attn_ker
       if (!wild) {
 #pragma unroll
         for (int k = 0; k < kGroups; k += 2) {
-          // P in the operands' type: its rounding (half a step) is of the size
-          // of the output's own
+          // P in the operands' type: its rounding (half a step) is of the size of
+          // the output's own. (A second product with what the rounding leaves took
+          // the error to the output's alone, and 6 % more time for 64 requests.)
           const uint32_t pa[4] = {pack2<kBF16>(s[k][0], s[k][1]), pack2<kBF16>(s[k][2], s[k][3]),
                                   pack2<kBF16>(s[k + 1][0], s[k + 1][1]), pack2<kBF16>(s[k + 1][2], s[k + 1][3])};
 #pragma unroll

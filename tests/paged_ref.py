@@ -35,6 +35,17 @@ def rope_ref(k, cos, sin, positions):
     return x * c + turned * s, (x * c).abs() + (turned * s).abs()
 
 
+def weighted(w, v, hidden):
+    """sum over the visible keys of w v; a hidden key's infinity or NaN does not count."""
+    wild = ~torch.isfinite(v).all(-1)
+    if not wild.any():
+        return w @ v
+    out = w[..., ~wild] @ v[~wild]
+    for m in torch.nonzero(wild).flatten().tolist():
+        out = out + torch.where(hidden[..., m, None], 0.0, w[..., m, None] * v[m])
+    return out
+
+
 def attend_ref(q, k_cache, v_cache, table, kv_lens, cu_q, positions, scale):
     """sqdk_paged_fwd in float64 and, per output, a bound on the error of a
     kernel that multiplies 16-bit operands, sums in float32 and rounds P and O
@@ -64,22 +75,27 @@ def attend_ref(q, k_cache, v_cache, table, kv_lens, cu_q, positions, scale):
         for g in range(Hkv):
             k = k_cache[pages, :, g].reshape(-1, hd)[:n].double()
             v = v_cache[pages, :, g].reshape(-1, hd)[:n].double()
-            for i in range(a, b):
-                vis = min(int(positions[i]) + 1, n)
-                if vis <= 0:
-                    continue
-                qq = q[i, g * G:(g + 1) * G].double()
-                s = (qq @ k[:vis].T) * scale
-                size = (qq.abs() @ k[:vis].abs().T).amax(-1, keepdim=True) * scale
-                w = torch.softmax(s, -1)
-                o[i, g * G:(g + 1) * G] = w @ v[:vis]
-                mass = w @ v[:vis].abs()
-                spread = (s.amax(-1, keepdim=True) - s.amin(-1, keepdim=True)) / math.log(2)
-                rel = u + 2 * (hd + 4) * e * size + (8 + spread) * e + 2 * (vis + 32) * e
-                t = rel * mass + u * o[i, g * G:(g + 1) * G].abs()
-                if q.dtype == torch.float16:
-                    t = t + 2.0 ** -25 * v[:vis].abs().sum(0)
-                tol[i, g * G:(g + 1) * G] = t
+            pos = positions[a:b].long()
+            rows = torch.nonzero(pos >= 0).flatten()  # the others see nothing
+            if rows.numel() == 0:
+                continue
+            hidden = torch.arange(n, device=q.device)[None, None, :] > pos[rows][:, None, None]
+            qq = q[a:b, g * G:(g + 1) * G][rows].double()  # [rows, G, hd]
+            s = (qq @ k.T) * scale
+            # a masked score must not reach the result, whatever it is
+            size = (qq.abs() @ k.abs().T).masked_fill(hidden, 0.0).amax(-1, keepdim=True) * scale
+            low = s.masked_fill(hidden, math.inf).amin(-1, keepdim=True)
+            s = s.masked_fill(hidden, -math.inf)
+            spread = (s.amax(-1, keepdim=True) - low) / math.log(2)
+            w = torch.softmax(s, -1)
+            out = weighted(w, v, hidden)
+            vis = torch.clamp(pos[rows] + 1, max=n)[:, None, None].double()
+            rel = u + 2 * (hd + 4) * e * size + (8 + spread) * e + 2 * (vis + 32) * e
+            t = rel * weighted(w, v.abs(), hidden) + u * out.abs()
+            if q.dtype == torch.float16:
+                t = t + 2.0 ** -25 * weighted((~hidden).double().expand_as(w), v.abs(), hidden)
+            at = (a + rows)[:, None].expand(-1, G), torch.arange(g * G, (g + 1) * G, device=q.device).expand(len(rows), G)
+            o[at], tol[at] = out, t
     return o, tol
 
 

@@ -312,11 +312,12 @@ def test_positions_behind_the_last_token_are_flagged_and_see_all():
     assert ops.device_errors() == N.DEVERR_POSITION
 
 
-def test_missing_pages_are_left_out_and_flagged():
+@pytest.mark.parametrize("H", [4, 16])  # 120 and 480 query rows a K/V head: either kernel
+def test_missing_pages_are_left_out_and_flagged(H):
     lens = [160, 64]
     for many in (False, True):
         positions = [list(range(100, 160)), [63] * (50 if many else 1)]
-        args = batch(lens, positions, 4, 2, 64, torch.bfloat16, 16, seed=8)
+        args = batch(lens, positions, H, 2, 64, torch.bfloat16, 16, seed=8)
         q, kc, vc, table, kv, cu, pos = args
         table[0, 3], table[0, 5] = -1, kc.shape[0]
         table[1] = 1 << 20
@@ -333,6 +334,69 @@ def test_missing_pages_are_left_out_and_flagged():
         want, tol = ref.attend_ref(q[:60], k2.view(-1, 16, 2, 64), v2.view(-1, 16, 2, 64),
                                    torch.arange(len(k2) // 16, device=DEV)[None], [n], [0, 60], pos[:60] - 32, 0.125)
         assert ((o[:60].double() - want).abs() <= tol).all()
+
+
+@pytest.mark.parametrize("big", [False, True])
+@pytest.mark.parametrize("H,Hkv,hd", [(16, 4, 128), (8, 8, 64), (6, 2, 96)])
+def test_short_runs(H, Hkv, hd, big):
+    """Requests of one to eight 16-row tiles, alone and beside one that is larger (they go to different kernels)."""
+    lens = [700, 33, 128, 129, 300, 64, 1000]
+    count = [5, 8, 16, 1, 31, 2, 40] if G(H, Hkv) > 1 else [17, 33, 100, 1, 16, 2, 128]
+    positions = [list(range(max(0, n - c), n)) for n, c in zip(lens, count)]
+    if big:
+        lens.append(350)
+        positions.append(list(range(0, 350)))
+    check(batch(lens, positions, H, Hkv, hd, torch.bfloat16, 16, seed=21 + hd), max_qs=(0,))
+    assert ops.device_errors() == 0
+
+
+def G(H, Hkv):
+    return H // Hkv
+
+
+@pytest.mark.parametrize("R,n", [(33, 40), (100, 37), (300, 33)])
+def test_many_chunks(R, n):
+    """More requests than a warp has lanes, each of several tiles; some without queries, some with one."""
+    lens = [n + 7 * (r % 11) for r in range(R)]
+    positions = [[] if r % 9 == 4 else [m - 1] if r % 9 == 5 else list(range(m - n, m)) for r, m in enumerate(lens)]
+    check(batch(lens, positions, 16, 2, 64, torch.float16, 32, seed=R), max_qs=(n,))
+    assert ops.device_errors() == 0
+
+
+@pytest.mark.parametrize("seed", range(12))
+def test_random_batches(seed):
+    """Runs cut anywhere: random lengths, query counts and order, heads, pages and types."""
+    import random
+    rng = random.Random(seed)
+    H, Hkv, hd = rng.choice(HEADS)
+    lens = [rng.randint(1, rng.choice((50, 500, 3000))) for _ in range(rng.randint(1, 12))]
+    positions = []
+    for m in lens:
+        count = rng.choice((0, 1, rng.randint(1, min(m, 40)), rng.randint(1, m)))
+        positions.append(sorted(rng.sample(range(m), count)))
+    check(batch(lens, positions, H, Hkv, hd, rng.choice((torch.bfloat16, torch.float16)), rng.choice((8, 16, 64, 128)),
+                seed=seed, joint=seed % 2 == 0, tail=seed % 3, fill=float("nan")), max_qs=(0,))
+    assert ops.device_errors() == 0
+
+
+def test_long_context():
+    """One token and one chunk over 70,001 keys."""
+    args = batch([70001], [[70000]], 8, 2, 128, torch.float16, 64, seed=15)
+    check(args, max_qs=(1,))
+    args = batch([70001], [list(range(69901, 70001))], 8, 2, 64, torch.bfloat16, 64, seed=16)
+    check(args, max_qs=(100,))
+    assert ops.device_errors() == 0
+
+
+def test_lengths_beyond_the_table_are_cut():
+    q, kc, vc, table, kv, cu, pos = batch([64], [[63]], 4, 2, 64, torch.bfloat16, 16, seed=17)
+    want = attend(q, kc, vc, table, [64], cu, pos)
+    assert torch.equal(attend(q, kc, vc, table, [2 ** 31 - 1], cu, pos), want)
+    assert ops.device_errors() == 0
+    none = attend(q, kc, vc, table[:, :0], [64], cu, pos)  # no page at all
+    assert not none.any() and ops.device_errors() == N.DEVERR_POSITION
+    none = attend(q, kc[:0], vc[:0], table, [64], cu, pos)  # an empty cache
+    assert not none.any() and ops.device_errors() == N.DEVERR_PAGE
 
 
 def test_strided_operands():
@@ -398,6 +462,45 @@ def test_other_stream():
         got = attend(*args, max_q=200)
     side.synchronize()
     assert torch.equal(got, want)
+
+
+def test_two_calls_at_once():
+    """Calls on two streams, in flight together, each with its own workspace."""
+    a = batch([9000, 400], [[8999], list(range(200, 400))], 16, 4, 128, torch.bfloat16, 64, seed=18)
+    b = batch([7000, 900], [[6999], list(range(100, 900, 2))], 16, 4, 128, torch.bfloat16, 64, seed=19)
+    want = [attend(*x, max_q=400) for x in (a, b)]
+    torch.cuda.synchronize()
+    streams, got = [torch.cuda.Stream(), torch.cuda.Stream()], [[], []]
+    for _ in range(20):
+        for i, x in enumerate((a, b)):
+            with torch.cuda.stream(streams[i]):
+                got[i].append(attend(*x, max_q=400))
+    torch.cuda.synchronize()
+    for i in range(2):
+        assert all(torch.equal(o, want[i]) for o in got[i])
+    assert ops.device_errors() == 0
+
+
+def test_two_graphs_in_turn():
+    """Two captured calls replayed in turn on new inputs."""
+    a = batch([600, 80], [[599], list(range(80))], 8, 2, 64, torch.bfloat16, 16, seed=22)
+    graphs, outs, queries = [], [], [a[0].clone(), a[0].clone()]
+    side = torch.cuda.Stream()
+    with torch.cuda.stream(side):
+        attend(*a, max_q=80)
+    torch.cuda.synchronize()
+    kv, cu = i32(a[4]), i32(a[5])
+    pool = torch.cuda.graph_pool_handle()
+    for q in queries:
+        graph = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(graph, pool=pool):
+            outs.append(ops.sqdk_paged_fwd(q, a[1], a[2], a[3], kv, cu, a[6], 0.125, 80))
+        graphs.append(graph)
+    for i in range(6):
+        queries[i % 2].copy_(torch.randn(a[0].shape, generator=torch.Generator().manual_seed(i)))
+        graphs[i % 2].replay()
+        want = attend(queries[i % 2], *a[1:], scale=0.125, max_q=80)
+        assert torch.equal(outs[i % 2], want)
 
 
 def test_captured_step_replays_with_new_lengths():
@@ -477,6 +580,87 @@ def test_prefill_in_chunks_and_decode_equal_the_whole_sequence():
     # two kernels, each within its bound
     assert ((got - dense).double().abs().reshape(-1, H, hd) <= 2 * tol + 2.0 ** -8 * want.abs()).all()
     assert ops.device_errors() == 0
+
+
+def test_refusals():
+    q, kc, vc, table, kv, cu, pos = batch([20], [[18, 19]], 4, 2, 64, torch.bfloat16, 16, seed=23)
+    kv, cu = i32(kv), i32(cu)
+
+    def fwd(q=q, kc=kc, vc=vc, table=table, kv=kv, cu=cu, pos=pos, scale=0.125, max_q=0):
+        return ops.sqdk_paged_fwd(q, kc, vc, table, kv, cu, pos, scale, max_q)
+
+    fwd()
+    for over in (dict(q=q[0]), dict(kc=kc[0]), dict(kc=kc[:, :8]), dict(kc=kc[..., :32], vc=vc[..., :32]),
+                 dict(table=table[0]), dict(table=table.long()), dict(kv=kv.long()), dict(kv=kv[:0]), dict(cu=cu[:1]),
+                 dict(pos=pos[:1]), dict(pos=pos.int()), dict(q=q[:, :3]),
+                 dict(kc=kc.transpose(2, 3).contiguous().transpose(2, 3))):
+        with pytest.raises(ValueError):
+            fwd(**over)
+    for over in (dict(q=q.float()), dict(q=q.half()), dict(vc=vc.half())):
+        with pytest.raises(TypeError):
+            fwd(**over)
+    for over in (dict(scale=-1.0), dict(scale=float("inf")), dict(max_q=-1), dict(kc=kc[:, :12], vc=vc[:, :12])):
+        with pytest.raises(N.HSPMNNativeError):
+            fwd(**over)
+    with pytest.raises(RuntimeError, match="CUDA tensors"):
+        fwd(pos=pos.cpu())
+    with pytest.raises(RuntimeError, match="no backward"):
+        fwd(q=q.clone().requires_grad_())
+    with torch.no_grad():
+        fwd(q=q.clone().requires_grad_())
+
+    k = torch.zeros((2, 2, 64), dtype=torch.bfloat16, device=DEV)
+    cos = torch.zeros((32, 64), dtype=torch.bfloat16, device=DEV)
+
+    def write(k=k, v=k, cos=cos, sin=cos, pos=pos, slots=pos, kc=kc, vc=vc):
+        ops.rope_paged_write_(k, v, cos, sin, pos, slots, kc, vc)
+
+    write()
+    write(k=k[:0], v=k[:0], pos=pos[:0], slots=pos[:0])
+    for over in (dict(k=k[0], v=k[0]), dict(v=k[:1]), dict(sin=None), dict(cos=cos[:, :32], sin=cos[:, :32]), dict(sin=cos[:5]),
+                 dict(pos=pos[:1]), dict(slots=pos.int()), dict(kc=kc[:, :, :1], vc=vc[:, :, :1])):
+        with pytest.raises(ValueError):
+            write(**over)
+    for over in (dict(v=k.half()), dict(cos=cos.half(), sin=cos.half()), dict(kc=kc.half()), dict(k=k.double(), v=k.double())):
+        with pytest.raises(TypeError):
+            write(**over)
+    with pytest.raises(RuntimeError, match="CUDA tensors"):
+        write(cos=cos.cpu(), sin=cos.cpu())
+    with pytest.raises(RuntimeError, match="no backward"):
+        write(k=k.clone().requires_grad_())
+
+    t = torch.zeros((2, 4), dtype=torch.int32, device=DEV)
+    n = i32([1, 2])
+    ops.paged_slots_(t, n, n, n, 16, 3)
+    for args in ((t[0], n, n, n, 16, 3), (t, n[:1], n, n, 16, 3), (t, n, n.long(), n, 16, 3), (t, n, n, t, 16, 3),
+                 (t, n, n, n, 16, -1), (t.t().contiguous().t(), n, n, n, 16, 3), (t[:1].expand(2, 4), n, n, n, 16, 3)):
+        with pytest.raises(ValueError):
+            ops.paged_slots_(*args)
+    with pytest.raises(N.HSPMNNativeError):
+        ops.paged_slots_(t, n, n, n, 20, 3)
+    assert ops.device_errors() == 0
+
+
+def test_calls_are_counted_and_timed():
+    q, kc, vc, table, kv, cu, pos = batch([20], [[19]], 4, 2, 64, torch.bfloat16, 16, seed=24)
+    before = ops.LaunchStats.launches
+    with ops.KernelTimer() as timer:
+        attend(q, kc, vc, table, kv, cu, pos)
+    torch.cuda.synchronize()
+    assert timer.results()["sqdk_paged_fwd"]["launches"] == 1 and ops.LaunchStats.launches == before + 1
+    attend(q, kc, vc, table, kv, cu, pos)
+    assert ops.LaunchStats.launches == before + 2
+
+
+def test_compiled_step_is_one_graph():
+    q, kc, vc, table, kv, cu, pos = batch([20, 50], [[19], [49]], 4, 2, 64, torch.bfloat16, 16, seed=25)
+    kv, cu = i32(kv), i32(cu)
+
+    def step(q, kc, vc):
+        return ops.sqdk_paged_fwd(q * 2, kc, vc, table, kv, cu, pos, 0.125, 1) + 1
+
+    got = torch.compile(step, backend="aot_eager", fullgraph=True)(q, kc, vc)
+    assert torch.equal(got, step(q, kc, vc))
 
 
 def test_registered_operators_trace():
