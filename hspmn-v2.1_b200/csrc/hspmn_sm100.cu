@@ -867,6 +867,14 @@ int launch_dependent(void (*kern)(Params...), unsigned grid, unsigned threads, s
   return cudaLaunchKernelEx(&cfg, kern, prm...) == cudaSuccess ? HSPMN_OK : HSPMN_ERR_CUDA;
 }
 
+// Shift that brings a list of up to `items` items of up to `cost` each (one added
+// to an item by rounding) below 2^30.
+int list_shift(int64_t items, int64_t cost) {
+  int s = 0;
+  while (s < 26 && static_cast<double>(items) * static_cast<double>((cost >> s) + 2) >= 1073741824.0) ++s;
+  return s;
+}
+
 // Whether a call has, by its arguments, requests that the chunk kernel may take.
 bool paged_has_chunks(int64_t N, int64_t G, int64_t max_q) {
   return (max_q > 0 ? std::min(max_q, N) : N) * G > kPagedRows;
@@ -1036,7 +1044,7 @@ int hspmn_sqdk_paged_fwd(const void* q, int64_t q_sn, int64_t q_sh, const void* 
   const int shift = page_shift(page_size);
   if (shift < 0 || hd < 8 || hd > 128 || hd % 8 != 0) return HSPMN_ERR_UNSUPPORTED;
   if (H % Hkv != 0 || H / Hkv > kSqdkBM) return HSPMN_ERR_UNSUPPORTED;
-  if (N > 0x7FFFFFFF / H || R > 0x7FFFFFFE || P > (0x7FFFFFFF >> shift) || num_pages > 0x7FFFFFFF)
+  if (N > 0x7FFFFFFF / H || R > 0x07FFFFFF / Hkv || P > (0x7FFFFFFF >> shift) || num_pages > 0x7FFFFFFF)
     return HSPMN_ERR_INVALID;
   const int64_t es = 2;
   // the stride of a dimension of one element is never used: any is accepted
@@ -1087,6 +1095,9 @@ int hspmn_sqdk_paged_fwd(const void* q, int64_t q_sn, int64_t q_sh, const void* 
   prm.hd = static_cast<int>(hd);
   prm.scale_log2 = sm_scale * 1.4426950408889634f;
   prm.has_chunks = 0;
+  // the lists' costs in 32 bits, whatever the lengths turn out to be
+  const int64_t keys = std::min<int64_t>(P << shift, 0x7FFFFFFF), unit = hd > 64 ? 64 : 128;
+  prm.cost_shift = list_shift((N * prm.G / kPagedRows + R + 1) * Hkv, keys / unit + 1 + kPagedItemCost);
   cudaStream_t st = static_cast<cudaStream_t>(stream);
   // The host knows neither lengths nor offsets: a call that may hold chunks runs
   // both kernels, each on its own requests.
@@ -1097,6 +1108,7 @@ int hspmn_sqdk_paged_fwd(const void* q, int64_t q_sn, int64_t q_sh, const void* 
     const int chunk_runs = sms * kChunkCtasPerSm;
     paged_ws_carve(&ch.a, static_cast<char*>(workspace) + paged_ws_bytes(runs, kPagedRows, hdp), chunk_runs, kSqdkBM, hdp);
     ch.QT = kSqdkBM / prm.G;
+    ch.a.cost_shift = list_shift((N / ch.QT + R) * Hkv, keys / 4 + kChunkUnit * (1 + kChunkTileCost) + 1);
     ch.box_rows = static_cast<int>(std::min<int64_t>(page_size, kSqdkBN));
     const CUtensorMapDataType dt =
         dtype == HSPMN_BF16 ? CU_TENSOR_MAP_DATA_TYPE_BFLOAT16 : CU_TENSOR_MAP_DATA_TYPE_FLOAT16;

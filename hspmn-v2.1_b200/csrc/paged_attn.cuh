@@ -57,6 +57,7 @@ struct PagedAttnParams {
   int64_t N;
   int R, P, num_pages, shift, H, Hkv, G, hd;
   int has_chunks;  // the chunk kernel takes part in the call
+  int cost_shift;  // the list is counted in 2^cost_shift units, so that 32 bits hold any
   float scale_log2;
 };
 
@@ -129,48 +130,50 @@ __device__ __forceinline__ PagedRequest paged_request(const PagedAttnParams& p, 
   return q;
 }
 
-// A request's cost in the list.
+// An item's share of the list, and a request's.
+__device__ __forceinline__ int item_cost(const PagedAttnParams& p, int nb) {
+  return ((nb + kPagedItemCost - 1) >> p.cost_shift) + 1;
+}
 template <int kKeys>
-__device__ __forceinline__ int64_t paged_cost(const PagedAttnParams& p, int split, int r) {
+__device__ __forceinline__ int paged_cost(const PagedAttnParams& p, int split, int r) {
   if (r > p.R) return 0;
   const PagedRequest q = paged_request<kKeys>(p, split, paged_raw(p, r), r);
-  return static_cast<int64_t>(q.tiles) * p.Hkv * (q.nb + kPagedItemCost);
+  return q.tiles * p.Hkv * item_cost(p, q.nb);
+}
+
+__device__ __forceinline__ int warp_scan(int x, int lane) {
+#pragma unroll
+  for (int d = 1; d < 32; d <<= 1) {
+    const int y = __shfl_up_sync(0xFFFFFFFFu, x, d);
+    if (lane >= d) x += y;
+  }
+  return x;
 }
 
 // The list of items, as one warp sees it: the first 32 requests' costs stay in
-// its lanes, later ones are read again.
+// its lanes, later ones are read again. (Everything that a CTA does before its
+// first load is done with few instructions, in 32 bits: they are fetched cold,
+// and that took longer than the loads.)
 template <int kKeys>
 struct PagedList {
   const PagedAttnParams& p;
   int split, lane;
-  int64_t own, upto;  // cost of request `lane`, and with all before it
+  int own, upto;  // cost of request `lane`, and with all before it
   __device__ __forceinline__ PagedList(const PagedAttnParams& p_, int split_, int lane_)
       : p(p_), split(split_), lane(lane_) {
     own = paged_cost<kKeys>(p, split, lane);
-    upto = scan(own);
+    upto = warp_scan(own, lane);
   }
-  __device__ __forceinline__ int64_t scan(int64_t x) const {
-#pragma unroll
-    for (int d = 1; d < 32; d <<= 1) {
-      const int64_t y = __shfl_up_sync(0xFFFFFFFFu, x, d);
-      if (lane >= d) x += y;
-    }
-    return x;
-  }
-  __device__ __forceinline__ int64_t total() const {
-    int64_t n = __shfl_sync(0xFFFFFFFFu, upto, 31);
-    if (p.R < 32) return n;
-    int64_t more = 0;
-    for (int r = lane + 32; r <= p.R; r += 32) more += paged_cost<kKeys>(p, split, r);
-#pragma unroll
-    for (int d = 16; d > 0; d >>= 1) more += __shfl_xor_sync(0xFFFFFFFFu, more, d);
-    return n + more;
+  __device__ __forceinline__ int total() const {
+    int n = own;
+    for (int r = lane + 32; r <= p.R; r += 32) n += paged_cost<kKeys>(p, split, r);
+    return __reduce_add_sync(0xFFFFFFFFu, n);
   }
   // The request that holds list place w (below the total) and the cost before it.
-  __device__ __forceinline__ int locate(int64_t w, int64_t& before) const {
-    int64_t base = 0, mine = own, sum = upto;
+  __device__ __forceinline__ int locate(int w, int& before) const {
+    int base = 0, mine = own, sum = upto;
     for (int r0 = 0; r0 <= p.R; r0 += 32) {
-      if (r0 > 0) mine = paged_cost<kKeys>(p, split, r0 + lane), sum = scan(mine);
+      if (r0 > 0) mine = paged_cost<kKeys>(p, split, r0 + lane), sum = warp_scan(mine, lane);
       const unsigned past = __ballot_sync(0xFFFFFFFFu, base + sum > w);
       if (past) {
         const int l = __ffs(past) - 1;
@@ -184,24 +187,17 @@ struct PagedList {
   }
 };
 
-// a / b; 64-bit divisions are slow, and most operands here fit 32 bits.
-__device__ __forceinline__ int64_t div_wide(int64_t a, int64_t b) {
-  if (((a | b) >> 32) == 0) return static_cast<uint32_t>(a) / static_cast<uint32_t>(b);
-  return a / b;
-}
-
 // A list of `total` units cut into n runs whose lengths differ by one at most.
 struct Runs {
-  int64_t share, rem;
-  int n;
-  __device__ __forceinline__ Runs(int64_t total, int64_t runs) {
-    n = static_cast<int>(runs);
-    share = div_wide(total, runs);
+  int share, rem, n;
+  __device__ __forceinline__ Runs(int total, int runs) {
+    n = runs;
+    share = static_cast<int>(static_cast<unsigned>(total) / static_cast<unsigned>(runs));
     rem = total - share * runs;
   }
-  __device__ __forceinline__ int64_t start(int64_t c) const { return share * c + min(c, rem); }
+  __device__ __forceinline__ int start(int c) const { return share * c + min(c, rem); }
   // The run that holds unit u.
-  __device__ __forceinline__ int of(int64_t u) const {
+  __device__ __forceinline__ int of(int u) const {
     int lo = 0, hi = n;
     while (hi - lo > 1) {
       const int mid = (lo + hi) >> 1;
@@ -220,35 +216,38 @@ struct PagedCursor {
   PagedRaw ahead;
   int split, r, tile, head;
   int j, jend;  // unit, and the end of this run's units of the item
-  int64_t a, end;  // the item's place in the list, the run's end
-  __device__ __forceinline__ void cut() {
-    const int64_t left = end - a - kPagedItemCost;
-    jend = static_cast<int>(min(max(left, static_cast<int64_t>(0)), static_cast<int64_t>(req.nb)));
+  int a, end;   // the item's place in the list, the run's end
+  // The item's unit at list place w: an item's fixed cost comes before its units.
+  __device__ __forceinline__ int unit_at(const PagedAttnParams& p, int w) const {
+    return min(max((min(w - a, item_cost(p, req.nb)) << p.cost_shift) - kPagedItemCost, 0), req.nb);
   }
   // To the run [w0, w1), whose start lies in request `request` with `before` before it.
-  __device__ __forceinline__ void open(const PagedAttnParams& p, int split_, int request, int64_t before, int64_t w0, int64_t w1) {
+  __device__ __forceinline__ void open(const PagedAttnParams& p, int split_, int request, int before, int w0, int w1) {
     split = split_;
     r = request;
     req = paged_request<kKeys>(p, split, paged_raw(p, r), r);
     ahead = paged_raw(p, r + 1);
-    const int64_t local = w0 - before, cost = req.nb + kPagedItemCost;
-    const int64_t item = div_wide(local, cost);
-    j = static_cast<int>(max(local - item * cost - kPagedItemCost, static_cast<int64_t>(0)));
-    tile = static_cast<int>(div_wide(item, p.Hkv));
-    head = static_cast<int>(item - static_cast<int64_t>(tile) * p.Hkv);
-    a = before + item * cost;
+    const unsigned cost = item_cost(p, req.nb), item = static_cast<unsigned>(w0 - before) / cost;
+    tile = static_cast<int>(item / static_cast<unsigned>(p.Hkv));
+    head = static_cast<int>(item) - tile * p.Hkv;
+    a = before + static_cast<int>(item * cost);
     end = w1;
-    cut();
+    j = unit_at(p, w0);
+    jend = unit_at(p, w1);
   }
   __device__ __forceinline__ bool valid() const { return j < jend; }
+  // Whether the run ends in front of the first unit of the item behind this one.
+  __device__ __forceinline__ bool last_item(const PagedAttnParams& p) const {
+    return end - a - item_cost(p, req.nb) <= kPagedItemCost >> p.cost_shift;
+  }
   // To the run's next unit, if there is one (valid() tells).
   __device__ __forceinline__ void next(const PagedAttnParams& p) {
     if (++j < jend) return;
-    a += req.nb + kPagedItemCost;
-    if (a + kPagedItemCost >= end) {  // the run ends in front of the next item's first unit
+    if (last_item(p)) {
       jend = 0;
       return;
     }
+    a += item_cost(p, req.nb);
     j = 0;
     if (++head == p.Hkv) {
       head = 0;
@@ -260,7 +259,7 @@ struct PagedCursor {
         } while (req.tiles == 0 && r < p.R);
       }
     }
-    cut();
+    jend = unit_at(p, end);
   }
 };
 
@@ -365,13 +364,13 @@ __global__ void __launch_bounds__(kPagedThreads, kPagedCtasPerSm) paged_attn_ker
   grid_dependents_launch();
   const int split = paged_split<L::kKeys>(p, lane);
   const PagedList<L::kKeys> list(p, split, lane);
-  const int64_t total = list.total();
-  const int64_t runs = min(static_cast<int64_t>(gridDim.x), total);
+  const int total = list.total();
+  const int runs = min(static_cast<int>(gridDim.x), total);
   PagedCursor<L::kKeys> cur, ahead;
-  const Runs run(total, max(runs, static_cast<int64_t>(1)));
-  if (blockIdx.x < runs) {
-    const int64_t w0 = run.start(blockIdx.x), w1 = run.start(blockIdx.x + 1);
-    int64_t before;
+  const Runs run(total, max(runs, 1));
+  if (static_cast<int>(blockIdx.x) < runs) {
+    const int w0 = run.start(blockIdx.x), w1 = run.start(blockIdx.x + 1);
+    int before;
     const int r0 = list.locate(w0, before);
     cur.open(p, split, r0, before, w0, w1);
   } else {
@@ -657,13 +656,13 @@ __global__ void __launch_bounds__(kPagedThreads, kPagedCtasPerSm) paged_attn_ker
       const bool item_end = cur.jend == cur.req.nb, whole = item_end && seg_j == 0;
       // the last item of this run: if it goes on behind it, its runs from the one
       // in which it opens to this one share its merge
-      if (threadIdx.x == 0 && (!item_end || cur.a + cur.req.nb + 2 * kPagedItemCost >= cur.end)) {
-        const int64_t first = cur.a + kPagedItemCost;
+      if (threadIdx.x == 0 && (!item_end || cur.last_item(p))) {
+        const int first = run.of(cur.a + (kPagedItemCost >> p.cost_shift));
+        const int last = run.of(cur.a + ((kPagedItemCost + cur.req.nb - 1) >> p.cost_shift));
         p.merges[blockIdx.x] =
             make_int4(cur.req.q0, cur.tile * kPagedRows,
                       cur.head * kPagedRows + min(kPagedRows, cur.req.rows - cur.tile * kPagedRows) - 1,
-                      item_end ? -1 : (seg_j == 0 ? static_cast<int>(blockIdx.x) : run.of(first)) << 16 |
-                                          run.of(first + cur.req.nb - 1));
+                      item_end ? -1 : first << 16 | last);
       }
       __syncthreads();
       // a run holds the last piece of one item at most, and the first of one

@@ -73,7 +73,10 @@ struct ChunkJob {
 // A request's tiles. Costs are linear in the tile number: first + t * slope.
 struct ChunkRequest {
   int q0, len, kv, tiles;
-  int64_t first, slope, head;  // head: the sum over a head's tiles
+  int first, slope, head;  // head: the sum over a head's tiles
+  __device__ __forceinline__ int before(int n) const {
+    return first * n + static_cast<int>(static_cast<int64_t>(n) * (n - 1) / 2 * slope);
+  }
 };
 
 __device__ __forceinline__ ChunkRequest chunk_request(const ChunkParams& p, int split, int r) {
@@ -86,24 +89,22 @@ __device__ __forceinline__ ChunkRequest chunk_request(const ChunkParams& p, int 
   c.first = c.slope = c.head = 0;
   if (q.rows <= split) return c;  // the 16-row kernel's
   c.tiles = (c.len + p.QT - 1) / p.QT;
-  const int64_t top = static_cast<int64_t>(c.kv) - 1;
-  const int64_t lo = min(max(__ldg(p.a.pos + c.q0 + min(p.QT, c.len) - 1), static_cast<int64_t>(0)), max(top, static_cast<int64_t>(0)));
-  const int64_t hi = min(max(__ldg(p.a.pos + c.q0 + c.len - 1), static_cast<int64_t>(0)), max(top, static_cast<int64_t>(0)));
+  const int64_t top = max(c.kv - 1, 0);
+  const int lo = static_cast<int>(min(max(__ldg(p.a.pos + c.q0 + min(p.QT, c.len) - 1), static_cast<int64_t>(0)), top));
+  const int hi = static_cast<int>(min(max(__ldg(p.a.pos + c.q0 + c.len - 1), static_cast<int64_t>(0)), top));
   constexpr int kShift = 2;  // 64 keys = kChunkUnit units
   static_assert(kSqdkBN >> kShift == kChunkUnit, "cost units");
-  c.first = (lo >> kShift) + kChunkUnit * (1 + kChunkTileCost);
-  c.slope = c.tiles > 1 ? div_wide(max((hi - lo) >> kShift, static_cast<int64_t>(0)), c.tiles - 1) : 0;
-  c.head = c.first * c.tiles + c.slope * (static_cast<int64_t>(c.tiles) * (c.tiles - 1) / 2);
+  const int sh = kShift + p.a.cost_shift;
+  c.first = (lo >> sh) + ((kChunkUnit * (1 + kChunkTileCost)) >> p.a.cost_shift) + 1;
+  c.slope = c.tiles > 1 ? static_cast<int>(static_cast<unsigned>(max(hi - lo, 0) >> sh) / static_cast<unsigned>(c.tiles - 1)) : 0;
+  c.head = c.before(c.tiles);
   return c;
 }
 
 struct ChunkTile {
   ChunkRequest req;
   int split, r, head, t;
-  int64_t start, cost;  // place in the list
-  __device__ __forceinline__ int64_t before(int n) const {
-    return req.first * n + req.slope * (static_cast<int64_t>(n) * (n - 1) / 2);
-  }
+  int start, cost;  // place in the list
   // Only called while a next tile exists.
   __device__ __forceinline__ void next(const ChunkParams& p) {
     start += cost;
@@ -124,35 +125,25 @@ struct ChunkTile {
 struct ChunkList {
   const ChunkParams& p;
   int split, lane;
-  int64_t mine, upto;  // cost of request `lane`, and with all before it
+  int mine, upto;  // cost of request `lane`, and with all before it
   __device__ __forceinline__ ChunkList(const ChunkParams& p_, int split_, int lane_)
       : p(p_), split(split_), lane(lane_) {
     mine = cost(lane);
-    upto = scan(mine);
+    upto = warp_scan(mine, lane);
   }
-  __device__ __forceinline__ int64_t cost(int r) const { return r < p.a.R ? chunk_request(p, split, r).head * p.a.Hkv : 0; }
-  __device__ __forceinline__ int64_t scan(int64_t x) const {
-#pragma unroll
-    for (int d = 1; d < 32; d <<= 1) {
-      const int64_t y = __shfl_up_sync(0xFFFFFFFFu, x, d);
-      if (lane >= d) x += y;
-    }
-    return x;
-  }
-  __device__ __forceinline__ int64_t total() const {
-    int64_t n = mine;
+  __device__ __forceinline__ int cost(int r) const { return r < p.a.R ? chunk_request(p, split, r).head * p.a.Hkv : 0; }
+  __device__ __forceinline__ int total() const {
+    int n = mine;
     for (int r = lane + 32; r < p.a.R; r += 32) n += cost(r);
-#pragma unroll
-    for (int d = 16; d > 0; d >>= 1) n += __shfl_xor_sync(0xFFFFFFFFu, n, d);
-    return n;
+    return __reduce_add_sync(0xFFFFFFFFu, n);
   }
   // The tile that holds list place w (below the total).
-  __device__ __forceinline__ ChunkTile locate(int64_t w) const {
+  __device__ __forceinline__ ChunkTile locate(int w) const {
     ChunkTile c;
-    int64_t base = 0, own = mine, sum = upto;
+    int base = 0, own = mine, sum = upto;
     c.r = p.a.R - 1;
     for (int r0 = 0; r0 < p.a.R; r0 += 32) {
-      if (r0 > 0) own = cost(r0 + lane), sum = scan(own);
+      if (r0 > 0) own = cost(r0 + lane), sum = warp_scan(own, lane);
       const unsigned past = __ballot_sync(0xFFFFFFFFu, base + sum > w);
       if (past) {
         const int l = __ffs(past) - 1;
@@ -164,18 +155,18 @@ struct ChunkList {
     }
     c.split = split;
     c.req = chunk_request(p, split, c.r);
-    const int64_t rel = w - base;
-    c.head = static_cast<int>(div_wide(rel, c.req.head));
-    const int64_t in_head = rel - c.head * c.req.head;
+    const unsigned rel = w - base;
+    c.head = static_cast<int>(rel / static_cast<unsigned>(c.req.head));
+    const int in_head = static_cast<int>(rel) - c.head * c.req.head;
     // the last tile t with first t + slope t (t - 1) / 2 <= in_head: the root
     // in float, set right in integers
     const float b = static_cast<float>(c.req.first) - 0.5f * static_cast<float>(c.req.slope);
     const float x = static_cast<float>(in_head), root = sqrtf(b * b + 2.0f * static_cast<float>(c.req.slope) * x);
-    int t = min(max(static_cast<int>(2.0f * x / (b + root)), 0), c.req.tiles - 1);
-    while (t > 0 && c.before(t) > in_head) --t;
-    while (t + 1 < c.req.tiles && c.before(t + 1) <= in_head) ++t;
+    int t = min(max(static_cast<int>(__fdividef(2.0f * x, b + root)), 0), c.req.tiles - 1);
+    while (t > 0 && c.req.before(t) > in_head) --t;
+    while (t + 1 < c.req.tiles && c.req.before(t + 1) <= in_head) ++t;
     c.t = t;
-    c.start = base + c.head * c.req.head + c.before(t);
+    c.start = base + c.head * c.req.head + c.req.before(t);
     c.cost = c.req.first + c.req.slope * t;
     return c;
   }
@@ -185,21 +176,13 @@ struct ChunkList {
 // would not be worth its merge is moved to that end.
 struct ChunkCuts {
   Runs run;
-  int64_t total, near;
-  __device__ __forceinline__ ChunkCuts(int64_t total_, int64_t most)
-      : run(total_, min(most, max(total_ / (kChunkUnit * kChunkMinPiece), static_cast<int64_t>(1)))),
+  int total, near;
+  __device__ __forceinline__ ChunkCuts(const ChunkParams& p, int total_, int most)
+      : run(total_, min(most, max(total_ / max((kChunkUnit * kChunkMinPiece) >> p.a.cost_shift, 1), 1))),
         total(total_),
-        near(min(run.share >> 4, static_cast<int64_t>(8 * kChunkUnit))) {}
-  __device__ __forceinline__ int64_t at(const ChunkList& list, int64_t c) const {
-    if (c >= run.n) return total;
-    const int64_t w = run.start(c);
-    const ChunkTile tile = list.locate(w);
-    if (w - tile.start <= near) return tile.start;
-    if (tile.start + tile.cost - w <= near) return tile.start + tile.cost;
-    return w;
-  }
+        near(min(run.share >> 4, (8 * kChunkUnit) >> p.a.cost_shift)) {}
   // The first run that begins behind list place w (the start of a tile that a cut divides).
-  __device__ __forceinline__ int first_inside(int64_t w) const {
+  __device__ __forceinline__ int first_inside(int w) const {
     int c = run.of(w) + 1;
     while (run.start(c) - w <= near) ++c;
     return c;
@@ -210,17 +193,28 @@ struct ChunkCuts {
 // start, then the one at its end.
 struct ChunkWalk {
   ChunkTile first, cur;
-  int64_t w0, w1;
+  int w0, w1;
   int stage;  // 0: whole tiles, 1: piece at the start, 2: piece at the end, 3: done
   bool started;
-  __device__ __forceinline__ void open(const ChunkList& list, const ChunkCuts& cuts, int64_t c) {
+  __device__ __forceinline__ void open(const ChunkList& list, const ChunkCuts& cuts, int c) {
     stage = 3;
     started = false;
+    w0 = w1 = 0;
     if (c >= cuts.run.n || cuts.total == 0) return;
-    w0 = cuts.at(list, c);
-    w1 = cuts.at(list, c + 1);
+    // the two ends, the start last: its tile is where the walk begins
+    w1 = cuts.total;
+#pragma unroll 1
+    for (int k = c + 1 < cuts.run.n ? 1 : 0; k >= 0; --k) {
+      w0 = cuts.run.start(c + k);
+      cur = list.locate(w0);
+      const int behind = cur.start + cur.cost;
+      if (w0 - cur.start <= cuts.near) w0 = cur.start;
+      else if (behind - w0 <= cuts.near) w0 = behind;
+      if (k == 1) w1 = w0;
+    }
     if (w0 >= w1) return;
-    first = cur = list.locate(w0);
+    if (w0 == cur.start + cur.cost) cur.next(list.p);
+    first = cur;
     stage = 0;
   }
   // The next piece's tile; slot and merge say what it is.
@@ -266,13 +260,15 @@ struct ChunkWalk {
 };
 
 // Key block at list place w of a tile with nblk blocks.
-__device__ __forceinline__ int chunk_block_at(const ChunkTile& c, int64_t w, int nblk) {
-  const int64_t x = min(max(w - c.start, static_cast<int64_t>(0)), c.cost);
-  return static_cast<int>(div_wide(x * nblk, c.cost));
+__device__ __forceinline__ int chunk_block_at(const ChunkTile& c, int w, int nblk) {
+  const int64_t x = static_cast<int64_t>(min(max(w - c.start, 0), c.cost)) * nblk;
+  // (64-bit divisions are slow, and most lists are short)
+  if ((x >> 32) == 0) return static_cast<int>(static_cast<unsigned>(x) / static_cast<unsigned>(c.cost));
+  return static_cast<int>(x / c.cost);
 }
 
 // Fills in a job for list places [a, b) of a tile (the whole warp).
-__device__ __forceinline__ void chunk_job(const ChunkParams& p, const ChunkTile& c, int64_t a, int64_t b, int slot,
+__device__ __forceinline__ void chunk_job(const ChunkParams& p, const ChunkTile& c, int a, int b, int slot,
                                           volatile ChunkJob& job, int lane) {
   int lo = 0x7FFFFFFF, hi = -1;
   const int n = min(p.QT, c.req.len - c.t * p.QT);
@@ -383,7 +379,7 @@ __global__ void __launch_bounds__(kChunkThreads, kChunkCtasPerSm)
     // ------------------------------------------------------------ producer
     const int boxes = kSqdkBN / p.box_rows;
     const ChunkList list(p, split, lane);
-    const ChunkCuts cuts(list.total(), gridDim.x);
+    const ChunkCuts cuts(p, list.total(), static_cast<int>(gridDim.x));
     ChunkWalk walk;
     walk.open(list, cuts, blockIdx.x);
     uint32_t nk = 0, nv = 0, segs = 0, posted = 0;
@@ -408,7 +404,7 @@ __global__ void __launch_bounds__(kChunkThreads, kChunkCtasPerSm)
       if (slot >= 0 && tile.start + tile.cost > walk.w1) {
         // the tile goes on behind this run: its runs from the one in which it
         // begins to the last that begins inside it share its merge
-        const int64_t end = tile.start + tile.cost;
+        const int end = tile.start + tile.cost;
         const int first = slot & 1 ? static_cast<int>(blockIdx.x) : cuts.first_inside(tile.start) - 1;
         int last = cuts.run.of(end - 1);
         if (end - cuts.run.start(last) <= cuts.near) --last;
@@ -887,7 +883,7 @@ __device__ __forceinline__ void chunk_merge(const ChunkParams& p, int run, int s
 // Both kernels' merges in one launch: blocks [0, paged_runs) those of the 16-row
 // kernel, then kChunkMergeBlocks a run of the chunks'.
 template <int HD, bool kBF16>
-__global__ void __launch_bounds__(32 * kMergeWarps)
+__global__ void __launch_bounds__(32 * kMergeWarps, 2)
     paged_both_merge_kernel(const __grid_constant__ PagedAttnParams p, const __grid_constant__ ChunkParams c, int paged_runs) {
   grid_dependency_wait();
   const int block = static_cast<int>(blockIdx.x) - paged_runs;
