@@ -83,6 +83,10 @@ __device__ __forceinline__ PagedRaw paged_raw(const PagedAttnParams& p, int r) {
   return x;
 }
 
+// Whether offsets do not begin at 0, descend or end behind q. Requests would
+// share rows and the lists outgrow their bounds: such a call computes nothing.
+__device__ __forceinline__ bool paged_offsets_bad(const PagedRaw& x, int r) { return x.a > x.b || (r == 0 && x.a != 0); }
+
 // The request's rows and keys (its tiles not counted).
 __device__ __forceinline__ PagedRequest paged_rows(const PagedAttnParams& p, const PagedRaw& x) {
   PagedRequest q;
@@ -135,9 +139,11 @@ __device__ __forceinline__ int item_cost(const PagedAttnParams& p, int nb) {
   return ((nb + kPagedItemCost - 1) >> p.cost_shift) + 1;
 }
 template <int kKeys>
-__device__ __forceinline__ int paged_cost(const PagedAttnParams& p, int split, int r) {
+__device__ __forceinline__ int paged_cost(const PagedAttnParams& p, int split, int r, bool& bad) {
   if (r > p.R) return 0;
-  const PagedRequest q = paged_request<kKeys>(p, split, paged_raw(p, r), r);
+  const PagedRaw x = paged_raw(p, r);
+  bad |= paged_offsets_bad(x, r);
+  const PagedRequest q = paged_request<kKeys>(p, split, x, r);
   return q.tiles * p.Hkv * item_cost(p, q.nb);
 }
 
@@ -159,21 +165,26 @@ struct PagedList {
   const PagedAttnParams& p;
   int split, lane;
   int own, upto;  // cost of request `lane`, and with all before it
+  bool bad = false;
   __device__ __forceinline__ PagedList(const PagedAttnParams& p_, int split_, int lane_)
       : p(p_), split(split_), lane(lane_) {
-    own = paged_cost<kKeys>(p, split, lane);
+    own = paged_cost<kKeys>(p, split, lane, bad);
     upto = warp_scan(own, lane);
   }
-  __device__ __forceinline__ int total() const {
-    int n = own;
-    for (int r = lane + 32; r <= p.R; r += 32) n += paged_cost<kKeys>(p, split, r);
-    return __reduce_add_sync(0xFFFFFFFFu, n);
+  // Its length; 0, and a device error, where the offsets are bad.
+  __device__ __forceinline__ int total() {
+    unsigned n = own;
+    for (int r = lane + 32; r <= p.R; r += 32) n += paged_cost<kKeys>(p, split, r, bad);
+    n = __reduce_add_sync(0xFFFFFFFFu, n);
+    if (!__any_sync(0xFFFFFFFFu, bad)) return static_cast<int>(n);
+    if (blockIdx.x == 0 && threadIdx.x == 0) raise_device_error(HSPMN_DEVERR_POSITION);
+    return 0;
   }
   // The request that holds list place w (below the total) and the cost before it.
-  __device__ __forceinline__ int locate(int w, int& before) const {
+  __device__ __forceinline__ int locate(int w, int& before) {
     int base = 0, mine = own, sum = upto;
     for (int r0 = 0; r0 <= p.R; r0 += 32) {
-      if (r0 > 0) mine = paged_cost<kKeys>(p, split, r0 + lane), sum = warp_scan(mine, lane);
+      if (r0 > 0) mine = paged_cost<kKeys>(p, split, r0 + lane, bad), sum = warp_scan(mine, lane);
       const unsigned past = __ballot_sync(0xFFFFFFFFu, base + sum > w);
       if (past) {
         const int l = __ffs(past) - 1;
@@ -363,7 +374,7 @@ __global__ void __launch_bounds__(kPagedThreads, kPagedCtasPerSm) paged_attn_ker
   const int g = lane >> 2, t2 = (lane & 3) * 2;  // accumulator row and first column of this lane
   grid_dependents_launch();
   const int split = paged_split<L::kKeys>(p, lane);
-  const PagedList<L::kKeys> list(p, split, lane);
+  PagedList<L::kKeys> list(p, split, lane);
   const int total = list.total();
   const int runs = min(static_cast<int>(gridDim.x), total);
   PagedCursor<L::kKeys> cur, ahead;

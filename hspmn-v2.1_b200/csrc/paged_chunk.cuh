@@ -336,11 +336,16 @@ __global__ void __launch_bounds__(kChunkThreads, kChunkCtasPerSm)
   const uint32_t sbase = (smem_u32(chunk_smem_raw) + 1023u) & ~1023u;
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   grid_dependents_launch();
-  // no request for this kernel: nothing to set up
+  // no request for this kernel, or bad offsets (the 16-row kernel says so):
+  // nothing to set up
   const int split = paged_split<PagedLayout<HD>::kKeys>(p.a, lane);
-  bool any = false;
-  for (int r = lane; r < p.a.R; r += 32) any |= paged_rows(p.a, paged_raw(p.a, r)).rows > split;
-  if (!__any_sync(0xFFFFFFFFu, any)) {
+  bool any = false, bad = false;
+  for (int r = lane; r <= p.a.R; r += 32) {
+    const PagedRaw x = paged_raw(p.a, r);
+    bad |= paged_offsets_bad(x, r);
+    any |= r < p.a.R && paged_rows(p.a, x).rows > split;
+  }
+  if (!__any_sync(0xFFFFFFFFu, any) || __any_sync(0xFFFFFFFFu, bad)) {
     if (threadIdx.x == 0) p.a.merges[blockIdx.x] = make_int4(0, 0, 0, -1);
     return;
   }

@@ -712,9 +712,10 @@ def sqdk_paged_fwd(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tensor
     hd] with H % Hkv == 0, read in place through ``block_table`` (int32 [R,P]).
     bf16 or f16. ``max_q``: the most rows any request has, 0 if unknown; it only
     helps to choose kernels. Returns [N,H,hd]; rows that see nothing and rows
-    behind ``cu_q[R]`` are zeros. A position beyond kv_lens sets
-    ``DEVERR_POSITION``, a page outside the cache ``DEVERR_PAGE`` (its keys are
-    left out) in ``device_errors()``. No backward."""
+    behind ``cu_q[R]`` are zeros. In ``device_errors()``, a position beyond
+    kv_lens (or beyond what P pages hold) sets ``DEVERR_POSITION``, as do offsets
+    that do not ascend from 0 to N at most (nothing is computed then), and a page
+    outside the cache ``DEVERR_PAGE`` (its keys are left out). No backward."""
     return _call_paged("sqdk_paged_fwd", q, k_cache, v_cache, block_table, kv_lens, cu_q,
                        positions, sm_scale, max_q)
 

@@ -371,7 +371,10 @@ HSPMN_API int64_t hspmn_sqdk_paged_workspace_size(int64_t N, int64_t H, int64_t 
  * A decode step (one query a request), a chunk of new tokens and the rows that
  * a router selected of one are all calls of this function; requests may differ.
  * Rows that see no key (position or kv_lens below 1 key) and rows i >= cu_q[R]
- * are written as zeros. A position >= kv_lens[r] sees all kv_lens[r] keys and
+ * are written as zeros. cu_q[0] is 0, and the offsets ascend (equal ones: no
+ * query) to N at most; where they do not, o is not written and
+ * HSPMN_DEVERR_POSITION is set. Of kv_lens[r], what P pages hold counts. A
+ * position >= that sees all the request's keys and
  * sets HSPMN_DEVERR_POSITION; keys whose page is outside the cache are left
  * out and set HSPMN_DEVERR_PAGE. Whatever the cache holds behind kv_lens[r],
  * NaN included, does not reach the result, nor does a key's value reach rows

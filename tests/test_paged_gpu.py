@@ -388,6 +388,21 @@ def test_long_context():
     assert ops.device_errors() == 0
 
 
+@pytest.mark.parametrize("R", [3, 70])
+@pytest.mark.parametrize("H", [2, 32])  # 40 and 640 query rows a request and K/V head
+def test_offsets_that_do_not_ascend_are_flagged(R, H):
+    args = batch([64] * R, [range(24, 64)] * R, H, 2, 64, torch.bfloat16, 16, seed=18)
+    q, kc, vc, table, kv, cu, pos = args
+    want = attend(*args)
+    assert ops.device_errors() == 0
+    for bad in ([1] + cu[1:], cu[:-1] + [len(q) + 1], cu[:2] + [cu[1] - 1] + cu[3:], [-1] + cu[1:],
+                cu[:2] + [2 ** 31 - 1] + cu[3:], [len(q) * (i % 2) for i in range(R + 1)]):
+        for max_q in (0, 1):
+            attend(q, kc, vc, table, kv, bad, pos, max_q=max_q)
+            assert ops.device_errors() == N.DEVERR_POSITION, bad
+    assert torch.equal(attend(*args), want) and ops.device_errors() == 0
+
+
 def test_lengths_beyond_the_table_are_cut():
     q, kc, vc, table, kv, cu, pos = batch([64], [[63]], 4, 2, 64, torch.bfloat16, 16, seed=17)
     want = attend(q, kc, vc, table, [64], cu, pos)
