@@ -1044,7 +1044,8 @@ int hspmn_sqdk_paged_fwd(const void* q, int64_t q_sn, int64_t q_sh, const void* 
   const int shift = page_shift(page_size);
   if (shift < 0 || hd < 8 || hd > 128 || hd % 8 != 0) return HSPMN_ERR_UNSUPPORTED;
   if (H % Hkv != 0 || H / Hkv > kSqdkBM) return HSPMN_ERR_UNSUPPORTED;
-  if (N > 0x7FFFFFFF / H || R > 0x07FFFFFF / Hkv || P > (0x7FFFFFFF >> shift) || num_pages > 0x7FFFFFFF)
+  // (key positions rounded up to a block stay below 2^31)
+  if (N > 0x7FFFFFFF / H || R > 0x07FFFFFF / Hkv || P > (0x7FFFF000 >> shift) || num_pages > 0x7FFFFFFF)
     return HSPMN_ERR_INVALID;
   const int64_t es = 2;
   // the stride of a dimension of one element is never used: any is accepted
@@ -1053,8 +1054,8 @@ int hspmn_sqdk_paged_fwd(const void* q, int64_t q_sn, int64_t q_sh, const void* 
   if (Hkv == 1) kc_sh = vc_sh = hd;
   if (num_pages == 1) kc_sp = vc_sp = page_size * Hkv * hd;
   if (int rc = check_strides({q_sn, q_sh, kc_sp, kc_ss, kc_sh, vc_sp, vc_ss, vc_sh, o_sn, o_sh}, es)) return rc;
-  // the kernels step through pages and slots with 32-bit strides
-  if (kc_sp >= (1LL << 30) || kc_ss >= (1LL << 30) || vc_sp >= (1LL << 30) || vc_ss >= (1LL << 30))
+  // the kernels step through pages and slots (up to four of these at a time) with 32-bit strides
+  if (kc_sp >= (1LL << 30) || kc_ss >= (1LL << 28) || vc_sp >= (1LL << 30) || vc_ss >= (1LL << 28))
     return HSPMN_ERR_UNSUPPORTED;
   if (!aligned(q, 16) || !aligned(k_cache, 16) || !aligned(v_cache, 16) || !aligned(o, 16) || !aligned(workspace, 16))
     return HSPMN_ERR_ALIGN;

@@ -373,17 +373,18 @@ HSPMN_API int64_t hspmn_sqdk_paged_workspace_size(int64_t N, int64_t H, int64_t 
  * Rows that see no key (position or kv_lens below 1 key) and rows i >= cu_q[R]
  * are written as zeros. cu_q[0] is 0, and the offsets ascend (equal ones: no
  * query) to N at most; where they do not, o is not written and
- * HSPMN_DEVERR_POSITION is set. Of kv_lens[r], what P pages hold counts. A
- * position >= that sees all the request's keys and
- * sets HSPMN_DEVERR_POSITION; keys whose page is outside the cache are left
- * out and set HSPMN_DEVERR_PAGE. Whatever the cache holds behind kv_lens[r],
+ * HSPMN_DEVERR_POSITION is set. Of kv_lens[r], what P pages hold counts; a
+ * position beyond it sees all the request's keys and sets
+ * HSPMN_DEVERR_POSITION. Keys whose page is outside the cache are left out and
+ * set HSPMN_DEVERR_PAGE. Whatever the cache holds behind kv_lens[r],
  * NaN included, does not reach the result, nor does a key's value reach rows
  * that do not see the key.
  * q, o: [N,H,hd], strides (elements) of row and head; caches as above, strides
  * of page, offset and head. dtype HSPMN_BF16 or HSPMN_F16. hd: a multiple of 8
  * up to 128; H % Hkv == 0, H / Hkv <= 128; strides of page and offset below
- * 2^30 elements. block_table, kv_lens, cu_q int32;
- * positions int64, in any order. Bases and strides multiples of 16 bytes.
+ * 2^30 and 2^28 elements; R * Hkv < 2^27, P * page_size <= 2^31 - 4096.
+ * block_table, kv_lens, cu_q int32; positions int64, in any order. Bases and
+ * strides multiples of 16 bytes.
  * max_q: the largest number of query rows of one request if the caller knows
  * it, else 0; it only chooses kernels, any value is correct.
  * workspace: hspmn_sqdk_paged_workspace_size() bytes (16-byte aligned);

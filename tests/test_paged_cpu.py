@@ -57,11 +57,13 @@ def test_attention_refusals():
 
     for over in (dict(q=None), dict(o=None), dict(kc=None), dict(vc=None), dict(table=None), dict(kv=None), dict(cu=None),
                  dict(pos=None), dict(n=-1), dict(R=-1), dict(rs=7), dict(scale=0.0), dict(scale=float("nan")),
-                 dict(max_q=-1), dict(sn=-2048), dict(n=1 << 28), dict(Pw=1 << 28, rs=1 << 28)):
+                 dict(max_q=-1), dict(sn=-2048), dict(n=1 << 28), dict(Pw=1 << 28, rs=1 << 28),
+                 dict(Pw=(1 << 27) - 255, rs=1 << 28), dict(R=1 << 25)):
         assert fwd(**over) == INVALID, over
     for over in (dict(dt=0), dict(dt=7)):
         assert fwd(**over) == DTYPE, over
-    for over in (dict(hd=12), dict(hd=136), dict(H=14), dict(H=516), dict(page=48), dict(sp=1 << 30)):
+    for over in (dict(hd=12), dict(hd=136), dict(H=14), dict(H=516), dict(page=48), dict(sp=1 << 30),
+                 dict(ss=1 << 28)):
         assert fwd(**over) == UNSUPPORTED, over
     odd = ctypes.c_void_p(4104)
     for over in (dict(q=odd), dict(o=odd), dict(kc=odd), dict(vc=odd), dict(ws=odd), dict(sn=2052), dict(ss=516)):
