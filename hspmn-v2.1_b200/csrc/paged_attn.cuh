@@ -5,9 +5,9 @@
 //   m over the positions of the query's request with m <= pos[i], m < kv_len
 //   and a page in the table
 //
-// Work unit: 64 keys (128 for head_dim <= 64) of one (request, K/V head, 16 query rows) item; the rows
-// of a request and K/V head are numbered query * G + head, so a single token's
-// G heads share the keys that are read. All units of a call form one list
+// Work unit: 64 keys (128 for head_dim <= 64) of one (request, K/V head, 16 query
+// rows) item; the rows of a request and K/V head are numbered query * G + head,
+// so a single token's G heads share the keys that are read. All units of a call form one list
 // (requests, then row tiles, then heads, then keys) which is cut into as many
 // equal contiguous runs as there are CTAs: ragged lengths cost no idle CTA and
 // need no plan from the host, which knows neither lengths nor offsets. An item
@@ -17,9 +17,16 @@
 //
 // Bound: reading K and V once (4 query heads a key: 4 flops a byte). Each of a
 // CTA's four warps owns 16 (32) keys of every unit and runs on its own: its K and
-// V rows come by cp.async into a private ring (kStages deep), Q K^T and P V are
+// V rows come by cp.async into a private ring (kPagedStages deep), Q K^T and P V are
 // m16n8k16 products with the softmax between them in registers, and the warps
-// meet only at the end of an item. Sums, maxima and O are fp32.
+// meet only at the end of an item. Sums, maxima and O are fp32. The products fill
+// a fifth of the tensor pipe, so 128-row tiles would not be faster; three stages
+// of two CTAs an SM keep 192 KB an SM on the way (three CTAs with two stages: 178
+// -> 221 us). 64 tokens over 1.15 GB of K and V (contexts to 32768, 16/4 heads of
+// 128) take 176 us, 6.5 TB/s; one token over 262144 keys 91 us (5.9 TB/s: the
+// start and the merge of 74 runs an item take 9 us); 37 tokens of 16 heads of 64
+// over up to 8192 keys 62 us (5.0 TB/s: 592 short items). One token over 500 keys
+// takes 7.8 us, two launches and a round of loads.
 #pragma once
 
 #include "sqdk.cuh"
@@ -30,7 +37,9 @@ constexpr int kPagedRows = 16;     // query rows of an item
 constexpr int kPagedWarps = 4;     // a quarter of a unit's keys each
 constexpr int kPagedThreads = 32 * kPagedWarps;
 constexpr int kPagedStages = 3;
-constexpr int kPagedItemCost = 2;  // what opening and closing an item takes, in units (68.0 us against 86.3 at 0, 68.7 at 1, 69.6 at 3: 37 x 16 items of 1 to 64 units)
+// What opening and closing an item takes, in units (68.0 us against 86.3 at 0,
+// 68.7 at 1, 69.6 at 3: 37 x 16 items of 1 to 64 units).
+constexpr int kPagedItemCost = 2;
 constexpr int kPagedCtasPerSm = 2;
 constexpr int kPagedMidRows = 128;      // see paged_split
 constexpr int kPagedMidScore = 14200;
