@@ -388,6 +388,18 @@ def test_long_context():
     assert ops.device_errors() == 0
 
 
+@pytest.mark.parametrize("width", [1000, 30000, 524287])  # work lists in units of one and of several blocks
+def test_wide_tables(width):
+    lens = [1, 70, 5000, 9000, 0, 300, 4097, 20000, 64, 640, 33, 1000]
+    positions = [[0], [69], [4999], range(8700, 9000), [], range(40), [5, 4096], range(19960, 20000, 3), [63],
+                 range(64, 640, 2), [32], [999]]
+    args = batch(lens, [list(p) for p in positions], 16, 4, 128, torch.bfloat16, 4096, seed=19)
+    table = torch.full((len(lens), width), -1, dtype=torch.int32, device=DEV)
+    table[:, :args[3].shape[1]] = args[3]
+    check((*args[:3], table, *args[4:]), max_qs=(0, 300))
+    assert ops.device_errors() == 0
+
+
 @pytest.mark.parametrize("R", [3, 70])
 @pytest.mark.parametrize("H", [2, 32])  # 40 and 640 query rows a request and K/V head
 def test_offsets_that_do_not_ascend_are_flagged(R, H):
