@@ -61,6 +61,15 @@ Tensor empty_on(c10::Device dev, at::IntArrayRef sizes, at::ScalarType dtype) {
   return at::detail::empty_cuda(sizes, dtype, dev, std::nullopt);
 }
 
+// n elements of `whole`'s memory from element `at` on, as a tensor of its own
+// (0.4 us less than an allocation).
+Tensor part_of(const Tensor& whole, int64_t at, int64_t n) {
+  Tensor t = at::detail::make_tensor<c10::TensorImpl>(c10::Storage(whole.storage()), whole.key_set(), whole.dtype());
+  t.unsafeGetTensorImpl()->set_sizes_contiguous({n});
+  t.unsafeGetTensorImpl()->set_storage_offset(at);
+  return t;
+}
+
 // A 1-D int32 / int64 argument of n elements, contiguous.
 Tensor vector_arg(const char* name, const char* what, const Tensor& t, at::ScalarType dtype, int64_t n) {
   TORCH_CHECK_VALUE(t.scalar_type() == dtype && t.dim() == 1 && (n < 0 || t.size(0) == n), name, ": ", what, " must be ",
@@ -86,6 +95,9 @@ void check_caches(const char* name, const Tensor& k, const Tensor& v, at::Scalar
                     ": the caches' last dimension must be contiguous (they are used in place)");
 }
 
+// kShare: the outputs of the requests, and those of the tokens, lie in one
+// allocation each (operators that are traced must give tensors that share nothing).
+template <bool kShare>
 std::tuple<Tensor, Tensor, Tensor, Tensor, Tensor> paged_slots_(const Tensor& block_table, const Tensor& seq_lens_,
                                                                 const Tensor& new_lens_, const Tensor& free_pages_,
                                                                 int64_t page_size, int64_t num_tokens) {
@@ -101,8 +113,16 @@ std::tuple<Tensor, Tensor, Tensor, Tensor, Tensor> paged_slots_(const Tensor& bl
                     ": block_table is written in place: its rows must be dense and must not overlap");
   TORCH_CHECK_VALUE(num_tokens >= 0, name, ": num_tokens=", num_tokens);
   const c10::cuda::CUDAGuard guard(dev);
-  Tensor cu = empty_on(dev, {R + 1}, at::kInt), kv_lens = empty_on(dev, {R}, at::kInt), taken = empty_on(dev, {1}, at::kInt);
-  Tensor positions = empty_on(dev, {num_tokens}, at::kLong), slots = empty_on(dev, {num_tokens}, at::kLong);
+  Tensor cu, kv_lens, taken, positions, slots;
+  if constexpr (kShare) {
+    const int64_t r4 = (R + 4) / 4 * 4, n2 = (num_tokens + 1) / 2 * 2;  // 16-byte boundaries
+    const Tensor requests = empty_on(dev, {2 * r4 + 1}, at::kInt), tokens = empty_on(dev, {n2 + num_tokens}, at::kLong);
+    cu = part_of(requests, 0, R + 1), kv_lens = part_of(requests, r4, R), taken = part_of(requests, 2 * r4, 1);
+    positions = part_of(tokens, 0, num_tokens), slots = part_of(tokens, n2, num_tokens);
+  } else {
+    cu = empty_on(dev, {R + 1}, at::kInt), kv_lens = empty_on(dev, {R}, at::kInt), taken = empty_on(dev, {1}, at::kInt);
+    positions = empty_on(dev, {num_tokens}, at::kLong), slots = empty_on(dev, {num_tokens}, at::kLong);
+  }
   const Range range("hspmn::paged_slots");
   check_status(
       hspmn_paged_slots(block_table.data_ptr<int32_t>(), R > 1 ? block_table.stride(0) : P,
@@ -222,13 +242,13 @@ TORCH_LIBRARY_FRAGMENT(hspmn, m) {
 }
 
 TORCH_LIBRARY_IMPL(hspmn, CompositeExplicitAutograd, m) {
-  m.impl("paged_slots_", paged_slots_);
+  m.impl("paged_slots_", paged_slots_<false>);
   m.impl("rope_paged_write_", rope_paged_write_);
   m.impl("sqdk_paged_fwd", sqdk_paged_fwd);
 }
 
 PYBIND11_MODULE(libhspmn_torch, m) {
-  m.def("paged_slots_", paged_slots_);
+  m.def("paged_slots_", paged_slots_<true>);
   m.def("rope_paged_write_", rope_paged_write_);
   m.def("sqdk_paged_fwd", sqdk_paged_fwd);
 }
