@@ -19,7 +19,9 @@
 // CTA's four warps owns 16 (32) keys of every unit and runs on its own: its K and
 // V rows come by cp.async into a private ring (kPagedStages deep), Q K^T and P V are
 // m16n8k16 products with the softmax between them in registers, and the warps
-// meet only at the end of an item. Sums, maxima and O are fp32. The products fill
+// meet only at the end of an item. Sums, maxima and O are fp32; the maximum is
+// kept in the products' own units and subtracted before the scale, so that scores
+// of any size weigh right. The products fill
 // a fifth of the tensor pipe, so 128-row tiles would not be faster; three stages
 // of two CTAs an SM keep 192 KB an SM on the way (three CTAs with two stages: 178
 // -> 221 us). 64 tokens over 1.15 GB of K and V (contexts to 32768, 16/4 heads of
@@ -61,7 +63,7 @@ struct PagedAttnParams {
   const int* cu_q;
   const int64_t* pos;
   float* part_o;   // [2 * runs][16][HD] unnormalised O
-  float* part_ml;  // [2 * runs][16][2] maximum (log2 units), row sum
+  float* part_ml;  // [2 * runs][16][2] maximum (of q.k, not scaled), row sum
   int4* merges;    // [runs] the item that goes on behind this run, for the merge; .w < 0: none
   int64_t N;
   int R, P, num_pages, shift, H, Hkv, G, hd;
@@ -569,16 +571,16 @@ __global__ void __launch_bounds__(kPagedThreads, kPagedCtasPerSm) paged_attn_ker
         for (int n = 1; n < kGroups; ++n) mx = fmaxf(mx, fmaxf(s[n][2 * i], s[n][2 * i + 1]));
         mx = fmaxf(mx, __shfl_xor_sync(0xFFFFFFFFu, mx, 1));
         mx = fmaxf(mx, __shfl_xor_sync(0xFFFFFFFFu, mx, 2));
-        const float m_new = fmaxf(m_run[i], mx * p.scale_log2);
-        alpha[i] = m_new > m_run[i] ? fast_exp2(m_run[i] - m_new) : 1.0f;
+        const float m_new = fmaxf(m_run[i], mx);
+        alpha[i] = m_new > m_run[i] ? fast_exp2((m_run[i] - m_new) * p.scale_log2) : 1.0f;
         grew |= m_new > m_run[i];
-        const float neg = m_new == -INFINITY ? 0.0f : -m_new;
+        const float base = m_new == -INFINITY ? 0.0f : m_new;
         float sum = 0.0f;
 #pragma unroll
         for (int n = 0; n < kGroups; ++n) {
 #pragma unroll
           for (int c = 0; c < 2; ++c) {
-            const float e = fast_exp2(fmaf(s[n][2 * i + c], p.scale_log2, neg));
+            const float e = fast_exp2((s[n][2 * i + c] - base) * p.scale_log2);
             s[n][2 * i + c] = e;
             sum += e;
           }
@@ -702,7 +704,7 @@ __global__ void __launch_bounds__(kPagedThreads, kPagedCtasPerSm) paged_attn_ker
         for (int w = 0; w < kPagedWarps; ++w) {
           if (s_l[w][lr] == kUnseen) continue;
           none = false;
-          const float mw = s_m[w][lr], f = mw == M ? 1.0f : fast_exp2(mw - M);
+          const float mw = s_m[w][lr], f = mw == M ? 1.0f : fast_exp2((mw - M) * p.scale_log2);
           const float4 x = *reinterpret_cast<const float4*>(
               reinterpret_cast<const float*>(paged_smem + w * L::kWarpStage + stage * L::kStage) +
               paged_o_word<HD>(lr, c));
@@ -742,8 +744,8 @@ __global__ void __launch_bounds__(kPagedThreads, kPagedCtasPerSm) paged_attn_ker
 constexpr int kMergeWarps = 16;
 
 // Adds the partial results of the item that goes on behind run `block`, as that
-// run noted: O = sum 2^(m_c - M) O_c / sum 2^(m_c - M) l_c over the item's runs in
-// order. All runs it goes on behind share its rows; a warp takes a row and a
+// run noted: O = sum w_c O_c / sum w_c l_c, w_c = 2^(scale_log2 (m_c - M)), over the
+// item's runs in order. All runs it goes on behind share its rows; a warp takes a row and a
 // share of the runs.
 template <int HD, bool kBF16>
 __device__ __forceinline__ void paged_merge(const PagedAttnParams& p, int block) {
@@ -776,7 +778,8 @@ __device__ __forceinline__ void paged_merge(const PagedAttnParams& p, int block)
       if (x.y == kUnseen) continue;
       none = false;
       const float top = fmaxf(M, x.x);
-      const float f = x.x == top ? 1.0f : fast_exp2(x.x - top), g = M == top ? 1.0f : fast_exp2(M - top);
+      const float f = x.x == top ? 1.0f : fast_exp2((x.x - top) * p.scale_log2);
+      const float g = M == top ? 1.0f : fast_exp2((M - top) * p.scale_log2);
       M = top;
       l = g * l + f * x.y;
       o.x = g * o.x + f * v.x, o.y = g * o.y + f * v.y, o.z = g * o.z + f * v.z, o.w = g * o.w + f * v.w;
@@ -795,7 +798,7 @@ __device__ __forceinline__ void paged_merge(const PagedAttnParams& p, int block)
     const float2 x = s_ml[w];
     if (x.y == kUnseen) continue;
     empty = false;
-    const float f = x.x == top ? 1.0f : fast_exp2(x.x - top);
+    const float f = x.x == top ? 1.0f : fast_exp2((x.x - top) * p.scale_log2);
     sum += f * x.y;
     if (lane < HD / 4) {
       const float4 v = s_o[w][lane];

@@ -45,6 +45,7 @@ constexpr int kChunkUnit = 16;           // cost units of a 64-key block
 constexpr int kChunkTileCost = 5;        // blocks' worth of time to open and close a tile (seven prompts: 247 us; at 3 256, 6 250, 7 252, 9 262)
 constexpr int kChunkMinPiece = 8;        // blocks of work below which another run is not opened
 constexpr int kChunkEpilogueBar = 1;     // named barrier of the four softmax warps
+constexpr float kChunkFmaMax = 512.0f;   // largest maximum (log2 units) of which the rounding may be left in P
 
 template <int HD>
 struct ChunkLayout {
@@ -618,15 +619,19 @@ __global__ void __launch_bounds__(kChunkThreads, kChunkCtasPerSm)
           }
         }
         uint32_t pk[kSqdkBN / 2];
-        // p = 2^(s*c2 - m), packed; returns the block's row sum
-        auto exponentiate = [&](float m) -> float {
-          const float neg_m = (m == -INFINITY) ? 0.0f : -m;
-          const uint64_t cc = f2_pack(c2, c2), nm = f2_pack(neg_m, neg_m);
+        // p = 2^((s - m) c2), packed; returns the block's row sum. kFma: as
+        // s c2 - (m c2), one operation instead of two, with the rounding of m c2
+        // (2^-15 at kChunkFmaMax) in every p.
+        auto exponentiate = [&](auto kFma, float m) -> float {
+          const float neg = (m == -INFINITY) ? 0.0f : kFma ? -(m * c2) : -m;
+          const uint64_t cc = f2_pack(c2, c2), nm = f2_pack(neg, neg);
           uint64_t acc0 = f2_pack(0.0f, 0.0f), acc1 = acc0;
 #pragma unroll
           for (int c = 0; c < kSqdkBN; c += 2) {
             float x0, x1;
-            f2_unpack(f2_fma(f2_pack(sv[c], sv[c + 1]), cc, nm), x0, x1);
+            const uint64_t s2 = f2_pack(sv[c], sv[c + 1]);
+            if constexpr (kFma) f2_unpack(f2_fma(s2, cc, nm), x0, x1);
+            else f2_unpack(f2_mul(f2_add(s2, nm), cc), x0, x1);
             const float p0 = fast_exp2(x0), p1 = fast_exp2(x1);
             if ((c >> 1) & 1) acc1 = f2_add(acc1, f2_pack(p0, p1));
             else acc0 = f2_add(acc0, f2_pack(p0, p1));
@@ -638,8 +643,8 @@ __global__ void __launch_bounds__(kChunkThreads, kChunkCtasPerSm)
           return (a0 + a1) + (b0 + b1);
         };
         bool done = false;
-        if (__all_sync(0xFFFFFFFFu, m_run != -INFINITY)) {
-          const float lb = exponentiate(m_run);
+        if (__all_sync(0xFFFFFFFFu, fabsf(m_run) * c2 <= kChunkFmaMax)) {
+          const float lb = exponentiate(std::true_type{}, m_run);
           if (__all_sync(0xFFFFFFFFu, lb < kSqdkSumBound<kBF16>)) {
             l_run += lb;
             done = true;
@@ -653,14 +658,14 @@ __global__ void __launch_bounds__(kChunkThreads, kChunkCtasPerSm)
             for (int u = 0; u < 4; ++u) mq[u] = fmaxf(mq[u], sv[c + u]);
           }
           const float mx = fmaxf(fmaxf(mq[0], mq[1]), fmaxf(mq[2], mq[3]));
-          const float m_new = fmaxf(m_run, mx * c2);
+          const float m_new = fmaxf(m_run, mx);
           const bool need_o = j > 0 && (m_run != -INFINITY) && (m_new > m_run);
           if (__any_sync(0xFFFFFFFFu, need_o)) {
             // P V of the block before must have landed in O
             ok = __all_sync(0xFFFFFFFFu, mbar_wait(&bar_vempty[(n - 1) & 1], ((n - 1) >> 1) & 1, &abort_flag));
             if (!ok) break;
             tc_fence_after();
-            const float alpha = need_o ? fast_exp2(m_run - m_new) : 1.0f;
+            const float alpha = need_o ? fast_exp2((m_run - m_new) * c2) : 1.0f;
 #pragma unroll 1
             for (int c = 0; c < HD; c += 32) {
               uint32_t x[32];
@@ -673,10 +678,10 @@ __global__ void __launch_bounds__(kChunkThreads, kChunkCtasPerSm)
             tmem_wait_st();
           }
           if (m_new != m_run) {
-            l_run = (m_run == -INFINITY) ? 0.0f : l_run * fast_exp2(m_run - m_new);
+            l_run = (m_run == -INFINITY) ? 0.0f : l_run * fast_exp2((m_run - m_new) * c2);
             m_run = m_new;
           }
-          l_run += exponentiate(m_run);
+          l_run += exponentiate(std::false_type{}, m_run);
         }
         tmem_st32(tS + sb * kSqdkBN, pk);
         tmem_wait_st();
@@ -815,7 +820,7 @@ __global__ void __launch_bounds__(kChunkThreads, kChunkCtasPerSm)
 }
 
 // Adds the pieces of the tile that goes on behind run `run`, as that run noted:
-// O = sum 2^(m_c - M) O_c / sum 2^(m_c - M) l_c over the runs in order. Every run
+// O = sum w_c O_c / sum w_c l_c, w_c = 2^(c2 (m_c - M)), over the runs in order. Every run
 // that the tile goes on behind gives kChunkMergeBlocks blocks to it. A warp takes
 // 8 rows by 16 columns at a time (128-byte reads of the pieces); where there are
 // more warps than that needs, several share the pieces.
@@ -850,7 +855,8 @@ __device__ __forceinline__ void chunk_merge(const ChunkParams& p, int run, int s
       if (s == kUnseen) return;
       none = false;
       const float top = fmaxf(M, m);
-      const float f = m == top ? 1.0f : fast_exp2(m - top), g = M == top ? 1.0f : fast_exp2(M - top);
+      const float f = m == top ? 1.0f : fast_exp2((m - top) * p.a.scale_log2);
+      const float g = M == top ? 1.0f : fast_exp2((M - top) * p.a.scale_log2);
       M = top;
       l = g * l + f * s;
       o.x = g * o.x + f * v.x, o.y = g * o.y + f * v.y, o.z = g * o.z + f * v.z, o.w = g * o.w + f * v.w;

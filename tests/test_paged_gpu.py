@@ -1,5 +1,7 @@
 """Paged K/V cache operators against their 64-bit forms (tests/paged_ref.py)."""
 
+import math
+
 import pytest
 import torch
 
@@ -303,6 +305,39 @@ def test_large_scores():
     kc.mul_(8.0)
     q.mul_(4.0)
     check(args, max_qs=(0, 200))
+    assert ops.device_errors() == 0
+
+
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16])
+@pytest.mark.parametrize("sign", [1, -1])
+@pytest.mark.parametrize("size", [1, 2 ** 7, 2 ** 15])
+def test_scores_of_any_size(dtype, sign, size):
+    """Scores of up to 2^30 that float32 holds exactly. The bound is the general one (paged_ref.attend_ref)
+    without the scores' rounding, an exponent of d having an error of d e, and 2^-15 for a maximum's rounding
+    (log2 units, up to 512) that P may keep."""
+    lens = [3000, 700, 300]
+    q, kc, vc, table, kv, cu, pos = batch(lens, [[2999], list(range(500, 700)), [100, 299]], 8, 2, 64, dtype, 16, seed=43)
+    q.zero_(), kc.zero_()
+    q[..., 0] = sign * size
+    u, e, rows = torch.finfo(dtype).eps / 2, 2.0 ** -23, []
+    for r, n in enumerate(lens):
+        m = torch.arange(n, device=DEV)
+        slots = table[r, m // 16].long() * 16 + m % 16
+        key = (16 * ((m * 7919 + 11) % (n // 2) + 1)).to(dtype)  # two keys of each value (more in bf16), all over
+        kc.view(-1, 2, 64)[slots, :, 0] = key[:, None]
+        s = sign * size * key.double()
+        v = vc.view(-1, 2, 64)[slots].double()
+        for i in range(cu[r], cu[r + 1]):
+            seen = int(pos[i]) + 1
+            d = (s[:seen].max() - s[:seen]) / math.log(2)
+            w = torch.softmax(s[:seen], 0)
+            out = torch.einsum("m,mgd->gd", w, v[:seen])
+            err = w * (u + 2.0 ** -15 + (8 + d) * e + 2 * (seen + 32) * e) + (2.0 ** -25 if dtype == torch.float16 else 0)
+            rows.append((out, torch.einsum("m,mgd->gd", err, v[:seen].abs()) + u * out.abs()))
+    want, tol = (torch.stack(x).repeat_interleave(4, dim=1) for x in zip(*rows))
+    for max_q in (0, 1, 200):
+        o = attend(q, kc, vc, table, kv, cu, pos, scale=1.0, max_q=max_q).double()
+        assert ((o - want).abs() <= tol).all(), (max_q, (o - want).abs().max().item())
     assert ops.device_errors() == 0
 
 
