@@ -358,11 +358,34 @@ __host__ __device__ constexpr uint32_t umma_idesc_f16(int M, int N, int ab, bool
 // dependent launches
 // ---------------------------------------------------------------------------
 
+// A kernel launched as a programmatic dependent may begin while the one before it
+// in the stream still runs; it calls grid_dependency_wait() before it touches
+// memory, and reads what earlier kernels wrote by coherent loads only (the
+// read-only path, __ldg, is for what does not change while a kernel is in flight,
+// and may be moved in front of the wait).
+
 // The next kernel of the stream, if launched as a programmatic dependent, may
-// begin; it waits for this grid's results with grid_dependency_wait().
+// begin.
 __device__ __forceinline__ void grid_dependents_launch() { asm volatile("griddepcontrol.launch_dependents;" ::: "memory"); }
 // Waits until the grid before this one has finished and its writes are visible.
 __device__ __forceinline__ void grid_dependency_wait() { asm volatile("griddepcontrol.wait;" ::: "memory"); }
+// A load that stays behind grid_dependency_wait() (what it reads may have been
+// written by the grid before, so not through the read-only path).
+__device__ __forceinline__ int load_now(const int* p) {
+  int x;
+  asm volatile("ld.global.s32 %0, [%1];" : "=r"(x) : "l"(p));
+  return x;
+}
+__device__ __forceinline__ int64_t load_now(const int64_t* p) {
+  int64_t x;
+  asm volatile("ld.global.s64 %0, [%1];" : "=l"(x) : "l"(p));
+  return x;
+}
+__device__ __forceinline__ unsigned short load_now(const unsigned short* p) {
+  unsigned short x;
+  asm volatile("ld.global.u16 %0, [%1];" : "=h"(x) : "l"(p));
+  return x;
+}
 
 // ---------------------------------------------------------------------------
 // small math

@@ -68,6 +68,8 @@ __global__ void __launch_bounds__(kSlotsThreads) paged_slots_kernel(const SlotsP
   int* s_page = slots_smem + (p.R + 1);  // [R+1]
   __shared__ int2 warp_sum[kSlotsWarps];
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+  grid_dependency_wait();
+  grid_dependents_launch();
   int2 carry = make_int2(0, 0);
   bool bad = false;
   if (threadIdx.x == 0) s_tok[0] = s_page[0] = 0;
@@ -75,7 +77,7 @@ __global__ void __launch_bounds__(kSlotsThreads) paged_slots_kernel(const SlotsP
     const int r = base + static_cast<int>(threadIdx.x);
     int2 v = make_int2(0, 0);
     if (r < p.R) {
-      const int c = __ldg(p.seq_lens + r), m = __ldg(p.new_lens + r);
+      const int c = p.seq_lens[r], m = p.new_lens[r];
       bad |= c < 0 || m < 0;
       const int64_t c0 = max(c, 0), kv = c0 + max(m, 0);
       v.x = max(m, 0);
@@ -112,21 +114,21 @@ __global__ void __launch_bounds__(kSlotsThreads) paged_slots_kernel(const SlotsP
   }
   for (int64_t j = tid; j < fresh; j += step) {
     const int r = last_not_above(s_page, p.R, static_cast<int>(j));
-    const int col = pages_of(max(__ldg(p.seq_lens + r), 0), p.shift, p.P) + static_cast<int>(j) - s_page[r];
-    if (col < p.P) p.table[r * p.table_rs + col] = j < p.F ? __ldg(p.free_pages + j) : -1;
+    const int col = pages_of(max(p.seq_lens[r], 0), p.shift, p.P) + static_cast<int>(j) - s_page[r];
+    if (col < p.P) p.table[r * p.table_rs + col] = j < p.F ? p.free_pages[j] : -1;
   }
   const int mask = (1 << p.shift) - 1;
   for (int64_t t = tid; t < p.N; t += step) {
     int64_t pos = -1, slot = -1;
     if (t < total) {
       const int r = last_not_above(s_tok, p.R, static_cast<int>(t));
-      const int64_t c0 = max(__ldg(p.seq_lens + r), 0);
+      const int64_t c0 = max(p.seq_lens[r], 0);
       pos = c0 + t - s_tok[r];
       const int64_t col = pos >> p.shift;
       const int held = pages_of(c0, p.shift, p.P);
       int page = -1;
       if (col < held) page = p.table[r * p.table_rs + col];
-      else if (col < p.P && s_page[r] + (col - held) < p.F) page = __ldg(p.free_pages + s_page[r] + (col - held));
+      else if (col < p.P && s_page[r] + (col - held) < p.F) page = p.free_pages[s_page[r] + (col - held)];
       if (page >= 0) slot = (static_cast<int64_t>(page) << p.shift) + (pos & mask);
     }
     p.pos[t] = pos;
@@ -174,7 +176,7 @@ __device__ __forceinline__ void load_table(const char* p, float (&out)[n]) {
   constexpr int per = 16 / sizeof(Tab);
 #pragma unroll
   for (int i = 0; i < n / per; ++i) {
-    const uint4 w = __ldg(reinterpret_cast<const uint4*>(p) + i);
+    const uint4 w = reinterpret_cast<const uint4*>(p)[i];
     const Tab* e = reinterpret_cast<const Tab*>(&w);
 #pragma unroll
     for (int j = 0; j < per; ++j) out[i * per + j] = elt_to_float(e[j]);
@@ -206,13 +208,15 @@ __global__ void __launch_bounds__(kRowThreads) rope_paged_write_kernel(const Pag
   const int vh1 = (lane + kLanes) / vgroups, vc1 = lane + kLanes - vh1 * vgroups;
   auto source = [](const char* row, int64_t sh, int h, int c) { return reinterpret_cast<const uint4*>(row + h * sh + c * 16); };
   const int64_t step = static_cast<int64_t>(gridDim.x) * kTokens;
+  grid_dependency_wait();
+  grid_dependents_launch();
   int64_t t = static_cast<int64_t>(blockIdx.x) * kTokens + threadIdx.x / kLanes;
-  int64_t slot = t < p.N ? __ldg(p.slots + t) : -1, pos = rope && t < p.N ? __ldg(p.pos + t) : 0;
+  int64_t slot = t < p.N ? p.slots[t] : -1, pos = rope && t < p.N ? p.pos[t] : 0;
   for (; t < p.N; t += step) {
     const int64_t slot_now = slot, pos_now = pos;
     if (t + step < p.N) {
-      slot = __ldg(p.slots + t + step);
-      if (rope) pos = __ldg(p.pos + t + step);
+      slot = p.slots[t + step];
+      if (rope) pos = p.pos[t + step];
     }
     if (slot_now < 0) continue;  // padding
     const int64_t page = slot_now >> p.shift, off = slot_now & ((1 << p.shift) - 1);

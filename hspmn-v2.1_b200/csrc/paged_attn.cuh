@@ -88,9 +88,9 @@ struct PagedRaw {
 
 __device__ __forceinline__ PagedRaw paged_raw(const PagedAttnParams& p, int r) {
   PagedRaw x;
-  x.a = r <= p.R ? __ldg(p.cu_q + r) : 0;
-  x.b = r < p.R ? __ldg(p.cu_q + r + 1) : static_cast<int>(p.N);
-  x.kv = r < p.R ? __ldg(p.kv_lens + r) : 0;
+  x.a = r <= p.R ? p.cu_q[r] : 0;
+  x.b = r < p.R ? p.cu_q[r + 1] : static_cast<int>(p.N);
+  x.kv = r < p.R ? p.kv_lens[r] : 0;
   return x;
 }
 
@@ -383,6 +383,8 @@ __global__ void __launch_bounds__(kPagedThreads, kPagedCtasPerSm) paged_attn_ker
   __shared__ __align__(8) int64_t s_pos[kPagedStages][kPagedRows];
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   const int g = lane >> 2, t2 = (lane & 3) * 2;  // accumulator row and first column of this lane
+  // (the chunk kernel lets this one begin behind its own wait)
+  if (!p.has_chunks) grid_dependency_wait();
   grid_dependents_launch();
   const int split = paged_split<L::kKeys>(p, lane);
   PagedList<L::kKeys> list(p, split, lane);
@@ -445,7 +447,7 @@ __global__ void __launch_bounds__(kPagedThreads, kPagedCtasPerSm) paged_attn_ker
     const char* vh = p.v + static_cast<int64_t>(ahead.head) * p.v_sh + ld_byte;
     int page[kGroups];
 #pragma unroll
-    for (int i = 0; i < kGroups; ++i) page[i] = 8 * i < left ? __ldg(row + ((key0 + 8 * i) >> p.shift)) : 0;
+    for (int i = 0; i < kGroups; ++i) page[i] = 8 * i < left ? row[(key0 + 8 * i) >> p.shift] : 0;
     uint32_t gone = 0;
 #pragma unroll
     for (int i = 0; i < kGroups; ++i) gone |= (static_cast<unsigned>(page[i]) >= static_cast<unsigned>(p.num_pages) ? 1u : 0u) << i;
@@ -817,6 +819,7 @@ __device__ __forceinline__ void paged_merge(const PagedAttnParams& p, int block)
 template <int HD, bool kBF16>
 __global__ void __launch_bounds__(32 * kMergeWarps) paged_merge_kernel(const __grid_constant__ PagedAttnParams p) {
   grid_dependency_wait();
+  grid_dependents_launch();
   paged_merge<HD, kBF16>(p, static_cast<int>(blockIdx.x));
 }
 

@@ -99,8 +99,8 @@ __device__ __forceinline__ ChunkRequest chunk_request(const ChunkParams& p, int 
   if (q.rows <= split) return c;  // the 16-row kernel's
   c.tiles = (c.len + p.QT - 1) / p.QT;
   const int64_t top = max(c.kv - 1, 0);
-  const int lo = static_cast<int>(min(max(__ldg(p.a.pos + c.q0 + min(p.QT, c.len) - 1), static_cast<int64_t>(0)), top));
-  const int hi = static_cast<int>(min(max(__ldg(p.a.pos + c.q0 + c.len - 1), static_cast<int64_t>(0)), top));
+  const int lo = static_cast<int>(min(max(load_now(p.a.pos + c.q0 + min(p.QT, c.len) - 1), static_cast<int64_t>(0)), top));
+  const int hi = static_cast<int>(min(max(load_now(p.a.pos + c.q0 + c.len - 1), static_cast<int64_t>(0)), top));
   constexpr int kShift = 2;  // 64 keys = kChunkUnit units
   static_assert(kSqdkBN >> kShift == kChunkUnit, "cost units");
   const int sh = kShift + p.a.cost_shift;
@@ -283,7 +283,7 @@ __device__ __forceinline__ void chunk_job(const ChunkParams& p, const ChunkTile&
   const int n = min(p.QT, c.req.len - c.t * p.QT);
   bool beyond = false;
   for (int i = lane; i < n; i += 32) {
-    const int64_t ps = __ldg(p.a.pos + c.req.q0 + c.t * p.QT + i);
+    const int64_t ps = load_now(p.a.pos + c.req.q0 + c.t * p.QT + i);
     const int lim = static_cast<int>(min(max(ps, static_cast<int64_t>(-1)), static_cast<int64_t>(c.req.kv) - 1));
     beyond |= ps >= c.req.kv;
     job.lim[i] = lim;
@@ -300,7 +300,7 @@ __device__ __forceinline__ void chunk_job(const ChunkParams& p, const ChunkTile&
     const int* row = p.a.table + static_cast<int64_t>(c.r) * p.a.table_rs;
     const int last = (min((j0 + nblk) * kSqdkBN, c.req.kv) - 1) >> p.a.shift;
     for (int pg = ((j0 * kSqdkBN) >> p.a.shift) + lane; pg <= last; pg += 32) {
-      const int x = __ldg(row + pg);
+      const int x = load_now(row + pg);
       holes |= x < 0 || x >= p.a.num_pages;
     }
     holes = __any_sync(0xFFFFFFFFu, holes);
@@ -344,6 +344,7 @@ __global__ void __launch_bounds__(kChunkThreads, kChunkCtasPerSm)
 
   const uint32_t sbase = (smem_u32(chunk_smem_raw) + 1023u) & ~1023u;
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  grid_dependency_wait();
   grid_dependents_launch();
   // no request for this kernel, or bad offsets (the 16-row kernel says so):
   // nothing to set up
@@ -445,7 +446,7 @@ __global__ void __launch_bounds__(kChunkThreads, kChunkCtasPerSm)
       auto page_at = [&](int j) -> int {
         const int key = (j0 + j) * kSqdkBN + lane * p.box_rows;
         if (lane >= boxes || key >= tile.req.kv) return p.a.num_pages;
-        const int pg = __ldg(row + (key >> p.a.shift));
+        const int pg = load_now(row + (key >> p.a.shift));
         return pg >= 0 && pg < p.a.num_pages ? pg : p.a.num_pages;
       };
       auto load = [&](const CUtensorMap* map, uint64_t* bar, uint32_t dst, int j, int page) {
@@ -610,7 +611,7 @@ __global__ void __launch_bounds__(kChunkThreads, kChunkCtasPerSm)
         if (holes) {
           const int* row = p.a.table + static_cast<int64_t>(job.r) * p.a.table_rs;
           for (int c0 = 0; c0 < kSqdkBN; c0 += 8) {
-            const int x = key0 + c0 < job.kv ? __ldg(row + ((key0 + c0) >> p.a.shift)) : -1;
+            const int x = key0 + c0 < job.kv ? load_now(row + ((key0 + c0) >> p.a.shift)) : -1;
             const bool gone = x < 0 || x >= p.a.num_pages;
             seen |= !gone && !blind && c0 <= left;
 #pragma unroll
@@ -754,14 +755,14 @@ __global__ void __launch_bounds__(kChunkThreads, kChunkCtasPerSm)
           const int* row = p.a.table + static_cast<int64_t>(job.r) * p.a.table_rs;
           const int from = max(tile_lo + 1, j0 * kSqdkBN), to = min(lim, (j0 + nblk) * kSqdkBN - 1);
           for (int key = from; key <= to; ++key) {
-            const int pg = __ldg(row + (key >> p.a.shift));
+            const int pg = load_now(row + (key >> p.a.shift));
             if (pg < 0 || pg >= p.a.num_pages) continue;
             const char* v = p.a.v + static_cast<int64_t>(pg) * p.a.v_sp +
                             static_cast<int64_t>(key & ((1 << p.a.shift) - 1)) * p.a.v_ss + head * p.a.v_sh;
 #pragma unroll
             for (int i = 0; i < 32; ++i) {
               if (c + i >= p.a.hd) continue;
-              const uint16_t w = __ldg(reinterpret_cast<const unsigned short*>(v) + c + i);
+              const uint16_t w = load_now(reinterpret_cast<const unsigned short*>(v) + c + i);
               if (not_finite2<kBF16>(w)) o[i] += half_to_float<kBF16>(w);
             }
           }
@@ -905,6 +906,7 @@ template <int HD, bool kBF16>
 __global__ void __launch_bounds__(32 * kMergeWarps, 2)
     paged_both_merge_kernel(const __grid_constant__ PagedAttnParams p, const __grid_constant__ ChunkParams c, int paged_runs) {
   grid_dependency_wait();
+  grid_dependents_launch();
   const int block = static_cast<int>(blockIdx.x) - paged_runs;
   if (block < 0) paged_merge<HD, kBF16>(p, static_cast<int>(blockIdx.x));
   else chunk_merge<HD, kBF16>(c, block / kChunkMergeBlocks, block % kChunkMergeBlocks);

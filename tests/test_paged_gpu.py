@@ -606,6 +606,75 @@ def test_captured_step_replays_with_new_lengths():
     assert ops.device_errors() == 0
 
 
+def serve(steps, sync):
+    """Steps of slots, write and attention (chunks and single tokens) whose operands the steps before wrote,
+    with small kernels and copies of other kinds between them; all that came out."""
+    R, H, Hkv, hd, page, pages = 6, 8, 2, 64, 16, 400
+    g = torch.Generator().manual_seed(41)
+    table = torch.full((R, 70), -1, dtype=torch.int32, device=DEV)
+    seq, free = torch.zeros(R, dtype=torch.int32, device=DEV), torch.arange(pages, dtype=torch.int32, device=DEV)
+    kc, vc = torch.zeros((2, pages, page, Hkv, hd), dtype=torch.bfloat16, device=DEV)
+    x = torch.randn((400, H, hd), generator=g).to(torch.bfloat16).to(DEV)
+    new = [torch.randint(0, 1 + most, (R,), generator=g, dtype=torch.int32).to(DEV) for most in (60, 1, 5, 1) * steps]
+    wait = torch.cuda.synchronize if sync else lambda: None
+    out = []
+    for lens in new:
+        wait()
+        cu, kv, pos, slots, taken = ops.paged_slots_(table, seq, lens, free, page, 400)
+        wait()
+        ops.rope_paged_write_(x[:, :Hkv], x[:, Hkv:2 * Hkv], None, None, pos, slots, kc, vc)
+        wait()
+        o = ops.sqdk_paged_fwd(x, kc, vc, table, kv, cu, pos, 0.125)
+        wait()
+        out.append(o)
+        x = torch.where(pos[:, None, None] >= 0, o + x, x) * 0.7
+        seq.copy_(kv)
+        free = free.gather(0, (torch.arange(pages, device=DEV) + taken) % pages)  # no page is given twice
+    return out, kc, vc, table
+
+
+def test_steps_in_a_row_equal_steps_one_by_one():
+    one_by_one = serve(12, True)
+    for _ in range(4):
+        in_a_row = serve(12, False)
+        assert all(torch.equal(a, b) for a, b in zip(one_by_one[0], in_a_row[0]))
+        assert all(torch.equal(a, b) for a, b in zip(one_by_one[1:], in_a_row[1:]))
+
+
+def test_capture_between_other_nodes():
+    """Operators captured behind a memset, a copy and a joined stream."""
+    lens = [33, 200]
+    q, kc, vc, table, kv, cu, pos = batch(lens, [[32], list(range(100, 200))], 8, 2, 64, torch.bfloat16, 16, seed=42)
+    kv_, cu_ = i32(kv), i32(cu)
+    want = ops.sqdk_paged_fwd(q, kc, vc, table, kv_, cu_, pos, 0.125)
+    q2, kv2, stamp, k2 = torch.empty_like(q), torch.empty_like(kv_), torch.ones(8, device=DEV), torch.zeros_like(kc)
+    side = torch.cuda.Stream()
+    g = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(g):
+        main = torch.cuda.current_stream()
+        stamp.zero_()
+        q2.copy_(q)
+        side.wait_stream(main)
+        with torch.cuda.stream(side):
+            kv2.copy_(kv_)
+            k2.copy_(kc)
+        first = ops.sqdk_paged_fwd(q, kc, vc, table, kv_, cu_, pos, 0.125)
+        main.wait_stream(side)
+        second = ops.sqdk_paged_fwd(q2, k2, vc, table, kv2, cu_, pos, 0.125)
+        side.wait_stream(main)
+        with torch.cuda.stream(side):
+            third = ops.sqdk_paged_fwd(q2, k2, vc, table, kv2, cu_, pos, 0.125, 1)
+        main.wait_stream(side)
+    one = torch.empty_like(third)
+    for _ in range(3):
+        for t in (q2, kv2, k2, first, second, third):
+            t.zero_()
+        g.replay()
+        one.copy_(third)
+        assert torch.equal(first, want) and torch.equal(second, want)
+        assert not stamp.any() and ((one.double() - want.double()).abs() <= 2.0 ** -6 * want.double().abs() + 2.0 ** -8).all()
+
+
 def test_prefill_in_chunks_and_decode_equal_the_whole_sequence():
     """Prompts brought in chunk by chunk and then token by token give what sqdk_fwd gives on the whole sequence."""
     B, S, H, Hkv, hd, page = 3, 200, 8, 2, 64, 16
