@@ -60,8 +60,8 @@ __device__ __forceinline__ int pages_of(int64_t len, int shift, int P) {
 // memory. No CTA reads what another writes: a token in a fresh page takes the
 // page from the free list, a token in an older page from the part of the table
 // that nobody writes. Latency bound: one launch and two dependent rounds of
-// loads, 3.1 us for 64 requests of one token; 6.4 us for 509 prompts of 1 to 4096
-// tokens (251,500 tokens, 4 MB).
+// loads, 3.3 us for 64 requests of one token; 6.5 us for 509 prompts of 1 to 4096
+// tokens (251,500 in all, 4 MB).
 __global__ void __launch_bounds__(kSlotsThreads) paged_slots_kernel(const SlotsParams p) {
   extern __shared__ int slots_smem[];
   int* s_tok = slots_smem;               // [R+1]
@@ -192,7 +192,7 @@ __device__ __forceinline__ void load_table(const char* p, float (&out)[n]) {
 // V groups (the whole rows up to 512 16-bit elements) together with the table
 // rows, so that a token waits for memory once. HBM bound: 65,536 tokens of 4 x 128
 // bf16 take 46.8 us, 5.85 TB/s (57 us when slots were read with the rows they
-// send); 61 tokens take 2.5 us, the launch.
+// send); 61 tokens take 2.4 us, the launch.
 template <typename T, typename Tab, int kLanes>
 __global__ void __launch_bounds__(kRowThreads) rope_paged_write_kernel(const PagedWriteParams p) {
   constexpr int n = 16 / sizeof(T);

@@ -7,13 +7,13 @@
 //
 // Work unit: 64 keys (128 for head_dim <= 64) of one (request, K/V head, 16 query
 // rows) item; the rows of a request and K/V head are numbered query * G + head,
-// so a single token's G heads share the keys that are read. All units of a call form one list
-// (requests, then row tiles, then heads, then keys) which is cut into as many
-// equal contiguous runs as there are CTAs: ragged lengths cost no idle CTA and
-// need no plan from the host, which knows neither lengths nor offsets. An item
-// that a cut divides leaves one partial result a run in the workspace (a run
-// has two at most: its first item and its last), and the merge kernel adds them
-// in run order, so results do not depend on timing.
+// so a single token's G heads share the keys that are read. All units of a call
+// form one list (requests, then row tiles, then heads, then keys) which is cut
+// into as many equal contiguous runs as there are CTAs: ragged lengths cost no
+// idle CTA and need no plan from the host, which knows neither lengths nor
+// offsets. An item that a cut divides leaves one partial result a run in the
+// workspace (a run has two at most: its first item and its last), and the merge
+// kernel adds them in run order, so results do not depend on timing.
 //
 // Bound: reading K and V once (4 query heads a key: 4 flops a byte). Each of a
 // CTA's four warps owns 16 (32) keys of every unit and runs on its own: its K and
@@ -21,14 +21,14 @@
 // m16n8k16 products with the softmax between them in registers, and the warps
 // meet only at the end of an item. Sums, maxima and O are fp32; the maximum is
 // kept in the products' own units and subtracted before the scale, so that scores
-// of any size weigh right. The products fill
-// a fifth of the tensor pipe, so 128-row tiles would not be faster; three stages
-// of two CTAs an SM keep 192 KB an SM on the way (three CTAs with two stages: 178
-// -> 221 us). 64 tokens over 1.15 GB of K and V (contexts to 32768, 16/4 heads of
-// 128) take 176 us, 6.5 TB/s; one token over 262144 keys 91 us (5.9 TB/s: the
-// start and the merge of 74 runs an item take 9 us); 37 tokens of 16 heads of 64
-// over up to 8192 keys 62 us (5.0 TB/s: 592 short items). One token over 500 keys
-// takes 7.8 us, two launches and a round of loads.
+// of any size weigh right. The products fill a fifth of the tensor pipe, so
+// 128-row tiles would not be faster; three stages of two CTAs an SM keep 192 KB
+// an SM on the way (three CTAs with two stages: 178 -> 221 us). 64 tokens over
+// 1.15 GB of K and V (contexts to 32768, 16/4 heads of 128) take 176 us, 6.5 TB/s;
+// one token over 262144 keys 92 us (5.8 TB/s: the start and the merge of 74 runs
+// an item take 9 us); 37 tokens of 16 heads of 64 over up to 8192 keys 63 us (4.9
+// TB/s: 592 short items). One token over 500 keys takes 7.7 us, two launches and a
+// few rounds of loads.
 #pragma once
 
 #include "sqdk.cuh"

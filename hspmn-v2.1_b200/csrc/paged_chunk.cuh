@@ -29,8 +29,8 @@
 // Bound: the chain of softmax and products of an SM's two CTAs (a block takes a
 // CTA about 1,800 cycles; tensor pipe and exponentials 50 % busy each), near the
 // card's 1 kW. A fifth of 8192 new tokens over 24576 cached, three requests of
-// 16/4 heads of 128: 1.23 ms, 940 TFLOP/s. Seven whole prompts of 511 to 4096
-// tokens: 249 us, 866 TFLOP/s (tiles of 23 blocks on average, each 5 blocks' time
+// 16/4 heads of 128: 1.24 ms, 930 TFLOP/s. Seven whole prompts of 511 to 4096
+// tokens: 250 us, 862 TFLOP/s (tiles of 23 blocks on average, each 5 blocks' time
 // to open and close). Eight softmax warps (258 us) and 128-key blocks with one S
 // buffer (283 us) were slower.
 #pragma once
