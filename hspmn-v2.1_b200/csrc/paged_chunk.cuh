@@ -30,7 +30,7 @@
 // CTA about 1,800 cycles; tensor pipe and exponentials 50 % busy each), near the
 // card's 1 kW. A fifth of 8192 new tokens over 24576 cached, three requests of
 // 16/4 heads of 128: 1.24 ms, 930 TFLOP/s. Seven whole prompts of 511 to 4096
-// tokens: 250 us, 862 TFLOP/s (tiles of 23 blocks on average, each 5 blocks' time
+// tokens: 247 us, 872 TFLOP/s (tiles of 23 blocks on average, each 5 blocks' time
 // to open and close). Eight softmax warps (258 us) and 128-key blocks with one S
 // buffer (283 us) were slower.
 #pragma once
@@ -45,6 +45,7 @@ constexpr int kChunkUnit = 16;           // cost units of a 64-key block
 constexpr int kChunkTileCost = 5;        // blocks' worth of time to open and close a tile (seven prompts: 247 us; at 3 256, 6 250, 7 252, 9 262)
 constexpr int kChunkMinPiece = 8;        // blocks of work below which another run is not opened
 constexpr int kChunkEpilogueBar = 1;     // named barrier of the four softmax warps
+constexpr int kChunkTilt = 3;            // see ChunkRuns, in 64ths
 constexpr float kChunkFmaMax = 512.0f;   // largest maximum (log2 units) of which the rounding may be left in P
 
 template <int HD>
@@ -181,13 +182,39 @@ struct ChunkList {
   }
 };
 
+// Runs of the list. Of the two CTAs that share an SM, the one launched first (the
+// first half of a full grid) is 10 % faster while both are at work, so its run is
+// longer: with a tilt of 0, 3, 5, 7 64ths, 285.0, 280.5, 280.6, 284.6 us for seven
+// prompts, 131.2, 128.5, 129.4, 130.2 for 52 requests of chunks and single tokens.
+struct ChunkRuns {
+  int share, rem, tilt, n;
+  __device__ __forceinline__ ChunkRuns(int total, int runs, int most) {
+    const Runs even(total, runs);
+    n = runs;
+    share = even.share;
+    rem = even.rem;
+    tilt = runs == most && (runs & 1) == 0 ? share / 64 * kChunkTilt : 0;
+  }
+  __device__ __forceinline__ int start(int c) const { return share * c + tilt * min(c, n - c) + min(c, rem); }
+  // The run that holds list place w.
+  __device__ __forceinline__ int of(int w) const {
+    int lo = 0, hi = n;
+    while (hi - lo > 1) {
+      const int mid = (lo + hi) >> 1;
+      if (start(mid) <= w) lo = mid;
+      else hi = mid;
+    }
+    return lo;
+  }
+};
+
 // The list cut into runs. A cut so near to an end of its tile that the piece
 // would not be worth its merge is moved to that end.
 struct ChunkCuts {
-  Runs run;
+  ChunkRuns run;
   int total, near;
   __device__ __forceinline__ ChunkCuts(const ChunkParams& p, int total_, int most)
-      : run(total_, min(most, max(total_ / max((kChunkUnit * kChunkMinPiece) >> p.a.cost_shift, 1), 1))),
+      : run(total_, min(most, max(total_ / max((kChunkUnit * kChunkMinPiece) >> p.a.cost_shift, 1), 1)), most),
         total(total_),
         near(min(run.share >> 4, (8 * kChunkUnit) >> p.a.cost_shift)) {}
   // The first run that begins behind list place w (the start of a tile that a cut divides).
