@@ -381,11 +381,6 @@ __device__ __forceinline__ int64_t load_now(const int64_t* p) {
   asm volatile("ld.global.s64 %0, [%1];" : "=l"(x) : "l"(p));
   return x;
 }
-__device__ __forceinline__ unsigned short load_now(const unsigned short* p) {
-  unsigned short x;
-  asm volatile("ld.global.u16 %0, [%1];" : "=h"(x) : "l"(p));
-  return x;
-}
 
 // ---------------------------------------------------------------------------
 // small math

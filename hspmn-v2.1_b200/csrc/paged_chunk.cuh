@@ -349,6 +349,18 @@ __device__ __forceinline__ void chunk_job(const ChunkParams& p, const ChunkTile&
   __syncwarp();
 }
 
+constexpr int kNoKey = 0x7FFFFFFF;
+
+// Notes in keys ([2][HD]: +inf, -inf) what element `h` of a key's V is, if it is an
+// infinity or NaN.
+template <bool kBF16, int HD>
+__device__ __forceinline__ void note_wild(int (&keys)[2][HD], int col, uint32_t h, int key) {
+  if (!not_finite2<kBF16>(h)) return;
+  const bool nan = (h & (kBF16 ? 0x7Fu : 0x3FFu)) != 0, negative = (h & 0x8000u) != 0;
+  if (nan || !negative) atomicMin(&keys[0][col], key);
+  if (nan || negative) atomicMin(&keys[1][col], key);
+}
+
 template <int HD, bool kBF16>
 __global__ void __launch_bounds__(kChunkThreads, kChunkCtasPerSm)
     paged_chunk_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant__ CUtensorMap tmK,
@@ -365,9 +377,12 @@ __global__ void __launch_bounds__(kChunkThreads, kChunkCtasPerSm)
   __shared__ int64_t row_off[kSqdkBM];  // of a tile's row in o, from the tile's first query and head; -1: no row
   __shared__ uint32_t tmem_base_sh;
   __shared__ volatile uint32_t abort_flag;
-  // an infinity or NaN was taken out of V for rows that do not see it (by the
-  // job's parity: one is cleared while the other is in use)
+  // an infinity or NaN was taken out of V for rows that do not see it, and the
+  // first key of each column at which a +inf, a -inf was (a NaN is both): rows see
+  // a prefix of the keys, so that is all they need to know, however many there are
+  // (both by the job's parity: one is cleared while the other is in use)
   __shared__ volatile uint32_t wild_flag[2];
+  __shared__ int wild_key[2][2][HD];
 
   const uint32_t sbase = (smem_u32(chunk_smem_raw) + 1023u) & ~1023u;
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
@@ -411,6 +426,8 @@ __global__ void __launch_bounds__(kChunkThreads, kChunkCtasPerSm)
   if (threadIdx.x >= 64) {
     const int rr = threadIdx.x - 64, ql = rr / p.a.G;
     row_off[rr] = ql < p.QT ? ql * p.a.o_sn + (rr - ql * p.a.G) * p.a.o_sh : -1;
+    for (int x = 0; x < 2; ++x)
+      if (rr < HD) wild_key[x][0][rr] = wild_key[x][1][rr] = kNoKey;
   }
   tc_fence_before();
   __syncthreads();
@@ -596,6 +613,7 @@ __global__ void __launch_bounds__(kChunkThreads, kChunkCtasPerSm)
       const bool posted = __all_sync(0xFFFFFFFFu, mbar_wait(&bar_job[walked & 1], (walked >> 1) & 1, &abort_flag));
       if (!named_bar_and(kChunkEpilogueBar, 128, posted)) break;
       if (threadIdx.x == 64) wild_flag[(walked + 1) & 1] = 0u;
+      if (r < HD) wild_key[(walked + 1) & 1][0][r] = wild_key[(walked + 1) & 1][1][r] = kNoKey;
       bool ok = true;
       volatile ChunkJob& job = jobs[walked & 1];
       const int nblk = job.nblk, j0 = job.j0;
@@ -717,8 +735,8 @@ __global__ void __launch_bounds__(kChunkThreads, kChunkCtasPerSm)
         if (edge) {
           // P is zero where a row does not see a key, but 0 * inf is not: V
           // rows that no row sees (the page's unwritten end) become zeros, and
-          // infinities and NaN leave the rows that only some see (the epilogue
-          // gives them back to those that do). 16 keys a warp.
+          // infinities and NaN leave the rows that only some see (they are noted,
+          // and the epilogue gives them back to those that do). 16 keys a warp.
           ok = __all_sync(0xFFFFFFFFu, mbar_wait(&bar_vfull[sb], (n >> 1) & 1, &abort_flag));
           if (!ok) break;
           const uint32_t vst = sbase + L::kVOff + sb * L::kKVBytes;
@@ -738,6 +756,14 @@ __global__ void __launch_bounds__(kChunkThreads, kChunkCtasPerSm)
                 if (not_finite2<kBF16>(w.x) || not_finite2<kBF16>(w.y) || not_finite2<kBF16>(w.z) ||
                     not_finite2<kBF16>(w.w)) {
                   found = true;
+                  // (the tile's 16-byte chunks lie swizzled by their row)
+                  const int col = (i >> 7) * 64 + (((i & 7) ^ (kr & 7)) << 3);
+                  const uint32_t pair[4] = {w.x, w.y, w.z, w.w};
+#pragma unroll
+                  for (int u = 0; u < 4; ++u) {
+                    note_wild<kBF16>(wild_key[walked & 1], col + 2 * u, pair[u] & 0xFFFFu, key);
+                    note_wild<kBF16>(wild_key[walked & 1], col + 2 * u + 1, pair[u] >> 16, key);
+                  }
                   w.x = finite2<kBF16>(w.x), w.y = finite2<kBF16>(w.y), w.z = finite2<kBF16>(w.z), w.w = finite2<kBF16>(w.w);
                   st_shared_v4(addr, w);
                 }
@@ -754,7 +780,8 @@ __global__ void __launch_bounds__(kChunkThreads, kChunkCtasPerSm)
       if (ok && nblk > 0) ok = __all_sync(0xFFFFFFFFu, mbar_wait(&bar_ofinal, segs & 1, &abort_flag));
       if (nblk > 0) ++segs;
       const bool live = named_bar_and(kChunkEpilogueBar, 128, ok);  // every warp has set this job's flag
-      const bool wild = wild_flag[walked & 1] != 0u;
+      const int parity = walked & 1;
+      const bool wild = wild_flag[parity] != 0u;
       ++walked;
       if (!live) break;
       tc_fence_after();
@@ -778,20 +805,11 @@ __global__ void __launch_bounds__(kChunkThreads, kChunkCtasPerSm)
           for (int i = 0; i < 32; ++i) o[i] = 0.0f;
         }
         if (wild && row_valid && !blind) {
-          // infinities and NaN that this row does see, from the cache
-          const int* row = p.a.table + static_cast<int64_t>(job.r) * p.a.table_rs;
-          const int from = max(tile_lo + 1, j0 * kSqdkBN), to = min(lim, (j0 + nblk) * kSqdkBN - 1);
-          for (int key = from; key <= to; ++key) {
-            const int pg = load_now(row + (key >> p.a.shift));
-            if (pg < 0 || pg >= p.a.num_pages) continue;
-            const char* v = p.a.v + static_cast<int64_t>(pg) * p.a.v_sp +
-                            static_cast<int64_t>(key & ((1 << p.a.shift) - 1)) * p.a.v_ss + head * p.a.v_sh;
+          // the infinities and NaN that this row does see
 #pragma unroll
-            for (int i = 0; i < 32; ++i) {
-              if (c + i >= p.a.hd) continue;
-              const uint16_t w = load_now(reinterpret_cast<const unsigned short*>(v) + c + i);
-              if (not_finite2<kBF16>(w)) o[i] += half_to_float<kBF16>(w);
-            }
+          for (int i = 0; i < 32; ++i) {
+            if (wild_key[parity][0][c + i] <= lim) o[i] += INFINITY;
+            if (wild_key[parity][1][c + i] <= lim) o[i] -= INFINITY;
           }
         }
         if (slot >= 0) {
@@ -835,7 +853,7 @@ __global__ void __launch_bounds__(kChunkThreads, kChunkCtasPerSm)
             make_float2(m_run, none ? kUnseen : l_run);
       tc_fence_before();  // O has been read: the next tile's first P V (behind this warp's arrival) may write it
       __syncwarp();
-      if (lane == 0) mbar_arrive(&bar_jobdone[(walked - 1) & 1]);
+      if (lane == 0) mbar_arrive(&bar_jobdone[parity]);
     }
   }
 

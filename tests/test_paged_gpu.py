@@ -297,6 +297,36 @@ def test_a_value_reaches_only_the_rows_that_see_its_key(bad, dtype):
         assert ((o - want).abs()[fine] <= tol.nan_to_num(0.0)[fine]).all()
 
 
+@pytest.mark.parametrize("hd,Hkv", [(128, 1), (64, 2)])
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16])
+def test_infinities_in_a_tile_whose_rows_lie_far_apart(dtype, hd, Hkv):
+    """A tile from the first keys to the last of a long context: infinities and NaN of one key or of many, in single
+    columns, beside a request that shares the CTAs. (One more look at every key a row and column took seconds.)"""
+    n = 100_000
+    spread = [0] + list(range(1500, n, 1600)) + [n - 1]
+    args = batch([n, 300], [spread, list(range(100, 300))], 4 * Hkv, Hkv, hd, dtype, 64, seed=44)
+    q, kc, vc, table, kv, cu, pos = args
+    q.mul_(0.25)  # every weight above the smallest f16
+
+    def put(p, col, x, head=0):
+        vc[table[0, p // 64].item(), p % 64, head, col] = x
+
+    inf, nan = float("inf"), float("nan")
+    for p, col, x in ((70, 0, inf), (40_000, 1, -inf), (40_001, 1, inf), (99_000, hd - 1, nan), (1500, 9, nan),
+                      (1501, 10, inf), (63, 17, -inf), (64, 18, -inf), (n - 1, 2, inf)):
+        put(p, col, x)
+    vc[table[0, 700:760].long(), :, 0, 33] = inf  # 3,840 keys of one column, and all of another key
+    vc[table[0, 1200].item(), 5, Hkv - 1] = nan
+    want, tol = ref.attend_ref(*args, hd ** -0.5)
+    for _ in range(2):
+        o = attend(*args, max_q=200).double()
+        assert torch.equal(o.isnan(), want.isnan())
+        assert torch.equal(o[o.isinf()], want[o.isinf()]) and torch.equal(o.isinf(), want.isinf())
+        fine = want.isfinite()
+        assert ((o - want).abs()[fine] <= tol.nan_to_num(0.0)[fine]).all()
+    assert ops.device_errors() == 0
+
+
 def test_large_scores():
     """Rows whose maximum grows by far from block to block, and ties at the top."""
     lens = [600, 600]
