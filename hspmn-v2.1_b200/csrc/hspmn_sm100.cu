@@ -797,6 +797,14 @@ int check_strides(std::initializer_list<int64_t> strides, int64_t es) {
   return HSPMN_OK;
 }
 
+// Status of a runtime call. A failed one leaves its error with the runtime, where
+// the next entry point's launch would find it and report it as its own: cleared here.
+int done(cudaError_t e) {
+  if (e == cudaSuccess) return HSPMN_OK;
+  (void)cudaGetLastError();
+  return HSPMN_ERR_CUDA;
+}
+
 // Lets kernel kKern use `bytes` of dynamic shared memory on the current device
 // (asked of the runtime once a device: the call takes as long as a launch).
 template <auto kKern>
@@ -805,8 +813,7 @@ int allow_smem(int bytes) {
   int dev = 0;
   if (cudaGetDevice(&dev) != cudaSuccess || dev < 0 || dev >= kMaxDevices) return HSPMN_ERR_CUDA;
   if (__atomic_load_n(&allowed[dev], __ATOMIC_ACQUIRE)) return HSPMN_OK;
-  if (cudaFuncSetAttribute(kKern, cudaFuncAttributeMaxDynamicSharedMemorySize, bytes) != cudaSuccess)
-    return HSPMN_ERR_CUDA;
+  if (int rc = done(cudaFuncSetAttribute(kKern, cudaFuncAttributeMaxDynamicSharedMemorySize, bytes))) return rc;
   __atomic_store_n(&allowed[dev], 1, __ATOMIC_RELEASE);
   return HSPMN_OK;
 }
@@ -846,7 +853,7 @@ int launch_dependent(void (*kern)(Params...), unsigned grid, unsigned threads, s
   attr[0].val.programmaticStreamSerializationAllowed = 1;
   cfg.attrs = attr;
   cfg.numAttrs = 1;
-  return cudaLaunchKernelEx(&cfg, kern, prm...) == cudaSuccess ? HSPMN_OK : HSPMN_ERR_CUDA;
+  return done(cudaLaunchKernelEx(&cfg, kern, prm...));
 }
 
 template <typename T, typename Tab, int kLanes>
@@ -952,9 +959,8 @@ int hspmn_paged_slots(int32_t* block_table, int64_t table_rs, const int32_t* seq
   prm.slots = slots;
   prm.taken = taken;
   const size_t smem = static_cast<size_t>(2 * (R + 1) * 4);
-  if (smem > 48 * 1024) {
-    if (int rc = allow_smem<paged_slots_kernel>(2 * (kSlotsMaxRequests + 1) * 4)) return rc;
-  }
+  // (always: what a launch may use without it is less than 48 KB by the kernel's own and the system's shared memory)
+  if (int rc = allow_smem<paged_slots_kernel>(2 * (kSlotsMaxRequests + 1) * 4)) return rc;
   const int64_t need = std::max<int64_t>(1, (N + kSlotsThreads - 1) / kSlotsThreads);
   const unsigned grid = static_cast<unsigned>(std::min<int64_t>(need, 2LL * sms));
   return launch_dependent(paged_slots_kernel, grid, kSlotsThreads, smem, static_cast<cudaStream_t>(stream), prm);

@@ -1,6 +1,8 @@
 """Paged K/V cache operators against their 64-bit forms (tests/paged_ref.py)."""
 
 import math
+import subprocess
+import sys
 
 import pytest
 import torch
@@ -8,6 +10,7 @@ import torch
 from hspmn_b200 import _native as N
 from hspmn_b200 import ops
 from tests import paged_ref as ref
+from tests.conftest import PKG, REPO
 
 pytestmark = pytest.mark.gpu
 DEV = "cuda"
@@ -65,6 +68,18 @@ def test_slots_many_requests(R):
     new = torch.randint(0, 40, (R,), generator=g).tolist()
     run_slots(seq, new, 16, sum(new) + 11)
     assert ops.device_errors() == 0
+
+
+def test_slots_in_a_fresh_process():
+    """From few requests to many in a process of its own: what one call asks of the runtime (more shared memory than
+    a kernel gets by default) must not be what a smaller one needs."""
+    code = ("import sys; sys.path[:0] = [%r, %r]\n"
+            "from tests.test_paged_gpu import ops, run_slots\n"
+            "for R in (1, 5800, 6000, 6014, 6015, 6016, 6017, 6080, 6134, 6135, 6136, 6143, 6144, 6145, 8191, 8192):\n"
+            "    run_slots([15] * R, [1 + (R & 1)] * R, 16, (1 + (R & 1)) * R)\n"
+            "    assert ops.device_errors() == 0\n" % (PKG, REPO))
+    r = subprocess.run([sys.executable, "-c", code], capture_output=True, text=True, timeout=300)
+    assert r.returncode == 0, r.stderr[-2000:]
 
 
 def test_slots_empty_batch():
