@@ -56,6 +56,14 @@ int dtype_code(const char* name, at::ScalarType t) {
   }
 }
 
+// Tells autograd that a tensor has been written in place: a backward that saved
+// what it held before then raises instead of using what it holds now. (No kernel of
+// the dispatcher does it: eager calls do not pass there.) Inference tensors have no
+// version.
+void written(const Tensor& t) {
+  if (!t.is_inference()) t.unsafeGetTensorImpl()->bump_version();
+}
+
 // at::empty without the dispatcher's part of its cost.
 Tensor empty_on(c10::Device dev, at::IntArrayRef sizes, at::ScalarType dtype) {
   return at::detail::empty_cuda(sizes, dtype, dev, std::nullopt);
@@ -132,6 +140,7 @@ std::tuple<Tensor, Tensor, Tensor, Tensor, Tensor> paged_slots_(const Tensor& bl
                         slots.data_ptr<int64_t>(), taken.data_ptr<int32_t>(),
                         c10::cuda::getCurrentCUDAStream(dev.index()).stream()),
       "hspmn_paged_slots");
+  written(block_table);
   return {cu, kv_lens, positions, slots, taken};
 }
 
@@ -180,6 +189,8 @@ void rope_paged_write_(const Tensor& k_, const Tensor& v_, const std::optional<T
                              v_cache.stride(2), n, heads, hd, k_cache.size(0), k_cache.size(1), code,
                              c10::cuda::getCurrentCUDAStream(dev.index()).stream()),
       "hspmn_rope_paged_write");
+  written(k_cache);
+  written(v_cache);
 }
 
 Tensor sqdk_paged_fwd(const Tensor& q_, const Tensor& k_cache, const Tensor& v_cache, const Tensor& block_table_,

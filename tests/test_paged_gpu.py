@@ -758,6 +758,62 @@ def test_prefill_in_chunks_and_decode_equal_the_whole_sequence():
     assert ops.device_errors() == 0
 
 
+def test_writes_raise_the_version_of_what_they_write():
+    n, Hkv, hd, page = 3, 2, 64, 16
+    kv = torch.zeros((4, 2, page, Hkv, hd), dtype=torch.bfloat16, device=DEV)
+    kc, vc = kv[:, 0], kv[:, 1]
+    k = torch.randn((n, Hkv, hd), device=DEV).to(torch.bfloat16)
+    slots = torch.arange(n, device=DEV)
+    lens = i32([0])
+    for write, make in ((ops.rope_paged_write_, ops.paged_slots_),
+                        (torch.ops.hspmn.rope_paged_write_, torch.ops.hspmn.paged_slots_)):
+        apart = [torch.zeros_like(kc) for _ in range(2)]
+        table = i32([[-1, -1]])
+        before = [t._version for t in (kv, *apart, table, k, slots, lens)]
+        write(k, k, None, None, slots, slots, kc, vc)
+        write(k, k, None, None, slots, slots, *apart)
+        make(table, lens, i32([3]), i32([0]), page, n)
+        after = [t._version for t in (kv, *apart, table, k, slots, lens)]
+        assert all(b > a for a, b in zip(before[:4], after[:4])) and before[4:] == after[4:]
+    assert ops.device_errors() == 0
+
+
+def test_backward_over_an_overwritten_cache_raises():
+    page, Hkv, hd = 16, 2, 64
+    kc, vc = (torch.randn((2, page, Hkv, hd), device=DEV).to(torch.bfloat16) for _ in range(2))
+    k = torch.randn((3, Hkv, hd), device=DEV).to(torch.bfloat16)
+    slots = torch.arange(3, device=DEV)
+    q = torch.randn((2, 5, 4, hd), device=DEV).to(torch.bfloat16).requires_grad_()
+    idx = torch.arange(5, device=DEV).expand(2, 5).contiguous()
+    for graph in (lambda: (q[:, :1, :Hkv] * kc).sum(), lambda: ops.sqdk_attention(q, kc, vc, idx, 0.125).float().sum()):
+        graph().backward()  # nothing written in between
+        y = graph()
+        ops.rope_paged_write_(k, k, None, None, slots, slots, kc, vc)
+        with pytest.raises(RuntimeError, match="modified by an inplace operation"):
+            y.backward()
+    table = i32([[-1, 5]])
+    w = torch.ones(8, device=DEV, requires_grad=True)
+    y = w[table.clamp(min=0).long()].sum() + (w[:2] * table).sum()
+    ops.paged_slots_(table, i32([0]), i32([3]), i32([0]), page, 3)
+    with pytest.raises(RuntimeError, match="modified by an inplace operation"):
+        y.backward()
+
+
+def test_caches_made_in_inference_mode():
+    n, Hkv, hd, page = 3, 2, 64, 16
+    k = torch.randn((n, Hkv, hd), device=DEV).to(torch.bfloat16)
+    slots, free = torch.arange(n, device=DEV), i32([0])
+    with torch.inference_mode():
+        kc, vc = (torch.zeros((1, page, Hkv, hd), dtype=torch.bfloat16, device=DEV) for _ in range(2))
+        table = i32([[-1]])
+        ops.rope_paged_write_(k, k, None, None, slots, slots, kc, vc)
+        ops.paged_slots_(table, i32([0]), i32([n]), free, page, n)
+    assert torch.equal(kc[0, :n], k) and table.tolist() == [[0]]
+    ops.rope_paged_write_(-k, k, None, None, slots, slots, kc, vc)  # and outside, as before
+    ops.paged_slots_(table, i32([0]), i32([n]), free, page, n)
+    assert torch.equal(kc[0, :n], -k)
+
+
 def test_refusals():
     q, kc, vc, table, kv, cu, pos = batch([20], [[18, 19]], 4, 2, 64, torch.bfloat16, 16, seed=23)
     kv, cu = i32(kv), i32(cu)
