@@ -130,6 +130,7 @@ __global__ void __launch_bounds__(kSlotsThreads) paged_slots_kernel(const SlotsP
       if (col < held) page = p.table[r * p.table_rs + col];
       else if (col < p.P && s_page[r] + (col - held) < p.F) page = p.free_pages[s_page[r] + (col - held)];
       if (page >= 0) slot = (static_cast<int64_t>(page) << p.shift) + (pos & mask);
+      else if (col < held) raise_device_error(HSPMN_DEVERR_PAGE);  // (the other causes are flagged above)
     }
     p.pos[t] = pos;
     p.slots[t] = slot;

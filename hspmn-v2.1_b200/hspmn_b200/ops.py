@@ -665,7 +665,8 @@ def paged_slots_(block_table: torch.Tensor, seq_lens: torch.Tensor, new_lens: to
     kv_lens int32 [R] = seq_lens + new_lens; positions int64 [N] and slots int64
     [N], -1 behind the last token; taken int32 [1], pages needed: the caller
     drops that many from ``free_pages``). Where ``free_pages`` ends, table
-    entries and slots are -1 and ``DEVERR_PAGE`` is set in ``device_errors()``;
+    entries and slots are -1 and ``DEVERR_PAGE`` is set in ``device_errors()``,
+    as for a new token in an older page whose entry is negative;
     negative lengths, tokens beyond N and lengths beyond P pages set
     ``DEVERR_POSITION``. At most 8192 requests a call."""
     return _call_paged("paged_slots_", block_table, seq_lens, new_lens, free_pages,

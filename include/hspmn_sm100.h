@@ -325,7 +325,8 @@ HSPMN_API int hspmn_sqdk_bwd(const void* q, const int64_t* q_strides,
  * slots, at least the number of new tokens (further ones are dropped and
  * HSPMN_DEVERR_POSITION is set, as for a negative length or one that P pages
  * do not hold). Where free_pages ends, entries and slots are -1 and
- * HSPMN_DEVERR_PAGE is set. R <= 8192. All lengths, cu_new, kv_lens, taken,
+ * HSPMN_DEVERR_PAGE is set, as where a new token belongs in an older page whose
+ * entry is negative (a page that was not to be had before). R <= 8192. All lengths, cu_new, kv_lens, taken,
  * block_table and free_pages are int32, positions and slots int64.
  */
 HSPMN_API int hspmn_paged_slots(int32_t* block_table, int64_t table_rs, const int32_t* seq_lens,

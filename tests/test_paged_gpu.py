@@ -104,6 +104,17 @@ def test_slots_flags_what_does_not_fit():
     assert ops.device_errors() == N.DEVERR_POSITION | N.DEVERR_PAGE
 
 
+def test_slots_flags_tokens_in_a_held_page_that_is_missing():
+    """A request whose last page was never had (a step before found the free list at its end): its new tokens have no
+    slot, and that is said; full pages that no new token goes to are not looked at."""
+    table, free = i32([[4, -1, -1], [-1, 2, -1], [-7, 6, 7]]), i32([9])
+    got = ops.paged_slots_(table, i32([12, 16, 20]), i32([3, 1, 0]), free, 8, 5)
+    assert got[2].tolist() == [12, 13, 14, 16, -1] and got[3].tolist() == [-1, -1, -1, 9 * 8, -1]
+    assert ops.device_errors() == N.DEVERR_PAGE
+    got = ops.paged_slots_(i32([[-1, 2, -1], [-7, 6, 7]]), i32([15, 20]), i32([1, 0]), free, 8, 1)
+    assert got[3].tolist() == [23] and ops.device_errors() == 0
+
+
 # ---------------------------------------------------------------------------
 # rope_paged_write_
 # ---------------------------------------------------------------------------
