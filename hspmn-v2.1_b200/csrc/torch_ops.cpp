@@ -7,6 +7,7 @@
 // the arguments costs 2 us more.
 #include <ATen/ATen.h>
 #include <ATen/cuda/EmptyTensor.h>
+#include <c10/core/AutogradState.h>
 #include <c10/cuda/CUDAGuard.h>
 #include <c10/cuda/CUDAStream.h>
 #include <nvtx3/nvToolsExt.h>
@@ -42,9 +43,12 @@ c10::Device require_cuda(std::initializer_list<const Tensor*> tensors) {
 }
 
 void no_grad_needed(const char* name, std::initializer_list<const Tensor*> tensors) {
-  if (!at::GradMode::is_enabled()) return;
-  for (const Tensor* t : tensors)
-    TORCH_CHECK(!t->requires_grad(), name, ": has no backward; call it under torch.no_grad() or detach its inputs");
+  const bool backward = at::GradMode::is_enabled(), forward = c10::AutogradState::get_tls_state().get_fw_grad_mode();
+  for (const Tensor* t : tensors) {
+    TORCH_CHECK(!(backward && t->requires_grad()), name,
+                ": has no backward; call it under torch.no_grad() or detach its inputs");
+    TORCH_CHECK(!(forward && t->_fw_grad(0).defined()), name, ": has no forward-mode derivative; give it the primals");
+  }
 }
 
 int dtype_code(const char* name, at::ScalarType t) {
@@ -165,6 +169,7 @@ void rope_paged_write_(const Tensor& k_, const Tensor& v_, const std::optional<T
   if (cos_.has_value()) {
     cos = *cos_, sin = *sin_;
     require_cuda({&k_, &cos, &sin});
+    no_grad_needed(name, {&cos, &sin});
     TORCH_CHECK_TYPE(cos.scalar_type() == sin.scalar_type() &&
                          (cos.scalar_type() == k_.scalar_type() || cos.scalar_type() == at::kFloat),
                      name, ": cos/sin must both have k's dtype or float32");

@@ -810,6 +810,39 @@ def test_backward_over_an_overwritten_cache_raises():
         y.backward()
 
 
+def test_derivatives_that_would_be_dropped_are_refused():
+    """Learned tables, and forward-mode tangents of any operand: there is no derivative, so none is dropped in silence."""
+    import torch.autograd.forward_ad as fw
+    page, Hkv, hd = 16, 2, 64
+    kc, vc = (torch.zeros((2, page, Hkv, hd), dtype=torch.bfloat16, device=DEV) for _ in range(2))
+    x = torch.randn((3, Hkv, hd), device=DEV).to(torch.bfloat16)
+    cos = torch.ones((8, hd), dtype=torch.float32, device=DEV)
+    at = torch.arange(3, device=DEV)
+    table, kv, cu = i32([[0, 1]]), i32([3]), i32([0, 3])
+    for cos_, sin_ in ((cos.clone().requires_grad_(), cos), (cos, cos.clone().requires_grad_())):
+        with pytest.raises(RuntimeError, match="no backward"):
+            ops.rope_paged_write_(x, x, cos_, sin_, at, at, kc, vc)
+        with torch.no_grad():
+            ops.rope_paged_write_(x, x, cos_, sin_, at, at, kc, vc)
+    with fw.dual_level():
+        def dual(t):
+            return fw.make_dual(t, torch.ones_like(t))
+
+        args = (x, x, cos, cos, at, at, kc, vc)
+        for i in (0, 1, 2, 3, 6, 7):
+            for grad_mode in (torch.enable_grad, torch.no_grad):
+                with grad_mode(), pytest.raises(RuntimeError, match="forward-mode"):
+                    ops.rope_paged_write_(*args[:i], dual(args[i]), *args[i + 1:])
+        args = (x, kc, vc, table, kv, cu, at, 0.125)
+        for i in range(3):
+            with pytest.raises(RuntimeError, match="forward-mode"):
+                ops.sqdk_paged_fwd(*args[:i], dual(args[i]), *args[i + 1:])
+        ops.sqdk_paged_fwd(*args)
+        with fw._set_fwd_grad_enabled(False):
+            ops.sqdk_paged_fwd(dual(x), *args[1:])
+    assert ops.device_errors() == 0
+
+
 def test_caches_made_in_inference_mode():
     n, Hkv, hd, page = 3, 2, 64, 16
     k = torch.randn((n, Hkv, hd), device=DEV).to(torch.bfloat16)
