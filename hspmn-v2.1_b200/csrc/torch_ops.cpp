@@ -97,6 +97,13 @@ Tensor rows_arg(const Tensor& t) {
   return ok ? t : t.clone(at::MemoryFormat::Contiguous);
 }
 
+// Whether a [L,hd] table can be read as it lies: dense rows, 16-byte stride and base.
+// (cos and sin share one stride, that of a table of one row included.)
+bool table_ok(const Tensor& t) {
+  return t.stride(1) == 1 && t.stride(0) >= t.size(1) && (t.stride(0) * t.element_size()) % 16 == 0 &&
+         reinterpret_cast<uintptr_t>(t.const_data_ptr()) % 16 == 0;
+}
+
 void check_caches(const char* name, const Tensor& k, const Tensor& v, at::ScalarType dtype, int64_t heads, int64_t hd) {
   TORCH_CHECK_VALUE(k.dim() == 4 && k.sizes() == v.sizes() && k.size(2) == heads && k.size(3) == hd, name,
                     ": caches must both be [num_pages, page_size, ", heads, ", ", hd, "], got ", k.sizes(), " and ",
@@ -173,11 +180,13 @@ void rope_paged_write_(const Tensor& k_, const Tensor& v_, const std::optional<T
     TORCH_CHECK_TYPE(cos.scalar_type() == sin.scalar_type() &&
                          (cos.scalar_type() == k_.scalar_type() || cos.scalar_type() == at::kFloat),
                      name, ": cos/sin must both have k's dtype or float32");
-    TORCH_CHECK_VALUE(cos.dim() >= 2 && cos.size(-1) == hd && cos.sizes() == sin.sizes(), name,
-                      ": cos/sin must both be [L,", hd, "], got ", cos.sizes(), " and ", sin.sizes());
-    if (cos.dim() != 2) cos = cos.reshape({-1, hd}), sin = sin.reshape({-1, hd});
-    if (cos.stride(1) != 1 || sin.stride(1) != 1 || cos.stride(0) != sin.stride(0) || cos.stride(0) < hd)
-      cos = cos.contiguous(), sin = sin.contiguous();
+    TORCH_CHECK_VALUE(cos.dim() >= 2 && cos.size(-1) == hd && sin.dim() >= 2 && sin.size(-1) == hd &&
+                          cos.numel() == sin.numel(),
+                      name, ": cos/sin must both be [L,", hd, "], got ", cos.sizes(), " and ", sin.sizes());
+    if (cos.dim() != 2) cos = cos.reshape({-1, hd});
+    if (sin.dim() != 2) sin = sin.reshape({-1, hd});
+    if (!table_ok(cos) || !table_ok(sin) || cos.stride(0) != sin.stride(0))
+      cos = cos.clone(at::MemoryFormat::Contiguous), sin = sin.clone(at::MemoryFormat::Contiguous);
     tab_code = dtype_code(name, cos.scalar_type());
   }
   if (n == 0) return;

@@ -177,6 +177,45 @@ def test_write_takes_views_and_block_tables():
     assert torch.equal(vc.view(-1, Hkv, hd)[3:3 + n], v)
 
 
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float32])
+def test_write_takes_tables_of_any_layout(dtype):
+    """Tables whose base or rows do not lie on 16 bytes, whose columns or rows are spread, of one row."""
+    L, Hkv, hd, page = 9, 2, 64, 8
+    g = torch.Generator().manual_seed(45)
+    k = torch.randn((L, Hkv, hd), generator=g).to(torch.bfloat16).to(DEV)
+    at = torch.arange(L, device=DEV)
+    cos, sin = tables(L, hd, dtype, g)
+
+    def write(cos, sin, rows=L):
+        kc, vc = (torch.zeros((2, page, Hkv, hd), dtype=torch.bfloat16, device=DEV) for _ in range(2))
+        ops.rope_paged_write_(k, k, cos, sin, at.clamp(max=rows - 1), at, kc, vc)
+        return kc
+
+    def shifted(t):
+        return torch.zeros(t.numel() + 1, dtype=t.dtype, device=DEV)[1:].view(t.shape).copy_(t)
+
+    def odd_rows(t):
+        return torch.zeros((L, hd + 1), dtype=t.dtype, device=DEV)[:, :hd].copy_(t)
+
+    def columns_apart(t):
+        return t.t().contiguous().t()
+
+    want = write(cos, sin)
+    for other in (shifted, odd_rows, columns_apart, lambda t: t[None, None], lambda t: odd_rows(t)[None, None]):
+        assert torch.equal(write(other(cos), other(sin)), want)
+        assert torch.equal(write(other(cos), sin), want) and torch.equal(write(cos, other(sin)), want)
+    one = write(cos[:1].contiguous(), sin[:1].contiguous(), 1)
+    for other in (lambda t: t[:1], lambda t: t[:1].as_strided((1, hd), (1, 1)), lambda t: t[:1].as_strided((1, hd), (0, 1)),
+                  lambda t: t[0]):
+        if other(cos).dim() == 1:
+            with pytest.raises(ValueError):
+                write(other(cos), other(sin), 1)
+        else:
+            assert torch.equal(write(other(cos), other(sin), 1), one)
+    assert torch.equal(write(cos[:1].expand(L, hd), sin[:1].expand(L, hd)), one)
+    assert ops.device_errors() == 0
+
+
 def test_write_flags_bad_slots_and_positions():
     Hkv, hd, page = 2, 32, 8
     kc, vc = (torch.zeros((2, page, Hkv, hd), dtype=torch.float16, device=DEV) for _ in range(2))
