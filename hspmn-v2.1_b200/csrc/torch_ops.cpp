@@ -2,9 +2,9 @@
 // from PyTorch's allocator, and the call into the C ABI on the caller's current
 // stream. They are in C++ because a decode step calls them for microseconds of
 // GPU work each (through Python checks and ctypes a call took 28 to 37 us of host
-// time). Registered as torch.ops.hspmn.*, for tracing, and as functions of the
-// Python module libhspmn_torch, which eager calls use: the dispatcher's boxing of
-// the arguments costs 2 us more.
+// time). Registered as torch.ops.hspmn.* for CUDA tensors, for traced calls, and as
+// functions of the Python module libhspmn_torch, which eager calls use: the
+// dispatcher's boxing of the arguments costs 2 us more.
 #include <ATen/ATen.h>
 #include <ATen/cuda/EmptyTensor.h>
 #include <c10/core/AutogradState.h>
@@ -254,19 +254,8 @@ Tensor sqdk_paged_fwd(const Tensor& q_, const Tensor& k_cache, const Tensor& v_c
 
 }  // namespace
 
-TORCH_LIBRARY_FRAGMENT(hspmn, m) {
-  m.def(
-      "paged_slots_(Tensor(a!) block_table, Tensor seq_lens, Tensor new_lens, Tensor free_pages, int page_size, "
-      "SymInt num_tokens) -> (Tensor, Tensor, Tensor, Tensor, Tensor)");
-  m.def(
-      "rope_paged_write_(Tensor k, Tensor v, Tensor? cos, Tensor? sin, Tensor positions, Tensor slots, "
-      "Tensor(a!) k_cache, Tensor(b!) v_cache) -> ()");
-  m.def(
-      "sqdk_paged_fwd(Tensor q, Tensor k_cache, Tensor v_cache, Tensor block_table, Tensor kv_lens, Tensor cu_q, "
-      "Tensor positions, float sm_scale, int max_q) -> Tensor");
-}
-
-TORCH_LIBRARY_IMPL(hspmn, CompositeExplicitAutograd, m) {
+// (the schemas are defined by the Python package, whether this library is loaded or not)
+TORCH_LIBRARY_IMPL(hspmn, CUDA, m) {
   m.impl("paged_slots_", paged_slots_<false>);
   m.impl("rope_paged_write_", rope_paged_write_);
   m.impl("sqdk_paged_fwd", sqdk_paged_fwd);

@@ -93,14 +93,11 @@ def lib() -> ctypes.CDLL:
     return _lib
 
 
-def torch_ops_available() -> bool:
-    return os.path.exists(TORCH_LIB_PATH) and available()
-
-
 def load_torch_ops():
     """Load libhspmn_torch.so: its operators are then registered with PyTorch.
-    Returns it as a Python module; raises if it is not built."""
-    if not torch_ops_available():
+    Returns it as a Python module; raises if it is not built, or not for this
+    PyTorch."""
+    if not os.path.exists(TORCH_LIB_PATH):
         raise RuntimeError(
             f"{os.path.basename(TORCH_LIB_PATH)} is not built (expected at {TORCH_LIB_PATH}); run "
             "`python hspmn-v2.1_b200/build_native.py` on a machine with the CUDA toolkit")
@@ -109,8 +106,13 @@ def load_torch_ops():
     import torch  # noqa: F401 (the module links against its libraries)
     lib()
     loader = importlib.machinery.ExtensionFileLoader("libhspmn_torch", TORCH_LIB_PATH)
-    module = importlib.util.module_from_spec(importlib.util.spec_from_loader("libhspmn_torch", loader))
-    loader.exec_module(module)
+    try:
+        module = importlib.util.module_from_spec(importlib.util.spec_from_loader("libhspmn_torch", loader))
+        loader.exec_module(module)
+    except ImportError as e:
+        raise RuntimeError(
+            f"{TORCH_LIB_PATH} does not load with PyTorch {torch.__version__} ({e}); run "
+            "`python hspmn-v2.1_b200/build_native.py --force` on a machine with the CUDA toolkit") from e
     return module
 
 

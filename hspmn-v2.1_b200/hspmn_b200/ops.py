@@ -610,20 +610,37 @@ def sqdk_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, indices: t
 # These operators are in C++ (csrc/torch_ops.cpp): a decode step calls them for
 # microseconds of GPU work each, so host time per call counts. Eager calls go to
 # the compiled functions directly, traced ones (and tensor subclasses) through
-# the operators registered as torch.ops.hspmn.*.
+# the operators registered as torch.ops.hspmn.*. Those are defined here, with
+# their fake forms, so that importing the package loads no library: the first
+# call does, and raises if it is not built or not for this PyTorch.
 
-_paged_direct = None  # the compiled functions
+_paged_direct = None  # the compiled functions, once loaded
 _paged_ops = {}       # the registered operators
+_paged_schemas = torch.library.Library("hspmn", "FRAGMENT")
 
 
-def _load_paged_ops() -> None:
+def _load_paged_ops():
     global _paged_direct
-    direct = N.load_torch_ops()
-    for name, fake in (("paged_slots_", _paged_slots_fake), ("rope_paged_write_", lambda *args: None),
-                       ("sqdk_paged_fwd", _sqdk_paged_fwd_fake)):
-        torch.library.register_fake("hspmn::" + name, fake)
-        _paged_ops[name] = getattr(torch.ops.hspmn, name).default
-    _paged_direct = direct
+    if _paged_direct is None:
+        _paged_direct = N.load_torch_ops()
+    return _paged_direct
+
+
+def _define_paged_op(schema: str, fake) -> None:
+    name = schema[:schema.index("(")]
+
+    def first_call(*args):
+        # reached for CUDA tensors until the library is loaded (it registers their
+        # implementation), and for those of other devices, which it refuses
+        direct = _load_paged_ops()
+        if any(isinstance(a, torch.Tensor) and a.device.type == "cuda" for a in args):
+            return _paged_ops[name](*args)
+        return getattr(direct, name)(*args)
+
+    _paged_schemas.define(schema)
+    _paged_schemas.impl(name, first_call, "CompositeExplicitAutograd")
+    torch.library.register_fake("hspmn::" + name, fake, lib=_paged_schemas)
+    _paged_ops[name] = getattr(torch.ops.hspmn, name).default
 
 
 def _call_paged(name: str, first: torch.Tensor, *args):
@@ -631,10 +648,8 @@ def _call_paged(name: str, first: torch.Tensor, *args):
     ``KernelTimer`` is active, timed as the other launches are."""
     if torch.compiler.is_compiling():
         return _paged_ops[name](first, *args)
-    if _paged_direct is None:
-        _load_paged_ops()  # raises: the library was not there at import
     plain = type(first) is torch.Tensor and torch._C._len_torch_dispatch_stack() == 0
-    op = getattr(_paged_direct, name) if plain else _paged_ops[name]
+    op = getattr(_paged_direct or _load_paged_ops(), name) if plain else _paged_ops[name]
     try:
         if LaunchStats.timer is not None:
             with _launch(name.rstrip("_"), first.device):
@@ -725,8 +740,15 @@ def _sqdk_paged_fwd_fake(q, k_cache, v_cache, block_table, kv_lens, cu_q, positi
     return torch.empty_like(q, memory_format=torch.contiguous_format)
 
 
-if N.torch_ops_available():
-    _load_paged_ops()
+_define_paged_op(
+    "paged_slots_(Tensor(a!) block_table, Tensor seq_lens, Tensor new_lens, Tensor free_pages, int page_size, "
+    "SymInt num_tokens) -> (Tensor, Tensor, Tensor, Tensor, Tensor)", _paged_slots_fake)
+_define_paged_op(
+    "rope_paged_write_(Tensor k, Tensor v, Tensor? cos, Tensor? sin, Tensor positions, Tensor slots, "
+    "Tensor(a!) k_cache, Tensor(b!) v_cache) -> ()", lambda *args: None)
+_define_paged_op(
+    "sqdk_paged_fwd(Tensor q, Tensor k_cache, Tensor v_cache, Tensor block_table, Tensor kv_lens, Tensor cu_q, "
+    "Tensor positions, float sm_scale, int max_q) -> Tensor", _sqdk_paged_fwd_fake)
 
 
 def device_errors(device: Optional[torch.device] = None, clear: bool = True) -> int:

@@ -3,6 +3,9 @@ of the Python entry points (no kernel launches), and the tests' plain forms
 against the oracle."""
 
 import ctypes
+import os
+import subprocess
+import sys
 
 import numpy as np
 import pytest
@@ -12,6 +15,7 @@ import oracle
 from hspmn_b200 import _native as N
 from hspmn_b200 import ops
 from tests import paged_ref as ref
+from tests.conftest import PKG
 
 P = ctypes.c_void_p(4096)
 INVALID, DTYPE, ALIGN, UNSUPPORTED = -1, -2, -3, -4
@@ -80,6 +84,53 @@ def test_ops_refuse_cpu_tensors():
         ops.rope_paged_write_(x, x, None, None, j, j, c, c)
     with pytest.raises(RuntimeError, match="CUDA tensors"):
         ops.sqdk_paged_fwd(x, c, c, t, i, i, j, 0.1)
+
+
+def python(code, path):
+    return subprocess.run([sys.executable, "-c", code], capture_output=True, text=True, timeout=300,
+                          env=dict(os.environ, PYTHONPATH=str(path), CUDA_VISIBLE_DEVICES=""))
+
+
+def test_importing_the_package_loads_no_library():
+    r = python("import hspmn_b200, torch\n"
+               "from hspmn_b200 import HSPMNBlock, HSPMNConfig\n"
+               "HSPMNBlock(HSPMNConfig(dim=64, num_heads=4, num_kv_heads=2))\n"
+               "for name in ('paged_slots_', 'rope_paged_write_', 'sqdk_paged_fwd'):\n"
+               "    getattr(torch.ops.hspmn, name).default\n"
+               "assert 'libhspmn' not in open('/proc/self/maps').read()\n"
+               "t = torch.zeros((1, 2), dtype=torch.int32)\n"
+               "for op in (hspmn_b200.ops.paged_slots_, torch.ops.hspmn.paged_slots_):\n"
+               "    try:\n"
+               "        op(t, t[0, :1], t[0, :1], t[0], 8, 1)\n"
+               "        assert False\n"
+               "    except RuntimeError as e:\n"
+               "        assert 'CUDA tensors' in str(e), e\n"
+               "assert 'libhspmn_torch' in open('/proc/self/maps').read()\n", PKG)
+    assert r.returncode == 0, r.stderr[-2000:]
+
+
+@pytest.mark.parametrize("torch_lib", [None, b"built for something else"])
+def test_package_without_a_fitting_operator_library(tmp_path, torch_lib):
+    """The rest of the package works; a paged operator says what to do, called or registered."""
+    pkg = tmp_path / "hspmn_b200"
+    pkg.mkdir()
+    for f in os.listdir(os.path.dirname(N.LIB_PATH)):
+        if f.endswith(".py") or f == N.LIB_NAME:
+            os.symlink(os.path.join(os.path.dirname(N.LIB_PATH), f), pkg / f)
+    if torch_lib is not None:
+        (pkg / os.path.basename(N.TORCH_LIB_PATH)).write_bytes(torch_lib)
+    r = python("import hspmn_b200, torch\n"
+               f"assert hspmn_b200.__file__.startswith({str(tmp_path)!r})\n"
+               "assert hspmn_b200.native_available() and hspmn_b200._native.lib().hspmn_version() > 0\n"
+               "t = torch.zeros((1, 2), dtype=torch.int32)\n"
+               "for op in (hspmn_b200.ops.paged_slots_, torch.ops.hspmn.paged_slots_):\n"
+               "    for _ in range(2):\n"
+               "        try:\n"
+               "            op(t, t[0, :1], t[0, :1], t[0], 8, 1)\n"
+               "            assert False\n"
+               "        except RuntimeError as e:\n"
+               "            assert 'build_native.py' in str(e), e\n", tmp_path)
+    assert r.returncode == 0, r.stderr[-2000:]
 
 
 def test_plain_attention_is_the_oracles():
