@@ -4,7 +4,8 @@ libhspmn_torch.so, which registers its paged-cache operators with PyTorch.
 Both are compiled in-tree (next to the Python package): the CUDA library with
 nvcc for ``sm_100a`` only (the product has no other target), the operators
 with the host compiler against the installed PyTorch. Each is rebuilt only
-when a source it is made from is newer.
+when a source it is made from is newer; the operators also when they were
+built for another PyTorch or Python.
 
     python hspmn-v2.1_b200/build_native.py [--force] [-v]
 """
@@ -13,6 +14,7 @@ from __future__ import annotations
 
 import argparse
 import glob
+import importlib.util
 import os
 import shutil
 import subprocess
@@ -72,9 +74,21 @@ def run(cmd, out: str, verbose: bool) -> None:
     os.replace(out + ".tmp", out)
 
 
+def native():
+    """The package's binding module, without the package."""
+    spec = importlib.util.spec_from_file_location("hspmn_native", os.path.join(HERE, "hspmn_b200", "_native.py"))
+    module = importlib.util.module_from_spec(spec)
+    spec.loader.exec_module(module)
+    return module
+
+
+def torch_ops_up_to_date() -> bool:
+    made_from = [TORCH_SOURCE, os.path.join(INCLUDE, "hspmn_sm100.h")]
+    return up_to_date(TORCH_LIB, made_from) and native().built_for_this_torch(TORCH_LIB)
+
+
 def build_torch_ops(force: bool = False, verbose: bool = False) -> str:
-    header = os.path.join(INCLUDE, "hspmn_sm100.h")
-    if not force and up_to_date(TORCH_LIB, [TORCH_SOURCE, header]):
+    if not force and torch_ops_up_to_date():
         return TORCH_LIB
     import sysconfig
     import torch
@@ -82,6 +96,7 @@ def build_torch_ops(force: bool = False, verbose: bool = False) -> str:
     cuda_include = os.path.join(os.path.dirname(os.path.dirname(os.path.realpath(nvcc()))), "include")
     cmd = [cxx(), "-O2", "-std=c++17", "-fPIC", "-shared", "-fvisibility=hidden",
            f"-D_GLIBCXX_USE_CXX11_ABI={int(torch._C._GLIBCXX_USE_CXX11_ABI)}",
+           f'-DHSPMN_TORCH_BUILD_ID="{native().torch_build_id()}"',
            *(f"-isystem{p}" for p in (*include_paths(), cuda_include, sysconfig.get_paths()["include"])), "-I", INCLUDE, TORCH_SOURCE,
            "-o", TORCH_LIB + ".tmp", "-L", os.path.dirname(LIB), "-l:" + os.path.basename(LIB), "-Wl,-rpath,$ORIGIN",
            *(f"-L{p}" for p in library_paths()), "-lc10", "-lc10_cuda", "-ltorch_cpu", "-ltorch_cuda",

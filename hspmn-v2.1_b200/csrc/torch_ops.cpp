@@ -261,6 +261,13 @@ TORCH_LIBRARY_IMPL(hspmn, CUDA, m) {
   m.impl("sqdk_paged_fwd", sqdk_paged_fwd);
 }
 
+// What this file was built for (found in the built file: a library that was built for
+// another PyTorch must not be loaded to ask it).
+extern "C" {
+extern const char hspmn_torch_build_id[];
+__attribute__((visibility("default"), used)) const char hspmn_torch_build_id[] = HSPMN_TORCH_BUILD_ID;
+}
+
 PYBIND11_MODULE(libhspmn_torch, m) {
   m.def("paged_slots_", paged_slots_<true>);
   m.def("rope_paged_write_", rope_paged_write_);

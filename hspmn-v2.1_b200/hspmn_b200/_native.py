@@ -93,6 +93,19 @@ def lib() -> ctypes.CDLL:
     return _lib
 
 
+def torch_build_id() -> str:
+    """What libhspmn_torch.so must have been built for, as it stands in the file."""
+    import sysconfig
+    import torch
+    return (f"hspmn_torch for torch {torch.__version__}, C++ ABI {int(torch._C._GLIBCXX_USE_CXX11_ABI)}, "
+            f"{sysconfig.get_config_var('SOABI')};")
+
+
+def built_for_this_torch(path: str) -> bool:
+    with open(path, "rb") as f:
+        return torch_build_id().encode() in f.read()
+
+
 def load_torch_ops():
     """Load libhspmn_torch.so: its operators are then registered with PyTorch.
     Returns it as a Python module; raises if it is not built, or not for this
@@ -105,6 +118,10 @@ def load_torch_ops():
     import importlib.util
     import torch  # noqa: F401 (the module links against its libraries)
     lib()
+    if not built_for_this_torch(TORCH_LIB_PATH):
+        raise RuntimeError(
+            f"{TORCH_LIB_PATH} was not built for PyTorch {torch.__version__} and this Python; run "
+            "`python hspmn-v2.1_b200/build_native.py` on a machine with the CUDA toolkit")
     loader = importlib.machinery.ExtensionFileLoader("libhspmn_torch", TORCH_LIB_PATH)
     try:
         module = importlib.util.module_from_spec(importlib.util.spec_from_loader("libhspmn_torch", loader))

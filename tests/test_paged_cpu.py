@@ -133,6 +133,30 @@ def test_package_without_a_fitting_operator_library(tmp_path, torch_lib):
     assert r.returncode == 0, r.stderr[-2000:]
 
 
+def test_operator_library_is_rebuilt_for_another_pytorch(tmp_path, monkeypatch):
+    """A file newer than its sources does not do: it must be built for this PyTorch and Python."""
+    import build_native
+    assert build_native.torch_ops_up_to_date()  # as built
+    lib = tmp_path / "libhspmn_torch.so"
+    monkeypatch.setattr(build_native, "TORCH_LIB", str(lib))
+    assert not build_native.torch_ops_up_to_date()
+    with open(N.TORCH_LIB_PATH, "rb") as f:
+        built = f.read()
+    mark = N.torch_build_id().encode()
+    assert built.count(mark) == 1 and torch.__version__.encode() in mark
+    lib.write_bytes(built)
+    assert build_native.torch_ops_up_to_date()
+    lib.write_bytes(built.replace(mark, mark.replace(torch.__version__.encode(), b"x" * len(torch.__version__))))
+    assert not build_native.torch_ops_up_to_date()
+    monkeypatch.setattr(torch, "__version__", torch.__version__ + "1")
+    lib.write_bytes(built)
+    assert not build_native.torch_ops_up_to_date()
+    # and is not loaded: entry points may have changed their meaning without changing their names
+    monkeypatch.setattr(N, "TORCH_LIB_PATH", str(lib))
+    with pytest.raises(RuntimeError, match="build_native.py"):
+        N.load_torch_ops()
+
+
 def test_plain_attention_is_the_oracles():
     g = torch.Generator().manual_seed(0)
     B, S, H, Hkv, hd, page = 2, 45, 6, 2, 16, 8
