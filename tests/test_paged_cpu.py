@@ -157,6 +157,21 @@ def test_operator_library_is_rebuilt_for_another_pytorch(tmp_path, monkeypatch):
         N.load_torch_ops()
 
 
+def test_cuda_library_is_built_without_the_operator_library(monkeypatch):
+    """A host without PyTorch or with another compiler still gets the library of the C ABI, and is told."""
+    import build_native
+
+    def fails(*args):
+        raise RuntimeError("g++ failed: no such header")
+
+    monkeypatch.setattr(build_native, "build_torch_ops", fails)
+    with pytest.warns(RuntimeWarning, match="paged-cache operators.*no such header"):
+        assert build_native.build() == build_native.LIB
+    monkeypatch.setattr(build_native, "run", fails)  # the CUDA library itself must build
+    with pytest.raises(RuntimeError, match="g.. failed"):
+        build_native.build(force=True)
+
+
 def test_plain_attention_is_the_oracles():
     g = torch.Generator().manual_seed(0)
     B, S, H, Hkv, hd, page = 2, 45, 6, 2, 16, 8
