@@ -359,7 +359,7 @@ __host__ __device__ constexpr uint32_t umma_idesc_f16(int M, int N, int ab, bool
 // ---------------------------------------------------------------------------
 
 // A kernel launched as a programmatic dependent may begin while the one before it
-// in the stream still runs; it calls grid_dependency_wait() before it touches
+// in the stream still runs; it calls grid_dependency_enter() before it touches
 // memory, and reads what earlier kernels wrote by coherent loads only (the
 // read-only path, __ldg, is for what does not change while a kernel is in flight,
 // and may be moved in front of the wait).
@@ -369,6 +369,22 @@ __host__ __device__ constexpr uint32_t umma_idesc_f16(int M, int N, int ab, bool
 __device__ __forceinline__ void grid_dependents_launch() { asm volatile("griddepcontrol.launch_dependents;" ::: "memory"); }
 // Waits until the grid before this one has finished and its writes are visible.
 __device__ __forceinline__ void grid_dependency_wait() { asm volatile("griddepcontrol.wait;" ::: "memory"); }
+// What such a kernel begins with, in this order: a grid begins once every CTA of the
+// one before it has let it, so by then all grids before that one have ended. One
+// kernel uses this: the 16-row attention kernel of a call with chunks needs nothing
+// of the chunk kernel in front of it, and would otherwise wait for all of it. It
+// begins with grid_dependency_behind() and reads what was written before the chunk
+// kernel on the strength of the chunk kernel's wait; it waits itself before it ends.
+__device__ __forceinline__ void grid_dependency_enter() {
+  grid_dependency_wait();
+  grid_dependents_launch();
+}
+// The fence is the acquire that its own wait would have been: nothing read from here
+// on is older (no line of L1 from before it either).
+__device__ __forceinline__ void grid_dependency_behind() {
+  __threadfence();
+  grid_dependents_launch();
+}
 // A load that stays behind grid_dependency_wait() (what it reads may have been
 // written by the grid before, so not through the read-only path).
 __device__ __forceinline__ int load_now(const int* p) {

@@ -68,8 +68,7 @@ __global__ void __launch_bounds__(kSlotsThreads) paged_slots_kernel(const SlotsP
   int* s_page = slots_smem + (p.R + 1);  // [R+1]
   __shared__ int2 warp_sum[kSlotsWarps];
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
-  grid_dependency_wait();
-  grid_dependents_launch();
+  grid_dependency_enter();
   int2 carry = make_int2(0, 0);
   bool bad = false;
   if (threadIdx.x == 0) s_tok[0] = s_page[0] = 0;
@@ -209,8 +208,7 @@ __global__ void __launch_bounds__(kRowThreads) rope_paged_write_kernel(const Pag
   const int vh1 = (lane + kLanes) / vgroups, vc1 = lane + kLanes - vh1 * vgroups;
   auto source = [](const char* row, int64_t sh, int h, int c) { return reinterpret_cast<const uint4*>(row + h * sh + c * 16); };
   const int64_t step = static_cast<int64_t>(gridDim.x) * kTokens;
-  grid_dependency_wait();
-  grid_dependents_launch();
+  grid_dependency_enter();
   int64_t t = static_cast<int64_t>(blockIdx.x) * kTokens + threadIdx.x / kLanes;
   int64_t slot = t < p.N ? p.slots[t] : -1, pos = rope && t < p.N ? p.pos[t] : 0;
   for (; t < p.N; t += step) {

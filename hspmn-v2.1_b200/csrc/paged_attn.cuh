@@ -383,9 +383,9 @@ __global__ void __launch_bounds__(kPagedThreads, kPagedCtasPerSm) paged_attn_ker
   __shared__ __align__(8) int64_t s_pos[kPagedStages][kPagedRows];
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   const int g = lane >> 2, t2 = (lane & 3) * 2;  // accumulator row and first column of this lane
-  // (the chunk kernel lets this one begin behind its own wait)
-  if (!p.has_chunks) grid_dependency_wait();
-  grid_dependents_launch();
+  // the chunk kernel in front of this one has entered: see grid_dependency_enter
+  if (p.has_chunks) grid_dependency_behind();
+  else grid_dependency_enter();
   const int split = paged_split<L::kKeys>(p, lane);
   PagedList<L::kKeys> list(p, split, lane);
   const int total = list.total();
@@ -818,8 +818,7 @@ __device__ __forceinline__ void paged_merge(const PagedAttnParams& p, int block)
 
 template <int HD, bool kBF16>
 __global__ void __launch_bounds__(32 * kMergeWarps) paged_merge_kernel(const __grid_constant__ PagedAttnParams p) {
-  grid_dependency_wait();
-  grid_dependents_launch();
+  grid_dependency_enter();
   paged_merge<HD, kBF16>(p, static_cast<int>(blockIdx.x));
 }
 

@@ -386,8 +386,7 @@ __global__ void __launch_bounds__(kChunkThreads, kChunkCtasPerSm)
 
   const uint32_t sbase = (smem_u32(chunk_smem_raw) + 1023u) & ~1023u;
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-  grid_dependency_wait();
-  grid_dependents_launch();
+  grid_dependency_enter();  // (the 16-row kernel counts on it too)
   // no request for this kernel, or bad offsets (the 16-row kernel says so):
   // nothing to set up
   const int split = paged_split<PagedLayout<HD>::kKeys>(p.a, lane);
@@ -950,8 +949,7 @@ __device__ __forceinline__ void chunk_merge(const ChunkParams& p, int run, int s
 template <int HD, bool kBF16>
 __global__ void __launch_bounds__(32 * kMergeWarps, 2)
     paged_both_merge_kernel(const __grid_constant__ PagedAttnParams p, const __grid_constant__ ChunkParams c, int paged_runs) {
-  grid_dependency_wait();
-  grid_dependents_launch();
+  grid_dependency_enter();
   const int block = static_cast<int>(blockIdx.x) - paged_runs;
   if (block < 0) paged_merge<HD, kBF16>(p, static_cast<int>(blockIdx.x));
   else chunk_merge<HD, kBF16>(c, block / kChunkMergeBlocks, block % kChunkMergeBlocks);

@@ -172,6 +172,24 @@ def test_cuda_library_is_built_without_the_operator_library(monkeypatch):
         build_native.build(force=True)
 
 
+def test_dependent_kernels_wait_before_they_release():
+    """A kernel that let the next one begin in front of its own wait would let the 16-row attention kernel, which
+    counts on the wait of the kernel before it, read what is still being written."""
+    import build_native
+    text = {os.path.basename(f): open(f).read() for f in build_native.sources() if f.endswith((".cu", ".cuh"))}
+    begins = ("grid_dependency_enter();", "grid_dependency_behind();")
+    kernels = 0
+    for name in ("paged.cuh", "paged_attn.cuh", "paged_chunk.cuh"):
+        assert "grid_dependents_launch" not in text[name] and "griddepcontrol" not in text[name], name
+        for body in text[name].split("__global__")[1:]:
+            kernels += 1
+            assert begins[0] in body, name
+    assert kernels == 6
+    assert sum(t.count(begins[1]) for n, t in text.items() if n != "common.cuh") == 1
+    enter = text["common.cuh"].split("void grid_dependency_enter() {")[1].split("}")[0]
+    assert enter.index("grid_dependency_wait();") < enter.index("grid_dependents_launch();")
+
+
 def test_plain_attention_is_the_oracles():
     g = torch.Generator().manual_seed(0)
     B, S, H, Hkv, hd, page = 2, 45, 6, 2, 16, 8
