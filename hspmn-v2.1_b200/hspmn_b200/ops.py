@@ -748,7 +748,7 @@ _define_paged_op(
     "Tensor(a!) k_cache, Tensor(b!) v_cache) -> ()", lambda *args: None)
 _define_paged_op(
     "sqdk_paged_fwd(Tensor q, Tensor k_cache, Tensor v_cache, Tensor block_table, Tensor kv_lens, Tensor cu_q, "
-    "Tensor positions, float sm_scale, int max_q) -> Tensor", _sqdk_paged_fwd_fake)
+    "Tensor positions, float sm_scale, SymInt max_q) -> Tensor", _sqdk_paged_fwd_fake)
 
 
 def device_errors(device: Optional[torch.device] = None, clear: bool = True) -> int:

@@ -978,6 +978,52 @@ def test_compiled_step_is_one_graph():
     assert torch.equal(got, step(q, kc, vc))
 
 
+@pytest.mark.parametrize("backend", ["eager", "aot_eager"])
+def test_compiled_serving_step(backend):
+    """The three operators in one graph: tables and caches that are its inputs are written in place, as eager calls
+    write them, and so are tensors that it makes itself."""
+    R, page, Hkv, H, hd, n = 2, 16, 2, 8, 64, 25
+    g = torch.Generator().manual_seed(46)
+    k, v = (torch.randn((n, Hkv, hd), generator=g).to(torch.bfloat16).to(DEV) for _ in range(2))
+    q = torch.randn((n, H, hd), generator=g).to(torch.bfloat16).to(DEV)
+    cos, sin = tables(64, hd, torch.float32, g)
+    free = i32([3, 1, 5, 0])
+    caches = torch.randn((2, 6, page, Hkv, hd), generator=g).to(torch.bfloat16).to(DEV)
+
+    def step(table, kc, vc, seq, new, k, v, q):
+        cu, kv, pos, slots, taken = ops.paged_slots_(table, seq, new, free, page, n)
+        ops.rope_paged_write_(k * 2, v, cos, sin, pos, slots, kc, vc)
+        own_k, own_v = kc + 1, torch.zeros_like(vc)
+        ops.rope_paged_write_(k, v, None, None, pos, slots, own_k, own_v)
+        return (ops.sqdk_paged_fwd(q + 1, kc, vc, table, kv, cu, pos, 0.125, 20), own_k.sum(), own_v, cu, kv, pos, slots,
+                taken)
+
+    def run(f):
+        table, (kc, vc) = i32([[4, -1, -1], [-1, -1, 9]]), caches.clone()
+        out = f(table, kc, vc, i32([9, 0]), i32([20, 4]), k, v, q)
+        return (*out, table, kc, vc)
+
+    want = run(step)
+    compiled = torch.compile(step, backend=backend, fullgraph=True)
+    for _ in range(2):
+        for a, b in zip(run(compiled), want):
+            assert torch.equal(a, b)
+    assert want[-3].tolist() == [[4, 3, -1], [1, -1, 9]]
+    assert ops.device_errors() == 0
+
+
+def test_compiled_step_takes_any_max_q():
+    from torch._dynamo.testing import CompileCounterWithBackend
+    args = batch([20, 50], [[19], [49, 48, 47]], 4, 2, 64, torch.bfloat16, 16, seed=47)
+    q, kc, vc, table, kv, cu, pos = args
+    kv, cu = i32(kv), i32(cu)
+    counter = CompileCounterWithBackend("aot_eager")
+    step = torch.compile(lambda m: ops.sqdk_paged_fwd(q, kc, vc, table, kv, cu, pos, 0.125, m), backend=counter, fullgraph=True)
+    for m in (3, 4, 5, 9, 60):
+        assert torch.equal(step(m), ops.sqdk_paged_fwd(q, kc, vc, table, kv, cu, pos, 0.125, m))
+    assert counter.frame_count <= 2  # the first value, and any other
+
+
 def test_registered_operators_trace():
     args = batch([20], [[19]], 4, 2, 64, torch.bfloat16, 16, seed=14)
     q, kc, vc, table, kv, cu, pos = args
