@@ -701,6 +701,60 @@ def test_captured_step_replays_with_new_lengths():
     assert ops.device_errors() == 0
 
 
+def test_captured_padded_step_with_rotated_queries():
+    """A whole step as a user has it, rotation of the queries included, of fewer tokens than it has room for: right,
+    and nothing is flagged (the places behind the last token have no position, which rope_gather_rows would flag)."""
+    R, P, page, H, Hkv, hd, cap, L = 3, 10, 16, 8, 2, 64, 40, 160
+    g = torch.Generator().manual_seed(48)
+    kc, vc = (torch.zeros((40, page, Hkv, hd), dtype=torch.bfloat16, device=DEV) for _ in range(2))
+    table = torch.full((R, P), -1, dtype=torch.int32, device=DEV)
+    seq, new, free = i32([0] * R), i32([0] * R), i32(list(range(40)))
+    cos, sin = tables(L, hd, torch.bfloat16, g)
+    k, v = (torch.zeros((cap, Hkv, hd), dtype=torch.bfloat16, device=DEV) for _ in range(2))
+    q = torch.zeros((cap, H, hd), dtype=torch.bfloat16, device=DEV)
+
+    def step():
+        cu, kv_lens, pos, slots, taken = ops.paged_slots_(table, seq, new, free, page, cap)
+        ops.rope_paged_write_(k, v, cos, sin, pos, slots, kc, vc)
+        turned = ops.rope_gather_rows(q[None], pos.clamp(min=0)[None], cos, sin, False)[0]
+        return cu, pos, taken, turned, ops.sqdk_paged_fwd(turned, kc, vc, table, kv_lens, cu, pos, 0.125)
+
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        step()
+    torch.cuda.current_stream().wait_stream(side)
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        out = step()
+    held, whole = [0] * R, [[] for _ in range(R)]  # each request's keys as they came, not rotated
+    u = torch.finfo(torch.bfloat16).eps / 2
+    for lens in ([30, 0, 7], [1, 33, 1], [1, 1, 1], [0, 1, 20], [0, 0, 0], [1, 1, 1]):
+        seq.copy_(i32(held))
+        new.copy_(i32(lens))
+        for t in (k, v, q):
+            t.copy_(torch.randn(t.shape, generator=g))
+        graph.replay()
+        assert ops.device_errors() == 0
+        cu, pos, taken, turned, o = out
+        n, at = cu[-1].item(), cu.tolist()
+        # three roundings of the reference's operations: two products and their sum
+        want, size = ref.rope_ref(q[:n], cos, sin, pos[:n])
+        assert ((turned[:n].double() - want).abs() <= u * (size + want.abs()) * (1 + 2 * u) + 2.0 ** -120).all()
+        held = [a + b for a, b in zip(held, lens)]
+        for r in range(R):
+            whole[r].append(k[at[r]:at[r + 1]].clone())
+            x = torch.cat(whole[r])
+            m = torch.arange(held[r], device=DEV)
+            got = kc[table[r, m // page].long(), m % page].double()
+            want, size = ref.rope_ref(x, cos, sin, m)
+            assert ((got - want).abs() <= u * want.abs() * (1 + 1e-6) + 3 * 2.0 ** -24 * size + 2.0 ** -120).all()
+        want, tol = ref.attend_ref(turned, kc, vc, table, held, at, pos, 0.125)
+        assert ((o.double() - want).abs() <= tol).all() and not o[n:].any()
+        free.copy_(torch.roll(free, -taken.item()))
+    assert ops.device_errors() == 0
+
+
 def serve(steps, sync):
     """Steps of slots, write and attention (chunks and single tokens) whose operands the steps before wrote,
     with small kernels and copies of other kinds between them; all that came out."""
