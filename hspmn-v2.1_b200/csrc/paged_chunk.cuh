@@ -427,6 +427,13 @@ __global__ void __launch_bounds__(kChunkThreads, kChunkCtasPerSm)
     row_off[rr] = ql < p.QT ? ql * p.a.o_sn + (rr - ql * p.a.G) * p.a.o_sh : -1;
     for (int x = 0; x < 2; ++x)
       if (rr < HD) wild_key[x][0][rr] = wild_key[x][1][rr] = kNoKey;
+    // rows behind the G * QT that the copies of Q fill: zeros, since what shared
+    // memory happens to hold there would share its warp's choice of a maximum
+    if (ql >= p.QT) {
+      for (int c = 0; c < L::kChunks * 8; ++c)
+        st_shared_v4(sbase + L::kQOff + (c >> 3) * L::kQChunkBytes + rr * 128 + (c & 7) * 16, make_uint4(0u, 0u, 0u, 0u));
+      fence_proxy_async_smem();
+    }
   }
   tc_fence_before();
   __syncthreads();

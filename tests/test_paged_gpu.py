@@ -583,6 +583,21 @@ def test_results_do_not_depend_on_the_run():
         assert torch.equal(attend(*args, max_q=400), first)
 
 
+@pytest.mark.parametrize("H,Hkv,hd", [(12, 4, 64), (6, 2, 96), (12, 4, 128), (10, 2, 64), (7, 1, 64), (96, 1, 64)])
+def test_results_do_not_depend_on_the_calls_before(H, Hkv, hd):
+    """Head groups that do not fill a tile's 128 rows: its other rows must not hold what a call before left in shared
+    memory (they share warps with real rows, whose way through the softmax they decide)."""
+    wide = 64 if hd <= 64 else 128
+    before = batch([600] * 8, [list(range(600))] * 8, 16, 4, wide, torch.bfloat16, 64, seed=49)
+    args = batch([900] * 4, [list(range(300, 900, 3))] * 4, H, Hkv, hd, torch.bfloat16, 64, seed=50)
+    check(args, max_qs=(200,))
+    outs = []
+    for x in (float("nan"), 0.0, float("inf"), 3.0e38, 1.0):
+        attend(torch.full_like(before[0], x), *before[1:], max_q=600)
+        outs.append(attend(*args, max_q=200))
+    assert all(torch.equal(o, outs[0]) for o in outs)
+
+
 def test_offsets_past_32_bits():
     """Pages far into a cache of more than 2^32 bytes."""
     page, Hkv, hd = 64, 4, 128
