@@ -24,8 +24,9 @@
 // of any size weigh right. The products fill a fifth of the tensor pipe, so
 // 128-row tiles would not be faster; three stages of two CTAs an SM keep 192 KB
 // an SM on the way (three CTAs with two stages: 178 -> 221 us). 64 tokens over
-// 1.15 GB of K and V (contexts to 32768, 16/4 heads of 128) take 176 us, 6.5 TB/s;
-// one token over 262144 keys 92 us (5.8 TB/s: the start and the merge of 74 runs
+// 1.15 GB of K and V (contexts to 32768, 16/4 heads of 128) take 176 us, 6.5 TB/s
+// (182 to 184 in calls in a row for seconds, at the card's 1 kW and 1.58 GHz); one
+// token over 262144 keys 92 us (5.8 TB/s: the start and the merge of 74 runs
 // an item take 9 us); 37 tokens of 16 heads of 64 over up to 8192 keys 63 us (4.9
 // TB/s: 592 short items). One token over 500 keys takes 7.7 us, two launches and a
 // few rounds of loads.
@@ -44,7 +45,7 @@ constexpr int kPagedStages = 3;
 constexpr int kPagedItemCost = 2;
 constexpr int kPagedCtasPerSm = 2;
 constexpr int kPagedMidRows = 128;      // see paged_split
-constexpr int kPagedMidScore = 14200;
+constexpr int kPagedMidScore = 14200;   // quarters of a microsecond: 12 us of 296 CTAs (148 SMs)
 
 // Row sum of a part that holds no key its row sees (a true sum is not negative).
 constexpr float kUnseen = -1.0f;
@@ -600,7 +601,7 @@ __global__ void __launch_bounds__(kPagedThreads, kPagedCtasPerSm) paged_attn_ker
       }
       // Where some row sees a key and another does not, an infinity or NaN in
       // that key's V must not reach the other (0 * inf): such a step adds its
-      // products one by one.
+      // products one by one (with P as it is: no operand to round it for).
       bool wild = false;
       if (masked) {
         bool mine = false;

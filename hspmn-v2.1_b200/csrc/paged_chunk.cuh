@@ -27,12 +27,14 @@
 // across tiles, so the next tile's keys load while this one ends.
 //
 // Bound: the chain of softmax and products of an SM's two CTAs (a block takes a
-// CTA about 1,800 cycles; tensor pipe and exponentials 50 % busy each), near the
-// card's 1 kW. A fifth of 8192 new tokens over 24576 cached, three requests of
-// 16/4 heads of 128: 1.24 ms, 930 TFLOP/s. Seven whole prompts of 511 to 4096
-// tokens: 247 us, 872 TFLOP/s (tiles of 23 blocks on average, each 5 blocks' time
-// to open and close). Eight softmax warps (258 us) and 128-key blocks with one S
-// buffer (283 us) were slower.
+// CTA about 1,700 cycles; tensor pipe and exponentials 43 % busy each), at the
+// card's 1 kW. Calls in a row for seconds: a fifth of 8192 new tokens over 24576
+// cached, three requests of 16/4 heads of 128, 1.27 to 1.30 ms, 890 to 910 TFLOP/s
+// (SM at 1.40 GHz); seven whole prompts of 511 to 4096 tokens 279 to 286 us, 754 to
+// 774 TFLOP/s (1.70 GHz; tiles of 23 blocks on average, each 5 blocks' time to open
+// and close). The prompts in bursts of 20 ms, before the power limit lowers the
+// clock: 245 to 247 us; there, eight softmax warps took 258 (against 249 then) and
+// 128-key blocks with one S buffer 283.
 #pragma once
 
 #include "paged_attn.cuh"
@@ -42,7 +44,7 @@ namespace hspmn {
 constexpr int kChunkThreads = 192;
 constexpr int kChunkCtasPerSm = 2;
 constexpr int kChunkUnit = 16;           // cost units of a 64-key block
-constexpr int kChunkTileCost = 5;        // blocks' worth of time to open and close a tile (seven prompts: 247 us; at 3 256, 6 250, 7 252, 9 262)
+constexpr int kChunkTileCost = 5;        // blocks' worth of time to open and close a tile (seven prompts in bursts of 20 ms: 247 us; at 3 256, 6 250, 7 252, 9 262)
 constexpr int kChunkMinPiece = 8;        // blocks of work below which another run is not opened
 constexpr int kChunkEpilogueBar = 1;     // named barrier of the four softmax warps
 constexpr int kChunkTilt = 3;            // see ChunkRuns, in 64ths
@@ -185,7 +187,8 @@ struct ChunkList {
 // Runs of the list. Of the two CTAs that share an SM, the one launched first (the
 // first half of a full grid) is 10 % faster while both are at work, so its run is
 // longer: with a tilt of 0, 3, 5, 7 64ths, 285.0, 280.5, 280.6, 284.6 us for seven
-// prompts, 131.2, 128.5, 129.4, 130.2 for 52 requests of chunks and single tokens.
+// prompts, 131.2, 128.5, 129.4, 130.2 for 52 requests of chunks and single tokens
+// (calls in a row for seconds).
 struct ChunkRuns {
   int share, rem, tilt, n;
   __device__ __forceinline__ ChunkRuns(int total, int runs, int most) {
@@ -671,7 +674,9 @@ __global__ void __launch_bounds__(kChunkThreads, kChunkCtasPerSm)
           }
         }
         uint32_t pk[kSqdkBN / 2];
-        // p = 2^((s - m) c2), packed; returns the block's row sum. kFma: as
+        // p = 2^((s - m) c2), packed in the operands' type (as in the 16-row kernel, for
+        // the same reason: half a step, the size of the output's own rounding; the row
+        // sum takes p before it); returns the block's row sum. kFma: as
         // s c2 - (m c2), one operation instead of two, with the rounding of m c2
         // (2^-15 at kChunkFmaMax) in every p.
         auto exponentiate = [&](auto kFma, float m) -> float {

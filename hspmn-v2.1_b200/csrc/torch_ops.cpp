@@ -4,7 +4,8 @@
 // GPU work each (through Python checks and ctypes a call took 28 to 37 us of host
 // time). Registered as torch.ops.hspmn.* for CUDA tensors, for traced calls, and as
 // functions of the Python module libhspmn_torch, which eager calls use: the
-// dispatcher's boxing of the arguments costs 2 us more.
+// dispatcher's boxing of the arguments costs 1 us more (6.9 and 7.9 us a call of
+// the attention of one token).
 #include <ATen/ATen.h>
 #include <ATen/cuda/EmptyTensor.h>
 #include <c10/core/AutogradState.h>
