@@ -25,7 +25,7 @@
 // 128-row tiles would not be faster; three stages of two CTAs an SM keep 192 KB
 // an SM on the way (three CTAs with two stages: 178 -> 221 us). 64 tokens over
 // 1.15 GB of K and V (contexts to 32768, 16/4 heads of 128) take 176 us, 6.5 TB/s
-// (182 to 184 in calls in a row for seconds, at the card's 1 kW and 1.58 GHz); one
+// (175 to 184 in calls in a row for seconds, at the card's 1 kW, by the card); one
 // token over 262144 keys 92 us (5.8 TB/s: the start and the merge of 74 runs
 // an item take 9 us); 37 tokens of 16 heads of 64 over up to 8192 keys 63 us (4.9
 // TB/s: 592 short items). One token over 500 keys takes 7.7 us, two launches and a

@@ -29,7 +29,7 @@
 // Bound: the chain of softmax and products of an SM's two CTAs (a block takes a
 // CTA about 1,700 cycles; tensor pipe and exponentials 43 % busy each), at the
 // card's 1 kW. Calls in a row for seconds: a fifth of 8192 new tokens over 24576
-// cached, three requests of 16/4 heads of 128, 1.27 to 1.30 ms, 890 to 910 TFLOP/s
+// cached, three requests of 16/4 heads of 128, 1.24 to 1.30 ms, 890 to 927 TFLOP/s
 // (SM at 1.40 GHz); seven whole prompts of 511 to 4096 tokens 279 to 286 us, 754 to
 // 774 TFLOP/s (1.70 GHz; tiles of 23 blocks on average, each 5 blocks' time to open
 // and close). The prompts in bursts of 20 ms, before the power limit lowers the
